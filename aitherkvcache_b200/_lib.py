@@ -167,6 +167,43 @@ class TriDecodeParams(C.Structure):
     ]
 
 
+class RotaryTables(C.Structure):
+    """Mirror of ``akv_rotary_tables``."""
+    _fields_ = [
+        ("head_dim", c_int), ("rotary_dim", c_int), ("num_axes", c_int), ("adjacent", c_int),
+        ("steps", c_vp), ("axes", c_vp),
+        ("scaling", c_f),
+    ]
+
+
+class RotaryParams(C.Structure):
+    """Mirror of ``akv_rotary_params``."""
+    _fields_ = [
+        ("tables", C.POINTER(RotaryTables)),
+        ("positions", c_vp), ("pos_dtype", c_int), ("pos_stride_axis", c_i64), ("pos_stride_tok", c_i64),
+        ("num_tokens", c_i64),
+        ("in_dtype", c_int), ("out_dtype", c_int),
+        ("query", c_vp), ("q_stride_tok", c_i64), ("q_stride_head", c_i64), ("num_q_heads", c_int),
+        ("q_out", c_vp), ("qo_stride_tok", c_i64), ("qo_stride_head", c_i64),
+        ("key", c_vp), ("k_stride_tok", c_i64), ("k_stride_head", c_i64), ("num_kv_heads", c_int),
+        ("k_out", c_vp), ("ko_stride_tok", c_i64), ("ko_stride_head", c_i64),
+        ("inverse", c_int),
+        ("stream", c_vp),
+    ]
+
+
+class RotaryAppendParams(C.Structure):
+    """Mirror of ``akv_rotary_append_params``."""
+    _fields_ = [
+        ("rotary", RotaryParams),
+        ("value", c_vp), ("v_stride_tok", c_i64), ("v_stride_head", c_i64),
+        ("slot_mapping", c_vp), ("slot_dtype", c_int),
+        ("k_cache", c_vp), ("kc_stride_blk", c_i64), ("kc_stride_pos", c_i64), ("kc_stride_head", c_i64),
+        ("v_cache", c_vp), ("vc_stride_blk", c_i64), ("vc_stride_pos", c_i64), ("vc_stride_head", c_i64),
+        ("block_size", c_int), ("num_blocks", c_i64),
+    ]
+
+
 _SIGNATURES = {
     "akv_version": (c_int, []),
     "akv_last_error": (C.c_char_p, []),
@@ -205,6 +242,8 @@ _SIGNATURES = {
     "akv_tri_encode_bits": (c_int, [c_vp, c_int, c_i64, c_i64, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp]),
     "akv_tri_decode_workspace_bytes": (C.c_size_t, [c_int] * 4),
     "akv_tri_decode_step": (c_int, [C.POINTER(TriDecodeParams)]),
+    "akv_rotary": (c_int, [C.POINTER(RotaryParams)]),
+    "akv_rotary_kv_append": (c_int, [C.POINTER(RotaryAppendParams)]),
     "akv_p2p_exchange_bytes": (C.c_size_t, [c_int] * 4),
     "akv_p2p_lse_merge": (c_int, [C.POINTER(P2PMergeParams)]),
     "akv_lse_merge": (c_int, [c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp, c_int, c_i64, c_i64, c_vp]),
@@ -288,6 +327,17 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def call(device: torch.device, name: str, params) -> None:
+    """Call entry point ``name`` with its argument block on ``device`` and raise what it refuses."""
+    fn = getattr(lib(), name)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(params)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(params)
+    check(rc, name)
 
 
 def ptr(t) -> int:

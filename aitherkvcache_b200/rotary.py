@@ -1,0 +1,151 @@
+"""Rotary positions with one or several axes.
+
+A vector's pair p turns by ``position[axis(p)] * frequency(p)``.  With one axis this is the usual rotary embedding; with
+several (time, height, width of image and video tokens) each pair follows one of the token's positions.  The rotation
+runs in ``akv_rotary``; ``rotary_kv_append`` (dense_kv.py) applies it while it writes keys and values to a paged cache.
+The reference has no rotation of its own: its callers hand it rotated keys, and its spectral codec wants unrotated ones
+(``inverse=True`` takes a rotation back).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from . import _lib
+
+MAX_AXES = 4
+
+
+def axis_of_pairs(pairs: int, sections: Optional[Sequence[int]], layout: str = "blocked") -> list:
+    """Axis of every pair.  ``sections[a]`` pairs belong to axis a: "blocked" gives the first ``sections[0]`` pairs to axis
+    0, the next ``sections[1]`` to axis 1 and so on; "cycled" lets the axes take turns until each has its share."""
+    if layout not in ("blocked", "cycled"):
+        raise ValueError(f"section_layout must be 'blocked' or 'cycled', got {layout!r}")
+    if sections is None:
+        return [0] * pairs
+    left = [int(n) for n in sections]
+    if not 1 <= len(left) <= MAX_AXES or min(left) < 0 or sum(left) != pairs:
+        raise ValueError(f"sections {tuple(sections)} must be 1 to {MAX_AXES} counts that add up to {pairs} pairs")
+    if layout == "blocked":
+        return [a for a, n in enumerate(left) for _ in range(n)]
+    axes, a = [], 0
+    while len(axes) < pairs:
+        if left[a % len(left)] > 0:
+            left[a % len(left)] -= 1
+            axes.append(a % len(left))
+        a += 1
+    return axes
+
+
+class RotaryPositions:
+    """``q, k = RotaryPositions(128, base=1e6).forward(query, key, positions)``.
+
+    head_dim        elements of a vector; ``rotary_dim`` of them (default all, even) are rotated, the rest pass through
+    base, inv_freq  frequency of pair p: ``base ** (-2 p / rotary_dim)``, or the ``rotary_dim / 2`` values given
+    sections        pairs of every axis (``None``: one axis); ``section_layout``: see ``axis_of_pairs``
+    pair_layout     "halves": pair p is elements (p, p + rotary_dim / 2); "adjacent": elements (2 p, 2 p + 1)
+    scaling         factor of the rotated elements (the attention factor of scaled rotary embeddings)
+    """
+
+    def __init__(self, head_dim: int, rotary_dim: Optional[int] = None, base: float = 10000.0,
+                 sections: Optional[Sequence[int]] = None, section_layout: str = "blocked", pair_layout: str = "halves",
+                 inv_freq=None, scaling: float = 1.0, device: str = "cuda"):
+        self.head_dim = int(head_dim)
+        self.rotary_dim = self.head_dim if rotary_dim is None else int(rotary_dim)
+        if self.head_dim <= 0 or not 0 < self.rotary_dim <= self.head_dim or self.rotary_dim % 2:
+            raise ValueError(f"rotary_dim must be even and in (0, head_dim], got {self.rotary_dim} of {self.head_dim}")
+        if pair_layout not in ("halves", "adjacent"):
+            raise ValueError(f"pair_layout must be 'halves' or 'adjacent', got {pair_layout!r}")
+        pairs = self.rotary_dim // 2
+        axes = axis_of_pairs(pairs, sections, section_layout)
+        self.num_axes = 1 if sections is None else len(sections)
+        self.pair_layout, self.section_layout = pair_layout, section_layout
+        self.sections = None if sections is None else tuple(int(n) for n in sections)
+        self.scaling = float(scaling)
+        if inv_freq is None:
+            freq = [float(base) ** (-2.0 * p / self.rotary_dim) for p in range(pairs)]
+        else:
+            freq = [float(f) for f in (inv_freq.tolist() if isinstance(inv_freq, torch.Tensor) else inv_freq)]
+            if len(freq) != pairs:
+                raise ValueError(f"inv_freq must have {pairs} values, got {len(freq)}")
+        if not all(math.isfinite(f) for f in freq) or not math.isfinite(self.scaling):
+            raise ValueError("frequencies and scaling must be finite")
+        # a frequency as a 64-bit fraction of a turn (radians / 2 pi * 2^64 modulo 2^64), kept as a signed 64-bit word
+        turns = [int(f / (2.0 * math.pi) * 2.0 ** 64) % (1 << 64) for f in freq]
+        self.inv_freq = torch.tensor(freq, dtype=torch.float64)
+        self.steps = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64, device=device)
+        self.axes = torch.tensor(axes, dtype=torch.int32, device=device)
+        self.device = self.steps.device
+        self._tables = _lib.RotaryTables(self.head_dim, self.rotary_dim, self.num_axes, int(pair_layout == "adjacent"),
+                                         self.steps.data_ptr(), self.axes.data_ptr(), self.scaling)
+        self._tables_ref = ctypes.pointer(self._tables)
+
+    def _positions(self, positions: torch.Tensor, tokens: int) -> Tuple[torch.Tensor, int, int]:
+        """(positions, stride over the axes, stride over the tokens) of [tokens] or [num_axes, tokens]."""
+        if positions.dim() == 1 and positions.shape[0] == tokens:
+            return positions, 0, positions.stride(0)      # text: the same position on every axis
+        if positions.dim() == 2 and positions.shape[0] == self.num_axes and positions.shape[1] == tokens:
+            return positions, positions.stride(0), positions.stride(1)
+        raise ValueError(f"positions {tuple(positions.shape)} must be [{tokens}] or [{self.num_axes}, {tokens}]")
+
+    def _heads(self, x: torch.Tensor, name: str, tokens: int) -> torch.Tensor:
+        if x.dim() != 3 or x.shape[2] != self.head_dim or x.shape[0] != tokens:
+            raise ValueError(f"{name} {tuple(x.shape)} must be [{tokens}, heads, {self.head_dim}]")
+        return x if x.stride(2) == 1 else x.contiguous()
+
+    def _params(self, query, key, positions, inverse, dev):
+        """The part of the argument block that the rotation and the append share, and tensors it must outlive."""
+        tokens = (query if query is not None else key).shape[0]
+        p = _lib.RotaryParams()
+        p.tables = self._tables_ref
+        pos, sa, st = self._positions(positions, tokens)
+        p.positions, p.pos_dtype, p.pos_stride_axis, p.pos_stride_tok = pos.data_ptr(), _lib.index_code(pos), sa, st
+        p.num_tokens = tokens
+        if query is not None:
+            query = self._heads(query, "query", tokens)
+            p.in_dtype = _lib.float_code(query)
+            p.query, p.q_stride_tok, p.q_stride_head, p.num_q_heads = query.data_ptr(), query.stride(0), query.stride(1), query.shape[1]
+        if key is not None:
+            key = self._heads(key, "key", tokens)
+            if query is not None and key.dtype != query.dtype:
+                raise TypeError(f"query and key must have one dtype, got {query.dtype} and {key.dtype}")
+            p.in_dtype = _lib.float_code(key)
+            p.key, p.k_stride_tok, p.k_stride_head, p.num_kv_heads = key.data_ptr(), key.stride(0), key.stride(1), key.shape[1]
+        p.inverse = int(inverse)
+        p.stream = _lib.stream_ptr(dev)
+        return p, query, key
+
+    @staticmethod
+    def _out(out, x, dtype, name, dev):
+        if out is None:
+            return torch.empty(x.shape, dtype=dtype, device=dev)
+        if out.shape != x.shape or out.stride(2) != 1 or out.dtype != dtype:
+            raise ValueError(f"{name} {tuple(out.shape)} {out.dtype} must be {tuple(x.shape)} {dtype} with a contiguous last "
+                             "dimension")
+        return out
+
+    def forward(self, query: Optional[torch.Tensor], key: Optional[torch.Tensor], positions: torch.Tensor,
+                query_out: Optional[torch.Tensor] = None, key_out: Optional[torch.Tensor] = None,
+                inverse: bool = False) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+        """``query`` [tokens, query_heads, head_dim] and ``key`` [tokens, kv_heads, head_dim] (either may be None, any
+        strides with a contiguous last dimension) turned to ``positions``: [tokens] or [num_axes, tokens], int32 or int64.
+        Returns (query, key) in their dtype.  ``query_out=query`` works in place.  ``inverse`` turns back; it is also the
+        gradient of the rotation."""
+        if query is None and key is None:
+            raise ValueError("query and key are both None")
+        dev = _lib.require_cuda(query, key, positions, query_out, key_out, self.steps)
+        p, query, key = self._params(query, key, positions, inverse, dev)
+        p.out_dtype = p.in_dtype
+        if query is not None:
+            query_out = self._out(query_out, query, query.dtype, "query_out", dev)
+            p.q_out, p.qo_stride_tok, p.qo_stride_head = query_out.data_ptr(), query_out.stride(0), query_out.stride(1)
+        if key is not None:
+            key_out = self._out(key_out, key, key.dtype, "key_out", dev)
+            p.k_out, p.ko_stride_tok, p.ko_stride_head = key_out.data_ptr(), key_out.stride(0), key_out.stride(1)
+        _lib.call(dev, "akv_rotary", ctypes.byref(p))
+        return (query_out if query is not None else None), (key_out if key is not None else None)
+
+    __call__ = forward

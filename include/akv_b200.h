@@ -418,6 +418,56 @@ size_t akv_tri_decode_workspace_bytes(int batch, int num_q_heads, int seq_len, i
 int akv_tri_decode_step(const akv_tri_decode_params* params);
 
 /* ------------------------------------------------------------------------
+ * Dense (16-bit) paged cache: rotary positions, append with rotation, attention.  No counterpart in the
+ * reference, whose uncompressed layers are served by vLLM's own kernels.
+ * ---------------------------------------------------------------------- */
+
+/* Tables of a rotation (HOST struct; its arrays are device arrays).  Pair p of a vector - elements (p, p +
+ * rotary_dim / 2), or (2p, 2p + 1) when `adjacent` - turns by position[axes[p]] * frequency(p).
+ *   steps [rotary_dim / 2] uint64: frequency(p) / (2 pi) * 2^64 modulo 2^64 (fraction of a turn per position)
+ *   axes  [rotary_dim / 2] int32 in [0, num_axes); may be NULL with one axis
+ *   scaling multiplies the rotated elements (1 for the plain rotation); elements behind rotary_dim pass through */
+typedef struct akv_rotary_tables {
+  int head_dim, rotary_dim, num_axes, adjacent;
+  const uint64_t* steps; const int* axes;
+  float scaling;
+} akv_rotary_tables;
+
+/* Rotate query and key vectors.
+ *   positions [num_axes, num_tokens] int32 / int64, any sign (stride 0 over the axes: one position for all of them)
+ *   query / q_out [num_tokens, num_q_heads, head_dim], key / k_out [num_tokens, num_kv_heads, head_dim], last dimension
+ *   contiguous; in place (out == in, same type and strides) is allowed.  num_q_heads or num_kv_heads may be 0.
+ *   inverse != 0 turns by the negative angle: takes a rotation back (scaling 1), and is its gradient. */
+typedef struct akv_rotary_params {
+  const akv_rotary_tables* tables;
+  const void* positions; int pos_dtype; int64_t pos_stride_axis, pos_stride_tok;
+  int64_t num_tokens;
+  int in_dtype, out_dtype;
+  const void* query; int64_t q_stride_tok, q_stride_head; int num_q_heads;
+  void* q_out; int64_t qo_stride_tok, qo_stride_head;
+  const void* key; int64_t k_stride_tok, k_stride_head; int num_kv_heads;
+  void* k_out; int64_t ko_stride_tok, ko_stride_head;
+  int inverse;
+  void* stream;
+} akv_rotary_params;
+int akv_rotary(const akv_rotary_params* params);
+
+/* Append new keys and values to a dense paged cache and rotate on the way, one launch: q_out = rotated query,
+ * k_cache[slot / block_size][slot % block_size][h] = rotated key, v_cache[...] = value (unrotated), all in
+ * rotary.out_dtype; rotary.k_out is ignored.  Tokens whose slot is negative or behind num_blocks are not written to the
+ * cache (their query is rotated all the same).  The slots of one call are distinct: two tokens with one slot leave a
+ * mixture of both. */
+typedef struct akv_rotary_append_params {
+  akv_rotary_params rotary;
+  const void* value; int64_t v_stride_tok, v_stride_head;      /* rotary.in_dtype */
+  const void* slot_mapping; int slot_dtype;                    /* [num_tokens] */
+  void* k_cache; int64_t kc_stride_blk, kc_stride_pos, kc_stride_head;
+  void* v_cache; int64_t vc_stride_blk, vc_stride_pos, vc_stride_head;
+  int block_size; int64_t num_blocks;
+} akv_rotary_append_params;
+int akv_rotary_kv_append(const akv_rotary_append_params* params);
+
+/* ------------------------------------------------------------------------
  * Cross-GPU merge of split-K partials over NVLink peer memory (no counterpart in the reference, which
  * has no multi-device path; the merge arithmetic is that of fused_attention.py:513-527)
  * ---------------------------------------------------------------------- */

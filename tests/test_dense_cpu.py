@@ -1,0 +1,137 @@
+"""Host side of the dense paged cache's operators: tables, argument checks, struct layouts (no GPU)."""
+import ctypes
+import math
+import os
+import re
+import subprocess
+
+import pytest
+import torch
+
+from conftest import ROOT
+
+
+def test_axis_of_pairs():
+    from aitherkvcache_b200.rotary import axis_of_pairs
+    assert axis_of_pairs(4, None) == [0, 0, 0, 0]
+    assert axis_of_pairs(6, (1, 2, 3)) == [0, 1, 1, 2, 2, 2]
+    assert axis_of_pairs(8, (4, 2, 2), "cycled") == [0, 1, 2, 0, 1, 2, 0, 0]
+    assert axis_of_pairs(6, (1, 3, 2), "cycled") == [0, 1, 2, 1, 2, 1]
+    for bad in ((3, 2), (1, 1, 1, 1, 2), (7, -1), ()):
+        with pytest.raises(ValueError):
+            axis_of_pairs(6, bad)
+    with pytest.raises(ValueError):
+        axis_of_pairs(6, None, "other")
+
+
+def test_steps_are_the_angles():
+    """pos * step modulo 2^64 is pos * frequency modulo a full turn: float64 angles agree to their own rounding."""
+    from aitherkvcache_b200 import RotaryPositions
+    freq = [1.0, 0.5, 3.9, -2.0, 1e-7, 7.1, 100.0, 1e-3]
+    rope = RotaryPositions(16, inv_freq=freq, device="cpu")
+    for p in (0, 1, -1, 12345, -99999, (1 << 24) + 1):
+        for f, step in zip(freq, rope.steps.tolist()):
+            turn = ((p * step) % (1 << 64)) / 2.0 ** 64
+            t = p * f
+            # the step is cut (2^-64 turns) after a float64 rounding of f / 2 pi (2^-52 of it)
+            tol = 2 * math.pi * (abs(p) * 2.0 ** -64 + abs(t) * 2.0 ** -51) + 1e-12
+            assert abs(math.cos(2 * math.pi * turn) - math.cos(t)) <= tol
+            assert abs(math.sin(2 * math.pi * turn) - math.sin(t)) <= tol
+
+
+def test_rotary_refuses():
+    from aitherkvcache_b200 import RotaryPositions
+    for kw in (dict(rotary_dim=7), dict(rotary_dim=18), dict(rotary_dim=0), dict(pair_layout="x"), dict(inv_freq=[1.0]),
+               dict(sections=(4, 3)), dict(section_layout="x"), dict(scaling=float("nan")), dict(inv_freq=[float("inf")] * 8)):
+        with pytest.raises(ValueError):
+            RotaryPositions(16, device="cpu", **kw)
+    rope = RotaryPositions(16, device="cpu", sections=(4, 4))
+    x = torch.zeros(3, 2, 16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        rope.forward(x, None, torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(ValueError):
+        rope.forward(None, None, torch.zeros(3, dtype=torch.int64))
+    for bad in (torch.zeros(2), torch.zeros(3, 3), torch.zeros(2, 2)):
+        with pytest.raises(ValueError):
+            rope._positions(bad, 3)
+    with pytest.raises(ValueError):
+        rope._heads(torch.zeros(3, 2, 15), "query", 3)
+    with pytest.raises(ValueError):
+        rope._heads(torch.zeros(3, 16), "query", 3)
+    with pytest.raises(ValueError):
+        RotaryPositions._out(torch.zeros(3, 2, 16).half(), x, torch.float32, "query_out", None)
+
+
+def test_rotary_entry_points_refuse():
+    """Argument blocks that the C entry points turn into errors before any launch."""
+    from aitherkvcache_b200 import _lib
+    L = _lib.lib()
+    good = dict(head_dim=16, rotary_dim=16, num_axes=1, adjacent=0, steps=64, axes=64, scaling=1.0)
+
+    def params(tables, **kw):
+        p = _lib.RotaryParams()
+        p.tables = ctypes.pointer(_lib.RotaryTables(**tables))
+        p.positions, p.num_tokens, p.query, p.q_out, p.num_q_heads = 64, 1, 64, 64, 1
+        for k, v in kw.items():
+            setattr(p, k, v)
+        return p
+
+    assert L.akv_rotary(None) == _lib.AKV_ERR_ARG
+    for t in (dict(good, rotary_dim=15), dict(good, rotary_dim=18), dict(good, head_dim=0), dict(good, num_axes=5),
+              dict(good, num_axes=0), dict(good, steps=None), dict(good, num_axes=2, axes=None)):
+        assert L.akv_rotary(ctypes.byref(params(t))) == _lib.AKV_ERR_ARG, t
+    for kw in (dict(num_tokens=-1), dict(in_dtype=3), dict(out_dtype=-1), dict(pos_dtype=2), dict(positions=None), dict(query=None),
+               dict(q_out=None), dict(num_kv_heads=2), dict(num_q_heads=-1), dict(num_kv_heads=2, key=64)):
+        assert L.akv_rotary(ctypes.byref(params(good, **kw))) == _lib.AKV_ERR_ARG, kw
+    assert L.akv_rotary(ctypes.byref(params(good, num_tokens=0))) == 0
+    assert L.akv_rotary_kv_append(None) == _lib.AKV_ERR_ARG
+
+    def append(**kw):
+        a = _lib.RotaryAppendParams()
+        a.rotary = params(good, num_kv_heads=1, key=64)
+        a.value = a.slot_mapping = a.k_cache = a.v_cache = 64
+        a.block_size, a.num_blocks = 16, 4
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return L.akv_rotary_kv_append(ctypes.byref(a))
+
+    for kw in (dict(block_size=0), dict(num_blocks=-1), dict(slot_dtype=7), dict(slot_mapping=None), dict(value=None),
+               dict(k_cache=None), dict(v_cache=None)):
+        assert append(**kw) == _lib.AKV_ERR_ARG, kw
+
+
+def test_append_refuses():
+    from aitherkvcache_b200 import dense_kv
+    a = torch.zeros(4, 16, 2, 32)
+    dense_kv._check_caches(a, a, 2, 32)
+    for k, v in ((a, a[:3]), (a[:, :, :1], a[:, :, :1]), (a[..., :16], a[..., :16]), (a.transpose(2, 3), a.transpose(2, 3)), (a[0], a[0])):
+        with pytest.raises(ValueError):
+            dense_kv._check_caches(k, v, 2, 32)
+    with pytest.raises(TypeError):
+        dense_kv._check_caches(a, a.half(), 2, 32)
+
+
+def test_dense_structures_match_the_header_layout(tmp_path):
+    """The parameter structs of the dense cache against their ctypes mirrors: sizeof and every offset, from gcc."""
+    from aitherkvcache_b200 import _lib
+    pairs = {"akv_rotary_tables": _lib.RotaryTables, "akv_rotary_params": _lib.RotaryParams,
+             "akv_rotary_append_params": _lib.RotaryAppendParams}
+    if hasattr(_lib, "DenseAttnParams"):
+        pairs["akv_dense_attn_params"] = _lib.DenseAttnParams
+    lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "akv_b200.h"', "int main(void) {"]
+    for cname, st in pairs.items():
+        lines.append('printf("%s %%zu", sizeof(%s));' % (cname, cname))
+        lines += ['printf(" %%zu", offsetof(%s, %s));' % (cname, f) for f, _ in st._fields_]
+        lines.append('printf("\\n");')
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["return 0;", "}"]))
+    subprocess.run(["gcc", "-std=c99", "-I", os.path.join(ROOT, "include"), "-o", str(exe), str(src)], check=True)
+    header = open(os.path.join(ROOT, "include", "akv_b200.h")).read()
+    for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.strip().splitlines():
+        cname, size, *offs = line.split()
+        st = pairs[cname]
+        assert ctypes.sizeof(st) == int(size), cname
+        assert [getattr(st, f).offset for f, _ in st._fields_] == [int(o) for o in offs], cname
+        body = re.sub(r"/\*.*?\*/", "", re.search(r"typedef struct %s \{(.*?)\} %s;" % (cname, cname), header, re.S).group(1), flags=re.S)
+        names = [re.findall(r"[A-Za-z_]\w*", part)[-1] for decl in body.split(";") if decl.strip() for part in decl.split(",")]
+        assert names == [f for f, _ in st._fields_], cname
