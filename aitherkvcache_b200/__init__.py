@@ -12,7 +12,7 @@ from .quantizer import TurboQuant, TurboQuantConfig
 from .fused_attention import TQPagedAttention
 from .fused_kv_update import fused_tq4_kv_update, fused_encode_and_store
 from .rotary import RotaryPositions
-from .dense_kv import rotary_kv_append
+from .dense_kv import DensePagedAttention, rotary_kv_append
 
 # kv-cache dtype names of the serving integration -> codec selection
 KV_CACHE_DTYPES = {
@@ -24,6 +24,7 @@ KV_CACHE_DTYPES = {
 
 __all__ = [
     "TurboQuant", "TurboQuantConfig", "TQPagedAttention",
-    "fused_tq4_kv_update", "fused_encode_and_store", "RotaryPositions", "rotary_kv_append", "KV_CACHE_DTYPES",
+    "fused_tq4_kv_update", "fused_encode_and_store", "RotaryPositions", "rotary_kv_append",
+    "DensePagedAttention", "KV_CACHE_DTYPES",
 ]
 __version__ = "0.1.0"

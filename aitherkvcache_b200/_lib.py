@@ -204,6 +204,26 @@ class RotaryAppendParams(C.Structure):
     ]
 
 
+class DenseAttnParams(C.Structure):
+    """Mirror of ``akv_dense_attn_params``."""
+    _fields_ = [
+        ("query", c_vp), ("dtype", c_int), ("q_stride_tok", c_i64), ("q_stride_head", c_i64),
+        ("k_cache", c_vp), ("k_stride_blk", c_i64), ("k_stride_pos", c_i64), ("k_stride_head", c_i64),
+        ("v_cache", c_vp), ("v_stride_blk", c_i64), ("v_stride_pos", c_i64), ("v_stride_head", c_i64),
+        ("block_tables", c_vp), ("bt_dtype", c_int), ("bt_stride_seq", c_i64),
+        ("seq_lens", c_vp), ("sl_dtype", c_int),
+        ("query_start_loc", c_vp), ("qs_dtype", c_int),
+        ("num_seqs", c_int), ("num_tokens", c_int), ("num_q_heads", c_int), ("num_kv_heads", c_int), ("head_dim", c_int),
+        ("block_size", c_int), ("max_blocks_per_seq", c_int),
+        ("num_blocks", c_i64),
+        ("scale", c_f), ("window", c_int),
+        ("out", c_vp), ("out_stride_tok", c_i64), ("out_stride_head", c_i64),
+        ("max_seq_len", c_int),
+        ("workspace", c_vp), ("workspace_bytes", C.c_size_t),
+        ("stream", c_vp),
+    ]
+
+
 _SIGNATURES = {
     "akv_version": (c_int, []),
     "akv_last_error": (C.c_char_p, []),
@@ -244,6 +264,8 @@ _SIGNATURES = {
     "akv_tri_decode_step": (c_int, [C.POINTER(TriDecodeParams)]),
     "akv_rotary": (c_int, [C.POINTER(RotaryParams)]),
     "akv_rotary_kv_append": (c_int, [C.POINTER(RotaryAppendParams)]),
+    "akv_dense_paged_attn_workspace_bytes": (C.c_size_t, [c_int] * 3),
+    "akv_dense_paged_attn": (c_int, [C.POINTER(DenseAttnParams)]),
     "akv_p2p_exchange_bytes": (C.c_size_t, [c_int] * 4),
     "akv_p2p_lse_merge": (c_int, [C.POINTER(P2PMergeParams)]),
     "akv_lse_merge": (c_int, [c_vp, c_int, c_int, c_int, c_int, c_vp, c_vp, c_int, c_i64, c_i64, c_vp]),

@@ -7,6 +7,7 @@ vLLM's kernels; here they run in ``akv_rotary_kv_append``, ``akv_dense_paged_att
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Optional
 
 import torch
@@ -62,3 +63,79 @@ def rotary_kv_append(query: Optional[torch.Tensor], key: torch.Tensor, value: to
         raise ValueError(f"caches {tuple(k_cache.shape)} hold no slot")
     _lib.call(dev, "akv_rotary_kv_append", ctypes.byref(p))
     return query_out
+
+
+class DensePagedAttention:
+    """``DensePagedAttention(head_dim, query_heads, kv_heads).forward(query, k_cache, v_cache, block_tables, context_lens)``.
+
+    The 16-bit counterpart of ``TQPagedAttention``: query and caches in one type (fp16 or bf16), head_dim 64, 128 or 256,
+    any number of query heads per KV head, any block size, caches in any strides whose rows start on 16-byte boundaries.
+    ``sliding_window``: keys a token sees, itself included (0: all).  ``scale`` defaults to 1/sqrt(head_dim).
+
+    A row that sees no key is zero.  Block-table entries outside the pool are clamped to it, and what pages hold behind
+    a sequence's end does not matter.  Scratch is allocated per call (stream-ordered, so calls on several streams and
+    captured graphs share nothing)."""
+
+    def __init__(self, head_dim: int, num_query_heads: int, num_kv_heads: int, scale: Optional[float] = None,
+                 sliding_window: int = 0):
+        if head_dim not in (64, 128, 256):
+            raise ValueError(f"head_dim must be 64, 128 or 256, got {head_dim}")
+        if num_kv_heads <= 0 or num_query_heads <= 0 or num_query_heads % num_kv_heads:
+            raise ValueError(f"{num_query_heads} query heads are not a multiple of {num_kv_heads} KV heads")
+        if sliding_window < 0:
+            raise ValueError(f"sliding_window must not be negative, got {sliding_window}")
+        self.head_dim, self.num_query_heads, self.num_kv_heads = head_dim, num_query_heads, num_kv_heads
+        self.scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+        self.sliding_window = int(sliding_window)
+        self._decode_bytes = _lib.lib().akv_dense_paged_attn_workspace_bytes(num_query_heads, num_kv_heads, head_dim)
+
+    @staticmethod
+    def _rows16(x: torch.Tensor) -> bool:
+        """Whether every row of a 16-bit [a, b, head_dim] tensor starts on a 16-byte boundary."""
+        return x.stride(2) == 1 and not (x.data_ptr() & 15 or (x.stride(0) | x.stride(1)) & 7)
+
+    def _params(self, dev, query, k_cache, v_cache, block_tables, seq_lens, num_seqs, out):
+        """Argument block of both entry points, and the output."""
+        if query.dim() != 3 or query.shape[1] != self.num_query_heads or query.shape[2] != self.head_dim:
+            raise ValueError(f"query {tuple(query.shape)} must be [tokens, {self.num_query_heads}, {self.head_dim}]")
+        _check_caches(k_cache, v_cache, self.num_kv_heads, self.head_dim)
+        if query.dtype not in (torch.float16, torch.bfloat16) or k_cache.dtype != query.dtype:
+            raise TypeError(f"query and caches must be fp16 or bf16 alike, got {query.dtype} and {k_cache.dtype}")
+        if block_tables.dim() != 2 or block_tables.shape[0] < num_seqs or seq_lens.dim() != 1 or seq_lens.shape[0] < num_seqs:
+            raise ValueError(f"block_tables {tuple(block_tables.shape)} / lengths {tuple(seq_lens.shape)} do not cover "
+                             f"{num_seqs} sequences")
+        if not self._rows16(query):
+            query = query.contiguous()
+        if block_tables.stride(1) != 1:
+            block_tables = block_tables.contiguous()
+        if seq_lens.stride(0) != 1:
+            seq_lens = seq_lens.contiguous()
+        if out is None:
+            out = torch.empty_like(query, memory_format=torch.contiguous_format)
+        elif out.shape != query.shape or out.dtype != query.dtype or not self._rows16(out):
+            raise ValueError(f"out {tuple(out.shape)} {out.dtype} must be {tuple(query.shape)} {query.dtype} with rows on 16-byte "
+                             "boundaries")
+        code = _lib._FLOAT_CODES[query.dtype]
+        p = _lib.DenseAttnParams(
+            query.data_ptr(), code, query.stride(0), query.stride(1),
+            k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
+            v_cache.data_ptr(), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2),
+            block_tables.data_ptr(), _lib.index_code(block_tables), block_tables.stride(0),
+            seq_lens.data_ptr(), _lib.index_code(seq_lens), None, 0,
+            num_seqs, query.shape[0], self.num_query_heads, self.num_kv_heads, self.head_dim,
+            k_cache.shape[1], block_tables.shape[1], k_cache.shape[0], self.scale, self.sliding_window,
+            out.data_ptr(), out.stride(0), out.stride(1))
+        p.stream = _lib.stream_ptr(dev)
+        return p, out, (query, block_tables, seq_lens)
+
+    def forward(self, query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                context_lens: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One token per sequence: ``query`` [num_seqs, query_heads, head_dim], the last of each sequence's
+        ``context_lens`` [num_seqs] tokens, over ``k_cache`` / ``v_cache`` [blocks, block_size, kv_heads, head_dim] through
+        ``block_tables`` [num_seqs, max_blocks].  Returns ``out`` [num_seqs, query_heads, head_dim]."""
+        dev = _lib.require_cuda(query, k_cache, v_cache, block_tables, context_lens, out)
+        p, out, keep = self._params(dev, query, k_cache, v_cache, block_tables, context_lens, query.shape[0], out)
+        ws = torch.empty(self._decode_bytes, dtype=torch.uint8, device=dev)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), self._decode_bytes
+        _lib.call(dev, "akv_dense_paged_attn", ctypes.byref(p))
+        return out

@@ -467,6 +467,34 @@ typedef struct akv_rotary_append_params {
 } akv_rotary_append_params;
 int akv_rotary_kv_append(const akv_rotary_append_params* params);
 
+/* Attention over the dense paged cache.  query [num_tokens, num_q_heads, head_dim], caches [num_blocks, block_size,
+ * num_kv_heads, head_dim] and out [num_tokens, num_q_heads, head_dim] all of `dtype` (AKV_F16 / AKV_BF16), any strides whose
+ * rows start on 16-byte boundaries, last dimension contiguous; num_q_heads a multiple of num_kv_heads; head_dim 64, 128 or
+ * 256; any block_size.  block_tables [num_seqs, max_blocks_per_seq] and seq_lens [num_seqs] int32 / int64; entries outside
+ * the pool are clamped to it, lengths to [0, max_blocks_per_seq * block_size].  window 0, or the number of keys a token
+ * sees, itself included.  A row that sees no key is zero.  Pages behind a sequence's end may hold anything, NaN included.
+ *
+ * akv_dense_paged_attn: one token per sequence, row s of query and out, the last of its seq_lens[s] tokens (rows behind
+ * num_seqs are left alone; query_start_loc is ignored).  Two launches, capturable; the workspace is used by the call alone
+ * until it has finished. */
+typedef struct akv_dense_attn_params {
+  const void* query; int dtype; int64_t q_stride_tok, q_stride_head;
+  const void* k_cache; int64_t k_stride_blk, k_stride_pos, k_stride_head;
+  const void* v_cache; int64_t v_stride_blk, v_stride_pos, v_stride_head;
+  const void* block_tables; int bt_dtype; int64_t bt_stride_seq;
+  const void* seq_lens; int sl_dtype;
+  const void* query_start_loc; int qs_dtype;
+  int num_seqs, num_tokens, num_q_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq;
+  int64_t num_blocks;
+  float scale; int window;
+  void* out; int64_t out_stride_tok, out_stride_head;
+  int max_seq_len;
+  void* workspace; size_t workspace_bytes;
+  void* stream;
+} akv_dense_attn_params;
+size_t akv_dense_paged_attn_workspace_bytes(int num_q_heads, int num_kv_heads, int head_dim);
+int akv_dense_paged_attn(const akv_dense_attn_params* params);
+
 /* ------------------------------------------------------------------------
  * Cross-GPU merge of split-K partials over NVLink peer memory (no counterpart in the reference, which
  * has no multi-device path; the merge arithmetic is that of fused_attention.py:513-527)

@@ -44,10 +44,19 @@ def rotate_bound(x, y, rotary_dim, adjacent, out_dtype, scaling=1.0):
 
 def attention(q, k_cache, v_cache, block_tables, seq_lens, starts, scale, window=0):
     """Chunk attention: token i of sequence s (rows starts[s] .. of q) sees keys j <= p, j > p - window (if window), with
-    p = seq_lens[s] - new + i; a row that sees nothing is zero.  Rows behind the last sequence: zero.  Float64."""
+    p = seq_lens[s] - new + i; a row that sees nothing is zero.  Rows behind the last sequence: zero.  Float64.
+
+    Returns (out, bound): the largest error that float32 scores, sums and accumulators and 16-bit probabilities may have.
+    A score is off by at most d = scale (D 2^-23 + 2^-22) sum|q k| (D accumulations of exact products, each off by a last
+    place; scaling, and the subtraction of the reference), its weight by the factor e^d and 2^-21 of the
+    exponential; the weight is rounded once to the type (half a step u, and for fp16 at most 2^-25 where it is
+    subnormal; the largest weight is at least 1); numerator and denominator are float32 sums of n terms (n 2^-23).  With
+    A = sum w|v| / sum w that is at most (2 d + 2 * 2^-21 + u + 2 n 2^-23) A + n 2^-25 max|v|, then u |out| for the result."""
     out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
-    bs, kvh = k_cache.shape[1], k_cache.shape[2]
+    bound = torch.zeros_like(out)
+    bs, kvh, dim = k_cache.shape[1], k_cache.shape[2], q.shape[2]
     group = q.shape[1] // kvh
+    u = torch.finfo(q.dtype).eps / 2
     for s in range(len(seq_lens)):
         lo, hi, total = int(starts[s]), int(starts[s + 1]), int(seq_lens[s])
         if hi <= lo or total <= 0:
@@ -61,10 +70,18 @@ def attention(q, k_cache, v_cache, block_tables, seq_lens, starts, scale, window
         if window:
             seen &= j > p - window
         for h in range(q.shape[1]):
-            sc = scale * (q[lo:hi, h].double() @ k[:, h // group].t())
-            sc = sc.masked_fill(~seen, -math.inf)
+            qh, kh, vh = q[lo:hi, h].double(), k[:, h // group], v[:, h // group]
+            sc = (scale * (qh @ kh.t())).masked_fill(~seen, -math.inf)
             top = sc.amax(1, keepdim=True)
             e = torch.exp(sc - torch.where(top == -math.inf, torch.zeros_like(top), top))
             tot = e.sum(1, keepdim=True)
-            out[lo:hi, h] = torch.where(tot > 0, (e / tot.clamp_min(1e-300)) @ v[:, h // group], torch.zeros_like(out[lo:hi, h]))
-    return out
+            some = tot > 0
+            w = torch.where(some, e / tot.clamp_min(1e-300), torch.zeros_like(e))
+            o = w @ vh
+            d = abs(scale) * (dim * 2.0 ** -23 + 2.0 ** -22) * (qh.abs() @ kh.abs().t()).masked_fill(~seen, 0).amax(1, keepdim=True)
+            n = seen.sum(1, keepdim=True).double()
+            vmax = vh.abs().max()
+            err = (2 * d + 2.0 ** -20 + u + n * 2.0 ** -22) * (w @ vh.abs()) + n * 2.0 ** -25 * vmax
+            out[lo:hi, h] = o
+            bound[lo:hi, h] = torch.where(some, err + u * (o.abs() + err) + 2.0 ** -25, torch.zeros_like(err))
+    return out, bound

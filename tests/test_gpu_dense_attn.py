@@ -1,0 +1,169 @@
+"""Attention over the dense paged cache against the definition in 64 bits (oracle/dense.py)."""
+import math
+
+import pytest
+import torch
+
+from oracle import dense as od
+
+pytestmark = pytest.mark.gpu
+
+
+def make(lens, new, qh, kvh, D, bs, dtype, seed=0, scale_q=1.0, stale=None, extra=2, tail=0):
+    """Random query, paged caches in a permuted pool (one tensor holds the keys and values of a block) and tables.
+    ``stale``: value of every slot behind a sequence's end and of the unused blocks."""
+    g = torch.Generator().manual_seed(seed)
+    need = [-(-n // bs) for n in lens]
+    nb = sum(need) + extra
+    kv = torch.randn(nb, 2, bs, kvh, D, generator=g).to(dtype)
+    perm = torch.randperm(nb, generator=g)
+    width = max(need + [1])
+    bt = torch.zeros(len(lens), width, dtype=torch.int32)
+    at = 0
+    used = torch.zeros(nb, bs, dtype=torch.bool)
+    for s, (n, c) in enumerate(zip(lens, need)):
+        bt[s, :c] = perm[at:at + c]
+        for i in range(c):
+            used[perm[at + i], :max(0, min(bs, n - i * bs))] = True
+        at += c
+    if stale is not None:
+        kv.transpose(1, 2)[~used] = stale
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    q = (torch.randn(starts[-1] + tail, qh, D, generator=g) * scale_q).to(dtype)
+    kv = kv.cuda()
+    return (q.cuda(), kv[:, 0], kv[:, 1], bt.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(),
+            torch.tensor(starts, dtype=torch.int32).cuda())
+
+
+def check(out, q, kc, vc, bt, lens, starts, window=0, scale=None, rows=None):
+    want, bound = od.attention(q, kc, vc, bt, lens.tolist(), starts.tolist(), scale or 1.0 / math.sqrt(q.shape[2]), window)
+    rows = slice(0, int(starts[-1])) if rows is None else rows
+    off = (out[rows].double() - want[rows]).abs() - bound[rows]
+    assert bool((off <= 0).all()), (float(off.max()), float(want.abs().max()))
+
+
+def attn(qh, kvh, D, **kw):
+    from aitherkvcache_b200 import DensePagedAttention
+    return DensePagedAttention(D, qh, kvh, **kw)
+
+
+LENS = [[1], [17, 0, 300], [1, 2, 15, 16, 17, 31, 32, 33, 511, 0, 1200], [5000, 3]]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("qh,kvh,D", [(32, 8, 128), (8, 8, 64), (7, 1, 128), (16, 1, 64), (40, 2, 128), (6, 2, 256), (12, 1, 256), (33, 3, 64)])
+@pytest.mark.parametrize("lens", LENS, ids=lambda x: str(len(x)))
+def test_single_tokens(dtype, qh, kvh, D, lens):
+    q, kc, vc, bt, cl, starts = make(lens, [1] * len(lens), qh, kvh, D, 16, dtype, seed=len(lens), scale_q=2.0, stale=math.nan)
+    out = attn(qh, kvh, D).forward(q, kc, vc, bt, cl)
+    check(out, q, kc, vc, bt, cl, starts)
+
+
+@pytest.mark.parametrize("bs", [1, 5, 8, 24, 48, 256])
+@pytest.mark.parametrize("window", [0, 1, 16, 100])
+def test_single_tokens_blocks_and_windows(bs, window):
+    lens = [1, 40, 129, 700, 0]
+    q, kc, vc, bt, cl, starts = make(lens, [1] * 5, 8, 2, 128, bs, torch.float16, seed=bs, stale=math.inf)
+    out = attn(8, 2, 128, sliding_window=window).forward(q, kc, vc, bt.long(), cl.long())
+    check(out, q, kc, vc, bt, cl, starts, window)
+
+
+def test_single_tokens_many_sequences():
+    g = torch.Generator().manual_seed(1)
+    lens = torch.randint(0, 90, (4500,), generator=g).tolist()      # more than one launch takes
+    q, kc, vc, bt, cl, starts = make(lens, [1] * len(lens), 2, 1, 64, 16, torch.bfloat16, stale=math.nan)
+    out = attn(2, 1, 64).forward(q, kc, vc, bt, cl)
+    check(out, q, kc, vc, bt, cl, starts)
+
+
+def test_single_tokens_large_scores_and_growing_maxima():
+    """Scores of hundreds that grow along the keys: the reference moves at every step."""
+    q, kc, vc, bt, cl, starts = make([900], [1], 4, 1, 128, 16, torch.float16, seed=3)
+    kc.mul_(0.02)
+    q.fill_(1.0)
+    ramp = torch.arange(900, device="cuda").half() / 64      # q.k grows by 2 per key
+    for i in range(57):
+        n = min(16, 900 - 16 * i)
+        kc[bt[0, i].long(), :n] += ramp[16 * i:16 * i + n, None, None]
+    out = attn(4, 1, 128, scale=1.0).forward(q, kc, vc, bt, cl)
+    check(out, q, kc, vc, bt, cl, starts, scale=1.0)
+
+
+def test_single_tokens_strides_padding_and_bad_tables():
+    lens = [70, 33, 100]
+    q, kc, vc, bt, cl, starts = make(lens, [1] * 3, 8, 2, 128, 16, torch.float16, seed=5)
+    a = attn(8, 2, 128)
+    want = a.forward(q, kc, vc, bt, cl)
+    # heads first inside a block, query rows inside a wider projection, output rows likewise
+    kh, vh = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in (kc, vc))
+    wide = torch.randn(3, 12, 128, device="cuda").half()
+    wide[:, 2:10] = q
+    out = torch.full((3, 9, 128), 7.0, dtype=torch.float16, device="cuda")
+    res = a.forward(wide[:, 2:10], kh, vh, bt, cl, out=out[:, :8])
+    assert res.data_ptr() == out.data_ptr() and torch.equal(out[:, :8], want) and bool((out[:, 8] == 7.0).all())
+    # rows that start anywhere are copied first
+    odd = torch.randn(3, 8 * 128 + 1, device="cuda").half()
+    odd[:, 1:] = q.flatten(1)
+    assert torch.equal(a.forward(odd[:, 1:].unflatten(1, (8, 128)), kc, vc, bt, cl), want)
+    # tables wider than needed with entries outside the pool behind the sequence, lengths clamped to the table
+    wide_bt = torch.full((5, 20), -9, dtype=torch.int64, device="cuda")
+    wide_bt[:, 10:] = 1 << 40
+    wide_bt[:3, :bt.shape[1]] = bt
+    for s, n in enumerate(lens):
+        wide_bt[s, -(-n // 16):] = 1 << 40
+    assert torch.equal(a.forward(q, kc, vc, wide_bt, torch.cat([cl, cl[:1]])), want)
+    clamped = a.forward(q, kc, vc, bt, torch.tensor([10 ** 9, -5, 100], dtype=torch.int32, device="cuda"))
+    full = a.forward(q, kc, vc, bt, torch.tensor([bt.shape[1] * 16, 0, 100], dtype=torch.int32, device="cuda"))
+    assert torch.equal(clamped, full) and bool((clamped[1] == 0).all())
+
+
+def test_single_tokens_nan_reaches_the_rows_that_see_it():
+    q, kc, vc, bt, cl, starts = make([40, 40], [1, 1], 8, 2, 64, 16, torch.bfloat16, seed=8)
+    q[0, 3, 5] = math.nan      # one head of one sequence
+    out = attn(8, 2, 64).forward(q, kc, vc, bt, cl)
+    assert bool(out[0, 3].isnan().all())
+    out[0, 3] = 0
+    assert bool(out.isfinite().all())
+
+
+def test_single_tokens_past_32_bit_offsets():
+    nb = (1 << 31) // (16 * 8 * 128) + 64      # over 2^31 elements per cache
+    kc, vc = (torch.zeros(nb, 16, 8, 128, dtype=torch.float16, device="cuda") for _ in range(2))
+    g = torch.Generator().manual_seed(0)
+    bt = torch.tensor([[nb - 1, 0, nb - 40], [3, nb - 2, 5]], dtype=torch.int32)
+    for b in bt.flatten().tolist():
+        kc[b] = torch.randn(16, 8, 128, generator=g).half().cuda()
+        vc[b] = torch.randn(16, 8, 128, generator=g).half().cuda()
+    q = torch.randn(2, 32, 128, generator=g).half().cuda()
+    cl = torch.tensor([48, 41], dtype=torch.int32).cuda()
+    out = attn(32, 8, 128).forward(q, kc, vc, bt.cuda(), cl)
+    check(out, q, kc, vc, bt.cuda(), cl, torch.tensor([0, 1, 2]))
+
+
+def test_single_tokens_graph_replay_and_streams():
+    lens = [700, 20, 4000]
+    q, kc, vc, bt, cl, starts = make(lens, [1] * 3, 32, 8, 128, 16, torch.float16, seed=9)
+    a = attn(32, 8, 128)
+    out = torch.empty_like(q)
+    a.forward(q, kc, vc, bt, cl, out=out)
+    graphs = []
+    for _ in range(2):      # two graphs of one object
+        o = torch.empty_like(q)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            a.forward(q, kc, vc, bt, cl, out=o)
+        graphs.append((graph, o, torch.cuda.Stream()))
+    for step in range(3):
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(step)).half())
+        cl.add_(-1)
+        want = a.forward(q, kc, vc, bt, cl)
+        for graph, o, s in graphs:      # replayed at the same time
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                graph.replay()
+        for graph, o, s in graphs:
+            s.synchronize()
+            assert torch.equal(o, want)
+    check(want, q, kc, vc, bt, cl, starts)
