@@ -218,7 +218,7 @@ class DenseAttnParams(C.Structure):
         ("num_blocks", c_i64),
         ("scale", c_f), ("window", c_int),
         ("out", c_vp), ("out_stride_tok", c_i64), ("out_stride_head", c_i64),
-        ("max_seq_len", c_int),
+        ("zero_tail", c_int),
         ("workspace", c_vp), ("workspace_bytes", C.c_size_t),
         ("stream", c_vp),
     ]
@@ -265,6 +265,8 @@ _SIGNATURES = {
     "akv_rotary": (c_int, [C.POINTER(RotaryParams)]),
     "akv_rotary_kv_append": (c_int, [C.POINTER(RotaryAppendParams)]),
     "akv_dense_paged_attn_workspace_bytes": (C.c_size_t, [c_int] * 3),
+    "akv_dense_prefill_attn_workspace_bytes": (C.c_size_t, [c_int]),
+    "akv_dense_prefill_attn": (c_int, [C.POINTER(DenseAttnParams)]),
     "akv_dense_paged_attn": (c_int, [C.POINTER(DenseAttnParams)]),
     "akv_p2p_exchange_bytes": (C.c_size_t, [c_int] * 4),
     "akv_p2p_lse_merge": (c_int, [C.POINTER(P2PMergeParams)]),

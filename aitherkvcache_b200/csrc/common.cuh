@@ -97,6 +97,8 @@ int launch_rot_rows(const void* src, int src_dtype, int64_t src_outer, int64_t s
                     int64_t out_inner, int64_t rows, cudaStream_t st);
 int prefill_tc_status(int* host_out, int reset);
 int prefill_tc_withhold(int tile);
+int dense_prefill_status(int* host_out, int reset);
+int dense_prefill_withhold(int tile);
 int hybrid_window_status(int* host_out, int reset);
 int tc_encode_withhold(int tile);
 int tc_decode_withhold(int tile);

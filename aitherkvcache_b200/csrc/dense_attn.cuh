@@ -34,7 +34,7 @@ struct akv_dense_attn_params {
   int64_t num_blocks;
   float scale; int window;
   void* out; int64_t out_stride_tok, out_stride_head;
-  int max_seq_len;
+  int zero_tail;
   void* workspace; size_t workspace_bytes;
   void* stream;
 };

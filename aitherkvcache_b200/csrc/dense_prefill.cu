@@ -1,0 +1,784 @@
+// Attention of chunks of new tokens over the dense (fp16 / bf16) paged cache, on the 5th-generation tensor cores.
+//
+//   o_i = sum_j w_ij v_j / sum_j w_ij,  w_ij = 2^(c q_i.k_j - m_i),  j in (p_i - window, p_i],  p_i = len - new + i
+//
+// Bound by the tensor pipe: 4 D flops per visible (row, key) pair, with one exponential per pair beside it - 128 x 128
+// scores take 1024 cycles of the exponential unit and, at D = 128, 1024 cycles of the tensor pipe for both products.
+//
+// Row tiles.  A CTA works on a row tile - up to 256 rows (token, query head) of one sequence and KV head, two halves of
+// 128 rows = TT = 128 / G tokens each - against key tiles of 128 keys.  Per half and key tile:
+//   S[128][128] = Q K^T      A = Q in shared memory, B = the keys as they lie in the pages (K-major);
+//   O[128][D]  += P V        A = P in tensor memory (over the columns of S), B = the values as they lie in the pages:
+//                            [key][dim] rows are the MN-major form of the operand, nothing is transposed.
+// K, V and Q come by TMA with the 128-byte swizzle straight out of the paged tensors (a box per run of keys inside a
+// block); rows of values behind the sequence's end are zeroed in shared memory, since 0 * NaN is NaN.
+//
+// Ten warps: 0-3 softmax of half 0 and 4-7 of half 1 (thread = row), 8 issues the MMAs, 9 the copies.  The two halves
+// are in ping-pong: while one half's warps take maxima and exponentials, the tensor pipe works for the other half.  Order
+// of the MMAs: P V of half h and tile g, then S of half h and tile g + 1, then the other half.  They complete in order, so
+// "S of tile g + 1 is there" (s_full) also says that O of the half is complete up to tile g (it may be rescaled) and that
+// P's columns may be overwritten; no further barrier is needed in the loop.  The row's reference maximum moves only when a
+// score exceeds it by more than 2^8 (fp16 and bf16 hold 2^8 exactly), so O is rescaled a few times per row.
+//
+// Work split.  The (row tile, key tile) pairs of the whole call are laid end to end and cut into equal ranges, one per SM:
+// every SM finishes at the same time whatever the lengths.  Row tiles that are cut (at most two per CTA) leave float32
+// partials in the workspace, joined by dense_prefill_merge_kernel in the order of the keys; a cut within DP_SNAP tiles of a
+// row tile's edge is moved to the edge (a partial costs about as much as two key tiles).
+//
+// Every wait is bounded (umma.cuh): a wait that gives up sets g_dense_prefill_status and a flag that ends all loops.
+#include "dense_attn.cuh"
+#include "umma.cuh"
+#include <cuda.h>
+#include <math_constants.h>
+
+namespace akv {
+namespace {
+
+__device__ int g_dense_prefill_status;           // 1: a bounded wait gave up, 2: tensor-memory columns were kept
+__device__ int g_dense_prefill_withhold = -1;    // test hook: CTA 0 issues neither the score MMAs nor the commit of this tile
+
+constexpr int DP_KT = 128;                       // keys per tile
+constexpr int DP_MAX_SEQS = 1024;                // sequences of one launch
+constexpr int DP_SNAP = 2;
+constexpr float DP_RESCALE = 8.0f;
+
+struct DpMaps { CUtensorMap q, k, v; };
+
+template <int D> struct DpL {
+  static constexpr int WARPS = 10, THREADS = 320, MMA_WARP = 8, LOAD_WARP = 9;
+  static constexpr int HALVES = D / 64;                    // 64-element columns of an operand
+  static constexpr int TILE = 128 * D * 2;                 // bytes of 128 rows
+  static constexpr int NB = D == 128 ? 4 : 8;              // ring slots (K and V tiles in turn)
+  static constexpr int Q = 0, KV = 2 * TILE, BAR = KV + NB * TILE;
+  static constexpr int PRE = BAR + 512;                    // int64 [DP_MAX_SEQS + 1]: units before a sequence
+  static constexpr int SMEM = PRE + (DP_MAX_SEQS + 1) * 8 + 1024;
+  static constexpr int T_O = 256;                          // tensor memory: S 0, S 1 (128 columns each), O 0, O 1
+  static_assert(SMEM + 512 <= 232448, "shared memory");
+};
+// barriers (bytes behind BAR)
+constexpr uint32_t P_KVFULL = 0, P_KVFREE = 64, P_QFULL = 128, P_QFREE = 144, P_SFULL = 160, P_PFULL = 176, P_OFULL = 192,
+                   P_DRAIN = 208, P_TMEM = 216, P_FAILED = 220;
+
+// What dense_prefill_merge_kernel needs to know about the row tile whose first part CTA c wrote (parts < 2: nothing)
+struct DpDesc { int parts, slot0, row0, ntok, kvh, pad[3]; };
+
+__device__ __forceinline__ void dp_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory");
+}
+__device__ __forceinline__ void dp_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void dp_tma4(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+               :: "r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ void dp_tma3(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+               :: "r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+// MN-major operand, 128-byte swizzle: a key's 64 dims are one 128-byte row; groups of 8 keys 1024 B apart (stride offset),
+// the next 64 dims 16 KB on (leading offset).
+__device__ __forceinline__ uint64_t dp_desc_mn(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// max(a, b, c) that keeps a NaN
+__device__ __forceinline__ float dp_max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+struct DpSeq { int q0, qlen, total; };           // first query row, new tokens, tokens
+struct DpTile { int tok0, ntok, t0, n; };        // first token and tokens of a row tile, its first key tile, key tiles
+
+__device__ __forceinline__ DpSeq dp_seq(const DenseArgs& a, int s) {
+  DpSeq r;
+  int64_t q0 = load_index(a.starts, a.qs_dtype, s), q1 = load_index(a.starts, a.qs_dtype, s + 1);
+  if (q0 < 0) q0 = 0;
+  if (q1 > a.n_tokens) q1 = a.n_tokens;
+  r.q0 = (int)q0;
+  r.qlen = q1 > q0 ? (int)(q1 - q0) : 0;
+  r.total = (int)load_ctx(a.seq_lens, a.sl_dtype, s, (int64_t)a.max_blocks_per_seq * a.block_size);
+  return r;
+}
+__device__ __forceinline__ int dp_tiles(const DpSeq& q, int tt2) { return (q.qlen + tt2 - 1) / tt2; }
+__device__ __forceinline__ DpTile dp_tile(const DenseArgs& a, const DpSeq& q, int tt2, int i) {
+  DpTile t;
+  t.tok0 = i * tt2;
+  t.ntok = q.qlen - t.tok0 < tt2 ? q.qlen - t.tok0 : tt2;
+  const int pos0 = q.total - q.qlen + t.tok0, kend = pos0 + t.ntok;      // kend <= total
+  const int klo = a.window > 0 && pos0 + 1 > a.window ? pos0 + 1 - a.window : 0;
+  t.t0 = klo / DP_KT;
+  t.n = kend > 0 ? (kend + DP_KT - 1) / DP_KT - t.t0 : 0;
+  if (t.n < 1) t.n = 1;                          // rows that see nothing: one masked tile, they come out as zeros
+  return t;
+}
+
+// A place in the call's list of units: row tile (s, kvh, i) with sequence and tile, and the unit inside it.
+struct DpPlace { int s, kvh, i, off; };
+
+// All lanes of a warp: the place of unit u, 0 <= u < pre[seqs].
+__device__ __forceinline__ DpPlace dp_locate(const DenseArgs& a, const int64_t* pre, int seqs, int tt2, int64_t u, int lane) {
+  DpPlace p;
+  int lo = 0, hi = seqs;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pre[mid] <= u) lo = mid; else hi = mid;
+  }
+  p.s = lo;
+  const int64_t per = (pre[lo + 1] - pre[lo]) / a.num_kv_heads, in = u - pre[lo];
+  p.kvh = (int)(in / per);
+  int64_t rem = in - (int64_t)p.kvh * per;
+  const DpSeq q = dp_seq(a, lo);
+  const int tiles = dp_tiles(q, tt2);
+  for (int base = 0;; base += 32) {
+    const int i = base + lane, n = i < tiles ? dp_tile(a, q, tt2, i).n : 0;
+    int inc = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += x;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, inc > rem);
+    if (hit != 0u || base + 32 >= tiles) {
+      const int l = hit != 0u ? __ffs(hit) - 1 : 31;
+      p.i = base + l;
+      p.off = (int)(rem - (__shfl_sync(0xffffffffu, inc, l) - __shfl_sync(0xffffffffu, n, l)));
+      return p;
+    }
+    rem -= __shfl_sync(0xffffffffu, inc, 31);
+  }
+}
+
+// All lanes of a warp: first unit of CTA c of n_ctas (moved to a row tile's edge where one is near), and its place.
+__device__ __forceinline__ int64_t dp_begin(const DenseArgs& a, const int64_t* pre, int seqs, int tt2, int n_ctas, int c, int lane,
+                                            DpPlace* place) {
+  const int64_t units = pre[seqs];
+  if (c >= n_ctas) return units;
+  int64_t u = units / n_ctas * c + units % n_ctas * c / n_ctas;
+  DpPlace p = dp_locate(a, pre, seqs, tt2, u, lane);
+  const int n = dp_tile(a, dp_seq(a, p.s), tt2, p.i).n;
+  if (p.off > 0 && p.off <= DP_SNAP) {
+    u -= p.off;
+    p.off = 0;
+  } else if (p.off > 0 && n - p.off <= DP_SNAP) {
+    u += n - p.off;
+    if (u >= units) return units;
+    p = dp_locate(a, pre, seqs, tt2, u, lane);
+  }
+  *place = p;
+  return u;
+}
+
+// A role's way through the CTA's range, piece by piece (a piece: consecutive key tiles of one row tile)
+struct DpCursor {
+  int s, kvh, i;
+  DpSeq q;
+  DpTile t;
+  int off, cnt;                 // key tiles t.t0 + off .. + cnt - 1
+  int64_t left;                 // units behind this piece
+  int nq;                       // halves with tokens
+
+  __device__ __forceinline__ void settle(const DenseArgs& a, int tt2, int64_t avail) {
+    t = dp_tile(a, q, tt2, i);
+    cnt = avail < t.n - off ? (int)avail : t.n - off;
+    left = avail - cnt;
+    nq = 2 * t.ntok > tt2 ? 2 : 1;
+  }
+  __device__ __forceinline__ bool next(const DenseArgs& a, int tt2) {
+    if (left <= 0) return false;
+    off = 0;
+    if (++i >= dp_tiles(q, tt2)) {
+      i = 0;
+      if (++kvh == a.num_kv_heads) {
+        kvh = 0;
+        do { ++s; q = dp_seq(a, s); } while (q.qlen == 0);      // left > 0: there is one with tokens
+      }
+    }
+    settle(a, tt2, left);
+    return true;
+  }
+};
+
+template <bool BF, int D>
+__global__ void __launch_bounds__(320, 1)
+dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant__ DpMaps maps, int seqs, int G, int TT, int box,
+                     DpDesc* desc, float* part_ml, float* part_acc) {
+  using L = DpL<D>;
+  constexpr int NB = L::NB;
+  extern __shared__ uint8_t dp_smem[];
+  const uint32_t raw_s = smem_u32(dp_smem);
+  const uint32_t base_s = (raw_s + 1023u) & ~1023u;
+  uint8_t* base = dp_smem + (base_s - raw_s);
+  const uint32_t bar_s = base_s + L::BAR, failed_s = bar_s + P_FAILED;
+  int64_t* pre = reinterpret_cast<int64_t*>(base + L::PRE);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tt2 = 2 * TT;
+  __shared__ int64_t s_u[2];
+  __shared__ DpPlace s_place;
+  __shared__ int s_tiles[L::WARPS];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  if (tid == 0) {
+    for (int i = 0; i < NB; ++i) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_KVFULL + 8 * i));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_KVFREE + 8 * i));
+    }
+    for (int i = 0; i < 2; ++i) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_QFULL + 8 * i));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_QFREE + 8 * i));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_SFULL + 8 * i));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 4;" :: "r"(bar_s + P_PFULL + 8 * i));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_OFULL + 8 * i));
+    }
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_DRAIN));
+    asm volatile("st.shared.u32 [%0], %1;" :: "r"(failed_s), "r"(0u) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
+  if (warp == L::MMA_WARP) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(bar_s + P_TMEM) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // ---- units per sequence (a warp per sequence, lanes over its row tiles), then their prefix sums ----
+  int my_tiles = 0;
+  for (int s = warp; s < seqs; s += L::WARPS) {
+    const DpSeq q = dp_seq(a, s);
+    const int tiles = dp_tiles(q, tt2);
+    int64_t n = 0;
+    for (int i = lane; i < tiles; i += 32) n += dp_tile(a, q, tt2, i).n;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
+    if (lane == 0) pre[s + 1] = n * a.num_kv_heads;
+    my_tiles += tiles;
+  }
+  if (lane == 0) s_tiles[warp] = my_tiles;
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (warp == 0) {
+    int64_t run = 0;
+    for (int b = 0; b < seqs; b += 32) {
+      int64_t x = b + lane < seqs ? pre[b + lane + 1] : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
+      }
+      x += run;
+      if (b + lane < seqs) pre[b + lane + 1] = x;
+      run = __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) pre[0] = 0;
+  }
+  __syncthreads();
+  const int64_t units = pre[seqs];
+  // CTAs that share them: all, but not more than there are row tiles or groups of four key tiles
+  int n_ctas;
+  {
+    int64_t rts = 0;
+    for (int w = 0; w < L::WARPS; ++w) rts += s_tiles[w];
+    rts *= a.num_kv_heads;
+    const int64_t want = units / 4 > rts ? units / 4 : rts;
+    n_ctas = want < (int64_t)gridDim.x ? (int)want : (int)gridDim.x;
+  }
+  if (warp < 2) {
+    DpPlace p{0, 0, 0, 0};
+    const int64_t u = units > 0 ? dp_begin(a, pre, seqs, tt2, n_ctas, (int)blockIdx.x + warp, lane, &p) : 0;
+    if (lane == 0) {
+      s_u[warp] = u;
+      if (warp == 0) s_place = p;
+    }
+  }
+  __syncthreads();
+  const int64_t u0 = s_u[0], u1 = s_u[1];
+  const uint32_t tmem = lds_u32(bar_s + P_TMEM);
+  const bool work = u1 > u0;
+  DpCursor cur;
+  cur.left = 0;
+  if (work) {
+    cur.s = s_place.s; cur.kvh = s_place.kvh; cur.i = s_place.i; cur.off = s_place.off;
+    cur.q = dp_seq(a, cur.s);
+    cur.settle(a, tt2, u1 - u0);
+  }
+
+  auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    if (done) return true;
+    if (lds_u32(failed_s) != 0u) return false;
+    if (mbar_wait(bar, parity)) return true;
+    g_dense_prefill_status = 1;
+    asm volatile("st.shared.u32 [%0], %1;" :: "r"(failed_s), "r"(1u) : "memory");
+    return false;
+  };
+  auto wait_warp = [&](uint32_t bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
+
+  if (work && warp == L::MMA_WARP) {
+    // ================= MMA warp: lane 0 issues, all lanes wait (and zero the values behind a sequence's end) =================
+    constexpr uint32_t TYPES = BF ? (1u << 7) | (1u << 10) : 0u;
+    constexpr uint32_t IDESC_S = (1u << 4) | TYPES | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+    constexpr uint32_t IDESC_O = (1u << 4) | TYPES | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
+    const int withhold = blockIdx.x == 0 ? g_dense_prefill_withhold : -1;
+    const uint32_t q_s = base_s + L::Q, kv_s = base_s + L::KV;
+    int pieces[2] = {0, 0};                 // pieces begun per half (phase of q_full)
+    int steps[2] = {0, 0};                  // P V products issued per half (phase of p_full)
+    // scores of half h, key tile number g of the CTA (tile j of piece c)
+    auto issue_s = [&](const DpCursor& c, int g, int j, int h) -> bool {
+      const uint32_t slot = (uint32_t)((2 * g) % NB);
+      if (h == 0 && !wait_warp(bar_s + P_KVFULL + 8 * slot, (uint32_t)((2 * g / NB) & 1))) return false;
+      if (j == 0) {
+        if (!wait_warp(bar_s + P_QFULL + 8 * h, (uint32_t)(pieces[h] & 1))) return false;
+        ++pieces[h];
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (g == withhold) return true;
+      if (lane == 0) {
+        const uint32_t qb = q_s + (uint32_t)(h * L::TILE), kb = kv_s + slot * L::TILE;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (uint32_t)((kk >> 2) * 16384 + (kk & 3) * 32);
+          umma_f16(tmem + (uint32_t)(h * 128), umma_desc(qb + off), umma_desc(kb + off), IDESC_S, (uint32_t)(kk != 0));
+        }
+        umma_commit(bar_s + P_SFULL + 8 * h);
+        if (j == c.cnt - 1) umma_commit(bar_s + P_QFREE + 8 * h);
+        if (h == c.nq - 1) umma_commit(bar_s + P_KVFREE + 8 * slot);
+      }
+      __syncwarp();
+      return true;
+    };
+    auto issue_pv = [&](const DpCursor& c, int g, int j, int h) -> bool {
+      const uint32_t slot = (uint32_t)((2 * g + 1) % NB);
+      const uint32_t vb = kv_s + slot * L::TILE;
+      if (h == 0) {
+        if (!wait_warp(bar_s + P_KVFULL + 8 * slot, (uint32_t)(((2 * g + 1) / NB) & 1))) return false;
+        int z = c.q.total - (c.t.t0 + c.off + j) * DP_KT;      // keys of the tile inside the sequence
+        if (z < DP_KT) {
+          if (z < 0) z = 0;
+          for (int e = z * 8 + lane; e < DP_KT * 8; e += 32)
+#pragma unroll
+            for (int x = 0; x < L::HALVES; ++x)
+              asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" :: "r"(vb + (uint32_t)(x * 16384 + e * 16)), "r"(0u) : "memory");
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+      }
+      if (!wait_warp(bar_s + P_PFULL + 8 * h, (uint32_t)(steps[h] & 1))) return false;
+      ++steps[h];
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (lane == 0) {
+#pragma unroll
+        for (int kk = 0; kk < DP_KT / 16; ++kk)
+          umma_f16_ta(tmem + (uint32_t)(L::T_O + h * 128), tmem + (uint32_t)(h * 128 + kk * 8), dp_desc_mn(vb + (uint32_t)(kk * 2048)),
+                      IDESC_O, (uint32_t)((j | kk) != 0));
+        if (j == c.cnt - 1) umma_commit(bar_s + P_OFULL + 8 * h);
+        if (h == c.nq - 1) umma_commit(bar_s + P_KVFREE + 8 * slot);
+      }
+      __syncwarp();
+      return true;
+    };
+    DpCursor ahead = cur;                   // the piece of the next scores
+    int ja = 0;
+    bool go = issue_s(ahead, 0, 0, 0) && (ahead.nq < 2 || issue_s(ahead, 0, 0, 1));
+    bool more = true;
+    int j = 0;
+    for (int g = 0; go; ++g) {
+      if (more && ++ja >= ahead.cnt) {
+        ja = 0;
+        more = ahead.next(a, tt2);
+      }
+#pragma unroll 1
+      for (int h = 0; h < 2 && go; ++h) {
+        if (h < cur.nq) go = issue_pv(cur, g, j, h);
+        if (go && more && h < ahead.nq) go = issue_s(ahead, g + 1, ja, h);
+      }
+      if (++j >= cur.cnt) {
+        j = 0;
+        if (!cur.next(a, tt2)) break;
+      }
+    }
+  } else if (work && warp == L::LOAD_WARP) {
+    // ================= copies: K of a tile, (Q of a new piece,) V of the tile =================
+    const int boxes = DP_KT / box;          // runs of keys inside a block
+    const uint32_t box_bytes = (uint32_t)box * 128u;
+    const bool mine = lane < boxes;
+    int seq = 0, pieces[2] = {0, 0};        // ring position
+    bool go = true;
+    auto fill = [&](const CUtensorMap* map, int64_t blk, int pos, int kvh) -> bool {
+      const uint32_t slot = (uint32_t)(seq % NB), bar = bar_s + P_KVFULL + 8 * slot;
+      if (seq >= NB && !wait_warp(bar_s + P_KVFREE + 8 * slot, (uint32_t)((seq / NB - 1) & 1))) return false;
+      if (lane == 0) dp_expect(bar, L::TILE);
+      __syncwarp();
+      if (mine)
+#pragma unroll
+        for (int x = 0; x < L::HALVES; ++x)
+          dp_tma4(base_s + L::KV + slot * L::TILE + (uint32_t)(x * 16384) + (uint32_t)lane * box_bytes, map, bar, 64 * x, kvh, pos, (int)blk);
+      ++seq;
+      return true;
+    };
+    do {
+      int64_t blk = 0;
+      int pos = 0;
+      auto find = [&](int j) {              // block and position of this lane's run of keys in tile j of the piece
+        if (mine && j < cur.cnt) {
+          const int key = (cur.t.t0 + cur.off + j) * DP_KT + lane * box;
+          const int b = key / a.block_size;
+          pos = key - b * a.block_size;
+          blk = dense_block(a, cur.s, b);
+        }
+      };
+      find(0);
+      for (int j = 0; j < cur.cnt && go; ++j) {
+        const int64_t blk_j = blk;
+        const int pos_j = pos;
+        find(j + 1);                        // in flight while the ring is waited for
+        go = fill(&maps.k, blk_j, pos_j, cur.kvh);
+        if (!go) break;
+        if (j == 0) {
+          for (int h = 0; h < cur.nq && go; ++h) {
+            if (pieces[h] > 0) go = wait_warp(bar_s + P_QFREE + 8 * h, (uint32_t)((pieces[h] - 1) & 1));
+            if (!go) break;
+            ++pieces[h];
+            if (lane == 0) {
+              dp_expect(bar_s + P_QFULL + 8 * h, (uint32_t)(TT * G * D * 2));
+#pragma unroll
+              for (int x = 0; x < L::HALVES; ++x)
+                dp_tma3(base_s + L::Q + (uint32_t)(h * L::TILE + x * 16384), &maps.q, bar_s + P_QFULL + 8 * h, 64 * x, cur.kvh * G,
+                        cur.q.q0 + cur.t.tok0 + h * TT);
+            }
+            __syncwarp();
+          }
+          if (!go) break;
+        }
+        go = fill(&maps.v, blk_j, pos_j, cur.kvh);
+      }
+    } while (go && cur.next(a, tt2));
+    // a CTA that gives up must not leave while copies into its shared memory are in flight
+    if (lds_u32(failed_s) != 0u) {
+      for (int q = seq - NB < 0 ? 0 : seq - NB; q < seq; ++q) mbar_wait(bar_s + P_KVFULL + 8 * (uint32_t)(q % NB), (uint32_t)((q / NB) & 1));
+      for (int h = 0; h < 2; ++h)
+        if (pieces[h] > 0) mbar_wait(bar_s + P_QFULL + 8 * h, (uint32_t)((pieces[h] - 1) & 1));
+    }
+  } else if (work) {
+    // ================= softmax warps: half = warp / 4, thread = row =================
+    const int half = warp >> 2, quad = warp & 3;
+    const int r = quad * 32 + lane;
+    const uint32_t t_lane = ((uint32_t)(quad * 32)) << 16;
+    const uint32_t t_s = tmem + t_lane + (uint32_t)(half * 128), t_o = tmem + t_lane + (uint32_t)(L::T_O + half * 128);
+    const int r_tok = r / G, r_head = r - r_tok * G;
+    const float c = a.scale_log2;
+    int step = 0, piece = 0;
+    bool ok = true, first = true;
+    do {
+      if (half < cur.nq) {
+        const int tok = cur.t.tok0 + half * TT + r_tok;
+        const bool live = r_tok < TT && tok < cur.q.qlen;
+        const int lim = live ? cur.q.total - cur.q.qlen + tok + 1 : 0x7fffffff;      // keys below it; a row without a token masks nothing
+        const int low = live && a.window > 0 && lim > a.window ? lim - a.window : 0;
+        const int lim_w = __reduce_min_sync(0xffffffffu, lim), low_w = __reduce_max_sync(0xffffffffu, low);
+        float m = -CUDART_INF_F, l = 0.f;      // reference in log2 units, sum of the weights
+        for (int j = 0; j < cur.cnt; ++j) {
+          if (!wait_warp(bar_s + P_SFULL + 8 * half, (uint32_t)(step & 1))) { ok = false; break; }
+          ++step;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          uint32_t v[128];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) tmem_ld32(t_s + 32 * x, *reinterpret_cast<uint32_t (*)[32]>(&v[32 * x]));
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          const int key0 = (cur.t.t0 + cur.off + j) * DP_KT;
+          if (key0 + DP_KT > lim_w || key0 < low_w) {
+            const int hi = lim - key0, lo = low - key0;
+#pragma unroll
+            for (int i = 0; i < 128; ++i) v[i] = i < hi && i >= lo ? v[i] : 0xff800000u;
+          }
+          float mx = __uint_as_float(v[0]), my = __uint_as_float(v[1]);
+#pragma unroll
+          for (int i = 2; i < 126; i += 4) {
+            mx = dp_max3(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+            my = dp_max3(my, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+          }
+          mx = dp_max3(mx, __uint_as_float(v[126]), __uint_as_float(v[127]));
+          mx = dp_max3(mx, my, my) * c;
+          const bool grow = live && !(mx <= m + DP_RESCALE);      // also for a NaN, which then stays
+          if (__any_sync(0xffffffffu, grow)) {
+            const float f = grow ? dense_ex2(m - mx) : 1.0f;      // m = -inf: 0
+            if (grow) { m = mx; l *= f; }
+            if (j > 0) {
+#pragma unroll 1
+              for (int x = 0; x < D / 32; ++x) {
+                uint32_t o[32];
+                tmem_ld32(t_o + 32 * x, o);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_st32(t_o + 32 * x, o);
+              }
+            }
+          }
+          const float ref = m == -CUDART_INF_F ? 0.f : -m;
+          float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint32_t ph[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float p0 = dense_ex2(fmaf(__uint_as_float(v[32 * x + 2 * i]), c, ref));
+              const float p1 = dense_ex2(fmaf(__uint_as_float(v[32 * x + 2 * i + 1]), c, ref));
+              l0 += p0;
+              l1 += p1;
+              ph[i] = dense_pack<BF>(p0, p1);
+            }
+            tmem_st16(t_s + 16 * x, ph);
+          }
+          l += l0 + l1;
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) dp_arrive(bar_s + P_PFULL + 8 * half);
+        }
+        if (!ok || !wait_warp(bar_s + P_OFULL + 8 * half, (uint32_t)(piece & 1))) { ok = false; break; }
+        ++piece;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const bool whole = cur.cnt == cur.t.n;
+        const int64_t row = cur.q.q0 + tok;
+        const int64_t slot = (int64_t)blockIdx.x * 2 + (first ? 0 : 1);
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll 1
+        for (int x = 0; x < D / 32; ++x) {
+          uint32_t o[32];
+          tmem_ld32(t_o + 32 * x, o);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          if (live && whole) {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.out_st + (int64_t)(cur.kvh * G + r_head) * a.out_sh + 32 * x);
+            // l == 0: no key was seen (0 * anything below would keep a NaN of a masked product)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = l == 0.f ? 0u : dense_pack<BF>(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+              dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else if (live) {
+            float4* dst = reinterpret_cast<float4*>(part_acc + (slot * 256 + half * 128 + r) * D + 32 * x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+          }
+        }
+        if (live && !whole) {
+          part_ml[(slot * 256 + half * 128 + r) * 2] = m;
+          part_ml[(slot * 256 + half * 128 + r) * 2 + 1] = l;
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      }
+      first = false;
+    } while (cur.next(a, tt2));
+  }
+
+  // ---- the row tile that this CTA begins and does not finish (its last piece): how many parts it has ----
+  if (warp == 0) {
+    DpDesc d{0, 0, 0, 0, 0, {0, 0, 0}};
+    if (work && lds_u32(failed_s) == 0u && cur.off == 0 && cur.cnt < cur.t.n) {
+      const int64_t begin = u1 - cur.cnt, end = begin + cur.t.n;
+      int c1 = (int)blockIdx.x + 1;
+      DpPlace p;
+      while (c1 + 1 < n_ctas && dp_begin(a, pre, seqs, tt2, n_ctas, c1 + 1, lane, &p) < end) ++c1;
+      d.parts = c1 - (int)blockIdx.x + 1;
+      d.slot0 = begin == u0 ? 0 : 1;
+      d.row0 = cur.q.q0 + cur.t.tok0;
+      d.ntok = cur.t.ntok;
+      d.kvh = cur.kvh;
+    }
+    if (lane == 0) desc[blockIdx.x] = d;
+  }
+
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  // a CTA in which a wait gave up may still have MMAs in flight: commit once more and wait (bounded) before the columns go back
+  int leak = 0;
+  if (warp == L::MMA_WARP && lane == 0 && lds_u32(failed_s) != 0u) {
+    umma_commit(bar_s + P_DRAIN);
+    leak = mbar_wait(bar_s + P_DRAIN, 0u) ? 0 : 1;
+    if (leak) g_dense_prefill_status = 2;
+  }
+  leak = __syncthreads_or(leak);
+  if (warp == L::MMA_WARP && !leak) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(tmem) : "memory");
+  }
+}
+
+// Row tiles that were cut: out = sum_p 2^(m_p - M) acc_p / sum_p 2^(m_p - M) l_p in the order of the keys.  Block (c, y):
+// rows 32 y .. + 31 of the row tile that CTA c began; a warp takes a row at a time.
+template <bool BF, int D>
+__global__ void __launch_bounds__(256)
+dense_prefill_merge_kernel(DenseArgs a, int G, int TT, int tail, const DpDesc* desc, const float* part_ml, const float* part_acc) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (tail >= 0) {               // rows behind the last sequence (`tail` of them in this launch) come out as zeros
+    int64_t row = load_index(a.starts, a.qs_dtype, tail);
+    if (row < 0) row = 0;
+    for (row += blockIdx.y * gridDim.x + blockIdx.x; row < a.n_tokens; row += gridDim.x * gridDim.y)
+      for (int e = threadIdx.x; e < a.num_q_heads * (D / 8); e += 256)
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.out_st + (int64_t)(e / (D / 8)) * a.out_sh + e % (D / 8) * 8) =
+            make_uint4(0u, 0u, 0u, 0u);
+  }
+  const DpDesc d = desc[blockIdx.x];
+  if (d.parts < 2) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int PER = D / 32;
+  for (int r = blockIdx.y * 32 + warp; r < blockIdx.y * 32 + 32; r += 8) {
+    const int in_half = r & 127, t = in_half / G, tok = (r >> 7) * TT + t;
+    if (t >= TT || tok >= d.ntok) continue;
+    auto at = [&](int p) -> int64_t { return ((int64_t)(blockIdx.x + p) * 2 + (p == 0 ? d.slot0 : 0)) * 256 + r; };
+    float top = -CUDART_INF_F;
+    for (int p = lane; p < d.parts; p += 32) top = fmaxf(top, part_ml[at(p) * 2]);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    float acc[PER], sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+    for (int p = 0; p < d.parts; ++p) {
+      const float mp = part_ml[at(p) * 2], f = mp == -CUDART_INF_F ? 0.f : dense_ex2(mp - top);
+      if (mp == -CUDART_INF_F) continue;      // the part saw no key of this row
+      sum += f * part_ml[at(p) * 2 + 1];
+      const float* src = part_acc + at(p) * D + lane * PER;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) acc[i] += f * src[i];
+    }
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (int64_t)(d.row0 + tok) * a.out_st +
+                                                (int64_t)(d.kvh * G + in_half - t * G) * a.out_sh + lane * PER);
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+    for (int i = 0; i < PER / 2; ++i) dst[i] = dense_pack<BF>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+  }
+}
+
+typedef CUresult (*dp_encode_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+dp_encode_fn dp_encoder() {
+  static const dp_encode_fn fn = []() -> dp_encode_fn {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+      return reinterpret_cast<dp_encode_fn>(p);
+    cudaGetLastError();
+    return nullptr;
+  }();
+  return fn;
+}
+
+int gcd(int a, int b) { return b == 0 ? a : gcd(b, a % b); }
+
+// Maps over the call's query and caches (this GPU's memory).  A stride of a dimension of one element is never used by a
+// copy but still checked by the driver: the row pitch stands in for it.
+bool dp_make_maps(const DenseArgs& a, bool bf, int G, int TT, int box, DpMaps* m) {
+  const dp_encode_fn enc = dp_encoder();
+  if (enc == nullptr) return false;
+  const CUtensorMapDataType type = bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const cuuint64_t row = (cuuint64_t)a.head_dim * 2;
+  auto pitch = [&](int64_t stride, int64_t n) -> cuuint64_t { return n > 1 ? (cuuint64_t)(stride * 2) : row; };
+  {
+    const cuuint64_t dims[3] = {(cuuint64_t)a.head_dim, (cuuint64_t)a.num_q_heads, (cuuint64_t)a.n_tokens};
+    const cuuint64_t strides[2] = {pitch(a.q_sh, a.num_q_heads), pitch(a.q_st, a.n_tokens)};
+    const cuuint32_t b[3] = {64, (cuuint32_t)G, (cuuint32_t)TT};
+    if (enc(&m->q, type, 3, const_cast<void*>(a.q), dims, strides, b, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) return false;
+  }
+  for (int side = 0; side < 2; ++side) {
+    const cuuint64_t dims[4] = {(cuuint64_t)a.head_dim, (cuuint64_t)a.num_kv_heads, (cuuint64_t)a.block_size, (cuuint64_t)a.num_blocks};
+    const cuuint64_t strides[3] = {pitch(side ? a.v_sh : a.k_sh, a.num_kv_heads), pitch(side ? a.v_sp : a.k_sp, a.block_size),
+                                   pitch(side ? a.v_sb : a.k_sb, a.num_blocks)};
+    const cuuint32_t b[4] = {64, 1, (cuuint32_t)box, 1};
+    if (enc(side ? &m->v : &m->k, type, 4, const_cast<void*>(side ? a.v : a.k), dims, strides, b, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) return false;
+  }
+  return true;
+}
+
+struct DpWorkspace { DpDesc* desc; float* ml; float* acc; };
+size_t dp_workspace(int head_dim, char* base, DpWorkspace* w) {
+  const size_t n = (size_t)sm_count();
+  const size_t d = (n * sizeof(DpDesc) + 255) / 256 * 256, ml = n * 2 * 256 * 2 * sizeof(float), acc = n * 2 * 256 * (size_t)head_dim * sizeof(float);
+  if (w != nullptr) *w = DpWorkspace{reinterpret_cast<DpDesc*>(base), reinterpret_cast<float*>(base + d), reinterpret_cast<float*>(base + d + ml)};
+  return d + ml + acc;
+}
+
+template <bool BF, int D>
+int dp_launch(const DenseArgs& all, const DpMaps& maps, int G, int TT, int box, bool zero_tail, const DpWorkspace& w, cudaStream_t st) {
+  using L = DpL<D>;
+  cudaError_t e = cudaFuncSetAttribute(dense_prefill_kernel<BF, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+  if (e != cudaSuccess) return fail((int)e, "dense prefill attention: smem attribute: %s", cudaGetErrorString(e));
+  const int grid = sm_count();
+  for (int s0 = 0; s0 < all.num_seqs; s0 += DP_MAX_SEQS) {
+    const int seqs = all.num_seqs - s0 < DP_MAX_SEQS ? all.num_seqs - s0 : DP_MAX_SEQS;
+    DenseArgs a = all;
+    a.starts = static_cast<const char*>(all.starts) + (size_t)s0 * (all.qs_dtype == AKV_I64 ? 8 : 4);
+    a.seq_lens = static_cast<const char*>(all.seq_lens) + (size_t)s0 * (all.sl_dtype == AKV_I64 ? 8 : 4);
+    a.block_tables = static_cast<const char*>(all.block_tables) + (int64_t)s0 * all.bt_stride * (all.bt_dtype == AKV_I64 ? 8 : 4);
+    dense_prefill_kernel<BF, D><<<grid, L::THREADS, L::SMEM, st>>>(a, maps, seqs, G, TT, box, w.desc, w.ml, w.acc);
+    if (int rc = check_launch("dense_prefill_attn_kernel")) return rc;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)grid, 8);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, dense_prefill_merge_kernel<BF, D>, a, G, TT, zero_tail && s0 + seqs == all.num_seqs ? seqs : -1, (const DpDesc*)w.desc, (const float*)w.ml, (const float*)w.acc);
+    if (e != cudaSuccess) return fail((int)e, "dense prefill merge: %s", cudaGetErrorString(e));
+    if (int rc = check_launch("dense_prefill_merge_kernel")) return rc;
+  }
+  return AKV_OK;
+}
+
+}  // namespace
+
+int dense_prefill_status(int* host_out, int reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(host_out, g_dense_prefill_status, sizeof(int));
+  if (e == cudaSuccess && reset) { const int z = 0; e = cudaMemcpyToSymbol(g_dense_prefill_status, &z, sizeof(int)); }
+  return e == cudaSuccess ? AKV_OK : fail((int)e, "dense prefill status: %s", cudaGetErrorString(e));
+}
+
+int dense_prefill_withhold(int tile) {
+  cudaError_t e = cudaMemcpyToSymbol(g_dense_prefill_withhold, &tile, sizeof(int));
+  return e == cudaSuccess ? AKV_OK : fail((int)e, "dense prefill test hook: %s", cudaGetErrorString(e));
+}
+
+}  // namespace akv
+
+AKV_EXPORT size_t akv_dense_prefill_attn_workspace_bytes(int head_dim) {
+  return head_dim > 0 ? akv::dp_workspace(head_dim, nullptr, nullptr) : 0;
+}
+
+AKV_EXPORT int akv_dense_prefill_attn(const akv_dense_attn_params* p) {
+  akv::DenseArgs a;
+  if (int rc = akv::dense_common(p, "akv_dense_prefill_attn", &a)) return rc;
+  if (a.num_seqs == 0 || a.n_tokens == 0) return AKV_OK;
+  if (!a.starts) return akv::fail(AKV_ERR_ARG, "akv_dense_prefill_attn: null query_start_loc");
+  const int G = a.num_q_heads / a.num_kv_heads;
+  const int box = a.block_size % 128 == 0 ? 128 : akv::gcd(a.block_size, 128);
+  if (a.head_dim == 256 || G > 128 || box < 8 || a.max_blocks_per_seq == 0 || a.num_blocks > 0x7fffffffll)
+    return akv::fail(AKV_ERR_UNSUPPORTED, "akv_dense_prefill_attn: head_dim %d, %d query heads per KV head, block_size %d, %d blocks per "
+                     "sequence (64 or 128, at most 128, a multiple of 8, at least 1)", a.head_dim, G, a.block_size, a.max_blocks_per_seq);
+  akv::DpWorkspace w;
+  const size_t need = akv::dp_workspace(a.head_dim, static_cast<char*>(p->workspace), &w);
+  if (!p->workspace || p->workspace_bytes < need || ((uintptr_t)p->workspace & 255))
+    return akv::fail(AKV_ERR_WORKSPACE, "akv_dense_prefill_attn: workspace of %zu bytes (256-byte aligned) needed, got %zu", need, p->workspace_bytes);
+  const int TT = 128 / G;
+  akv::DpMaps maps;
+  const bool bf = p->dtype == AKV_BF16;
+  if (!akv::dp_make_maps(a, bf, G, TT, box, &maps))
+    return akv::fail(AKV_ERR_UNSUPPORTED, "akv_dense_prefill_attn: these strides cannot be described to the copy unit");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(p->stream);
+  if (a.head_dim == 128) return bf ? akv::dp_launch<true, 128>(a, maps, G, TT, box, p->zero_tail != 0, w, st) : akv::dp_launch<false, 128>(a, maps, G, TT, box, p->zero_tail != 0, w, st);
+  return bf ? akv::dp_launch<true, 64>(a, maps, G, TT, box, p->zero_tail != 0, w, st) : akv::dp_launch<false, 64>(a, maps, G, TT, box, p->zero_tail != 0, w, st);
+}

@@ -87,12 +87,14 @@ class DensePagedAttention:
         self.head_dim, self.num_query_heads, self.num_kv_heads = head_dim, num_query_heads, num_kv_heads
         self.scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
         self.sliding_window = int(sliding_window)
+        self._prefill_bytes = _lib.lib().akv_dense_prefill_attn_workspace_bytes(head_dim)
         self._decode_bytes = _lib.lib().akv_dense_paged_attn_workspace_bytes(num_query_heads, num_kv_heads, head_dim)
 
     @staticmethod
     def _rows16(x: torch.Tensor) -> bool:
         """Whether every row of a 16-bit [a, b, head_dim] tensor starts on a 16-byte boundary."""
-        return x.stride(2) == 1 and not (x.data_ptr() & 15 or (x.stride(0) | x.stride(1)) & 7)
+        return (x.stride(2) == 1 and x.stride(0) > 0 and x.stride(1) > 0
+                and not (x.data_ptr() & 15 or (x.stride(0) | x.stride(1)) & 7))
 
     def _params(self, dev, query, k_cache, v_cache, block_tables, seq_lens, num_seqs, out):
         """Argument block of both entry points, and the output."""
@@ -138,4 +140,53 @@ class DensePagedAttention:
         ws = torch.empty(self._decode_bytes, dtype=torch.uint8, device=dev)
         p.workspace, p.workspace_bytes = ws.data_ptr(), self._decode_bytes
         _lib.call(dev, "akv_dense_paged_attn", ctypes.byref(p))
+        return out
+
+    def prefill(self, query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                seq_lens: torch.Tensor, query_start_loc: torch.Tensor, out: Optional[torch.Tensor] = None,
+                max_seq_len: Optional[int] = None) -> torch.Tensor:
+        """Chunks of new tokens: rows ``query_start_loc[s] .. query_start_loc[s + 1]`` of ``query`` [tokens, query_heads,
+        head_dim] are the last tokens of sequence s, whose keys and values (counted in ``seq_lens``) are in the cache
+        already; each attends causally up to its own position.  Rows behind the last sequence are left as they are in
+        ``out`` (zero when ``out`` is allocated here).  Lengths stay on the device: ``max_seq_len``, which
+        ``TQPagedAttention.prefill`` sizes its scratch by, is accepted and not needed.
+
+        Chunks run on the tensor cores for head_dim 64 and 128, at most 128 query heads per KV head and block sizes that
+        are multiples of 8; other shapes attend token by token through ``forward``'s kernels."""
+        dev = _lib.require_cuda(query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, out)
+        if query_start_loc.dim() != 1 or query_start_loc.shape[0] < 1:
+            raise ValueError(f"query_start_loc {tuple(query_start_loc.shape)} must be [sequences + 1]")
+        if query_start_loc.stride(0) != 1:
+            query_start_loc = query_start_loc.contiguous()
+        qs_code = _lib.index_code(query_start_loc)
+        zero_tail = out is None
+        p, out, keep = self._params(dev, query, k_cache, v_cache, block_tables, seq_lens, query_start_loc.shape[0] - 1, out)
+        if not (self.head_dim <= 128 and self.num_query_heads <= 128 * self.num_kv_heads and k_cache.shape[1] % 8 == 0
+                and block_tables.shape[1] > 0):
+            if zero_tail:
+                out.zero_()
+            return self._prefill_by_rows(query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, out)
+        ws = torch.empty(self._prefill_bytes, dtype=torch.uint8, device=dev)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), self._prefill_bytes
+        p.query_start_loc, p.qs_dtype, p.zero_tail = query_start_loc.data_ptr(), qs_code, int(zero_tail)
+        _lib.call(dev, "akv_dense_prefill_attn", ctypes.byref(p))
+        return out
+
+    ROWS = 2048      # tokens of one call of the single-token kernels
+
+    def _prefill_by_rows(self, query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, out):
+        """Every token as a sequence of its own: its context length and its sequence's row of the block tables."""
+        n = query.shape[0]
+        if n == 0 or query_start_loc.shape[0] < 2:
+            return out
+        tok = torch.arange(n, device=query.device, dtype=torch.int64)
+        ends = query_start_loc[1:].to(torch.int64).contiguous()
+        seq = torch.bucketize(tok, ends, right=True)
+        there = (seq < ends.shape[0])[:, None, None]
+        seq = seq.clamp_(max=ends.shape[0] - 1)
+        ctx = (seq_lens.to(torch.int64)[seq] - (ends[seq] - 1 - tok)).clamp_(min=0)
+        for lo in range(0, n, self.ROWS):
+            hi = min(n, lo + self.ROWS)
+            rows = self.forward(query[lo:hi], k_cache, v_cache, block_tables[seq[lo:hi]], ctx[lo:hi])
+            out[lo:hi].copy_(torch.where(there[lo:hi], rows, out[lo:hi]))
         return out

@@ -57,13 +57,13 @@ const char* akv_last_split_kernel(void);
  *   out[2] akv_tq_paged_attn / akv_tq_decode_step, out[3] akv_hybrid_paged_attn: 1 = a kernel that keeps
  *          tables at fixed shared-memory addresses found its window taken and returned without writing
  *          partials (the host checks the window before choosing such a kernel, so this stays 0); for the
- *          TMA-fed attention kernel 2 = a bounded wait on a copy barrier ran out.
+ *          TMA-fed attention kernel and the tensor-core prefill kernels (packed or dense cache) 2 = a bounded wait ran out.
  *   out[4] akv_p2p_lse_merge: 1 = the bounded wait for the peers' partials ran out (a peer is late or gone).
  * A diagnostic call for health checks and tests, not part of a serving step. */
 int akv_device_status(int* out, int reset);
 
 /* Test hook for those bounded waits: CTA 0 of later encoder (which = 0), decoder (which = 1) or
- * tensor-core prefill attention (which = 2: the score MMAs of key tile `tile`) launches issues neither
+ * tensor-core prefill attention (which = 2 packed, 3 dense cache: the score MMAs of key tile `tile`) launches issues neither
  * the MMAs nor the commit of its tile number `tile`, so the wait on that tile runs out with no tensor
  * work in flight and the CTA leaves through its give-up path.  tile < 0 (the default) switches the
  * hook off. */
@@ -476,7 +476,15 @@ int akv_rotary_kv_append(const akv_rotary_append_params* params);
  *
  * akv_dense_paged_attn: one token per sequence, row s of query and out, the last of its seq_lens[s] tokens (rows behind
  * num_seqs are left alone; query_start_loc is ignored).  Two launches, capturable; the workspace is used by the call alone
- * until it has finished. */
+ * until it has finished.
+ *
+ * akv_dense_prefill_attn: chunks of new tokens.  Sequence s brings rows query_start_loc[s] .. query_start_loc[s + 1] - 1
+ * (int32 / int64, [num_seqs + 1], ascending, from 0), the last of its seq_lens[s] tokens, whose keys and values are in the
+ * cache already; token i of n sees the first seq_lens[s] - (n - 1 - i) keys, the last `window` of them with a window.
+ * Rows behind the last sequence are left alone, or zeroed with zero_tail.  Two launches, capturable, no host bound on any length needed; workspace as
+ * above, 256-byte aligned.  head_dim 64 or 128, at most 128 query heads per KV head, block_size a multiple of 8:
+ * AKV_ERR_UNSUPPORTED otherwise (attend row by row with akv_dense_paged_attn then).  A value that is not finite reaches the
+ * rows of its sequence that see its key, and may reach rows of the same 128 keys' tile that do not. */
 typedef struct akv_dense_attn_params {
   const void* query; int dtype; int64_t q_stride_tok, q_stride_head;
   const void* k_cache; int64_t k_stride_blk, k_stride_pos, k_stride_head;
@@ -488,12 +496,14 @@ typedef struct akv_dense_attn_params {
   int64_t num_blocks;
   float scale; int window;
   void* out; int64_t out_stride_tok, out_stride_head;
-  int max_seq_len;
+  int zero_tail;   /* akv_dense_prefill_attn: write zeros to the rows behind the last sequence */
   void* workspace; size_t workspace_bytes;
   void* stream;
 } akv_dense_attn_params;
 size_t akv_dense_paged_attn_workspace_bytes(int num_q_heads, int num_kv_heads, int head_dim);
 int akv_dense_paged_attn(const akv_dense_attn_params* params);
+size_t akv_dense_prefill_attn_workspace_bytes(int head_dim);
+int akv_dense_prefill_attn(const akv_dense_attn_params* params);
 
 /* ------------------------------------------------------------------------
  * Cross-GPU merge of split-K partials over NVLink peer memory (no counterpart in the reference, which

@@ -167,3 +167,180 @@ def test_single_tokens_graph_replay_and_streams():
             s.synchronize()
             assert torch.equal(o, want)
     check(want, q, kc, vc, bt, cl, starts)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# chunks of new tokens
+# ---------------------------------------------------------------------------------------------------------------------
+CHUNKS = {      # (tokens with the chunk's, the chunk's)
+    "one": ([1], [1]),
+    "prompt": ([130], [130]),
+    "tiles": ([127, 128, 129, 256, 257], [127, 128, 129, 256, 257]),
+    "behind": ([1000, 40, 513], [3, 40, 70]),
+    "mixed": ([700, 0, 5, 90, 33, 1500], [1, 1, 5, 0, 33, 200]),
+    "long": ([5000], [300]),
+}
+
+
+def run_chunks(lens, new, qh, kvh, D, bs, dtype, window=0, seed=0, tail=0, **kw):
+    q, kc, vc, bt, cl, starts = make(lens, new, qh, kvh, D, bs, dtype, seed=seed, stale=math.nan, tail=tail, **kw)
+    out = attn(qh, kvh, D, sliding_window=window).prefill(q, kc, vc, bt, cl, starts)
+    from aitherkvcache_b200 import _lib
+    assert _lib.device_status()["attn_window"] == 0
+    check(out, q, kc, vc, bt, cl, starts, window)
+    return out
+
+
+@pytest.mark.parametrize("chunks", CHUNKS)
+@pytest.mark.parametrize("qh,kvh,D", [(8, 2, 128), (8, 1, 64), (3, 3, 128), (14, 2, 64), (20, 4, 128), (64, 1, 64)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_chunks(dtype, qh, kvh, D, chunks):
+    lens, new = CHUNKS[chunks]
+    run_chunks(lens, new, qh, kvh, D, 16, dtype, seed=len(lens), scale_q=2.0)
+
+
+@pytest.mark.parametrize("bs", [8, 24, 32, 128, 384])
+@pytest.mark.parametrize("window", [0, 1, 100, 128, 1000])
+def test_chunks_blocks_and_windows(bs, window):
+    run_chunks([900, 77, 2000, 1], [300, 77, 9, 1], 8, 2, 128, bs, torch.float16, window, seed=bs)
+
+
+@pytest.mark.parametrize("qh,kvh,D,bs", [(4, 2, 256, 16), (4, 2, 128, 5), (129, 1, 64, 16)])
+def test_chunks_that_attend_token_by_token(qh, kvh, D, bs):
+    out = run_chunks([300, 20, 0], [40, 20, 2], qh, kvh, D, bs, torch.bfloat16, 30, tail=3)
+    assert bool((out[-3:] == 0).all())
+
+
+def test_chunks_more_query_tokens_than_cached_tokens():
+    """The first tokens of a chunk longer than its sequence see nothing and come out as zeros."""
+    q, kc, vc, bt, cl, starts = make([50, 60], [50, 60], 8, 2, 128, 16, torch.float16, seed=4)
+    cl[0] = 20
+    out = attn(8, 2, 128).prefill(q, kc, vc, bt, cl, starts)
+    assert bool((out[:30] == 0).all())
+    check(out, q, kc, vc, bt, cl, starts)
+
+
+def test_chunks_rows_behind_the_last_sequence():
+    lens, new = [200, 40], [33, 40]
+    q, kc, vc, bt, cl, starts = make(lens, new, 8, 2, 64, 16, torch.float16, seed=6, tail=700)
+    a = attn(8, 2, 64)
+    want = a.prefill(q, kc, vc, bt, cl, starts)
+    assert bool((want[73:] == 0).all())
+    check(want, q, kc, vc, bt, cl, starts)
+    out = torch.full((773, 10, 64), 5.0, dtype=torch.float16, device="cuda")
+    res = a.prefill(q, kc, vc, bt.long(), cl.long(), starts.long(), out=out[:, :8], max_seq_len=200)
+    assert res.data_ptr() == out.data_ptr() and torch.equal(out[:73, :8], want[:73])
+    assert bool((out[73:] == 5.0).all()) and bool((out[:, 8:] == 5.0).all())
+
+
+def test_chunks_large_scores_and_growing_maxima():
+    q, kc, vc, bt, cl, starts = make([900], [200], 4, 1, 128, 16, torch.bfloat16, seed=3)
+    kc.mul_(0.02)
+    q.fill_(1.0)
+    ramp = (torch.arange(912, device="cuda") / 64).to(torch.bfloat16).view(57, 16)
+    kc[bt[0, :57].long()] += ramp[:, :, None, None]
+    out = attn(4, 1, 128, scale=1.0).prefill(q, kc, vc, bt, cl, starts)
+    check(out, q, kc, vc, bt, cl, starts, scale=1.0)
+
+
+def test_chunks_strides_and_bad_tables():
+    lens, new = [300, 100], [50, 100]
+    q, kc, vc, bt, cl, starts = make(lens, new, 8, 2, 128, 16, torch.float16, seed=5)
+    a = attn(8, 2, 128)
+    want = a.prefill(q, kc, vc, bt, cl, starts)
+    kh, vh = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in (kc, vc))      # heads first inside a block
+    wide = torch.randn(150, 12, 128, device="cuda").half()
+    wide[:, 2:10] = q
+    assert torch.equal(a.prefill(wide[:, 2:10], kh, vh, bt, cl, starts), want)
+    odd = torch.randn(150, 8 * 128 + 1, device="cuda").half()
+    odd[:, 1:] = q.flatten(1)
+    assert torch.equal(a.prefill(odd[:, 1:].unflatten(1, (8, 128)), kc, vc, bt, cl, starts), want)
+    far = torch.full((2, 40), 1 << 40, dtype=torch.int64, device="cuda")
+    for s, n in enumerate(lens):
+        far[s, :-(-n // 16)] = bt[s, :-(-n // 16)]
+    far[0, 30:] = -7
+    assert torch.equal(a.prefill(q, kc, vc, far, cl, starts), want)
+    one = attn(8, 2, 128).prefill(q, kc, vc, bt, torch.tensor([10 ** 9, 100], dtype=torch.int32, device="cuda"), starts)
+    full = attn(8, 2, 128).prefill(q, kc, vc, bt, torch.tensor([bt.shape[1] * 16, 100], dtype=torch.int32, device="cuda"), starts)
+    assert torch.equal(one, full)
+
+
+def test_chunks_nan_of_a_query_or_key_reaches_the_rows_that_see_it():
+    q, kc, vc, bt, cl, starts = make([300], [300], 4, 2, 128, 16, torch.float16, seed=8)
+    q[7, 1, 5] = math.nan
+    out = attn(4, 2, 128).prefill(q, kc, vc, bt, cl, starts)
+    assert bool(out[7, 1].isnan().all()) and int(out.isnan().any(-1).sum()) == 1
+    q[7, 1, 5] = 0
+    kc[bt[0, 6].long(), 4, 0, 9] = math.nan      # key 100 of KV head 0: query heads 0 and 1 from token 100 on
+    out = attn(4, 2, 128).prefill(q, kc, vc, bt, cl, starts)
+    assert bool(out[100:, :2].isnan().all()) and bool(out[:100].isfinite().all()) and bool(out[:, 2:].isfinite().all())
+
+
+def test_chunks_many_sequences_and_repeatability():
+    g = torch.Generator().manual_seed(2)
+    new = torch.randint(0, 4, (2300,), generator=g).tolist()      # more than one launch takes
+    lens = [n + int(x) for n, x in zip(new, torch.randint(0, 300, (2300,), generator=g))]
+    q, kc, vc, bt, cl, starts = make(lens, new, 2, 1, 64, 16, torch.bfloat16, seed=1, stale=math.nan)
+    a = attn(2, 1, 64)
+    out = a.prefill(q, kc, vc, bt, cl, starts)
+    check(out, q, kc, vc, bt, cl, starts)
+    for _ in range(3):
+        assert torch.equal(a.prefill(q, kc, vc, bt, cl, starts), out)
+
+
+def test_chunks_past_32_bit_offsets():
+    nb = (1 << 31) // (16 * 8 * 128) + 64
+    kc, vc = (torch.zeros(nb, 16, 8, 128, dtype=torch.float16, device="cuda") for _ in range(2))
+    g = torch.Generator().manual_seed(0)
+    bt = torch.tensor([[nb - 1, 0, nb - 40], [3, nb - 2, 5]], dtype=torch.int32)
+    for b in bt.flatten().tolist():
+        kc[b] = torch.randn(16, 8, 128, generator=g).half().cuda()
+        vc[b] = torch.randn(16, 8, 128, generator=g).half().cuda()
+    q = torch.randn(50, 16, 128, generator=g).half().cuda()
+    cl, starts = torch.tensor([48, 41], dtype=torch.int32).cuda(), torch.tensor([0, 30, 50], dtype=torch.int32).cuda()
+    out = attn(16, 8, 128).prefill(q, kc, vc, bt.cuda(), cl, starts)
+    check(out, q, kc, vc, bt.cuda(), cl, starts)
+
+
+def test_chunks_graph_replay_and_streams():
+    lens, new = [700, 20, 1800], [100, 20, 130]
+    q, kc, vc, bt, cl, starts = make(lens, new, 32, 8, 128, 16, torch.float16, seed=9)
+    a = attn(32, 8, 128)
+    a.prefill(q, kc, vc, bt, cl, starts)
+    graphs = []
+    for _ in range(2):
+        o = torch.empty_like(q)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            a.prefill(q, kc, vc, bt, cl, starts, out=o)
+        graphs.append((graph, o, torch.cuda.Stream()))
+    for step in range(3):
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(step)).half())
+        cl.add_(-3)
+        want = a.prefill(q, kc, vc, bt, cl, starts)
+        for graph, o, s in graphs:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                graph.replay()
+        for graph, o, s in graphs:
+            s.synchronize()
+            assert torch.equal(o, want)
+    check(want, q, kc, vc, bt, cl, starts)
+
+
+def test_chunks_a_wait_that_runs_out_is_reported():
+    """Test hook: CTA 0 withholds the scores of key tile 1; its waits run out, the status word says so, nothing hangs, and
+    the next call is whole again."""
+    from aitherkvcache_b200 import _lib
+    q, kc, vc, bt, cl, starts = make([600], [300], 8, 2, 128, 16, torch.float16, seed=1)
+    a = attn(8, 2, 128)
+    want = a.prefill(q, kc, vc, bt, cl, starts)
+    assert _lib.device_status(reset=True)["attn_window"] == 0
+    _lib.check(_lib.lib().akv_debug_tc_withhold(3, 1), "hook")
+    try:
+        a.prefill(q, kc, vc, bt, cl, starts)
+        assert _lib.device_status(reset=True)["attn_window"] == 2
+    finally:
+        _lib.check(_lib.lib().akv_debug_tc_withhold(3, -1), "hook")
+    assert torch.equal(a.prefill(q, kc, vc, bt, cl, starts), want)
+    assert _lib.device_status()["attn_window"] == 0
