@@ -13,12 +13,17 @@
 // K, V and Q come by TMA with the 128-byte swizzle straight out of the paged tensors (a box per run of keys inside a
 // block); rows of values behind the sequence's end are zeroed in shared memory, since 0 * NaN is NaN.
 //
-// Ten warps: 0-3 softmax of half 0 and 4-7 of half 1 (thread = row), 8 issues the MMAs, 9 the copies.  The two halves
-// are in ping-pong: while one half's warps take maxima and exponentials, the tensor pipe works for the other half.  Order
-// of the MMAs: P V of half h and tile g, then S of half h and tile g + 1, then the other half.  They complete in order, so
-// "S of tile g + 1 is there" (s_full) also says that O of the half is complete up to tile g (it may be rescaled) and that
-// P's columns may be overwritten; no further barrier is needed in the loop.  The row's reference maximum moves only when a
-// score exceeds it by more than 2^8 (fp16 and bf16 hold 2^8 exactly), so O is rescaled a few times per row.
+// Ten warps: 0-3 softmax of half 0 and 4-7 of half 1 (thread = row), 8 issues the MMAs, 9 the copies.  A half's tile goes
+// through in two sub-tiles of 64 keys with a score buffer each, and the MMAs are issued in the order
+//   P V of (half 0, sub-tile u), S of (half 0, u + 2), then the same of half 1,
+// so while a softmax warp works on sub-tile u the scores of u + 1 are there already: it never waits for the tensor pipe's
+// round trip (P written -> P V and the next S: 1300 cycles and more), and the two halves' warps, two per scheduler, fill
+// each other's gaps in the exponential unit.  64-key scores cost the tensor pipe 385 cycles instead of 256 (the operands'
+// shared-memory traffic), 2485 per tile pair in all where 2048 would be the least; with whole 128-key tiles in one buffer a
+// tile pair took 4850 cycles, 2900 of each half's period waiting for that round trip.
+// MMAs complete in order, so "S of u is there" also says that P V of u - 2 is done and the buffer of P u - 2 was free.
+// The row's reference maximum moves only when a score exceeds it by more than 2^8 (fp16 and bf16 hold 2^8 exactly), so O
+// is rescaled a few times per row; that waits for P V of u - 1.
 //
 // Work split.  The (row tile, key tile) pairs of the whole call are laid end to end and cut into equal ranges, one per SM:
 // every SM finishes at the same time whatever the lengths.  Row tiles that are cut (at most two per CTA) leave float32
@@ -41,23 +46,28 @@ constexpr int DP_KT = 128;                       // keys per tile
 constexpr int DP_MAX_SEQS = 1024;                // sequences of one launch
 constexpr int DP_SNAP = 2;
 constexpr float DP_RESCALE = 8.0f;
+constexpr int DP_POLY = 4;
+template <bool B> struct DpBool { static constexpr bool value = B; };
 
 struct DpMaps { CUtensorMap q, k, v; };
 
 template <int D> struct DpL {
-  static constexpr int WARPS = 10, THREADS = 320, MMA_WARP = 8, LOAD_WARP = 9;
+  static constexpr int WARPS = 11, THREADS = 352, MMA_WARP = 8, LOAD_WARP = 9, MMA_WARP2 = 10;
   static constexpr int HALVES = D / 64;                    // 64-element columns of an operand
   static constexpr int TILE = 128 * D * 2;                 // bytes of 128 rows
   static constexpr int NB = D == 128 ? 4 : 8;              // ring slots (K and V tiles in turn)
   static constexpr int Q = 0, KV = 2 * TILE, BAR = KV + NB * TILE;
   static constexpr int PRE = BAR + 512;                    // int64 [DP_MAX_SEQS + 1]: units before a sequence
-  static constexpr int SMEM = PRE + (DP_MAX_SEQS + 1) * 8 + 1024;
+  static constexpr int SROW = 80;                          // staging of results: 64 bytes of a row, padded to other banks
+  static constexpr int STAGE = PRE + (DP_MAX_SEQS + 2) * 8;      // [8 warps][32 rows][SROW]
+  static constexpr int SMEM = STAGE + 8 * 32 * SROW + 1024;
+  static_assert(STAGE % 16 == 0, "staging");
   static constexpr int T_O = 256;                          // tensor memory: S 0, S 1 (128 columns each), O 0, O 1
   static_assert(SMEM + 512 <= 232448, "shared memory");
 };
 // barriers (bytes behind BAR)
-constexpr uint32_t P_KVFULL = 0, P_KVFREE = 64, P_QFULL = 128, P_QFREE = 144, P_SFULL = 160, P_PFULL = 176, P_OFULL = 192,
-                   P_DRAIN = 208, P_TMEM = 216, P_FAILED = 220;
+constexpr uint32_t P_KVFULL = 0, P_KVFREE = 64, P_QFULL = 128, P_QFREE = 144, P_SFULL = 160, P_PFULL = 192, P_PVDONE = 224,
+                   P_TAIL = 240, P_DRAIN = 248, P_TMEM = 264, P_FAILED = 268;
 
 // What dense_prefill_merge_kernel needs to know about the row tile whose first part CTA c wrote (parts < 2: nothing)
 struct DpDesc { int parts, slot0, row0, ntok, kvh, pad[3]; };
@@ -81,6 +91,46 @@ __device__ __forceinline__ void dp_tma3(uint32_t dst, const CUtensorMap* m, uint
 __device__ __forceinline__ uint64_t dp_desc_mn(uint32_t saddr) {
   return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ bool dp_elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+  return p != 0;
+}
+// two floats per register pair: the FMA pipe's packed instructions
+__device__ __forceinline__ uint64_t dp_pk(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void dp_upk(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t dp_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t dp_add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// 2^x of two numbers without the exponential unit: x = n + f with n the nearest integer (found by adding 1.5 * 2^23, whose
+// low bits then hold n), 2^f on [-1/2, 1/2] by the polynomial of smallest relative error (fitted by weighted least
+// squares: degree 4, 2^-18.5 with its float32 evaluation; the result is rounded to 11 bits at most), n added to the
+// exponent.  x is cut off at -126.
+__device__ __forceinline__ void dp_exp2_fma(float x0, float x1, float& y0, float& y1) {
+  const uint64_t x = dp_pk(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const uint64_t r = dp_add2(x, dp_pk(12582912.f, 12582912.f));
+  const uint64_t f = dp_fma2(dp_add2(r, dp_pk(-12582912.f, -12582912.f)), dp_pk(-1.f, -1.f), x);
+  uint64_t p = dp_fma2(dp_pk(0.009570102207362652f, 0.009570102207362652f), f, dp_pk(0.05591786280274391f, 0.05591786280274391f));
+  p = dp_fma2(p, f, dp_pk(0.240247443318367f, 0.240247443318367f));
+  p = dp_fma2(p, f, dp_pk(0.6931217908859253f, 0.6931217908859253f));
+  p = dp_fma2(p, f, dp_pk(0.9999992847442627f, 0.9999992847442627f));
+  float p0, p1, r0, r1;
+  dp_upk(p, p0, p1);
+  dp_upk(r, r0, r1);
+  y0 = __int_as_float(__float_as_int(p0) + (__float_as_int(r0) << 23));
+  y1 = __int_as_float(__float_as_int(p1) + (__float_as_int(r1) << 23));
 }
 // max(a, b, c) that keeps a NaN
 __device__ __forceinline__ float dp_max3(float a, float b, float c) {
@@ -202,7 +252,7 @@ struct DpCursor {
 };
 
 template <bool BF, int D>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(352, 1)
 dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant__ DpMaps maps, int seqs, int G, int TT, int box,
                      DpDesc* desc, float* part_ml, float* part_acc) {
   using L = DpL<D>;
@@ -213,7 +263,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
   uint8_t* base = dp_smem + (base_s - raw_s);
   const uint32_t bar_s = base_s + L::BAR, failed_s = bar_s + P_FAILED;
   int64_t* pre = reinterpret_cast<int64_t*>(base + L::PRE);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int tt2 = 2 * TT;
   __shared__ int64_t s_u[2];
   __shared__ DpPlace s_place;
@@ -223,16 +273,19 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
   if (tid == 0) {
     for (int i = 0; i < NB; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_KVFULL + 8 * i));
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_KVFREE + 8 * i));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 2;" :: "r"(bar_s + P_KVFREE + 8 * i));      // both halves
     }
     for (int i = 0; i < 2; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_QFULL + 8 * i));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_QFREE + 8 * i));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_PVDONE + 8 * i));
+    }
+    for (int i = 0; i < 4; ++i) {           // half, sub-tile
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_SFULL + 8 * i));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 4;" :: "r"(bar_s + P_PFULL + 8 * i));
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_OFULL + 8 * i));
     }
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_DRAIN));
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_TAIL));
+    for (int i = 0; i < 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_DRAIN + 8 * i));
     asm volatile("st.shared.u32 [%0], %1;" :: "r"(failed_s), "r"(0u) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -319,83 +372,90 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
   };
   auto wait_warp = [&](uint32_t bar, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait(bar, parity)); };
 
-  if (work && warp == L::MMA_WARP) {
-    // ================= MMA warp: lane 0 issues, all lanes wait (and zero the values behind a sequence's end) =================
+  if (work && (warp == L::MMA_WARP || warp == L::MMA_WARP2)) {
+    // ================= MMA warps, one per half: all lanes follow the loop, one elected lane issues =================
+    // (uniform control flow, so that an MMA's operands are computed in uniform registers: with one lane in a divergent
+    // loop the issue of a sub-tile's 12 MMAs took 1200 cycles of the 621 they need; and two warps, so that one's waits
+    // are covered by the other's MMAs)
     constexpr uint32_t TYPES = BF ? (1u << 7) | (1u << 10) : 0u;
-    constexpr uint32_t IDESC_S = (1u << 4) | TYPES | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+    constexpr uint32_t IDESC_S = (1u << 4) | TYPES | ((64u >> 3) << 17) | ((128u >> 4) << 24);
     constexpr uint32_t IDESC_O = (1u << 4) | TYPES | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
+    const int h = warp == L::MMA_WARP ? 0 : 1;
     const int withhold = blockIdx.x == 0 ? g_dense_prefill_withhold : -1;
-    const uint32_t q_s = base_s + L::Q, kv_s = base_s + L::KV;
-    int pieces[2] = {0, 0};                 // pieces begun per half (phase of q_full)
-    int steps[2] = {0, 0};                  // P V products issued per half (phase of p_full)
-    // scores of half h, key tile number g of the CTA (tile j of piece c)
-    auto issue_s = [&](const DpCursor& c, int g, int j, int h) -> bool {
-      const uint32_t slot = (uint32_t)((2 * g) % NB);
-      if (h == 0 && !wait_warp(bar_s + P_KVFULL + 8 * slot, (uint32_t)((2 * g / NB) & 1))) return false;
-      if (j == 0) {
-        if (!wait_warp(bar_s + P_QFULL + 8 * h, (uint32_t)(pieces[h] & 1))) return false;
-        ++pieces[h];
-      }
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (g == withhold) return true;
-      if (lane == 0) {
-        const uint32_t qb = q_s + (uint32_t)(h * L::TILE), kb = kv_s + slot * L::TILE;
+    const uint32_t q_s = base_s + L::Q + (uint32_t)(h * L::TILE), kv_s = base_s + L::KV;
+    const uint32_t t_s = tmem + (uint32_t)(h * 128), t_o = tmem + (uint32_t)(L::T_O + h * 128);
+    uint32_t q_phase = 0, p_phase = 0;      // parities of the next waits
+    auto full = [&](int n) -> bool { return wait_warp(bar_s + P_KVFULL + 8 * (uint32_t)(n % NB), (uint32_t)((n / NB) & 1)); };
+    auto free_bar = [&](int n) -> uint32_t { return bar_s + P_KVFREE + 8 * (uint32_t)(n % NB); };
+    // scores of sub-tile u of tile number g of the CTA; last: the piece's last tile
+    auto issue_s = [&](int g, int u, bool last) {
+      const uint32_t kb = kv_s + (uint32_t)((2 * g) % NB) * L::TILE + (uint32_t)(u * 8192);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (uint32_t)((kk >> 2) * 16384 + (kk & 3) * 32);
-          umma_f16(tmem + (uint32_t)(h * 128), umma_desc(qb + off), umma_desc(kb + off), IDESC_S, (uint32_t)(kk != 0));
-        }
-        umma_commit(bar_s + P_SFULL + 8 * h);
-        if (j == c.cnt - 1) umma_commit(bar_s + P_QFREE + 8 * h);
-        if (h == c.nq - 1) umma_commit(bar_s + P_KVFREE + 8 * slot);
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t off = (uint32_t)((kk >> 2) * 16384 + (kk & 3) * 32);
+        umma_f16(t_s + (uint32_t)(u * 64), umma_desc(q_s + off), umma_desc(kb + off), IDESC_S, (uint32_t)(kk != 0));
       }
-      __syncwarp();
-      return true;
+      umma_commit(bar_s + P_SFULL + 8 * (uint32_t)(2 * h + u));
+      if (u == 1 && last) umma_commit(bar_s + P_QFREE + 8 * h);
+      if (u == 1) umma_commit(free_bar(2 * g));
     };
-    auto issue_pv = [&](const DpCursor& c, int g, int j, int h) -> bool {
-      const uint32_t slot = (uint32_t)((2 * g + 1) % NB);
-      const uint32_t vb = kv_s + slot * L::TILE;
-      if (h == 0) {
-        if (!wait_warp(bar_s + P_KVFULL + 8 * slot, (uint32_t)(((2 * g + 1) / NB) & 1))) return false;
-        int z = c.q.total - (c.t.t0 + c.off + j) * DP_KT;      // keys of the tile inside the sequence
-        if (z < DP_KT) {
-          if (z < 0) z = 0;
-          for (int e = z * 8 + lane; e < DP_KT * 8; e += 32)
+    // O += P V of sub-tile u; first: the piece's first tile
+    auto issue_pv = [&](int g, int u, bool first) {
+      const uint32_t vb = kv_s + (uint32_t)((2 * g + 1) % NB) * L::TILE + (uint32_t)(u * 8192);
 #pragma unroll
-            for (int x = 0; x < L::HALVES; ++x)
-              asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" :: "r"(vb + (uint32_t)(x * 16384 + e * 16)), "r"(0u) : "memory");
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-        }
-      }
-      if (!wait_warp(bar_s + P_PFULL + 8 * h, (uint32_t)(steps[h] & 1))) return false;
-      ++steps[h];
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      if (lane == 0) {
-#pragma unroll
-        for (int kk = 0; kk < DP_KT / 16; ++kk)
-          umma_f16_ta(tmem + (uint32_t)(L::T_O + h * 128), tmem + (uint32_t)(h * 128 + kk * 8), dp_desc_mn(vb + (uint32_t)(kk * 2048)),
-                      IDESC_O, (uint32_t)((j | kk) != 0));
-        if (j == c.cnt - 1) umma_commit(bar_s + P_OFULL + 8 * h);
-        if (h == c.nq - 1) umma_commit(bar_s + P_KVFREE + 8 * slot);
-      }
-      __syncwarp();
-      return true;
+      for (int kk = 0; kk < 4; ++kk)
+        umma_f16_ta(t_o, t_s + (uint32_t)(u * 64 + kk * 8), dp_desc_mn(vb + (uint32_t)(kk * 2048)), IDESC_O, (u | kk) != 0 || !first ? 1u : 0u);
+      umma_commit(bar_s + P_PVDONE + 8 * h);
+      if (u == 1) umma_commit(free_bar(2 * g + 1));
+    };
+    auto q_there = [&]() -> bool {
+      const uint32_t parity = q_phase;
+      q_phase ^= 1u;
+      return wait_warp(bar_s + P_QFULL + 8 * h, parity);
     };
     DpCursor ahead = cur;                   // the piece of the next scores
-    int ja = 0;
-    bool go = issue_s(ahead, 0, 0, 0) && (ahead.nq < 2 || issue_s(ahead, 0, 0, 1));
-    bool more = true;
-    int j = 0;
+    int ja = 0, j = 0;
+    bool go = full(0), more = true;
+    if (go && h < ahead.nq) {
+      go = q_there();
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      if (go && withhold != 0 && dp_elect()) {
+        issue_s(0, 0, ahead.cnt == 1);
+        issue_s(0, 1, ahead.cnt == 1);
+      }
+      __syncwarp();
+    } else if (go && lane == 0) {
+      dp_arrive(free_bar(0));               // no rows in this half: the tile is free as far as it goes
+    }
     for (int g = 0; go; ++g) {
       if (more && ++ja >= ahead.cnt) {
         ja = 0;
         more = ahead.next(a, tt2);
       }
-#pragma unroll 1
-      for (int h = 0; h < 2 && go; ++h) {
-        if (h < cur.nq) go = issue_pv(cur, g, j, h);
-        if (go && more && h < ahead.nq) go = issue_s(ahead, g + 1, ja, h);
+      if (!full(2 * g + 1) || (more && !full(2 * g + 2))) break;
+      const bool pv = h < cur.nq, sc = more && h < ahead.nq, issue = g + 1 != withhold;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (go && pv) {
+          go = wait_warp(bar_s + P_PFULL + 8 * (uint32_t)(2 * h + u), p_phase);
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (go && dp_elect()) issue_pv(g, u, j == 0);
+          __syncwarp();
+        }
+        if (go && sc) {
+          if (u == 0 && ja == 0) {
+            go = q_there();
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          }
+          if (go && issue && dp_elect()) issue_s(g + 1, u, ja == ahead.cnt - 1);
+          __syncwarp();
+        }
+      }
+      if (!go) break;
+      if (pv) p_phase ^= 1u;
+      if (lane == 0) {
+        if (!pv) dp_arrive(free_bar(2 * g + 1));
+        if (more && !sc) dp_arrive(free_bar(2 * g + 2));
       }
       if (++j >= cur.cnt) {
         j = 0;
@@ -407,17 +467,35 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
     const int boxes = DP_KT / box;          // runs of keys inside a block
     const uint32_t box_bytes = (uint32_t)box * 128u;
     const bool mine = lane < boxes;
-    int seq = 0, pieces[2] = {0, 0};        // ring position
+    int seq = 0;                            // ring position
+    uint32_t q_used = 0, q_phase = 0;       // a bit per half: Q was loaded before; parity of its last load's barriers
     bool go = true;
-    auto fill = [&](const CUtensorMap* map, int64_t blk, int pos, int kvh) -> bool {
-      const uint32_t slot = (uint32_t)(seq % NB), bar = bar_s + P_KVFULL + 8 * slot;
+    int tails = 0;
+    // tile number seq of the ring from the maps; the last `128 - z` rows are zeroed before the tile is handed over (z < 128)
+    auto fill = [&](const CUtensorMap* map, int64_t blk, int pos, int kvh, int z) -> bool {
+      const uint32_t slot = (uint32_t)(seq % NB), full = bar_s + P_KVFULL + 8 * slot, dst = base_s + L::KV + slot * L::TILE;
       if (seq >= NB && !wait_warp(bar_s + P_KVFREE + 8 * slot, (uint32_t)((seq / NB - 1) & 1))) return false;
+      const uint32_t bar = z < DP_KT ? bar_s + P_TAIL : full;
       if (lane == 0) dp_expect(bar, L::TILE);
       __syncwarp();
       if (mine)
 #pragma unroll
-        for (int x = 0; x < L::HALVES; ++x)
-          dp_tma4(base_s + L::KV + slot * L::TILE + (uint32_t)(x * 16384) + (uint32_t)lane * box_bytes, map, bar, 64 * x, kvh, pos, (int)blk);
+        for (int x = 0; x < L::HALVES; ++x) dp_tma4(dst + (uint32_t)(x * 16384) + (uint32_t)lane * box_bytes, map, bar, 64 * x, kvh, pos, (int)blk);
+      if (z < DP_KT) {
+        const bool there = __all_sync(0xffffffffu, mbar_wait(bar, (uint32_t)(tails++ & 1)));      // also when others gave up: the copy is in flight
+        if (!there) {
+          g_dense_prefill_status = 1;
+          asm volatile("st.shared.u32 [%0], %1;" :: "r"(failed_s), "r"(1u) : "memory");
+          return false;
+        }
+        for (int e = (z < 0 ? 0 : z) * 8 + lane; e < DP_KT * 8; e += 32)
+#pragma unroll
+          for (int x = 0; x < L::HALVES; ++x)
+            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" :: "r"(dst + (uint32_t)(x * 16384 + e * 16)), "r"(0u) : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) dp_arrive(full);
+      }
       ++seq;
       return true;
     };
@@ -437,13 +515,16 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
         const int64_t blk_j = blk;
         const int pos_j = pos;
         find(j + 1);                        // in flight while the ring is waited for
-        go = fill(&maps.k, blk_j, pos_j, cur.kvh);
+        go = fill(&maps.k, blk_j, pos_j, cur.kvh, DP_KT);
         if (!go) break;
         if (j == 0) {
           for (int h = 0; h < cur.nq && go; ++h) {
-            if (pieces[h] > 0) go = wait_warp(bar_s + P_QFREE + 8 * h, (uint32_t)((pieces[h] - 1) & 1));
+            if ((q_used >> h) & 1u) {
+              go = wait_warp(bar_s + P_QFREE + 8 * h, (q_phase >> h) & 1u);
+              q_phase ^= 1u << h;
+            }
             if (!go) break;
-            ++pieces[h];
+            q_used |= 1u << h;
             if (lane == 0) {
               dp_expect(bar_s + P_QFULL + 8 * h, (uint32_t)(TT * G * D * 2));
 #pragma unroll
@@ -455,14 +536,14 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
           }
           if (!go) break;
         }
-        go = fill(&maps.v, blk_j, pos_j, cur.kvh);
+        go = fill(&maps.v, blk_j, pos_j, cur.kvh, cur.q.total - (cur.t.t0 + cur.off + j) * DP_KT);
       }
     } while (go && cur.next(a, tt2));
     // a CTA that gives up must not leave while copies into its shared memory are in flight
     if (lds_u32(failed_s) != 0u) {
       for (int q = seq - NB < 0 ? 0 : seq - NB; q < seq; ++q) mbar_wait(bar_s + P_KVFULL + 8 * (uint32_t)(q % NB), (uint32_t)((q / NB) & 1));
       for (int h = 0; h < 2; ++h)
-        if (pieces[h] > 0) mbar_wait(bar_s + P_QFULL + 8 * h, (uint32_t)((pieces[h] - 1) & 1));
+        if ((q_used >> h) & 1u) mbar_wait(bar_s + P_QFULL + 8 * h, (q_phase >> h) & 1u);
     }
   } else if (work) {
     // ================= softmax warps: half = warp / 4, thread = row =================
@@ -470,9 +551,17 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
     const int r = quad * 32 + lane;
     const uint32_t t_lane = ((uint32_t)(quad * 32)) << 16;
     const uint32_t t_s = tmem + t_lane + (uint32_t)(half * 128), t_o = tmem + t_lane + (uint32_t)(L::T_O + half * 128);
-    const int r_tok = r / G, r_head = r - r_tok * G;
+    const int r_tok = r / G;
     const float c = a.scale_log2;
-    int step = 0, piece = 0;
+    uint8_t* stage = base + L::STAGE + warp * 32 * L::SROW;
+    uint32_t rows4 = 0, heads4 = 0;      // token and head of rows 8 e + lane / 4 of the warp, a byte each
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int rr = quad * 32 + 8 * e + (lane >> 2), t = rr / G;
+      rows4 |= (uint32_t)t << (8 * e);
+      heads4 |= (uint32_t)(rr - t * G) << (8 * e);
+    }
+    int step = 0;               // sub-tiles of this half
     bool ok = true, first = true;
     do {
       if (half < cur.nq) {
@@ -482,93 +571,141 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
         const int low = live && a.window > 0 && lim > a.window ? lim - a.window : 0;
         const int lim_w = __reduce_min_sync(0xffffffffu, lim), low_w = __reduce_max_sync(0xffffffffu, low);
         float m = -CUDART_INF_F, l = 0.f;      // reference in log2 units, sum of the weights
-        for (int j = 0; j < cur.cnt; ++j) {
-          if (!wait_warp(bar_s + P_SFULL + 8 * half, (uint32_t)(step & 1))) { ok = false; break; }
+        for (int x = 0; x < 2 * cur.cnt; ++x) {
+          const int u = x & 1;
+          if (!wait_warp(bar_s + P_SFULL + 8 * (uint32_t)(2 * half + u), (uint32_t)((step >> 1) & 1))) { ok = false; break; }
           ++step;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          uint32_t v[128];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) tmem_ld32(t_s + 32 * x, *reinterpret_cast<uint32_t (*)[32]>(&v[32 * x]));
+          uint32_t v[64];
+          tmem_ld32(t_s + 64 * u, *reinterpret_cast<uint32_t (*)[32]>(&v[0]));
+          tmem_ld32(t_s + 64 * u + 32, *reinterpret_cast<uint32_t (*)[32]>(&v[32]));
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          const int key0 = (cur.t.t0 + cur.off + j) * DP_KT;
-          if (key0 + DP_KT > lim_w || key0 < low_w) {
+          const int key0 = (cur.t.t0 + cur.off) * DP_KT + 64 * x;
+          const bool masked = key0 + 64 > lim_w || key0 < low_w;
+          if (masked) {
             const int hi = lim - key0, lo = low - key0;
 #pragma unroll
-            for (int i = 0; i < 128; ++i) v[i] = i < hi && i >= lo ? v[i] : 0xff800000u;
+            for (int i = 0; i < 64; ++i) v[i] = i < hi && i >= lo ? v[i] : 0xff800000u;
           }
-          float mx = __uint_as_float(v[0]), my = __uint_as_float(v[1]);
+          float mx[4];
 #pragma unroll
-          for (int i = 2; i < 126; i += 4) {
-            mx = dp_max3(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-            my = dp_max3(my, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
-          }
-          mx = dp_max3(mx, __uint_as_float(v[126]), __uint_as_float(v[127]));
-          mx = dp_max3(mx, my, my) * c;
-          const bool grow = live && !(mx <= m + DP_RESCALE);      // also for a NaN, which then stays
+          for (int i = 0; i < 4; ++i) mx[i] = dp_max3(__uint_as_float(v[i]), __uint_as_float(v[4 + i]), __uint_as_float(v[8 + i]));
+#pragma unroll
+          for (int i = 12; i < 60; i += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = dp_max3(mx[e], __uint_as_float(v[i + e]), __uint_as_float(v[i + 4 + e]));
+          mx[0] = dp_max3(mx[0], __uint_as_float(v[60]), __uint_as_float(v[61]));
+          mx[1] = dp_max3(mx[1], __uint_as_float(v[62]), __uint_as_float(v[63]));
+          const float top = dp_max3(mx[0], mx[1], dp_max3(mx[2], mx[3], mx[3])) * c;
+          const bool grow = live && !(top <= m + DP_RESCALE);      // also for a NaN, which then stays
           if (__any_sync(0xffffffffu, grow)) {
-            const float f = grow ? dense_ex2(m - mx) : 1.0f;      // m = -inf: 0
-            if (grow) { m = mx; l *= f; }
-            if (j > 0) {
+            const float f = grow ? dense_ex2(m - top) : 1.0f;      // m = -inf: 0
+            if (grow) { m = top; l *= f; }
+            if (x > 0) {                    // O holds the products of the sub-tiles before: P V of the last one may still run
+              if (!wait_warp(bar_s + P_PVDONE + 8 * half, (uint32_t)((step - 2) & 1))) { ok = false; break; }
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-              for (int x = 0; x < D / 32; ++x) {
+              for (int y = 0; y < D / 32; ++y) {
                 uint32_t o[32];
-                tmem_ld32(t_o + 32 * x, o);
+                tmem_ld32(t_o + 32 * y, o);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                tmem_st32(t_o + 32 * x, o);
+                tmem_st32(t_o + 32 * y, o);
               }
             }
           }
           const float ref = m == -CUDART_INF_F ? 0.f : -m;
-          float l0 = 0.f, l1 = 0.f;
+          // weights, rounded once to the cache's type for the product; the sum takes them before.  One pair in DP_POLY goes
+          // through the FMA pipe: the exponential unit (8 cycles per warp and instruction) is what the softmax is bound by.
+          const uint64_t c2 = dp_pk(c, c), ref2 = dp_pk(ref, ref);
+          uint64_t sum = 0;
+          auto weights = [&](auto poly) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            uint32_t ph[16];
+            for (int y = 0; y < 2; ++y) {
+              uint32_t ph[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float p0 = dense_ex2(fmaf(__uint_as_float(v[32 * x + 2 * i]), c, ref));
-              const float p1 = dense_ex2(fmaf(__uint_as_float(v[32 * x + 2 * i + 1]), c, ref));
-              l0 += p0;
-              l1 += p1;
-              ph[i] = dense_pack<BF>(p0, p1);
+              for (int i = 0; i < 16; ++i) {
+                float x0, x1, p0, p1;
+                dp_upk(dp_fma2(dp_pk(__uint_as_float(v[32 * y + 2 * i]), __uint_as_float(v[32 * y + 2 * i + 1])), c2, ref2), x0, x1);
+                if (decltype(poly)::value && i % DP_POLY == DP_POLY - 1) {
+                  dp_exp2_fma(x0, x1, p0, p1);
+                } else {
+                  p0 = dense_ex2(x0);
+                  p1 = dense_ex2(x1);
+                }
+                sum = dp_add2(sum, dp_pk(p0, p1));
+                ph[i] = dense_pack<BF>(p0, p1);
+              }
+              tmem_st16(t_s + 64 * u + 16 * y, ph);
             }
-            tmem_st16(t_s + 16 * x, ph);
+          };
+          if (masked) weights(DpBool<false>{});      // 2^-126 instead of 0 for a masked score would be wrong
+          else weights(DpBool<true>{});
+          {
+            float l0, l1;
+            dp_upk(sum, l0, l1);
+            l += l0 + l1;
           }
-          l += l0 + l1;
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
-          if (lane == 0) dp_arrive(bar_s + P_PFULL + 8 * half);
+          if (lane == 0) dp_arrive(bar_s + P_PFULL + 8 * (uint32_t)(2 * half + u));
         }
-        if (!ok || !wait_warp(bar_s + P_OFULL + 8 * half, (uint32_t)(piece & 1))) { ok = false; break; }
-        ++piece;
+        // the last two products (the scores of the last sub-tile say that the ones before are done)
+        if (!ok || !wait_warp(bar_s + P_PVDONE + 8 * half, (uint32_t)((step - 2) & 1)) ||
+            !wait_warp(bar_s + P_PVDONE + 8 * half, (uint32_t)((step - 1) & 1))) { ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const bool whole = cur.cnt == cur.t.n;
-        const int64_t row = cur.q.q0 + tok;
         const int64_t slot = (int64_t)blockIdx.x * 2 + (first ? 0 : 1);
         const float inv = l == 0.f ? 0.f : 1.0f / l;
+        // A thread holds a row, but a store instruction should write whole pieces of few rows: 64 bytes of each of the warp's
+        // 32 rows at a time go through shared memory, four lanes then write a row's piece (thread by thread, the stores
+        // of a row tile took 10000 cycles: 32 lines per instruction).
+        const int c4 = lane & 3;
+        if (whole) {
 #pragma unroll 1
-        for (int x = 0; x < D / 32; ++x) {
-          uint32_t o[32];
-          tmem_ld32(t_o + 32 * x, o);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          if (live && whole) {
-            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.out_st + (int64_t)(cur.kvh * G + r_head) * a.out_sh + 32 * x);
-            // l == 0: no key was seen (0 * anything below would keep a NaN of a masked product)
+          for (int x = 0; x < D / 32; ++x) {
+            uint32_t o[32];
+            tmem_ld32(t_o + 32 * x, o);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t w[4];
+            for (int e = 0; e < 16; ++e)      // l == 0: no key was seen (0 times whatever is there would keep a NaN)
+              w[e] = l == 0.f ? 0u : dense_pack<BF>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(stage + lane * L::SROW + 16 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int rr = 8 * e + (lane >> 2), t = (rows4 >> (8 * e)) & 255, hd = (heads4 >> (8 * e)) & 255;
+              if (t < TT && cur.t.tok0 + half * TT + t < cur.q.qlen)
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (int64_t)(cur.q.q0 + cur.t.tok0 + half * TT + t) * a.out_st +
+                                          (int64_t)(cur.kvh * G + hd) * a.out_sh + 32 * x + 8 * c4) =
+                    *reinterpret_cast<const uint4*>(stage + rr * L::SROW + 16 * c4);
+            }
+          }
+        } else {
+          float* part = part_acc + (slot * 256 + half * 128 + quad * 32) * D;
+#pragma unroll 1
+          for (int x = 0; x < D / 32; ++x) {
+            uint32_t o[32];
+            tmem_ld32(t_o + 32 * x, o);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              __syncwarp();
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                w[e] = l == 0.f ? 0u : dense_pack<BF>(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-              dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          } else if (live) {
-            float4* dst = reinterpret_cast<float4*>(part_acc + (slot * 256 + half * 128 + r) * D + 32 * x);
+                *reinterpret_cast<uint4*>(stage + lane * L::SROW + 16 * e) = make_uint4(o[16 * y + 4 * e], o[16 * y + 4 * e + 1], o[16 * y + 4 * e + 2], o[16 * y + 4 * e + 3]);
+              __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+              for (int e = 0; e < 4; ++e) {
+                const int rr = 8 * e + (lane >> 2);
+                *reinterpret_cast<uint4*>(part + rr * D + 32 * x + 16 * y + 4 * c4) = *reinterpret_cast<const uint4*>(stage + rr * L::SROW + 16 * c4);
+              }
+            }
           }
         }
         if (live && !whole) {
@@ -602,11 +739,13 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
   __syncthreads();
   // a CTA in which a wait gave up may still have MMAs in flight: commit once more and wait (bounded) before the columns go back
   int leak = 0;
-  if (warp == L::MMA_WARP && lane == 0 && lds_u32(failed_s) != 0u) {
-    umma_commit(bar_s + P_DRAIN);
-    leak = mbar_wait(bar_s + P_DRAIN, 0u) ? 0 : 1;
+  if ((warp == L::MMA_WARP || warp == L::MMA_WARP2) && lds_u32(failed_s) != 0u && dp_elect()) {
+    const uint32_t bar = bar_s + P_DRAIN + (warp == L::MMA_WARP ? 0u : 8u);
+    umma_commit(bar);
+    leak = mbar_wait(bar, 0u) ? 0 : 1;
     if (leak) g_dense_prefill_status = 2;
   }
+  __syncwarp();
   leak = __syncthreads_or(leak);
   if (warp == L::MMA_WARP && !leak) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(tmem) : "memory");
