@@ -46,8 +46,6 @@ constexpr int DP_KT = 128;                       // keys per tile
 constexpr int DP_MAX_SEQS = 1024;                // sequences of one launch
 constexpr int DP_SNAP = 2;
 constexpr float DP_RESCALE = 8.0f;
-constexpr int DP_POLY = 4;
-template <bool B> struct DpBool { static constexpr bool value = B; };
 
 struct DpMaps { CUtensorMap q, k, v; };
 
@@ -55,8 +53,8 @@ template <int D> struct DpL {
   static constexpr int WARPS = 11, THREADS = 352, MMA_WARP = 8, LOAD_WARP = 9, MMA_WARP2 = 10;
   static constexpr int HALVES = D / 64;                    // 64-element columns of an operand
   static constexpr int TILE = 128 * D * 2;                 // bytes of 128 rows
-  static constexpr int NB = D == 128 ? 4 : 8;              // ring slots (K and V tiles in turn)
-  static constexpr int Q = 0, KV = 2 * TILE, BAR = KV + NB * TILE;
+  static constexpr int NP = D == 128 ? 2 : 4;              // ring slots of K tiles, and of V tiles
+  static constexpr int Q = 0, KV = 2 * TILE, BAR = KV + 2 * NP * TILE;      // K slot, V slot, K slot ...
   static constexpr int PRE = BAR + 512;                    // int64 [DP_MAX_SEQS + 1]: units before a sequence
   static constexpr int SROW = 80;                          // staging of results: 64 bytes of a row, padded to other banks
   static constexpr int STAGE = PRE + (DP_MAX_SEQS + 2) * 8;      // [8 warps][32 rows][SROW]
@@ -66,7 +64,7 @@ template <int D> struct DpL {
   static_assert(SMEM + 512 <= 232448, "shared memory");
 };
 // barriers (bytes behind BAR)
-constexpr uint32_t P_KVFULL = 0, P_KVFREE = 64, P_QFULL = 128, P_QFREE = 144, P_SFULL = 160, P_PFULL = 192, P_PVDONE = 224,
+constexpr uint32_t P_PAIR = 0 /* V of tile g and K of tile g + 1 are there */, P_KFREE = 32, P_VFREE = 64, P_KFIRST = 96, P_QFULL = 128, P_QFREE = 144, P_SFULL = 160, P_PFULL = 192, P_PVDONE = 224,
                    P_TAIL = 240, P_DRAIN = 248, P_TMEM = 264, P_FAILED = 268;
 
 // What dense_prefill_merge_kernel needs to know about the row tile whose first part CTA c wrote (parts < 2: nothing)
@@ -113,24 +111,6 @@ __device__ __forceinline__ uint64_t dp_add2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
-}
-// 2^x of two numbers without the exponential unit: x = n + f with n the nearest integer (found by adding 1.5 * 2^23, whose
-// low bits then hold n), 2^f on [-1/2, 1/2] by the polynomial of smallest relative error (fitted by weighted least
-// squares: degree 4, 2^-18.5 with its float32 evaluation; the result is rounded to 11 bits at most), n added to the
-// exponent.  x is cut off at -126.
-__device__ __forceinline__ void dp_exp2_fma(float x0, float x1, float& y0, float& y1) {
-  const uint64_t x = dp_pk(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-  const uint64_t r = dp_add2(x, dp_pk(12582912.f, 12582912.f));
-  const uint64_t f = dp_fma2(dp_add2(r, dp_pk(-12582912.f, -12582912.f)), dp_pk(-1.f, -1.f), x);
-  uint64_t p = dp_fma2(dp_pk(0.009570102207362652f, 0.009570102207362652f), f, dp_pk(0.05591786280274391f, 0.05591786280274391f));
-  p = dp_fma2(p, f, dp_pk(0.240247443318367f, 0.240247443318367f));
-  p = dp_fma2(p, f, dp_pk(0.6931217908859253f, 0.6931217908859253f));
-  p = dp_fma2(p, f, dp_pk(0.9999992847442627f, 0.9999992847442627f));
-  float p0, p1, r0, r1;
-  dp_upk(p, p0, p1);
-  dp_upk(r, r0, r1);
-  y0 = __int_as_float(__float_as_int(p0) + (__float_as_int(r0) << 23));
-  y1 = __int_as_float(__float_as_int(p1) + (__float_as_int(r1) << 23));
 }
 // max(a, b, c) that keeps a NaN
 __device__ __forceinline__ float dp_max3(float a, float b, float c) {
@@ -256,7 +236,7 @@ __global__ void __launch_bounds__(352, 1)
 dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant__ DpMaps maps, int seqs, int G, int TT, int box,
                      DpDesc* desc, float* part_ml, float* part_acc) {
   using L = DpL<D>;
-  constexpr int NB = L::NB;
+  constexpr int NP = L::NP;
   extern __shared__ uint8_t dp_smem[];
   const uint32_t raw_s = smem_u32(dp_smem);
   const uint32_t base_s = (raw_s + 1023u) & ~1023u;
@@ -271,10 +251,12 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (tid == 0) {
-    for (int i = 0; i < NB; ++i) {
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_KVFULL + 8 * i));
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 2;" :: "r"(bar_s + P_KVFREE + 8 * i));      // both halves
+    for (int i = 0; i < NP; ++i) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 2;" :: "r"(bar_s + P_PAIR + 8 * i));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 2;" :: "r"(bar_s + P_KFREE + 8 * i));      // both halves
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 2;" :: "r"(bar_s + P_VFREE + 8 * i));
     }
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_KFIRST));
     for (int i = 0; i < 2; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_QFULL + 8 * i));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_QFREE + 8 * i));
@@ -385,11 +367,9 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
     const uint32_t q_s = base_s + L::Q + (uint32_t)(h * L::TILE), kv_s = base_s + L::KV;
     const uint32_t t_s = tmem + (uint32_t)(h * 128), t_o = tmem + (uint32_t)(L::T_O + h * 128);
     uint32_t q_phase = 0, p_phase = 0;      // parities of the next waits
-    auto full = [&](int n) -> bool { return wait_warp(bar_s + P_KVFULL + 8 * (uint32_t)(n % NB), (uint32_t)((n / NB) & 1)); };
-    auto free_bar = [&](int n) -> uint32_t { return bar_s + P_KVFREE + 8 * (uint32_t)(n % NB); };
     // scores of sub-tile u of tile number g of the CTA; last: the piece's last tile
     auto issue_s = [&](int g, int u, bool last) {
-      const uint32_t kb = kv_s + (uint32_t)((2 * g) % NB) * L::TILE + (uint32_t)(u * 8192);
+      const uint32_t kb = kv_s + (uint32_t)(2 * (g % NP)) * L::TILE + (uint32_t)(u * 8192);
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         const uint32_t off = (uint32_t)((kk >> 2) * 16384 + (kk & 3) * 32);
@@ -397,25 +377,34 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
       }
       umma_commit(bar_s + P_SFULL + 8 * (uint32_t)(2 * h + u));
       if (u == 1 && last) umma_commit(bar_s + P_QFREE + 8 * h);
-      if (u == 1) umma_commit(free_bar(2 * g));
+      if (u == 1) umma_commit(bar_s + P_KFREE + 8 * (uint32_t)(g % NP));
     };
     // O += P V of sub-tile u; first: the piece's first tile
     auto issue_pv = [&](int g, int u, bool first) {
-      const uint32_t vb = kv_s + (uint32_t)((2 * g + 1) % NB) * L::TILE + (uint32_t)(u * 8192);
+      const uint32_t vb = kv_s + (uint32_t)(2 * (g % NP) + 1) * L::TILE + (uint32_t)(u * 8192);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
         umma_f16_ta(t_o, t_s + (uint32_t)(u * 64 + kk * 8), dp_desc_mn(vb + (uint32_t)(kk * 2048)), IDESC_O, (u | kk) != 0 || !first ? 1u : 0u);
       umma_commit(bar_s + P_PVDONE + 8 * h);
-      if (u == 1) umma_commit(free_bar(2 * g + 1));
+      if (u == 1) umma_commit(bar_s + P_VFREE + 8 * (uint32_t)(g % NP));
     };
     auto q_there = [&]() -> bool {
       const uint32_t parity = q_phase;
       q_phase ^= 1u;
       return wait_warp(bar_s + P_QFULL + 8 * h, parity);
     };
+    auto test_warp = [&](uint32_t bar, uint32_t parity) -> bool {
+      uint32_t done;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}\n"
+          : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+      return __all_sync(0xffffffffu, done != 0u);
+    };
     DpCursor ahead = cur;                   // the piece of the next scores
     int ja = 0, j = 0;
-    bool go = full(0), more = true;
+    bool go = wait_warp(bar_s + P_KFIRST, 0u), more = true, there = false;
     if (go && h < ahead.nq) {
       go = q_there();
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -425,38 +414,40 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
       }
       __syncwarp();
     } else if (go && lane == 0) {
-      dp_arrive(free_bar(0));               // no rows in this half: the tile is free as far as it goes
+      dp_arrive(bar_s + P_KFREE);           // no rows in this half: the tile is free as far as it goes
     }
     for (int g = 0; go; ++g) {
       if (more && ++ja >= ahead.cnt) {
         ja = 0;
         more = ahead.next(a, tt2);
       }
-      if (!full(2 * g + 1) || (more && !full(2 * g + 2))) break;
-      const bool pv = h < cur.nq, sc = more && h < ahead.nq, issue = g + 1 != withhold;
+      const bool pv = h < cur.nq, sc = more && h < ahead.nq, issue = sc && g + 1 != withhold;
+      // V of this tile, K of the next: tested before the previous step's last MMAs were issued, so that nothing is waited
+      // for in the regular flow (the tensor pipe's queue lasts some 350 cycles)
+      if (!there && !wait_warp(bar_s + P_PAIR + 8 * (uint32_t)(g % NP), (uint32_t)((g / NP) & 1))) break;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        if (go && pv) {
-          go = wait_warp(bar_s + P_PFULL + 8 * (uint32_t)(2 * h + u), p_phase);
+        if (pv) {
+          if (!wait_warp(bar_s + P_PFULL + 8 * (uint32_t)(2 * h + u), p_phase)) { go = false; break; }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          if (go && dp_elect()) issue_pv(g, u, j == 0);
+          if (dp_elect()) issue_pv(g, u, j == 0);
           __syncwarp();
         }
-        if (go && sc) {
-          if (u == 0 && ja == 0) {
-            go = q_there();
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          }
-          if (go && issue && dp_elect()) issue_s(g + 1, u, ja == ahead.cnt - 1);
+        if (u == 0 && sc && ja == 0) {      // a new piece's scores
+          if (!q_there()) { go = false; break; }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
+        if (u == 1) there = test_warp(bar_s + P_PAIR + 8 * (uint32_t)((g + 1) % NP), (uint32_t)(((g + 1) / NP) & 1));
+        if (issue) {
+          if (dp_elect()) issue_s(g + 1, u, ja == ahead.cnt - 1);
           __syncwarp();
         }
       }
       if (!go) break;
       if (pv) p_phase ^= 1u;
-      if (lane == 0) {
-        if (!pv) dp_arrive(free_bar(2 * g + 1));
-        if (more && !sc) dp_arrive(free_bar(2 * g + 2));
-      }
+      else if (lane == 0) dp_arrive(bar_s + P_VFREE + 8 * (uint32_t)(g % NP));
+      if (more && !sc && lane == 0) dp_arrive(bar_s + P_KFREE + 8 * (uint32_t)((g + 1) % NP));
+      __syncwarp();
       if (++j >= cur.cnt) {
         j = 0;
         if (!cur.next(a, tt2)) break;
@@ -467,22 +458,29 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
     const int boxes = DP_KT / box;          // runs of keys inside a block
     const uint32_t box_bytes = (uint32_t)box * 128u;
     const bool mine = lane < boxes;
-    int seq = 0;                            // ring position
     uint32_t q_used = 0, q_phase = 0;       // a bit per half: Q was loaded before; parity of its last load's barriers
+    int tails = 0, g = 0;                   // tiles copied
     bool go = true;
-    int tails = 0;
-    // tile number seq of the ring from the maps; the last `128 - z` rows are zeroed before the tile is handed over (z < 128)
-    auto fill = [&](const CUtensorMap* map, int64_t blk, int pos, int kvh, int z) -> bool {
-      const uint32_t slot = (uint32_t)(seq % NB), full = bar_s + P_KVFULL + 8 * slot, dst = base_s + L::KV + slot * L::TILE;
-      if (seq >= NB && !wait_warp(bar_s + P_KVFREE + 8 * slot, (uint32_t)((seq / NB - 1) & 1))) return false;
-      const uint32_t bar = z < DP_KT ? bar_s + P_TAIL : full;
+    auto copy = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar, int64_t blk, int pos, int kvh) {
       if (lane == 0) dp_expect(bar, L::TILE);
       __syncwarp();
       if (mine)
 #pragma unroll
         for (int x = 0; x < L::HALVES; ++x) dp_tma4(dst + (uint32_t)(x * 16384) + (uint32_t)lane * box_bytes, map, bar, 64 * x, kvh, pos, (int)blk);
+    };
+    // K of tile g: announced on the pair barrier of tile g - 1
+    auto fill_k = [&](int64_t blk, int pos, int kvh) -> bool {
+      if (g >= NP && !wait_warp(bar_s + P_KFREE + 8 * (uint32_t)(g % NP), (uint32_t)((g / NP - 1) & 1))) return false;
+      copy(&maps.k, base_s + L::KV + (uint32_t)(2 * (g % NP)) * L::TILE, g == 0 ? bar_s + P_KFIRST : bar_s + P_PAIR + 8 * (uint32_t)((g - 1) % NP), blk, pos, kvh);
+      return true;
+    };
+    // V of tile g; with z < 128 its last 128 - z rows are zeroed before it is handed over
+    auto fill_v = [&](int64_t blk, int pos, int kvh, int z) -> bool {
+      if (g >= NP && !wait_warp(bar_s + P_VFREE + 8 * (uint32_t)(g % NP), (uint32_t)((g / NP - 1) & 1))) return false;
+      const uint32_t full = bar_s + P_PAIR + 8 * (uint32_t)(g % NP), dst = base_s + L::KV + (uint32_t)(2 * (g % NP) + 1) * L::TILE;
+      copy(&maps.v, dst, z < DP_KT ? bar_s + P_TAIL : full, blk, pos, kvh);
       if (z < DP_KT) {
-        const bool there = __all_sync(0xffffffffu, mbar_wait(bar, (uint32_t)(tails++ & 1)));      // also when others gave up: the copy is in flight
+        const bool there = __all_sync(0xffffffffu, mbar_wait(bar_s + P_TAIL, (uint32_t)(tails++ & 1)));      // also when others gave up: the copy is in flight
         if (!there) {
           g_dense_prefill_status = 1;
           asm volatile("st.shared.u32 [%0], %1;" :: "r"(failed_s), "r"(1u) : "memory");
@@ -496,9 +494,9 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
         __syncwarp();
         if (lane == 0) dp_arrive(full);
       }
-      ++seq;
       return true;
     };
+    bool more = true;
     do {
       int64_t blk = 0;
       int pos = 0;
@@ -515,7 +513,8 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
         const int64_t blk_j = blk;
         const int pos_j = pos;
         find(j + 1);                        // in flight while the ring is waited for
-        go = fill(&maps.k, blk_j, pos_j, cur.kvh, DP_KT);
+        go = fill_k(blk_j, pos_j, cur.kvh);
+        if (!go && g > 0 && lane == 0) dp_arrive(bar_s + P_PAIR + 8 * (uint32_t)((g - 1) % NP));      // announced by V alone
         if (!go) break;
         if (j == 0) {
           for (int h = 0; h < cur.nq && go; ++h) {
@@ -536,12 +535,18 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
           }
           if (!go) break;
         }
-        go = fill(&maps.v, blk_j, pos_j, cur.kvh, cur.q.total - (cur.t.t0 + cur.off + j) * DP_KT);
+        go = fill_v(blk_j, pos_j, cur.kvh, cur.q.total - (cur.t.t0 + cur.off + j) * DP_KT);
+        ++g;
       }
-    } while (go && cur.next(a, tt2));
-    // a CTA that gives up must not leave while copies into its shared memory are in flight
+      if (go) more = cur.next(a, tt2);
+    } while (go && more);
+    if (go && lane == 0) dp_arrive(bar_s + P_PAIR + 8 * (uint32_t)((g - 1) % NP));      // no K behind the last tile
+    __syncwarp();
+    // a CTA that gives up must not leave while copies into its shared memory are in flight: their barriers once more (a V
+    // tile that is waited for on P_TAIL has been, above)
     if (lds_u32(failed_s) != 0u) {
-      for (int q = seq - NB < 0 ? 0 : seq - NB; q < seq; ++q) mbar_wait(bar_s + P_KVFULL + 8 * (uint32_t)(q % NB), (uint32_t)((q / NB) & 1));
+      mbar_wait(bar_s + P_KFIRST, 0u);
+      for (int p = g - NP < 0 ? 0 : g - NP; p < g; ++p) mbar_wait(bar_s + P_PAIR + 8 * (uint32_t)(p % NP), (uint32_t)((p / NP) & 1));
       for (int h = 0; h < 2; ++h)
         if ((q_used >> h) & 1u) mbar_wait(bar_s + P_QFULL + 8 * h, (q_phase >> h) & 1u);
     }
@@ -581,8 +586,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
           tmem_ld32(t_s + 64 * u + 32, *reinterpret_cast<uint32_t (*)[32]>(&v[32]));
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
           const int key0 = (cur.t.t0 + cur.off) * DP_KT + 64 * x;
-          const bool masked = key0 + 64 > lim_w || key0 < low_w;
-          if (masked) {
+          if (key0 + 64 > lim_w || key0 < low_w) {
             const int hi = lim - key0, lo = low - key0;
 #pragma unroll
             for (int i = 0; i < 64; ++i) v[i] = i < hi && i >= lo ? v[i] : 0xff800000u;
@@ -616,32 +620,22 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
             }
           }
           const float ref = m == -CUDART_INF_F ? 0.f : -m;
-          // weights, rounded once to the cache's type for the product; the sum takes them before.  One pair in DP_POLY goes
-          // through the FMA pipe: the exponential unit (8 cycles per warp and instruction) is what the softmax is bound by.
+          // weights, rounded once to the cache's type for the product; the sum takes them before
           const uint64_t c2 = dp_pk(c, c), ref2 = dp_pk(ref, ref);
           uint64_t sum = 0;
-          auto weights = [&](auto poly) {
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              uint32_t ph[16];
+          for (int y = 0; y < 2; ++y) {
+            uint32_t ph[16];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                float x0, x1, p0, p1;
-                dp_upk(dp_fma2(dp_pk(__uint_as_float(v[32 * y + 2 * i]), __uint_as_float(v[32 * y + 2 * i + 1])), c2, ref2), x0, x1);
-                if (decltype(poly)::value && i % DP_POLY == DP_POLY - 1) {
-                  dp_exp2_fma(x0, x1, p0, p1);
-                } else {
-                  p0 = dense_ex2(x0);
-                  p1 = dense_ex2(x1);
-                }
-                sum = dp_add2(sum, dp_pk(p0, p1));
-                ph[i] = dense_pack<BF>(p0, p1);
-              }
-              tmem_st16(t_s + 64 * u + 16 * y, ph);
+            for (int i = 0; i < 16; ++i) {
+              float x0, x1;
+              dp_upk(dp_fma2(dp_pk(__uint_as_float(v[32 * y + 2 * i]), __uint_as_float(v[32 * y + 2 * i + 1])), c2, ref2), x0, x1);
+              const float p0 = dense_ex2(x0), p1 = dense_ex2(x1);
+              sum = dp_add2(sum, dp_pk(p0, p1));
+              ph[i] = dense_pack<BF>(p0, p1);
             }
-          };
-          if (masked) weights(DpBool<false>{});      // 2^-126 instead of 0 for a masked score would be wrong
-          else weights(DpBool<true>{});
+            tmem_st16(t_s + 64 * u + 16 * y, ph);
+          }
           {
             float l0, l1;
             dp_upk(sum, l0, l1);
