@@ -119,6 +119,23 @@ __device__ __forceinline__ float dp_max3(float a, float b, float c) {
   return d;
 }
 
+// MMAs of kind::f16 with descriptors given as halves: operands that differ in the address field only share the upper
+// half, and an unrolled sequence costs one addition per operand (short code matters: the issuing warps share the
+// instruction caches with eight softmax warps in long loops).
+template <bool ACC>
+__device__ __forceinline__ void dp_mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}\n"
+      :: "r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "n"(ACC ? 1 : 0) : "memory");
+}
+__device__ __forceinline__ void dp_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 db, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}\n"
+      :: "r"(d), "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc) : "memory");
+}
+
 struct DpSeq { int q0, qlen, total; };           // first query row, new tokens, tokens
 struct DpTile { int tok0, ntok, t0, n; };        // first token and tokens of a row tile, its first key tile, key tiles
 
@@ -364,16 +381,20 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
     constexpr uint32_t IDESC_O = (1u << 4) | TYPES | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
     const int h = warp == L::MMA_WARP ? 0 : 1;
     const int withhold = blockIdx.x == 0 ? g_dense_prefill_withhold : -1;
-    const uint32_t q_s = base_s + L::Q + (uint32_t)(h * L::TILE), kv_s = base_s + L::KV;
+    // descriptors: upper halves, and lower halves of the half's Q and of the first K and V slots
+    const uint32_t k_hi = (uint32_t)(umma_desc(0u) >> 32), v_hi = (uint32_t)(dp_desc_mn(0u) >> 32);
+    const uint32_t q_d = (uint32_t)umma_desc(base_s + L::Q + (uint32_t)(h * L::TILE)), k_d = (uint32_t)umma_desc(base_s + L::KV);
+    const uint32_t v_d = (uint32_t)dp_desc_mn(base_s + L::KV + L::TILE);
     const uint32_t t_s = tmem + (uint32_t)(h * 128), t_o = tmem + (uint32_t)(L::T_O + h * 128);
     uint32_t q_phase = 0, p_phase = 0;      // parities of the next waits
     // scores of sub-tile u of tile number g of the CTA; last: the piece's last tile
     auto issue_s = [&](int g, int u, bool last) {
-      const uint32_t kb = kv_s + (uint32_t)(2 * (g % NP)) * L::TILE + (uint32_t)(u * 8192);
+      const uint32_t kd = k_d + (uint32_t)(2 * (g % NP)) * (L::TILE >> 4) + (uint32_t)(u * (8192 >> 4));
+      dp_mma_ss<false>(t_s + (uint32_t)(u * 64), q_d, kd, k_hi, IDESC_S);
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const uint32_t off = (uint32_t)((kk >> 2) * 16384 + (kk & 3) * 32);
-        umma_f16(t_s + (uint32_t)(u * 64), umma_desc(q_s + off), umma_desc(kb + off), IDESC_S, (uint32_t)(kk != 0));
+      for (int kk = 1; kk < D / 16; ++kk) {
+        const uint32_t off = (uint32_t)((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+        dp_mma_ss<true>(t_s + (uint32_t)(u * 64), q_d + off, kd + off, k_hi, IDESC_S);
       }
       umma_commit(bar_s + P_SFULL + 8 * (uint32_t)(2 * h + u));
       if (u == 1 && last) umma_commit(bar_s + P_QFREE + 8 * h);
@@ -381,10 +402,10 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
     };
     // O += P V of sub-tile u; first: the piece's first tile
     auto issue_pv = [&](int g, int u, bool first) {
-      const uint32_t vb = kv_s + (uint32_t)(2 * (g % NP) + 1) * L::TILE + (uint32_t)(u * 8192);
+      const uint32_t vd = v_d + (uint32_t)(2 * (g % NP)) * (L::TILE >> 4) + (uint32_t)(u * (8192 >> 4));
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
-        umma_f16_ta(t_o, t_s + (uint32_t)(u * 64 + kk * 8), dp_desc_mn(vb + (uint32_t)(kk * 2048)), IDESC_O, (u | kk) != 0 || !first ? 1u : 0u);
+        dp_mma_ts(t_o, t_s + (uint32_t)(u * 64 + kk * 8), vd + (uint32_t)(kk * (2048 >> 4)), v_hi, IDESC_O, (u | kk) != 0 || !first ? 1u : 0u);
       umma_commit(bar_s + P_PVDONE + 8 * h);
       if (u == 1) umma_commit(bar_s + P_VFREE + 8 * (uint32_t)(g % NP));
     };
