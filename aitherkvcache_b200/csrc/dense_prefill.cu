@@ -423,56 +423,93 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
           : "=r"(done) : "r"(bar), "r"(parity) : "memory");
       return __all_sync(0xffffffffu, done != 0u);
     };
-    DpCursor ahead = cur;                   // the piece of the next scores
-    int ja = 0, j = 0;
-    bool go = wait_warp(bar_s + P_KFIRST, 0u), more = true, there = false;
-    if (go && h < ahead.nq) {
+    bool go = wait_warp(bar_s + P_KFIRST, 0u), there = false;
+    if (go && h < cur.nq) {
       go = q_there();
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (go && withhold != 0 && dp_elect()) {
-        issue_s(0, 0, ahead.cnt == 1);
-        issue_s(0, 1, ahead.cnt == 1);
+        issue_s(0, 0, cur.cnt == 1);
+        issue_s(0, 1, cur.cnt == 1);
       }
       __syncwarp();
     } else if (go && lane == 0) {
       dp_arrive(bar_s + P_KFREE);           // no rows in this half: the tile is free as far as it goes
     }
-    for (int g = 0; go; ++g) {
-      if (more && ++ja >= ahead.cnt) {
-        ja = 0;
-        more = ahead.next(a, tt2);
-      }
-      const bool pv = h < cur.nq, sc = more && h < ahead.nq, issue = sc && g + 1 != withhold;
-      // V of this tile, K of the next: tested before the previous step's last MMAs were issued, so that nothing is waited
-      // for in the regular flow (the tensor pipe's queue lasts some 350 cycles)
-      if (!there && !wait_warp(bar_s + P_PAIR + 8 * (uint32_t)(g % NP), (uint32_t)((g / NP) & 1))) break;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (pv) {
-          if (!wait_warp(bar_s + P_PFULL + 8 * (uint32_t)(2 * h + u), p_phase)) { go = false; break; }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          if (dp_elect()) issue_pv(g, u, j == 0);
+    __syncwarp();
+    // one tile: P V of its sub-tiles, each followed by the scores of the next tile's (K of tile g + 1 in ring order).  The
+    // barrier of V of this tile and K of the next was tested before the previous tile's last MMAs were issued, so that
+    // nothing is waited for in the regular flow (the tensor pipe's queue lasts some 350 cycles).
+    auto pair_there = [&](int g) -> bool {
+      return there || wait_warp(bar_s + P_PAIR + 8 * (uint32_t)(g % NP), (uint32_t)((g / NP) & 1));
+    };
+    auto test_pair = [&](int g) { there = test_warp(bar_s + P_PAIR + 8 * (uint32_t)(g % NP), (uint32_t)((g / NP) & 1)); };
+    auto p_there = [&](int u) -> bool {
+      if (!wait_warp(bar_s + P_PFULL + 8 * (uint32_t)(2 * h + u), p_phase)) return false;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      return true;
+    };
+    int g = 0;
+    while (go) {
+      // ---- tiles of the piece that are followed by another of the same piece: the loop that counts ----
+      if (h < cur.nq) {
+        for (int j = 0; j + 1 < cur.cnt; ++j, ++g) {
+          if (!pair_there(g) || !p_there(0)) { go = false; break; }
+          if (dp_elect()) {
+            issue_pv(g, 0, j == 0);
+            if (g + 1 != withhold) issue_s(g + 1, 0, false);
+          }
           __syncwarp();
+          if (!p_there(1)) { go = false; break; }
+          test_pair(g + 1);
+          if (dp_elect()) {
+            issue_pv(g, 1, false);
+            if (g + 1 != withhold) issue_s(g + 1, 1, j + 2 == cur.cnt);
+          }
+          __syncwarp();
+          p_phase ^= 1u;
         }
-        if (u == 0 && sc && ja == 0) {      // a new piece's scores
-          if (!q_there()) { go = false; break; }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        }
-        if (u == 1) there = test_warp(bar_s + P_PAIR + 8 * (uint32_t)((g + 1) % NP), (uint32_t)(((g + 1) / NP) & 1));
-        if (issue) {
-          if (dp_elect()) issue_s(g + 1, u, ja == ahead.cnt - 1);
+      } else {                              // no rows in this half: the tiles are free as far as it goes
+        for (int j = 0; j + 1 < cur.cnt; ++j, ++g) {
+          there = false;
+          if (!pair_there(g)) { go = false; break; }
+          if (lane == 0) {
+            dp_arrive(bar_s + P_VFREE + 8 * (uint32_t)(g % NP));
+            dp_arrive(bar_s + P_KFREE + 8 * (uint32_t)((g + 1) % NP));
+          }
           __syncwarp();
         }
       }
       if (!go) break;
-      if (pv) p_phase ^= 1u;
-      else if (lane == 0) dp_arrive(bar_s + P_VFREE + 8 * (uint32_t)(g % NP));
-      if (more && !sc && lane == 0) dp_arrive(bar_s + P_KFREE + 8 * (uint32_t)((g + 1) % NP));
-      __syncwarp();
-      if (++j >= cur.cnt) {
-        j = 0;
-        if (!cur.next(a, tt2)) break;
+      // ---- the piece's last tile, with the scores of the next piece's first ----
+      DpCursor ahead = cur;
+      const bool more = ahead.next(a, tt2), pv = h < cur.nq, sc = more && h < ahead.nq;
+      if (!pair_there(g)) break;
+#pragma unroll 1
+      for (int u = 0; u < 2 && go; ++u) {
+        if (pv) {
+          go = p_there(u);
+          if (go && dp_elect()) issue_pv(g, u, cur.cnt == 1);
+          __syncwarp();
+        }
+        if (go && sc) {
+          if (u == 0) {
+            go = q_there();
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          }
+          if (go && g + 1 != withhold && dp_elect()) issue_s(g + 1, u, ahead.cnt == 1);
+          __syncwarp();
+        }
       }
+      if (!go || !more) break;
+      there = false;
+      if (pv) p_phase ^= 1u;
+      if (lane == 0) {
+        if (!pv) dp_arrive(bar_s + P_VFREE + 8 * (uint32_t)(g % NP));
+        if (!sc) dp_arrive(bar_s + P_KFREE + 8 * (uint32_t)((g + 1) % NP));
+      }
+      __syncwarp();
+      ++g;
+      cur = ahead;
     }
   } else if (work && warp == L::LOAD_WARP) {
     // ================= copies: K of a tile, (Q of a new piece,) V of the tile =================
