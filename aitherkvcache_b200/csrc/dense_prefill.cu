@@ -50,7 +50,7 @@ constexpr float DP_RESCALE = 8.0f;
 struct DpMaps { CUtensorMap q, k, v; };
 
 template <int D> struct DpL {
-  static constexpr int WARPS = 11, THREADS = 352, MMA_WARP = 8, LOAD_WARP = 9, MMA_WARP2 = 10;
+  static constexpr int WARPS = 12, THREADS = 384, MMA_WARP = 8, K_WARP = 9, MMA_WARP2 = 10, V_WARP = 11;
   static constexpr int HALVES = D / 64;                    // 64-element columns of an operand
   static constexpr int TILE = 128 * D * 2;                 // bytes of 128 rows
   static constexpr int NP = D == 128 ? 2 : 4;              // ring slots of K tiles, and of V tiles
@@ -64,7 +64,7 @@ template <int D> struct DpL {
   static_assert(SMEM + 512 <= 232448, "shared memory");
 };
 // barriers (bytes behind BAR)
-constexpr uint32_t P_PAIR = 0 /* V of tile g and K of tile g + 1 are there */, P_KFREE = 32, P_VFREE = 64, P_KFIRST = 96, P_QFULL = 128, P_QFREE = 144, P_SFULL = 160, P_PFULL = 192, P_PVDONE = 224,
+constexpr uint32_t P_PAIR = 0 /* V of tile g and K of tile g + 1 are there */, P_KFIRST = 32, P_KFREE = 64, P_VFREE = 96, P_QFULL = 128, P_QFREE = 144, P_SFULL = 160, P_PFULL = 192, P_PVDONE = 224,
                    P_TAIL = 240, P_DRAIN = 248, P_TMEM = 264, P_FAILED = 268;
 
 // What dense_prefill_merge_kernel needs to know about the row tile whose first part CTA c wrote (parts < 2: nothing)
@@ -249,7 +249,7 @@ struct DpCursor {
 };
 
 template <bool BF, int D>
-__global__ void __launch_bounds__(352, 1)
+__global__ void __launch_bounds__(384, 1)
 dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant__ DpMaps maps, int seqs, int G, int TT, int box,
                      DpDesc* desc, float* part_ml, float* part_acc) {
   using L = DpL<D>;
@@ -264,7 +264,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
   const int tt2 = 2 * TT;
   __shared__ int64_t s_u[2];
   __shared__ DpPlace s_place;
-  __shared__ int s_tiles[L::WARPS];
+  __shared__ int s_tiles[L::WARPS], s_copied[2];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (tid == 0) {
@@ -273,7 +273,6 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 2;" :: "r"(bar_s + P_KFREE + 8 * i));      // both halves
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 2;" :: "r"(bar_s + P_VFREE + 8 * i));
     }
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_KFIRST));
     for (int i = 0; i < 2; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_QFULL + 8 * i));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_QFREE + 8 * i));
@@ -284,6 +283,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 4;" :: "r"(bar_s + P_PFULL + 8 * i));
     }
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_TAIL));
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_KFIRST));
     for (int i = 0; i < 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_DRAIN + 8 * i));
     asm volatile("st.shared.u32 [%0], %1;" :: "r"(failed_s), "r"(0u) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -436,9 +436,9 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
       dp_arrive(bar_s + P_KFREE);           // no rows in this half: the tile is free as far as it goes
     }
     __syncwarp();
-    // one tile: P V of its sub-tiles, each followed by the scores of the next tile's (K of tile g + 1 in ring order).  The
-    // barrier of V of this tile and K of the next was tested before the previous tile's last MMAs were issued, so that
-    // nothing is waited for in the regular flow (the tensor pipe's queue lasts some 350 cycles).
+    // One tile: P V of its sub-tiles, each followed by the scores of the next tile's.  V of this tile and K of the next are
+    // tested for before the previous tile's last MMAs are issued, so that nothing is waited for in the regular flow (the
+    // tensor pipe's queue lasts some 350 cycles).
     auto pair_there = [&](int g) -> bool {
       return there || wait_warp(bar_s + P_PAIR + 8 * (uint32_t)(g % NP), (uint32_t)((g / NP) & 1));
     };
@@ -511,103 +511,107 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
       ++g;
       cur = ahead;
     }
-  } else if (work && warp == L::LOAD_WARP) {
-    // ================= copies: K of a tile, (Q of a new piece,) V of the tile =================
+  } else if (work && (warp == L::K_WARP || warp == L::V_WARP)) {
+    // ================= copies: one warp brings the keys (and Q), one the values =================
+    // (two warps and uniform issue: a tile of 16-key blocks is 32 copies of 2 KB, and with a lane per block, which the
+    // hardware runs through one by one, their issue alone took 3000 cycles per tile)
+    const bool of_k = warp == L::K_WARP;
     const int boxes = DP_KT / box;          // runs of keys inside a block
     const uint32_t box_bytes = (uint32_t)box * 128u;
-    const bool mine = lane < boxes;
     uint32_t q_used = 0, q_phase = 0;       // a bit per half: Q was loaded before; parity of its last load's barriers
     int tails = 0, g = 0;                   // tiles copied
     bool go = true;
-    auto copy = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar, int64_t blk, int pos, int kvh) {
-      if (lane == 0) dp_expect(bar, L::TILE);
+    // lane p's block and position hold run p of the tile
+    auto copy = [&](const CUtensorMap* map, uint32_t dst, uint32_t bar, int blk, int pos, int kvh) {
+      if (dp_elect()) dp_expect(bar, L::TILE);
       __syncwarp();
-      if (mine)
+      for (int p = 0; p < boxes; ++p) {
+        const int b = __shfl_sync(0xffffffffu, blk, p), z = __shfl_sync(0xffffffffu, pos, p);
+        if (dp_elect()) {
 #pragma unroll
-        for (int x = 0; x < L::HALVES; ++x) dp_tma4(dst + (uint32_t)(x * 16384) + (uint32_t)lane * box_bytes, map, bar, 64 * x, kvh, pos, (int)blk);
-    };
-    // K of tile g: announced on the pair barrier of tile g - 1
-    auto fill_k = [&](int64_t blk, int pos, int kvh) -> bool {
-      if (g >= NP && !wait_warp(bar_s + P_KFREE + 8 * (uint32_t)(g % NP), (uint32_t)((g / NP - 1) & 1))) return false;
-      copy(&maps.k, base_s + L::KV + (uint32_t)(2 * (g % NP)) * L::TILE, g == 0 ? bar_s + P_KFIRST : bar_s + P_PAIR + 8 * (uint32_t)((g - 1) % NP), blk, pos, kvh);
-      return true;
-    };
-    // V of tile g; with z < 128 its last 128 - z rows are zeroed before it is handed over
-    auto fill_v = [&](int64_t blk, int pos, int kvh, int z) -> bool {
-      if (g >= NP && !wait_warp(bar_s + P_VFREE + 8 * (uint32_t)(g % NP), (uint32_t)((g / NP - 1) & 1))) return false;
-      const uint32_t full = bar_s + P_PAIR + 8 * (uint32_t)(g % NP), dst = base_s + L::KV + (uint32_t)(2 * (g % NP) + 1) * L::TILE;
-      copy(&maps.v, dst, z < DP_KT ? bar_s + P_TAIL : full, blk, pos, kvh);
-      if (z < DP_KT) {
-        const bool there = __all_sync(0xffffffffu, mbar_wait(bar_s + P_TAIL, (uint32_t)(tails++ & 1)));      // also when others gave up: the copy is in flight
-        if (!there) {
-          g_dense_prefill_status = 1;
-          asm volatile("st.shared.u32 [%0], %1;" :: "r"(failed_s), "r"(1u) : "memory");
-          return false;
+          for (int x = 0; x < L::HALVES; ++x) dp_tma4(dst + (uint32_t)(x * 16384) + (uint32_t)p * box_bytes, map, bar, 64 * x, kvh, z, b);
         }
-        for (int e = (z < 0 ? 0 : z) * 8 + lane; e < DP_KT * 8; e += 32)
+        __syncwarp();
+      }
+    };
+    // Q of the halves of piece c, each as soon as the last scores of its previous one are done
+    auto load_q = [&](const DpCursor& c) -> bool {
+      for (int h = 0; h < c.nq; ++h) {
+        if ((q_used >> h) & 1u) {
+          const uint32_t parity = (q_phase >> h) & 1u;
+          if (!wait_warp(bar_s + P_QFREE + 8 * h, parity)) return false;
+          q_phase ^= 1u << h;
+        }
+        q_used |= 1u << h;
+        if (dp_elect()) {
+          dp_expect(bar_s + P_QFULL + 8 * h, (uint32_t)(TT * G * D * 2));
 #pragma unroll
           for (int x = 0; x < L::HALVES; ++x)
-            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" :: "r"(dst + (uint32_t)(x * 16384 + e * 16)), "r"(0u) : "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            dp_tma3(base_s + L::Q + (uint32_t)(h * L::TILE + x * 16384), &maps.q, bar_s + P_QFULL + 8 * h, 64 * x, c.kvh * G,
+                    c.q.q0 + c.t.tok0 + h * TT);
+        }
         __syncwarp();
-        if (lane == 0) dp_arrive(full);
       }
       return true;
     };
-    bool more = true;
     do {
-      int64_t blk = 0;
-      int pos = 0;
+      int blk = 0, pos = 0;
       auto find = [&](int j) {              // block and position of this lane's run of keys in tile j of the piece
-        if (mine && j < cur.cnt) {
+        if (lane < boxes && j < cur.cnt) {
           const int key = (cur.t.t0 + cur.off + j) * DP_KT + lane * box;
           const int b = key / a.block_size;
           pos = key - b * a.block_size;
-          blk = dense_block(a, cur.s, b);
+          blk = (int)dense_block(a, cur.s, b);
         }
       };
       find(0);
-      for (int j = 0; j < cur.cnt && go; ++j) {
-        const int64_t blk_j = blk;
-        const int pos_j = pos;
+      for (int j = 0; j < cur.cnt && go; ++j, ++g) {
+        const int blk_j = blk, pos_j = pos;
         find(j + 1);                        // in flight while the ring is waited for
-        go = fill_k(blk_j, pos_j, cur.kvh);
-        if (!go && g > 0 && lane == 0) dp_arrive(bar_s + P_PAIR + 8 * (uint32_t)((g - 1) % NP));      // announced by V alone
-        if (!go) break;
-        if (j == 0) {
-          for (int h = 0; h < cur.nq && go; ++h) {
-            if ((q_used >> h) & 1u) {
-              go = wait_warp(bar_s + P_QFREE + 8 * h, (q_phase >> h) & 1u);
-              q_phase ^= 1u << h;
+        const uint32_t slot = (uint32_t)(g % NP);
+        if (of_k) {
+          if (g >= NP) go = wait_warp(bar_s + P_KFREE + 8 * slot, (uint32_t)((g / NP - 1) & 1));
+          if (!go) break;
+          copy(&maps.k, base_s + L::KV + 2 * slot * L::TILE, g == 0 ? bar_s + P_KFIRST : bar_s + P_PAIR + 8 * (uint32_t)((g - 1) % NP), blk_j, pos_j, cur.kvh);
+          if (j == 0) go = load_q(cur);
+        } else {
+          if (g >= NP) go = wait_warp(bar_s + P_VFREE + 8 * slot, (uint32_t)((g / NP - 1) & 1));
+          if (!go) break;
+          const uint32_t full = bar_s + P_PAIR + 8 * slot, dst = base_s + L::KV + (2 * slot + 1) * L::TILE;
+          const int z = cur.q.total - (cur.t.t0 + cur.off + j) * DP_KT;      // rows inside the sequence
+          copy(&maps.v, dst, z < DP_KT ? bar_s + P_TAIL : full, blk_j, pos_j, cur.kvh);
+          if (z < DP_KT) {                  // values behind the sequence's end are zeroed before the tile is handed over
+            const bool there = __all_sync(0xffffffffu, mbar_wait(bar_s + P_TAIL, (uint32_t)(tails++ & 1)));      // also when others gave up: the copy is in flight
+            if (!there) {
+              g_dense_prefill_status = 1;
+              asm volatile("st.shared.u32 [%0], %1;" :: "r"(failed_s), "r"(1u) : "memory");
+              go = false;
+              break;
             }
-            if (!go) break;
-            q_used |= 1u << h;
-            if (lane == 0) {
-              dp_expect(bar_s + P_QFULL + 8 * h, (uint32_t)(TT * G * D * 2));
+            for (int e = (z < 0 ? 0 : z) * 8 + lane; e < DP_KT * 8; e += 32)
 #pragma unroll
               for (int x = 0; x < L::HALVES; ++x)
-                dp_tma3(base_s + L::Q + (uint32_t)(h * L::TILE + x * 16384), &maps.q, bar_s + P_QFULL + 8 * h, 64 * x, cur.kvh * G,
-                        cur.q.q0 + cur.t.tok0 + h * TT);
-            }
+                asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" :: "r"(dst + (uint32_t)(x * 16384 + e * 16)), "r"(0u) : "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
+            if (lane == 0) dp_arrive(full);
           }
-          if (!go) break;
         }
-        go = fill_v(blk_j, pos_j, cur.kvh, cur.q.total - (cur.t.t0 + cur.off + j) * DP_KT);
-        ++g;
       }
-      if (go) more = cur.next(a, tt2);
-    } while (go && more);
-    if (go && lane == 0) dp_arrive(bar_s + P_PAIR + 8 * (uint32_t)((g - 1) % NP));      // no K behind the last tile
+    } while (go && cur.next(a, tt2));
+    // A CTA must not leave while copies into its shared memory are in flight, also when it gives up: the last barriers once
+    // more.  The values are announced for tiles < gv, the keys on the barriers of tiles < gk - 1 (there are no keys behind
+    // the last tile, and a side that gave up announces nothing more): the side that is behind stands in.
+    if (lane == 0) s_copied[of_k ? 1 : 0] = g;
+    asm volatile("bar.sync 2, 64;" ::: "memory");
+    const int gv = s_copied[0], gk = s_copied[1], all = gv > gk - 1 ? gv : gk - 1;
+    if (lane == 0)
+      for (int p = of_k ? (gk > 0 ? gk - 1 : 0) : gv; p < all; ++p) dp_arrive(bar_s + P_PAIR + 8 * (uint32_t)(p % NP));
     __syncwarp();
-    // a CTA that gives up must not leave while copies into its shared memory are in flight: their barriers once more (a V
-    // tile that is waited for on P_TAIL has been, above)
-    if (lds_u32(failed_s) != 0u) {
-      mbar_wait(bar_s + P_KFIRST, 0u);
-      for (int p = g - NP < 0 ? 0 : g - NP; p < g; ++p) mbar_wait(bar_s + P_PAIR + 8 * (uint32_t)(p % NP), (uint32_t)((p / NP) & 1));
-      for (int h = 0; h < 2; ++h)
-        if ((q_used >> h) & 1u) mbar_wait(bar_s + P_QFULL + 8 * h, (q_phase >> h) & 1u);
-    }
+    if (gk > 0) mbar_wait(bar_s + P_KFIRST, 0u);
+    for (int p = all - NP < 0 ? 0 : all - NP; p < all; ++p) mbar_wait(bar_s + P_PAIR + 8 * (uint32_t)(p % NP), (uint32_t)((p / NP) & 1));
+    for (int h = 0; h < 2; ++h)
+      if ((q_used >> h) & 1u) mbar_wait(bar_s + P_QFULL + 8 * h, (q_phase >> h) & 1u);
   } else if (work) {
     // ================= softmax warps: half = warp / 4, thread = row =================
     const int half = warp >> 2, quad = warp & 3;
