@@ -30,10 +30,16 @@
 // partials in the workspace, joined by dense_prefill_merge_kernel in the order of the keys; a cut within DP_SNAP tiles of a
 // row tile's edge is moved to the edge (a partial costs about as much as two key tiles).
 //
+// Rounds.  The CTAs' ranges begin anywhere in the keys, so a KV head's keys and values are wanted at all times of its round,
+// and what does not fit into L2 comes from HBM again for every row tile: at a power limit that costs clock (131 MB of
+// keys and values ran at 1.34 GHz, 24 MB at 1.47).  So the (sequence, KV head) pairs are taken in rounds of about
+// DP_ROUND_BYTES of keys and values, each cut into ranges for all SMs.
+//
 // Every wait is bounded (umma.cuh): a wait that gives up sets g_dense_prefill_status and a flag that ends all loops.
 #include "dense_attn.cuh"
 #include "umma.cuh"
 #include <cuda.h>
+#include <math.h>
 #include <math_constants.h>
 
 namespace akv {
@@ -43,7 +49,9 @@ __device__ int g_dense_prefill_status;           // 1: a bounded wait gave up, 2
 __device__ int g_dense_prefill_withhold = -1;    // test hook: CTA 0 issues neither the score MMAs nor the commit of this tile
 
 constexpr int DP_KT = 128;                       // keys per tile
-constexpr int DP_MAX_SEQS = 1024;                // sequences of one launch
+constexpr int DP_MAX_SEQS = 512;                 // sequences of one launch
+constexpr int DP_MAX_ROUNDS = 4;
+constexpr int64_t DP_ROUND_BYTES = 68 << 20;     // keys and values of a round
 constexpr int DP_SNAP = 2;
 constexpr float DP_RESCALE = 8.0f;
 
@@ -55,9 +63,10 @@ template <int D> struct DpL {
   static constexpr int TILE = 128 * D * 2;                 // bytes of 128 rows
   static constexpr int NP = D == 128 ? 2 : 4;              // ring slots of K tiles, and of V tiles
   static constexpr int Q = 0, KV = 2 * TILE, BAR = KV + 2 * NP * TILE;      // K slot, V slot, K slot ...
-  static constexpr int PRE = BAR + 512;                    // int64 [DP_MAX_SEQS + 1]: units before a sequence
+  static constexpr int PRE = BAR + 512;                    // int64 [DP_MAX_SEQS + 1]: units before a sequence ...
+  static constexpr int PREK = PRE + (DP_MAX_SEQS + 1) * 8; // ... and keys before it
   static constexpr int SROW = 80;                          // staging of results: 64 bytes of a row, padded to other banks
-  static constexpr int STAGE = PRE + (DP_MAX_SEQS + 2) * 8;      // [8 warps][32 rows][SROW]
+  static constexpr int STAGE = PRE + (DP_MAX_SEQS + 1) * 16;     // [8 warps][32 rows][SROW]
   static constexpr int SMEM = STAGE + 8 * 32 * SROW + 1024;
   static_assert(STAGE % 16 == 0, "staging");
   static constexpr int T_O = 256;                          // tensor memory: S 0, S 1 (128 columns each), O 0, O 1
@@ -198,25 +207,29 @@ __device__ __forceinline__ DpPlace dp_locate(const DenseArgs& a, const int64_t* 
   }
 }
 
-// All lanes of a warp: first unit of CTA c of n_ctas (moved to a row tile's edge where one is near), and its place.
-__device__ __forceinline__ int64_t dp_begin(const DenseArgs& a, const int64_t* pre, int seqs, int tt2, int n_ctas, int c, int lane,
-                                            DpPlace* place) {
-  const int64_t units = pre[seqs];
-  if (c >= n_ctas) return units;
-  int64_t u = units / n_ctas * c + units % n_ctas * c / n_ctas;
+// All lanes of a warp: first unit of CTA c of the n that share units [lo, hi) (moved to a row tile's edge where one is
+// near), and its place.
+__device__ __forceinline__ int64_t dp_begin(const DenseArgs& a, const int64_t* pre, int seqs, int tt2, int64_t lo, int64_t hi, int n, int c,
+                                            int lane, DpPlace* place) {
+  const int64_t units = hi - lo;
+  if (c >= n) return hi;
+  int64_t u = lo + units / n * c + units % n * c / n;
   DpPlace p = dp_locate(a, pre, seqs, tt2, u, lane);
-  const int n = dp_tile(a, dp_seq(a, p.s), tt2, p.i).n;
+  const int m = dp_tile(a, dp_seq(a, p.s), tt2, p.i).n;
   if (p.off > 0 && p.off <= DP_SNAP) {
     u -= p.off;
     p.off = 0;
-  } else if (p.off > 0 && n - p.off <= DP_SNAP) {
-    u += n - p.off;
-    if (u >= units) return units;
+  } else if (p.off > 0 && m - p.off <= DP_SNAP) {
+    u += m - p.off;
+    if (u >= hi) return hi;
     p = dp_locate(a, pre, seqs, tt2, u, lane);
   }
   *place = p;
   return u;
 }
+
+// A round: the units [lo, hi) of consecutive (sequence, KV head) pairs, shared by n CTAs; this CTA's part [u0, u1) of it
+struct DpRound { int64_t lo, hi, u0, u1; int n; DpPlace place; };
 
 // A role's way through the CTA's range, piece by piece (a piece: consecutive key tiles of one row tile)
 struct DpCursor {
@@ -226,6 +239,8 @@ struct DpCursor {
   int off, cnt;                 // key tiles t.t0 + off .. + cnt - 1
   int64_t left;                 // units behind this piece
   int nq;                       // halves with tokens
+  int round;
+  bool first;                   // the first piece of this CTA's part of the round
 
   __device__ __forceinline__ void settle(const DenseArgs& a, int tt2, int64_t avail) {
     t = dp_tile(a, q, tt2, i);
@@ -233,9 +248,22 @@ struct DpCursor {
     left = avail - cnt;
     nq = 2 * t.ntok > tt2 ? 2 : 1;
   }
-  __device__ __forceinline__ bool next(const DenseArgs& a, int tt2) {
-    if (left <= 0) return false;
+  // the part of the next round that has one; false: there is none
+  __device__ __forceinline__ bool next_round(const DenseArgs& a, int tt2, const DpRound* rounds, int n_rounds) {
+    do {
+      if (++round >= n_rounds) return false;
+    } while (rounds[round].u1 <= rounds[round].u0);
+    const DpRound& r = rounds[round];
+    s = r.place.s; kvh = r.place.kvh; i = r.place.i; off = r.place.off;
+    q = dp_seq(a, s);
+    first = true;
+    settle(a, tt2, r.u1 - r.u0);
+    return true;
+  }
+  __device__ __forceinline__ bool next(const DenseArgs& a, int tt2, const DpRound* rounds, int n_rounds) {
+    if (left <= 0) return next_round(a, tt2, rounds, n_rounds);
     off = 0;
+    first = false;
     if (++i >= dp_tiles(q, tt2)) {
       i = 0;
       if (++kvh == a.num_kv_heads) {
@@ -251,7 +279,7 @@ struct DpCursor {
 template <bool BF, int D>
 __global__ void __launch_bounds__(384, 1)
 dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant__ DpMaps maps, int seqs, int G, int TT, int box,
-                     DpDesc* desc, float* part_ml, float* part_acc) {
+                     int max_rounds, DpDesc* desc, float* part_ml, float* part_acc) {
   using L = DpL<D>;
   constexpr int NP = L::NP;
   extern __shared__ uint8_t dp_smem[];
@@ -260,10 +288,10 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
   uint8_t* base = dp_smem + (base_s - raw_s);
   const uint32_t bar_s = base_s + L::BAR, failed_s = bar_s + P_FAILED;
   int64_t* pre = reinterpret_cast<int64_t*>(base + L::PRE);
+  int64_t* prek = reinterpret_cast<int64_t*>(base + L::PREK);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int tt2 = 2 * TT;
-  __shared__ int64_t s_u[2];
-  __shared__ DpPlace s_place;
+  __shared__ DpRound s_round[DP_MAX_ROUNDS];
   __shared__ int s_tiles[L::WARPS], s_copied[2];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -302,58 +330,84 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
     for (int i = lane; i < tiles; i += 32) n += dp_tile(a, q, tt2, i).n;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
-    if (lane == 0) pre[s + 1] = n * a.num_kv_heads;
+    if (lane == 0) {
+      pre[s + 1] = n * a.num_kv_heads;
+      prek[s + 1] = tiles == 0 ? 0 : (a.window > 0 && a.window + q.qlen < q.total ? a.window + q.qlen : q.total);
+    }
     my_tiles += tiles;
   }
   if (lane == 0) s_tiles[warp] = my_tiles;
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  if (warp == 0) {
+  if (warp < 2) {
+    int64_t* p = warp == 0 ? pre : prek;
     int64_t run = 0;
     for (int b = 0; b < seqs; b += 32) {
-      int64_t x = b + lane < seqs ? pre[b + lane + 1] : 0;
+      int64_t x = b + lane < seqs ? p[b + lane + 1] : 0;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
         if (lane >= d) x += y;
       }
       x += run;
-      if (b + lane < seqs) pre[b + lane + 1] = x;
+      if (b + lane < seqs) p[b + lane + 1] = x;
       run = __shfl_sync(0xffffffffu, x, 31);
     }
-    if (lane == 0) pre[0] = 0;
+    if (lane == 0) p[0] = 0;
   }
   __syncthreads();
   const int64_t units = pre[seqs];
-  // CTAs that share them: all, but not more than there are row tiles or groups of four key tiles
-  int n_ctas;
-  {
-    int64_t rts = 0;
-    for (int w = 0; w < L::WARPS; ++w) rts += s_tiles[w];
-    rts *= a.num_kv_heads;
-    const int64_t want = units / 4 > rts ? units / 4 : rts;
-    n_ctas = want < (int64_t)gridDim.x ? (int)want : (int)gridDim.x;
-  }
-  if (warp < 2) {
-    DpPlace p{0, 0, 0, 0};
-    const int64_t u = units > 0 ? dp_begin(a, pre, seqs, tt2, n_ctas, (int)blockIdx.x + warp, lane, &p) : 0;
-    if (lane == 0) {
-      s_u[warp] = u;
-      if (warp == 0) s_place = p;
+  // rounds: as many as it takes for a round's keys and values to stay in L2 while the CTAs walk over them
+  const int64_t kv_bytes = prek[seqs] * a.num_kv_heads * (4 * D);
+  int n_rounds = (int)((kv_bytes + DP_ROUND_BYTES - 1) / DP_ROUND_BYTES < max_rounds ? (kv_bytes + DP_ROUND_BYTES - 1) / DP_ROUND_BYTES : max_rounds);
+  if (n_rounds < 1) n_rounds = 1;
+  if (units == 0) n_rounds = 0;
+  if (warp < n_rounds) {
+    // first unit of round r: that of the first (sequence, KV head) pair with r / n_rounds of all keys before it
+    auto edge = [&](int r) -> int64_t {
+      if (r <= 0) return 0;
+      if (r >= n_rounds) return units;
+      const int64_t want = prek[seqs] * a.num_kv_heads * r / n_rounds;
+      int lo = 0, hi = seqs;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (prek[mid] * a.num_kv_heads <= want) lo = mid; else hi = mid;
+      }
+      const int64_t keys = prek[lo + 1] - prek[lo], in = want - prek[lo] * a.num_kv_heads;
+      int64_t h = keys > 0 ? (in + keys - 1) / keys : a.num_kv_heads;
+      if (h > a.num_kv_heads) h = a.num_kv_heads;
+      return pre[lo] + h * ((pre[lo + 1] - pre[lo]) / a.num_kv_heads);
+    };
+    DpRound r;
+    r.lo = edge(warp);
+    r.hi = edge(warp + 1);
+    // CTAs that share it: all, but not more than there are row tiles or groups of four key tiles
+    int64_t want = (r.hi - r.lo) / 4;
+    if (n_rounds == 1) {
+      int64_t rts = 0;
+      for (int w = 0; w < L::WARPS; ++w) rts += s_tiles[w];
+      rts *= a.num_kv_heads;
+      if (want < rts) want = rts;
+    } else if (want < 1) {
+      want = 1;
     }
+    r.n = want < (int64_t)gridDim.x ? (int)want : (int)gridDim.x;
+    r.place = DpPlace{0, 0, 0, 0};
+    r.u0 = r.u1 = r.hi;
+    if (r.hi > r.lo) {
+      DpPlace end;
+      r.u0 = dp_begin(a, pre, seqs, tt2, r.lo, r.hi, r.n, (int)blockIdx.x, lane, &r.place);
+      r.u1 = dp_begin(a, pre, seqs, tt2, r.lo, r.hi, r.n, (int)blockIdx.x + 1, lane, &end);
+    }
+    if (lane == 0) s_round[warp] = r;
   }
   __syncthreads();
-  const int64_t u0 = s_u[0], u1 = s_u[1];
   const uint32_t tmem = lds_u32(bar_s + P_TMEM);
-  const bool work = u1 > u0;
   DpCursor cur;
+  cur.round = -1;
   cur.left = 0;
-  if (work) {
-    cur.s = s_place.s; cur.kvh = s_place.kvh; cur.i = s_place.i; cur.off = s_place.off;
-    cur.q = dp_seq(a, cur.s);
-    cur.settle(a, tt2, u1 - u0);
-  }
+  const bool work = cur.next_round(a, tt2, s_round, n_rounds);
 
   auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
     uint32_t done;
@@ -482,7 +536,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
       if (!go) break;
       // ---- the piece's last tile, with the scores of the next piece's first ----
       DpCursor ahead = cur;
-      const bool more = ahead.next(a, tt2), pv = h < cur.nq, sc = more && h < ahead.nq;
+      const bool more = ahead.next(a, tt2, s_round, n_rounds), pv = h < cur.nq, sc = more && h < ahead.nq;
       if (!pair_there(g)) break;
 #pragma unroll 1
       for (int u = 0; u < 2 && go; ++u) {
@@ -598,7 +652,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
           }
         }
       }
-    } while (go && cur.next(a, tt2));
+    } while (go && cur.next(a, tt2, s_round, n_rounds));
     // A CTA must not leave while copies into its shared memory are in flight, also when it gives up: the last barriers once
     // more.  The values are announced for tiles < gv, the keys on the barriers of tiles < gk - 1 (there are no keys behind
     // the last tile, and a side that gave up announces nothing more): the side that is behind stands in.
@@ -629,7 +683,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
       heads4 |= (uint32_t)(rr - t * G) << (8 * e);
     }
     int step = 0;               // sub-tiles of this half
-    bool ok = true, first = true;
+    bool ok = true;
     do {
       if (half < cur.nq) {
         const int tok = cur.t.tok0 + half * TT + r_tok;
@@ -713,7 +767,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
             !wait_warp(bar_s + P_PVDONE + 8 * half, (uint32_t)((step - 1) & 1))) { ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const bool whole = cur.cnt == cur.t.n;
-        const int64_t slot = (int64_t)blockIdx.x * 2 + (first ? 0 : 1);
+        const int64_t slot = ((int64_t)cur.round * gridDim.x + blockIdx.x) * 2 + (cur.first ? 0 : 1);
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         // A thread holds a row, but a store instruction should write whole pieces of few rows: 64 bytes of each of the warp's
         // 32 rows at a time go through shared memory, four lanes then write a row's piece (thread by thread, the stores
@@ -743,25 +797,16 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
             }
           }
         } else {
-          float* part = part_acc + (slot * 256 + half * 128 + quad * 32) * D;
+          // float4 of 4 columns, rows fastest: a store instruction writes 512 bytes in a row
+          float4* part = reinterpret_cast<float4*>(part_acc) + slot * 64 * D + half * 128 + r;
 #pragma unroll 1
           for (int x = 0; x < D / 32; ++x) {
             uint32_t o[32];
             tmem_ld32(t_o + 32 * x, o);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              __syncwarp();
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                *reinterpret_cast<uint4*>(stage + lane * L::SROW + 16 * e) = make_uint4(o[16 * y + 4 * e], o[16 * y + 4 * e + 1], o[16 * y + 4 * e + 2], o[16 * y + 4 * e + 3]);
-              __syncwarp();
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int rr = 8 * e + (lane >> 2);
-                *reinterpret_cast<uint4*>(part + rr * D + 32 * x + 16 * y + 4 * c4) = *reinterpret_cast<const uint4*>(stage + rr * L::SROW + 16 * c4);
-              }
-            }
+            for (int e = 0; e < 8; ++e)
+              part[(8 * x + e) * 256] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
           }
         }
         if (live && !whole) {
@@ -770,25 +815,31 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       }
-      first = false;
-    } while (cur.next(a, tt2));
+    } while (cur.next(a, tt2, s_round, n_rounds));
   }
 
-  // ---- the row tile that this CTA begins and does not finish (its last piece): how many parts it has ----
-  if (warp == 0) {
+  // ---- per round, the row tile that this CTA begins and does not finish (the last of its part): how many parts it has ----
+  if (warp < max_rounds) {
     DpDesc d{0, 0, 0, 0, 0, {0, 0, 0}};
-    if (work && lds_u32(failed_s) == 0u && cur.off == 0 && cur.cnt < cur.t.n) {
-      const int64_t begin = u1 - cur.cnt, end = begin + cur.t.n;
-      int c1 = (int)blockIdx.x + 1;
-      DpPlace p;
-      while (c1 + 1 < n_ctas && dp_begin(a, pre, seqs, tt2, n_ctas, c1 + 1, lane, &p) < end) ++c1;
-      d.parts = c1 - (int)blockIdx.x + 1;
-      d.slot0 = begin == u0 ? 0 : 1;
-      d.row0 = cur.q.q0 + cur.t.tok0;
-      d.ntok = cur.t.ntok;
-      d.kvh = cur.kvh;
+    if (warp < n_rounds && s_round[warp].u1 > s_round[warp].u0 && s_round[warp].u1 < s_round[warp].hi && lds_u32(failed_s) == 0u) {
+      const DpRound& r = s_round[warp];
+      DpPlace p;                            // where the next CTA's part begins: inside a row tile, or at its edge
+      dp_begin(a, pre, seqs, tt2, r.lo, r.hi, r.n, (int)blockIdx.x + 1, lane, &p);
+      const int64_t begin = r.u1 - p.off;
+      if (p.off > 0 && begin >= r.u0) {
+        const DpSeq q = dp_seq(a, p.s);
+        const DpTile t = dp_tile(a, q, tt2, p.i);
+        int c1 = (int)blockIdx.x + 1;
+        DpPlace e;
+        while (c1 + 1 < r.n && dp_begin(a, pre, seqs, tt2, r.lo, r.hi, r.n, c1 + 1, lane, &e) < begin + t.n) ++c1;
+        d.parts = c1 - (int)blockIdx.x + 1;
+        d.slot0 = begin == r.u0 ? 0 : 1;
+        d.row0 = q.q0 + t.tok0;
+        d.ntok = t.ntok;
+        d.kvh = p.kvh;
+      }
     }
-    if (lane == 0) desc[blockIdx.x] = d;
+    if (lane == 0) desc[warp * gridDim.x + blockIdx.x] = d;
   }
 
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -808,13 +859,14 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
   }
 }
 
-// Row tiles that were cut: out = sum_p 2^(m_p - M) acc_p / sum_p 2^(m_p - M) l_p in the order of the keys.  Block (c, y):
-// rows 32 y .. + 31 of the row tile that CTA c began; a warp takes a row at a time.
+// Row tiles that were cut: out = sum_p 2^(m_p - M) acc_p / sum_p 2^(m_p - M) l_p in the order of the keys.  Block (c, y, r):
+// rows 32 y .. + 31 of the row tile that CTA c began in round r; a thread takes 4 columns of one row, neighbouring threads
+// neighbouring rows (the partials' layout).
 template <bool BF, int D>
 __global__ void __launch_bounds__(256)
 dense_prefill_merge_kernel(DenseArgs a, int G, int TT, int tail, const DpDesc* desc, const float* part_ml, const float* part_acc) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (tail >= 0) {               // rows behind the last sequence (`tail` of them in this launch) come out as zeros
+  if (tail >= 0 && blockIdx.z == 0) {      // rows behind the last sequence (`tail` of them in this launch) come out as zeros
     int64_t row = load_index(a.starts, a.qs_dtype, tail);
     if (row < 0) row = 0;
     for (row += blockIdx.y * gridDim.x + blockIdx.x; row < a.n_tokens; row += gridDim.x * gridDim.y)
@@ -822,34 +874,29 @@ dense_prefill_merge_kernel(DenseArgs a, int G, int TT, int tail, const DpDesc* d
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.out_st + (int64_t)(e / (D / 8)) * a.out_sh + e % (D / 8) * 8) =
             make_uint4(0u, 0u, 0u, 0u);
   }
-  const DpDesc d = desc[blockIdx.x];
+  const DpDesc d = desc[blockIdx.z * gridDim.x + blockIdx.x];
   if (d.parts < 2) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int PER = D / 32;
-  for (int r = blockIdx.y * 32 + warp; r < blockIdx.y * 32 + 32; r += 8) {
+  constexpr int ROWS = 256 / (D / 4);      // rows of the block at a time
+  const int c4 = threadIdx.x / ROWS;
+  for (int r = blockIdx.y * 32 + threadIdx.x % ROWS; r < blockIdx.y * 32 + 32; r += ROWS) {
     const int in_half = r & 127, t = in_half / G, tok = (r >> 7) * TT + t;
     if (t >= TT || tok >= d.ntok) continue;
-    auto at = [&](int p) -> int64_t { return ((int64_t)(blockIdx.x + p) * 2 + (p == 0 ? d.slot0 : 0)) * 256 + r; };
+    auto slot = [&](int p) -> int64_t { return ((int64_t)blockIdx.z * gridDim.x + blockIdx.x + p) * 2 + (p == 0 ? d.slot0 : 0); };
     float top = -CUDART_INF_F;
-    for (int p = lane; p < d.parts; p += 32) top = fmaxf(top, part_ml[at(p) * 2]);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    float acc[PER], sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+    for (int p = 0; p < d.parts; ++p) top = fmaxf(top, part_ml[(slot(p) * 256 + r) * 2]);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
     for (int p = 0; p < d.parts; ++p) {
-      const float mp = part_ml[at(p) * 2], f = mp == -CUDART_INF_F ? 0.f : dense_ex2(mp - top);
-      if (mp == -CUDART_INF_F) continue;      // the part saw no key of this row
-      sum += f * part_ml[at(p) * 2 + 1];
-      const float* src = part_acc + at(p) * D + lane * PER;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) acc[i] += f * src[i];
+      const float2 ml = *reinterpret_cast<const float2*>(part_ml + (slot(p) * 256 + r) * 2);
+      if (ml.x == -CUDART_INF_F) continue;      // the part saw no key of this row
+      const float f = dense_ex2(ml.x - top);
+      const float4 v = reinterpret_cast<const float4*>(part_acc)[slot(p) * 64 * D + c4 * 256 + r];
+      sum += f * ml.y;
+      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
     }
-    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (int64_t)(d.row0 + tok) * a.out_st +
-                                                (int64_t)(d.kvh * G + in_half - t * G) * a.out_sh + lane * PER);
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-#pragma unroll
-    for (int i = 0; i < PER / 2; ++i) dst[i] = dense_pack<BF>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (int64_t)(d.row0 + tok) * a.out_st + (int64_t)(d.kvh * G + in_half - t * G) * a.out_sh + 4 * c4) =
+        make_uint2(dense_pack<BF>(acc.x * inv, acc.y * inv), dense_pack<BF>(acc.z * inv, acc.w * inv));
   }
 }
 
@@ -898,15 +945,22 @@ bool dp_make_maps(const DenseArgs& a, bool bf, int G, int TT, int box, DpMaps* m
 }
 
 struct DpWorkspace { DpDesc* desc; float* ml; float* acc; };
-size_t dp_workspace(int head_dim, char* base, DpWorkspace* w) {
-  const size_t n = (size_t)sm_count();
+size_t dp_workspace(int head_dim, int rounds, char* base, DpWorkspace* w) {
+  const size_t n = (size_t)sm_count() * rounds;
   const size_t d = (n * sizeof(DpDesc) + 255) / 256 * 256, ml = n * 2 * 256 * 2 * sizeof(float), acc = n * 2 * 256 * (size_t)head_dim * sizeof(float);
   if (w != nullptr) *w = DpWorkspace{reinterpret_cast<DpDesc*>(base), reinterpret_cast<float*>(base + d), reinterpret_cast<float*>(base + d + ml)};
   return d + ml + acc;
 }
 
+// Rounds that a call may need: its keys and values are at most those of the pool, or of full block-table rows.
+int dp_rounds(int num_kv_heads, int head_dim, int64_t num_blocks, int block_size, int num_seqs, int max_blocks_per_seq) {
+  const double rows = (double)num_seqs * max_blocks_per_seq, blocks = rows < (double)num_blocks ? rows : (double)num_blocks;
+  const double n = blocks * block_size * num_kv_heads * 4.0 * head_dim / (double)DP_ROUND_BYTES;
+  return n <= 1.0 ? 1 : (n >= DP_MAX_ROUNDS ? DP_MAX_ROUNDS : (int)ceil(n));
+}
+
 template <bool BF, int D>
-int dp_launch(const DenseArgs& all, const DpMaps& maps, int G, int TT, int box, bool zero_tail, const DpWorkspace& w, cudaStream_t st) {
+int dp_launch(const DenseArgs& all, const DpMaps& maps, int G, int TT, int box, int rounds, bool zero_tail, const DpWorkspace& w, cudaStream_t st) {
   using L = DpL<D>;
   cudaError_t e = cudaFuncSetAttribute(dense_prefill_kernel<BF, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
   if (e != cudaSuccess) return fail((int)e, "dense prefill attention: smem attribute: %s", cudaGetErrorString(e));
@@ -917,13 +971,13 @@ int dp_launch(const DenseArgs& all, const DpMaps& maps, int G, int TT, int box, 
     a.starts = static_cast<const char*>(all.starts) + (size_t)s0 * (all.qs_dtype == AKV_I64 ? 8 : 4);
     a.seq_lens = static_cast<const char*>(all.seq_lens) + (size_t)s0 * (all.sl_dtype == AKV_I64 ? 8 : 4);
     a.block_tables = static_cast<const char*>(all.block_tables) + (int64_t)s0 * all.bt_stride * (all.bt_dtype == AKV_I64 ? 8 : 4);
-    dense_prefill_kernel<BF, D><<<grid, L::THREADS, L::SMEM, st>>>(a, maps, seqs, G, TT, box, w.desc, w.ml, w.acc);
+    dense_prefill_kernel<BF, D><<<grid, L::THREADS, L::SMEM, st>>>(a, maps, seqs, G, TT, box, rounds, w.desc, w.ml, w.acc);
     if (int rc = check_launch("dense_prefill_attn_kernel")) return rc;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)grid, 8);
+    cfg.gridDim = dim3((unsigned)grid, 8, (unsigned)rounds);
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cfg.attrs = &at;
@@ -950,8 +1004,10 @@ int dense_prefill_withhold(int tile) {
 
 }  // namespace akv
 
-AKV_EXPORT size_t akv_dense_prefill_attn_workspace_bytes(int head_dim) {
-  return head_dim > 0 ? akv::dp_workspace(head_dim, nullptr, nullptr) : 0;
+AKV_EXPORT size_t akv_dense_prefill_attn_workspace_bytes(int num_kv_heads, int head_dim, int64_t num_blocks, int block_size, int num_seqs,
+                                                          int max_blocks_per_seq) {
+  if (num_kv_heads <= 0 || head_dim <= 0 || num_blocks < 0 || block_size <= 0 || num_seqs < 0 || max_blocks_per_seq < 0) return 0;
+  return akv::dp_workspace(head_dim, akv::dp_rounds(num_kv_heads, head_dim, num_blocks, block_size, num_seqs, max_blocks_per_seq), nullptr, nullptr);
 }
 
 AKV_EXPORT int akv_dense_prefill_attn(const akv_dense_attn_params* p) {
@@ -965,7 +1021,8 @@ AKV_EXPORT int akv_dense_prefill_attn(const akv_dense_attn_params* p) {
     return akv::fail(AKV_ERR_UNSUPPORTED, "akv_dense_prefill_attn: head_dim %d, %d query heads per KV head, block_size %d, %d blocks per "
                      "sequence (64 or 128, at most 128, a multiple of 8, at least 1)", a.head_dim, G, a.block_size, a.max_blocks_per_seq);
   akv::DpWorkspace w;
-  const size_t need = akv::dp_workspace(a.head_dim, static_cast<char*>(p->workspace), &w);
+  const int rounds = akv::dp_rounds(a.num_kv_heads, a.head_dim, a.num_blocks, a.block_size, a.num_seqs, a.max_blocks_per_seq);
+  const size_t need = akv::dp_workspace(a.head_dim, rounds, static_cast<char*>(p->workspace), &w);
   if (!p->workspace || p->workspace_bytes < need || ((uintptr_t)p->workspace & 255))
     return akv::fail(AKV_ERR_WORKSPACE, "akv_dense_prefill_attn: workspace of %zu bytes (256-byte aligned) needed, got %zu", need, p->workspace_bytes);
   const int TT = 128 / G;
@@ -974,6 +1031,6 @@ AKV_EXPORT int akv_dense_prefill_attn(const akv_dense_attn_params* p) {
   if (!akv::dp_make_maps(a, bf, G, TT, box, &maps))
     return akv::fail(AKV_ERR_UNSUPPORTED, "akv_dense_prefill_attn: these strides cannot be described to the copy unit");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(p->stream);
-  if (a.head_dim == 128) return bf ? akv::dp_launch<true, 128>(a, maps, G, TT, box, p->zero_tail != 0, w, st) : akv::dp_launch<false, 128>(a, maps, G, TT, box, p->zero_tail != 0, w, st);
-  return bf ? akv::dp_launch<true, 64>(a, maps, G, TT, box, p->zero_tail != 0, w, st) : akv::dp_launch<false, 64>(a, maps, G, TT, box, p->zero_tail != 0, w, st);
+  if (a.head_dim == 128) return bf ? akv::dp_launch<true, 128>(a, maps, G, TT, box, rounds, p->zero_tail != 0, w, st) : akv::dp_launch<false, 128>(a, maps, G, TT, box, rounds, p->zero_tail != 0, w, st);
+  return bf ? akv::dp_launch<true, 64>(a, maps, G, TT, box, rounds, p->zero_tail != 0, w, st) : akv::dp_launch<false, 64>(a, maps, G, TT, box, rounds, p->zero_tail != 0, w, st);
 }

@@ -87,7 +87,6 @@ class DensePagedAttention:
         self.head_dim, self.num_query_heads, self.num_kv_heads = head_dim, num_query_heads, num_kv_heads
         self.scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
         self.sliding_window = int(sliding_window)
-        self._prefill_bytes = _lib.lib().akv_dense_prefill_attn_workspace_bytes(head_dim)
         self._decode_bytes = _lib.lib().akv_dense_paged_attn_workspace_bytes(num_query_heads, num_kv_heads, head_dim)
 
     @staticmethod
@@ -166,8 +165,10 @@ class DensePagedAttention:
             if zero_tail:
                 out.zero_()
             return self._prefill_by_rows(query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, out)
-        ws = torch.empty(self._prefill_bytes, dtype=torch.uint8, device=dev)
-        p.workspace, p.workspace_bytes = ws.data_ptr(), self._prefill_bytes
+        nbytes = _lib.lib().akv_dense_prefill_attn_workspace_bytes(p.num_kv_heads, p.head_dim, p.num_blocks, p.block_size, p.num_seqs,
+                                                                   p.max_blocks_per_seq)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
         p.query_start_loc, p.qs_dtype, p.zero_tail = query_start_loc.data_ptr(), qs_code, int(zero_tail)
         _lib.call(dev, "akv_dense_prefill_attn", ctypes.byref(p))
         return out

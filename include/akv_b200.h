@@ -502,7 +502,8 @@ typedef struct akv_dense_attn_params {
 } akv_dense_attn_params;
 size_t akv_dense_paged_attn_workspace_bytes(int num_q_heads, int num_kv_heads, int head_dim);
 int akv_dense_paged_attn(const akv_dense_attn_params* params);
-size_t akv_dense_prefill_attn_workspace_bytes(int head_dim);
+size_t akv_dense_prefill_attn_workspace_bytes(int num_kv_heads, int head_dim, int64_t num_blocks, int block_size, int num_seqs,
+                                              int max_blocks_per_seq);
 int akv_dense_prefill_attn(const akv_dense_attn_params* params);
 
 /* ------------------------------------------------------------------------

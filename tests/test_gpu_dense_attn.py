@@ -288,6 +288,12 @@ def test_chunks_many_sequences_and_repeatability():
         assert torch.equal(a.prefill(q, kc, vc, bt, cl, starts), out)
 
 
+def test_chunks_in_rounds():
+    """Keys and values of 245 MB: the call goes over its (sequence, KV head) pairs in rounds, every one of them cut into
+    ranges for all SMs (four rounds of three sequences: rounds begin between the KV heads of a sequence)."""
+    run_chunks([20000, 300, 25000, 14700], [70, 300, 130, 1], 16, 8, 128, 16, torch.float16, seed=12)
+
+
 def test_chunks_past_32_bit_offsets():
     nb = (1 << 31) // (16 * 8 * 128) + 64
     kc, vc = (torch.zeros(nb, 16, 8, 128, dtype=torch.float16, device="cuda") for _ in range(2))
