@@ -49,10 +49,11 @@ __device__ int g_dense_prefill_status;           // 1: a bounded wait gave up, 2
 __device__ int g_dense_prefill_withhold = -1;    // test hook: CTA 0 issues neither the score MMAs nor the commit of this tile
 
 constexpr int DP_KT = 128;                       // keys per tile
-constexpr int DP_MAX_SEQS = 512;                 // sequences of one launch
+constexpr int DP_MAX_SEQS = 384;                 // sequences of one launch
 constexpr int DP_MAX_ROUNDS = 4;
 constexpr int64_t DP_ROUND_BYTES = 68 << 20;     // keys and values of a round
 constexpr int DP_SNAP = 2;
+constexpr int DP_PIECE = 2;                      // what a row tile costs besides its key tiles, in key tiles
 constexpr float DP_RESCALE = 8.0f;
 
 struct DpMaps { CUtensorMap q, k, v; };
@@ -66,7 +67,8 @@ template <int D> struct DpL {
   static constexpr int PRE = BAR + 512;                    // int64 [DP_MAX_SEQS + 1]: units before a sequence ...
   static constexpr int PREK = PRE + (DP_MAX_SEQS + 1) * 8; // ... and keys before it
   static constexpr int SROW = 80;                          // staging of results: 64 bytes of a row, padded to other banks
-  static constexpr int STAGE = PRE + (DP_MAX_SEQS + 1) * 16;     // [8 warps][32 rows][SROW]
+  static constexpr int SEQ = PRE + (DP_MAX_SEQS + 1) * 16;       // int [DP_MAX_SEQS][3]: DpSeq of every sequence
+  static constexpr int STAGE = (SEQ + DP_MAX_SEQS * 12 + 15) / 16 * 16;     // [8 warps][32 rows][SROW]
   static constexpr int SMEM = STAGE + 8 * 32 * SROW + 1024;
   static_assert(STAGE % 16 == 0, "staging");
   static constexpr int T_O = 256;                          // tensor memory: S 0, S 1 (128 columns each), O 0, O 1
@@ -171,25 +173,36 @@ __device__ __forceinline__ DpTile dp_tile(const DenseArgs& a, const DpSeq& q, in
   return t;
 }
 
-// A place in the call's list of units: row tile (s, kvh, i) with sequence and tile, and the unit inside it.
-struct DpPlace { int s, kvh, i, off; };
+// The call's work, laid end to end: sequences, their KV heads, their row tiles; a row tile counts DP_PIECE + key tiles units.
+// A place in that list: row tile (s, kvh, i) of tile t, and the unit inside it.
+struct DpPlace { int s, kvh, i, off; DpTile t; };
+
+struct DpWork {                                  // what every role of the CTA knows about the call
+  const int64_t* pre;                            // units before a sequence
+  const DpSeq* seq;
+  int seqs, tt2, n_rounds;
+};
+
+__device__ __forceinline__ uint32_t dp_div(int64_t a, int64_t b) {      // quotients below 2^32
+  return ((a | b) >> 32) == 0 ? (uint32_t)a / (uint32_t)b : (uint32_t)(a / b);
+}
 
 // All lanes of a warp: the place of unit u, 0 <= u < pre[seqs].
-__device__ __forceinline__ DpPlace dp_locate(const DenseArgs& a, const int64_t* pre, int seqs, int tt2, int64_t u, int lane) {
+__device__ __forceinline__ DpPlace dp_locate(const DenseArgs& a, const DpWork& w, int64_t u, int lane) {
   DpPlace p;
-  int lo = 0, hi = seqs;
+  int lo = 0, hi = w.seqs;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (pre[mid] <= u) lo = mid; else hi = mid;
+    if (w.pre[mid] <= u) lo = mid; else hi = mid;
   }
   p.s = lo;
-  const int64_t per = (pre[lo + 1] - pre[lo]) / a.num_kv_heads, in = u - pre[lo];
-  p.kvh = (int)(in / per);
+  const int64_t in = u - w.pre[lo], per = dp_div(w.pre[lo + 1] - w.pre[lo], a.num_kv_heads);
+  p.kvh = (int)dp_div(in, per);
   int64_t rem = in - (int64_t)p.kvh * per;
-  const DpSeq q = dp_seq(a, lo);
-  const int tiles = dp_tiles(q, tt2);
+  const DpSeq q = w.seq[lo];
+  const int tiles = dp_tiles(q, w.tt2);
   for (int base = 0;; base += 32) {
-    const int i = base + lane, n = i < tiles ? dp_tile(a, q, tt2, i).n : 0;
+    const int i = base + lane, n = i < tiles ? DP_PIECE + dp_tile(a, q, w.tt2, i).n : 0;
     int inc = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -201,77 +214,85 @@ __device__ __forceinline__ DpPlace dp_locate(const DenseArgs& a, const int64_t* 
       const int l = hit != 0u ? __ffs(hit) - 1 : 31;
       p.i = base + l;
       p.off = (int)(rem - (__shfl_sync(0xffffffffu, inc, l) - __shfl_sync(0xffffffffu, n, l)));
+      p.t = dp_tile(a, q, w.tt2, p.i);
       return p;
     }
     rem -= __shfl_sync(0xffffffffu, inc, 31);
   }
 }
 
+// The row tile behind p's (there is one)
+__device__ __forceinline__ void dp_advance(const DenseArgs& a, const DpWork& w, DpPlace* p) {
+  p->off = 0;
+  if (++p->i >= dp_tiles(w.seq[p->s], w.tt2)) {
+    p->i = 0;
+    if (++p->kvh == a.num_kv_heads) {
+      p->kvh = 0;
+      do { ++p->s; } while (w.seq[p->s].qlen == 0);
+    }
+  }
+  p->t = dp_tile(a, w.seq[p->s], w.tt2, p->i);
+}
+
 // All lanes of a warp: first unit of CTA c of the n that share units [lo, hi) (moved to a row tile's edge where one is
-// near), and its place.
-__device__ __forceinline__ int64_t dp_begin(const DenseArgs& a, const int64_t* pre, int seqs, int tt2, int64_t lo, int64_t hi, int n, int c,
-                                            int lane, DpPlace* place) {
+// near, so that an offset inside a row tile is above DP_PIECE), and its place.
+__device__ __forceinline__ int64_t dp_begin(const DenseArgs& a, const DpWork& w, int64_t lo, int64_t hi, int n, int c, int lane, DpPlace* place) {
   const int64_t units = hi - lo;
   if (c >= n) return hi;
-  int64_t u = lo + units / n * c + units % n * c / n;
-  DpPlace p = dp_locate(a, pre, seqs, tt2, u, lane);
-  const int m = dp_tile(a, dp_seq(a, p.s), tt2, p.i).n;
-  if (p.off > 0 && p.off <= DP_SNAP) {
+  int64_t u = lo;
+  if ((units >> 32) == 0) u += (int64_t)((uint32_t)units / (uint32_t)n) * c + (uint32_t)units % (uint32_t)n * (uint32_t)c / (uint32_t)n;
+  else u += units / n * c + units % n * c / n;
+  DpPlace p = dp_locate(a, w, u, lane);
+  const int m = DP_PIECE + p.t.n;
+  if (p.off > 0 && p.off <= DP_PIECE + DP_SNAP) {
     u -= p.off;
     p.off = 0;
   } else if (p.off > 0 && m - p.off <= DP_SNAP) {
     u += m - p.off;
     if (u >= hi) return hi;
-    p = dp_locate(a, pre, seqs, tt2, u, lane);
+    dp_advance(a, w, &p);
   }
   *place = p;
   return u;
 }
 
 // A round: the units [lo, hi) of consecutive (sequence, KV head) pairs, shared by n CTAs; this CTA's part [u0, u1) of it
-struct DpRound { int64_t lo, hi, u0, u1; int n; DpPlace place; };
+// (the end: end_off units inside a row tile, 0 at an edge)
+struct DpRound { int64_t lo, hi, u0, u1; int n, end_off; DpPlace place; };
 
-// A role's way through the CTA's range, piece by piece (a piece: consecutive key tiles of one row tile)
+// A role's way through the CTA's part, piece by piece (a piece: consecutive key tiles of one row tile)
 struct DpCursor {
-  int s, kvh, i;
+  DpPlace at;
   DpSeq q;
-  DpTile t;
-  int off, cnt;                 // key tiles t.t0 + off .. + cnt - 1
+  int off, cnt;                 // key tiles at.t.t0 + off .. + cnt - 1
   int64_t left;                 // units behind this piece
   int nq;                       // halves with tokens
   int round;
   bool first;                   // the first piece of this CTA's part of the round
 
-  __device__ __forceinline__ void settle(const DenseArgs& a, int tt2, int64_t avail) {
-    t = dp_tile(a, q, tt2, i);
-    cnt = avail < t.n - off ? (int)avail : t.n - off;
-    left = avail - cnt;
-    nq = 2 * t.ntok > tt2 ? 2 : 1;
+  __device__ __forceinline__ void settle(const DpWork& w, int64_t avail) {      // avail > DP_PIECE where at.off == 0
+    q = w.seq[at.s];
+    const int m = DP_PIECE + at.t.n, end = avail < m - at.off ? at.off + (int)avail : m;
+    off = at.off > DP_PIECE ? at.off - DP_PIECE : 0;
+    cnt = end - DP_PIECE - off;
+    left = avail - (end - at.off);
+    nq = 2 * at.t.ntok > w.tt2 ? 2 : 1;
   }
   // the part of the next round that has one; false: there is none
-  __device__ __forceinline__ bool next_round(const DenseArgs& a, int tt2, const DpRound* rounds, int n_rounds) {
+  __device__ __forceinline__ bool next_round(const DpWork& w, const DpRound* rounds) {
     do {
-      if (++round >= n_rounds) return false;
+      if (++round >= w.n_rounds) return false;
     } while (rounds[round].u1 <= rounds[round].u0);
-    const DpRound& r = rounds[round];
-    s = r.place.s; kvh = r.place.kvh; i = r.place.i; off = r.place.off;
-    q = dp_seq(a, s);
+    at = rounds[round].place;
     first = true;
-    settle(a, tt2, r.u1 - r.u0);
+    settle(w, rounds[round].u1 - rounds[round].u0);
     return true;
   }
-  __device__ __forceinline__ bool next(const DenseArgs& a, int tt2, const DpRound* rounds, int n_rounds) {
-    if (left <= 0) return next_round(a, tt2, rounds, n_rounds);
-    off = 0;
+  __device__ __forceinline__ bool next(const DenseArgs& a, const DpWork& w, const DpRound* rounds) {
+    if (left <= 0) return next_round(w, rounds);
     first = false;
-    if (++i >= dp_tiles(q, tt2)) {
-      i = 0;
-      if (++kvh == a.num_kv_heads) {
-        kvh = 0;
-        do { ++s; q = dp_seq(a, s); } while (q.qlen == 0);      // left > 0: there is one with tokens
-      }
-    }
-    settle(a, tt2, left);
+    dp_advance(a, w, &at);
+    settle(w, left);
     return true;
   }
 };
@@ -321,13 +342,17 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" :: "r"(bar_s + P_TMEM) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // ---- units per sequence (a warp per sequence, lanes over its row tiles), then their prefix sums ----
+  asm volatile("griddepcontrol.wait;" ::: "memory");      // what the kernel before this one wrote is read from here on
+  // ---- the sequences, units per sequence (a warp per sequence, lanes over its row tiles), then prefix sums ----
+  DpSeq* seq = reinterpret_cast<DpSeq*>(base + L::SEQ);
+  for (int s = tid; s < seqs; s += L::THREADS) seq[s] = dp_seq(a, s);
+  __syncthreads();
   int my_tiles = 0;
   for (int s = warp; s < seqs; s += L::WARPS) {
-    const DpSeq q = dp_seq(a, s);
+    const DpSeq q = seq[s];
     const int tiles = dp_tiles(q, tt2);
     int64_t n = 0;
-    for (int i = lane; i < tiles; i += 32) n += dp_tile(a, q, tt2, i).n;
+    for (int i = lane; i < tiles; i += 32) n += DP_PIECE + dp_tile(a, q, tt2, i).n;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
     if (lane == 0) {
@@ -363,7 +388,8 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
   int n_rounds = (int)((kv_bytes + DP_ROUND_BYTES - 1) / DP_ROUND_BYTES < max_rounds ? (kv_bytes + DP_ROUND_BYTES - 1) / DP_ROUND_BYTES : max_rounds);
   if (n_rounds < 1) n_rounds = 1;
   if (units == 0) n_rounds = 0;
-  if (warp < n_rounds) {
+  const DpWork w{pre, seq, seqs, tt2, n_rounds};
+  if (warp < 2 * n_rounds) {              // two warps per round: where this CTA's part begins and where it ends
     // first unit of round r: that of the first (sequence, KV head) pair with r / n_rounds of all keys before it
     auto edge = [&](int r) -> int64_t {
       if (r <= 0) return 0;
@@ -379,35 +405,39 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
       if (h > a.num_kv_heads) h = a.num_kv_heads;
       return pre[lo] + h * ((pre[lo + 1] - pre[lo]) / a.num_kv_heads);
     };
-    DpRound r;
-    r.lo = edge(warp);
-    r.hi = edge(warp + 1);
-    // CTAs that share it: all, but not more than there are row tiles or groups of four key tiles
-    int64_t want = (r.hi - r.lo) / 4;
+    const int round = warp >> 1;
+    const int64_t lo = edge(round), hi = edge(round + 1);
+    // CTAs that share it: all, but not more than there are row tiles or groups of eight units (less is not worth a cut)
+    int64_t want = (hi - lo) >> 3;
     if (n_rounds == 1) {
       int64_t rts = 0;
-      for (int w = 0; w < L::WARPS; ++w) rts += s_tiles[w];
+      for (int x = 0; x < L::WARPS; ++x) rts += s_tiles[x];
       rts *= a.num_kv_heads;
       if (want < rts) want = rts;
     } else if (want < 1) {
       want = 1;
     }
-    r.n = want < (int64_t)gridDim.x ? (int)want : (int)gridDim.x;
-    r.place = DpPlace{0, 0, 0, 0};
-    r.u0 = r.u1 = r.hi;
-    if (r.hi > r.lo) {
-      DpPlace end;
-      r.u0 = dp_begin(a, pre, seqs, tt2, r.lo, r.hi, r.n, (int)blockIdx.x, lane, &r.place);
-      r.u1 = dp_begin(a, pre, seqs, tt2, r.lo, r.hi, r.n, (int)blockIdx.x + 1, lane, &end);
+    const int n = want < (int64_t)gridDim.x ? (int)want : (int)gridDim.x;
+    DpPlace place{0, 0, 0, 0, {0, 0, 0, 0}};
+    const int64_t u = hi > lo ? dp_begin(a, w, lo, hi, n, (int)blockIdx.x + (warp & 1), lane, &place) : hi;
+    if (lane == 0) {
+      DpRound& r = s_round[round];
+      if (warp & 1) {
+        r.u1 = u;
+        r.end_off = place.off;
+      } else {
+        r.lo = lo; r.hi = hi; r.n = n;
+        r.u0 = u;
+        r.place = place;
+      }
     }
-    if (lane == 0) s_round[warp] = r;
   }
   __syncthreads();
   const uint32_t tmem = lds_u32(bar_s + P_TMEM);
   DpCursor cur;
   cur.round = -1;
   cur.left = 0;
-  const bool work = cur.next_round(a, tt2, s_round, n_rounds);
+  const bool work = cur.next_round(w, s_round);
 
   auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
     uint32_t done;
@@ -536,7 +566,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
       if (!go) break;
       // ---- the piece's last tile, with the scores of the next piece's first ----
       DpCursor ahead = cur;
-      const bool more = ahead.next(a, tt2, s_round, n_rounds), pv = h < cur.nq, sc = more && h < ahead.nq;
+      const bool more = ahead.next(a, w, s_round), pv = h < cur.nq, sc = more && h < ahead.nq;
       if (!pair_there(g)) break;
 #pragma unroll 1
       for (int u = 0; u < 2 && go; ++u) {
@@ -601,8 +631,8 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
           dp_expect(bar_s + P_QFULL + 8 * h, (uint32_t)(TT * G * D * 2));
 #pragma unroll
           for (int x = 0; x < L::HALVES; ++x)
-            dp_tma3(base_s + L::Q + (uint32_t)(h * L::TILE + x * 16384), &maps.q, bar_s + P_QFULL + 8 * h, 64 * x, c.kvh * G,
-                    c.q.q0 + c.t.tok0 + h * TT);
+            dp_tma3(base_s + L::Q + (uint32_t)(h * L::TILE + x * 16384), &maps.q, bar_s + P_QFULL + 8 * h, 64 * x, c.at.kvh * G,
+                    c.q.q0 + c.at.t.tok0 + h * TT);
         }
         __syncwarp();
       }
@@ -612,10 +642,10 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
       int blk = 0, pos = 0;
       auto find = [&](int j) {              // block and position of this lane's run of keys in tile j of the piece
         if (lane < boxes && j < cur.cnt) {
-          const int key = (cur.t.t0 + cur.off + j) * DP_KT + lane * box;
+          const int key = (cur.at.t.t0 + cur.off + j) * DP_KT + lane * box;
           const int b = key / a.block_size;
           pos = key - b * a.block_size;
-          blk = (int)dense_block(a, cur.s, b);
+          blk = (int)dense_block(a, cur.at.s, b);
         }
       };
       find(0);
@@ -626,14 +656,14 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
         if (of_k) {
           if (g >= NP) go = wait_warp(bar_s + P_KFREE + 8 * slot, (uint32_t)((g / NP - 1) & 1));
           if (!go) break;
-          copy(&maps.k, base_s + L::KV + 2 * slot * L::TILE, g == 0 ? bar_s + P_KFIRST : bar_s + P_PAIR + 8 * (uint32_t)((g - 1) % NP), blk_j, pos_j, cur.kvh);
+          copy(&maps.k, base_s + L::KV + 2 * slot * L::TILE, g == 0 ? bar_s + P_KFIRST : bar_s + P_PAIR + 8 * (uint32_t)((g - 1) % NP), blk_j, pos_j, cur.at.kvh);
           if (j == 0) go = load_q(cur);
         } else {
           if (g >= NP) go = wait_warp(bar_s + P_VFREE + 8 * slot, (uint32_t)((g / NP - 1) & 1));
           if (!go) break;
           const uint32_t full = bar_s + P_PAIR + 8 * slot, dst = base_s + L::KV + (2 * slot + 1) * L::TILE;
-          const int z = cur.q.total - (cur.t.t0 + cur.off + j) * DP_KT;      // rows inside the sequence
-          copy(&maps.v, dst, z < DP_KT ? bar_s + P_TAIL : full, blk_j, pos_j, cur.kvh);
+          const int z = cur.q.total - (cur.at.t.t0 + cur.off + j) * DP_KT;      // rows inside the sequence
+          copy(&maps.v, dst, z < DP_KT ? bar_s + P_TAIL : full, blk_j, pos_j, cur.at.kvh);
           if (z < DP_KT) {                  // values behind the sequence's end are zeroed before the tile is handed over
             const bool there = __all_sync(0xffffffffu, mbar_wait(bar_s + P_TAIL, (uint32_t)(tails++ & 1)));      // also when others gave up: the copy is in flight
             if (!there) {
@@ -652,7 +682,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
           }
         }
       }
-    } while (go && cur.next(a, tt2, s_round, n_rounds));
+    } while (go && cur.next(a, w, s_round));
     // A CTA must not leave while copies into its shared memory are in flight, also when it gives up: the last barriers once
     // more.  The values are announced for tiles < gv, the keys on the barriers of tiles < gk - 1 (there are no keys behind
     // the last tile, and a side that gave up announces nothing more): the side that is behind stands in.
@@ -686,7 +716,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
     bool ok = true;
     do {
       if (half < cur.nq) {
-        const int tok = cur.t.tok0 + half * TT + r_tok;
+        const int tok = cur.at.t.tok0 + half * TT + r_tok;
         const bool live = r_tok < TT && tok < cur.q.qlen;
         const int lim = live ? cur.q.total - cur.q.qlen + tok + 1 : 0x7fffffff;      // keys below it; a row without a token masks nothing
         const int low = live && a.window > 0 && lim > a.window ? lim - a.window : 0;
@@ -701,7 +731,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
           tmem_ld32(t_s + 64 * u, *reinterpret_cast<uint32_t (*)[32]>(&v[0]));
           tmem_ld32(t_s + 64 * u + 32, *reinterpret_cast<uint32_t (*)[32]>(&v[32]));
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          const int key0 = (cur.t.t0 + cur.off) * DP_KT + 64 * x;
+          const int key0 = (cur.at.t.t0 + cur.off) * DP_KT + 64 * x;
           if (key0 + 64 > lim_w || key0 < low_w) {
             const int hi = lim - key0, lo = low - key0;
 #pragma unroll
@@ -766,35 +796,44 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
         if (!ok || !wait_warp(bar_s + P_PVDONE + 8 * half, (uint32_t)((step - 2) & 1)) ||
             !wait_warp(bar_s + P_PVDONE + 8 * half, (uint32_t)((step - 1) & 1))) { ok = false; break; }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const bool whole = cur.cnt == cur.t.n;
+        const bool whole = cur.cnt == cur.at.t.n;
         const int64_t slot = ((int64_t)cur.round * gridDim.x + blockIdx.x) * 2 + (cur.first ? 0 : 1);
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         // A thread holds a row, but a store instruction should write whole pieces of few rows: 64 bytes of each of the warp's
         // 32 rows at a time go through shared memory, four lanes then write a row's piece (thread by thread, the stores
         // of a row tile took 10000 cycles: 32 lines per instruction).
         const int c4 = lane & 3;
+        uint32_t alive = 0;                 // of rows 8 e + lane / 4
+        char* dst4[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int t = (rows4 >> (8 * e)) & 255, hd = (heads4 >> (8 * e)) & 255, tok_e = cur.at.t.tok0 + half * TT + t;
+          if (t < TT && tok_e < cur.q.qlen) alive |= 1u << e;
+          dst4[e] = static_cast<char*>(a.out) + 2 * ((int64_t)(cur.q.q0 + tok_e) * a.out_st + (int64_t)(cur.at.kvh * G + hd) * a.out_sh + 8 * c4);
+        }
         if (whole) {
-#pragma unroll 1
-          for (int x = 0; x < D / 32; ++x) {
-            uint32_t o[32];
-            tmem_ld32(t_o + 32 * x, o);
+          uint32_t w[D / 2];
+#pragma unroll
+          for (int x = 0; x < D / 64; ++x) {
+            uint32_t o[64];
+            tmem_ld32(t_o + 64 * x, *reinterpret_cast<uint32_t (*)[32]>(&o[0]));
+            tmem_ld32(t_o + 64 * x + 32, *reinterpret_cast<uint32_t (*)[32]>(&o[32]));
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            uint32_t w[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e)      // l == 0: no key was seen (0 times whatever is there would keep a NaN)
-              w[e] = l == 0.f ? 0u : dense_pack<BF>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+            for (int e = 0; e < 32; ++e)      // l == 0: no key was seen (0 times whatever is there would keep a NaN)
+              w[32 * x + e] = l == 0.f ? 0u : dense_pack<BF>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+          }
+#pragma unroll
+          for (int x = 0; x < D / 32; ++x) {
             __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(stage + lane * L::SROW + 16 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(stage + lane * L::SROW + 16 * e) = make_uint4(w[16 * x + 4 * e], w[16 * x + 4 * e + 1], w[16 * x + 4 * e + 2], w[16 * x + 4 * e + 3]);
             __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int rr = 8 * e + (lane >> 2), t = (rows4 >> (8 * e)) & 255, hd = (heads4 >> (8 * e)) & 255;
-              if (t < TT && cur.t.tok0 + half * TT + t < cur.q.qlen)
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (int64_t)(cur.q.q0 + cur.t.tok0 + half * TT + t) * a.out_st +
-                                          (int64_t)(cur.kvh * G + hd) * a.out_sh + 32 * x + 8 * c4) =
-                    *reinterpret_cast<const uint4*>(stage + rr * L::SROW + 16 * c4);
-            }
+            for (int e = 0; e < 4; ++e)
+              if ((alive >> e) & 1u)
+                *reinterpret_cast<uint4*>(dst4[e] + 64 * x) = *reinterpret_cast<const uint4*>(stage + (8 * e + (lane >> 2)) * L::SROW + 16 * c4);
           }
         } else {
           // float4 of 4 columns, rows fastest: a store instruction writes 512 bytes in a row
@@ -815,27 +854,24 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       }
-    } while (cur.next(a, tt2, s_round, n_rounds));
+    } while (cur.next(a, w, s_round));
   }
 
   // ---- per round, the row tile that this CTA begins and does not finish (the last of its part): how many parts it has ----
   if (warp < max_rounds) {
     DpDesc d{0, 0, 0, 0, 0, {0, 0, 0}};
-    if (warp < n_rounds && s_round[warp].u1 > s_round[warp].u0 && s_round[warp].u1 < s_round[warp].hi && lds_u32(failed_s) == 0u) {
+    if (warp < n_rounds && s_round[warp].u1 > s_round[warp].u0 && s_round[warp].end_off > 0 && lds_u32(failed_s) == 0u) {
       const DpRound& r = s_round[warp];
-      DpPlace p;                            // where the next CTA's part begins: inside a row tile, or at its edge
-      dp_begin(a, pre, seqs, tt2, r.lo, r.hi, r.n, (int)blockIdx.x + 1, lane, &p);
-      const int64_t begin = r.u1 - p.off;
-      if (p.off > 0 && begin >= r.u0) {
-        const DpSeq q = dp_seq(a, p.s);
-        const DpTile t = dp_tile(a, q, tt2, p.i);
+      const int64_t begin = r.u1 - r.end_off;
+      if (begin >= r.u0) {
+        const DpPlace p = dp_locate(a, w, begin, lane);
         int c1 = (int)blockIdx.x + 1;
         DpPlace e;
-        while (c1 + 1 < r.n && dp_begin(a, pre, seqs, tt2, r.lo, r.hi, r.n, c1 + 1, lane, &e) < begin + t.n) ++c1;
+        while (c1 + 1 < r.n && dp_begin(a, w, r.lo, r.hi, r.n, c1 + 1, lane, &e) < begin + DP_PIECE + p.t.n) ++c1;
         d.parts = c1 - (int)blockIdx.x + 1;
         d.slot0 = begin == r.u0 ? 0 : 1;
-        d.row0 = q.q0 + t.tok0;
-        d.ntok = t.ntok;
+        d.row0 = w.seq[p.s].q0 + p.t.tok0;
+        d.ntok = p.t.ntok;
         d.kvh = p.kvh;
       }
     }
@@ -971,17 +1007,24 @@ int dp_launch(const DenseArgs& all, const DpMaps& maps, int G, int TT, int box, 
     a.starts = static_cast<const char*>(all.starts) + (size_t)s0 * (all.qs_dtype == AKV_I64 ? 8 : 4);
     a.seq_lens = static_cast<const char*>(all.seq_lens) + (size_t)s0 * (all.sl_dtype == AKV_I64 ? 8 : 4);
     a.block_tables = static_cast<const char*>(all.block_tables) + (int64_t)s0 * all.bt_stride * (all.bt_dtype == AKV_I64 ? 8 : 4);
-    dense_prefill_kernel<BF, D><<<grid, L::THREADS, L::SMEM, st>>>(a, maps, seqs, G, TT, box, rounds, w.desc, w.ml, w.acc);
-    if (int rc = check_launch("dense_prefill_attn_kernel")) return rc;
+    // programmatic launches: the kernels set up (barriers, tensor memory) while the one before them ends, and wait for its
+    // end before they read anything
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)grid, 8, (unsigned)rounds);
-    cfg.blockDim = dim3(256);
     cfg.stream = st;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(L::THREADS);
+    cfg.dynamicSmemBytes = L::SMEM;
+    e = cudaLaunchKernelEx(&cfg, dense_prefill_kernel<BF, D>, a, maps, seqs, G, TT, box, rounds, w.desc, w.ml, w.acc);
+    if (e != cudaSuccess) return fail((int)e, "dense prefill attention: %s", cudaGetErrorString(e));
+    if (int rc = check_launch("dense_prefill_attn_kernel")) return rc;
+    cfg.dynamicSmemBytes = 0;
+    cfg.gridDim = dim3((unsigned)grid, 8, (unsigned)rounds);
+    cfg.blockDim = dim3(256);
     e = cudaLaunchKernelEx(&cfg, dense_prefill_merge_kernel<BF, D>, a, G, TT, zero_tail && s0 + seqs == all.num_seqs ? seqs : -1, (const DpDesc*)w.desc, (const float*)w.ml, (const float*)w.acc);
     if (e != cudaSuccess) return fail((int)e, "dense prefill merge: %s", cudaGetErrorString(e));
     if (int rc = check_launch("dense_prefill_merge_kernel")) return rc;
