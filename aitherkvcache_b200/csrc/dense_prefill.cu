@@ -52,7 +52,7 @@ constexpr int DP_KT = 128;                       // keys per tile
 constexpr int DP_MAX_SEQS = 384;                 // sequences of one launch
 constexpr int DP_MAX_ROUNDS = 4;
 constexpr int64_t DP_ROUND_BYTES = 68 << 20;     // keys and values of a round
-constexpr int DP_SNAP = 2;
+constexpr int DP_SNAP = 4;
 constexpr int DP_PIECE = 2;                      // what a row tile costs besides its key tiles, in key tiles
 constexpr float DP_RESCALE = 8.0f;
 
@@ -733,9 +733,16 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
           const int key0 = (cur.at.t.t0 + cur.off) * DP_KT + 64 * x;
           if (key0 + 64 > lim_w || key0 < low_w) {
+            // a bit per key: those below the limit and not below the window's edge (bits by constant position become predicates
+            // several at a time)
             const int hi = lim - key0, lo = low - key0;
+            const uint64_t upto = hi >= 64 ? ~0ull : (hi <= 0 ? 0ull : (1ull << hi) - 1), from = lo >= 64 ? 0ull : (lo <= 0 ? ~0ull : ~0ull << lo);
+            const uint32_t see0 = (uint32_t)(upto & from), see1 = (uint32_t)((upto & from) >> 32);
 #pragma unroll
-            for (int i = 0; i < 64; ++i) v[i] = i < hi && i >= lo ? v[i] : 0xff800000u;
+            for (int i = 0; i < 32; ++i) {
+              v[i] = (see0 & (1u << i)) != 0u ? v[i] : 0xff800000u;
+              v[32 + i] = (see1 & (1u << i)) != 0u ? v[32 + i] : 0xff800000u;
+            }
           }
           float mx[4];
 #pragma unroll
