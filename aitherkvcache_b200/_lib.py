@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -353,15 +354,61 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def call(device: torch.device, name: str, params) -> None:
-    """Call entry point ``name`` with its argument block on ``device`` and raise what it refuses."""
-    fn = getattr(lib(), name)
-    if torch.cuda.current_device() == device.index:
-        rc = fn(params)
+# ---- lean calls: an argument block packed in one go, for entry points whose calls last about as long as their launch ----
+
+_PACK_CODES = {c_int: "i", c_i64: "q", c_vp: "P", c_f: "f", C.c_size_t: "N"}
+
+
+def packer(cls):
+    """``pack(*values) -> bytes`` of a ctypes structure: all its fields in order, those of nested structures in their
+    place, pointers as integers."""
+    def codes(c):
+        for _, t in c._fields_:
+            if isinstance(t, type) and issubclass(t, C.Structure):
+                yield from codes(t)
+            else:
+                yield _PACK_CODES.get(t, "P")
+    s = struct.Struct("@" + "".join(codes(cls)))
+    pad = C.sizeof(cls) - s.size      # trailing alignment
+    if not 0 <= pad < 8:
+        raise TypeError(f"{cls.__name__} cannot be packed")
+    return s.pack if pad == 0 else lambda *v: s.pack(*v) + b"\0" * pad
+
+
+def cuda_index(*tensors) -> int:
+    """Index of the one CUDA device that the tensors (None: left out) are on."""
+    index = -1
+    for t in tensors:
+        if t is not None:
+            i = t.get_device()
+            if i != index:
+                if index >= 0 or i < 0:
+                    require_cuda(*tensors)      # raises what is wrong
+                index = i
+    return index
+
+
+_raw: dict = {}
+
+
+def call(index: int, name: str, block: bytes) -> None:
+    """Call entry point ``name`` with a packed argument block on device ``index``; raises what it refuses."""
+    fn = _raw.get(name)
+    if fn is None:
+        fn = lib()[name]      # a function object of its own, which takes the block as bytes
+        fn.restype, fn.argtypes = c_int, [C.c_char_p]
+        _raw[name] = fn
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(block)
     else:
-        with torch.cuda.device(device):
-            rc = fn(params)
-    check(rc, name)
+        with torch.cuda.device(index):
+            rc = fn(block)
+    if rc:
+        check(rc, name)
+
+
+def raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def ptr(t) -> int:

@@ -78,28 +78,39 @@ __device__ __forceinline__ void rot_cs(int64_t pos, unsigned long long step, con
   s *= a.scaling;
 }
 
-template <typename T> __device__ __forceinline__ void rot_load8(const T* p, float (&f)[8]);
-template <> __device__ __forceinline__ void rot_load8<__half>(const __half* p, float (&f)[8]) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+// eight elements as they lie in memory, and as floats
+template <typename T> struct Raw8 { uint4 w[sizeof(T) / 2]; };
+template <typename T> __device__ __forceinline__ Raw8<T> rot_load8(const T* p) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.w[i].x), "=r"(r.w[i].y), "=r"(r.w[i].z), "=r"(r.w[i].w) : "l"(reinterpret_cast<const uint4*>(p) + i));
+  return r;
+}
+template <typename T> __device__ __forceinline__ void rot_floats(const Raw8<T>& r, float (&f)[8]);
+template <> __device__ __forceinline__ void rot_floats<__half>(const Raw8<__half>& r, float (&f)[8]) {
+  const uint32_t u[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
     f[2 * i] = t.x; f[2 * i + 1] = t.y;
   }
 }
-template <> __device__ __forceinline__ void rot_load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&f)[8]) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+template <> __device__ __forceinline__ void rot_floats<__nv_bfloat16>(const Raw8<__nv_bfloat16>& r, float (&f)[8]) {
+  const uint32_t u[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     f[2 * i] = __uint_as_float(u[i] << 16);
     f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
   }
 }
-template <> __device__ __forceinline__ void rot_load8<float>(const float* p, float (&f)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+template <> __device__ __forceinline__ void rot_floats<float>(const Raw8<float>& r, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    f[4 * i] = __uint_as_float(r.w[i].x); f[4 * i + 1] = __uint_as_float(r.w[i].y);
+    f[4 * i + 2] = __uint_as_float(r.w[i].z); f[4 * i + 3] = __uint_as_float(r.w[i].w);
+  }
 }
 template <typename T> __device__ __forceinline__ void rot_store8(T* p, const float (&f)[8]);
 template <> __device__ __forceinline__ void rot_store8<__half>(__half* p, const float (&f)[8]) {
@@ -169,6 +180,21 @@ rotary_rows_kernel(RotArgs a) {
   // element offsets of the thread's two groups of eight
   const int e0 = turned ? (a.adjacent ? 16 * u : 8 * u) : 16 * u;
   const int e1 = turned && !a.adjacent ? half + 8 * u : e0 + 8;
+  // the first batch of loads is on its way while the angles are worked out
+  constexpr int B = sizeof(TI) == 4 ? 2 : 4;
+  Raw8<TI> r0[B], r1[B];
+  auto load = [&](int h) {
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const TI* src;
+      TO* dst;
+      if (h + b * a.head_slices < a.heads && rot_row<TI, TO>(a, t, h + b * a.head_slices, blk, in_blk, src, dst)) {
+        r0[b] = rot_load8<TI>(src + e0);
+        r1[b] = rot_load8<TI>(src + e1);
+      }
+    }
+  };
+  load(h0);
   float c[8], s[8];
   if (turned && h0 < a.qh + a.kh) {
     int64_t pos[ROT_MAX_AXES];
@@ -185,35 +211,42 @@ rotary_rows_kernel(RotArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) { c[i] = 1.f; s[i] = 0.f; }
   }
-#pragma unroll 2
-  for (int h = h0; h < a.heads; h += a.head_slices) {
-    const TI* src;
-    TO* dst;
-    if (!rot_row<TI, TO>(a, t, h, blk, in_blk, src, dst)) continue;
-    float x0[8], x1[8];
-    rot_load8<TI>(src + e0, x0);
-    rot_load8<TI>(src + e1, x1);
-    if (turned && h < a.qh + a.kh) {
-      if (a.adjacent) {          // x0: pairs 0..3 of the unit, x1: pairs 4..7
+#pragma unroll 1
+  for (int h1 = h0;;) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = x0[2 * i], q = x0[2 * i + 1], r = x1[2 * i], w = x1[2 * i + 1];
-          x0[2 * i] = p * c[i] - q * s[i];
-          x0[2 * i + 1] = q * c[i] + p * s[i];
-          x1[2 * i] = r * c[4 + i] - w * s[4 + i];
-          x1[2 * i + 1] = w * c[4 + i] + r * s[4 + i];
-        }
-      } else {
+    for (int b = 0; b < B; ++b) {
+      const int h = h1 + b * a.head_slices;
+      const TI* src;
+      TO* dst;
+      if (h >= a.heads || !rot_row<TI, TO>(a, t, h, blk, in_blk, src, dst)) continue;
+      float x0[8], x1[8];
+      rot_floats<TI>(r0[b], x0);
+      rot_floats<TI>(r1[b], x1);
+      if (turned && h < a.qh + a.kh) {
+        if (a.adjacent) {        // x0: pairs 0..3 of the unit, x1: pairs 4..7
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float p = x0[i], q = x1[i];
-          x0[i] = p * c[i] - q * s[i];
-          x1[i] = q * c[i] + p * s[i];
+          for (int i = 0; i < 4; ++i) {
+            const float p = x0[2 * i], q = x0[2 * i + 1], r = x1[2 * i], w = x1[2 * i + 1];
+            x0[2 * i] = p * c[i] - q * s[i];
+            x0[2 * i + 1] = q * c[i] + p * s[i];
+            x1[2 * i] = r * c[4 + i] - w * s[4 + i];
+            x1[2 * i + 1] = w * c[4 + i] + r * s[4 + i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float p = x0[i], q = x1[i];
+            x0[i] = p * c[i] - q * s[i];
+            x1[i] = q * c[i] + p * s[i];
+          }
         }
       }
+      rot_store8<TO>(dst + e0, x0);
+      rot_store8<TO>(dst + e1, x1);
     }
-    rot_store8<TO>(dst + e0, x0);
-    rot_store8<TO>(dst + e1, x1);
+    h1 += B * a.head_slices;
+    if (h1 >= a.heads) break;
+    load(h1);
   }
 }
 

@@ -6,7 +6,6 @@ vLLM's kernels; here they run in ``akv_rotary_kv_append``, ``akv_dense_paged_att
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Optional
 
@@ -16,13 +15,20 @@ from . import _lib
 from .rotary import RotaryPositions
 
 
-def _check_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_heads: int, head_dim: int) -> None:
-    if (k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[2] != kv_heads or k_cache.shape[3] != head_dim
-            or k_cache.stride(3) != 1 or v_cache.stride(3) != 1):
-        raise ValueError(f"caches {tuple(k_cache.shape)} / {tuple(v_cache.shape)} must both be [blocks, block_size, {kv_heads}, "
+_HALVES = {torch.float16: _lib.AKV_F16, torch.bfloat16: _lib.AKV_BF16}
+_pack_append = _lib.packer(_lib.RotaryAppendParams)
+_pack_attn = _lib.packer(_lib.DenseAttnParams)
+
+
+def _check_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, kv_heads: int, head_dim: int):
+    """(shape, strides of the keys, strides of the values) of two caches that belong together."""
+    shape, ks, vs = k_cache.shape, k_cache.stride(), v_cache.stride()
+    if (len(shape) != 4 or shape != v_cache.shape or shape[2] != kv_heads or shape[3] != head_dim or ks[3] != 1 or vs[3] != 1):
+        raise ValueError(f"caches {tuple(shape)} / {tuple(v_cache.shape)} must both be [blocks, block_size, {kv_heads}, "
                          f"{head_dim}] with a contiguous last dimension")
     if k_cache.dtype != v_cache.dtype:
         raise TypeError(f"caches must have one dtype, got {k_cache.dtype} and {v_cache.dtype}")
+    return shape, ks, vs
 
 
 def rotary_kv_append(query: Optional[torch.Tensor], key: torch.Tensor, value: torch.Tensor, positions: torch.Tensor,
@@ -34,34 +40,33 @@ def rotary_kv_append(query: Optional[torch.Tensor], key: torch.Tensor, value: to
 
     Tokens with a negative slot, or one behind the cache, are skipped (padding).  The slots of one call must be distinct.
     ``query_out`` may be the query itself when their dtypes agree."""
-    dev = _lib.require_cuda(query, key, value, positions, slot_mapping, k_cache, v_cache, query_out, rope.steps)
-    p = _lib.RotaryAppendParams()
-    r, query, key = rope._params(query, key, positions, False, dev)
-    tokens, kv_heads, head_dim = key.shape
-    _check_caches(k_cache, v_cache, kv_heads, head_dim)
+    index = _lib.cuda_index(key, query, value, positions, slot_mapping, k_cache, v_cache, query_out, rope.steps)
+    tokens = key.shape[0]
+    key = rope._heads(key, "key", tokens)
+    shape, ks, vs = _check_caches(k_cache, v_cache, key.shape[1], key.shape[2])
     if value.shape != key.shape or value.dtype != key.dtype:
         raise ValueError(f"value {tuple(value.shape)} {value.dtype} must match key {tuple(key.shape)} {key.dtype}")
-    if value.stride(2) != 1:
+    st = value.stride()
+    if st[2] != 1:
         value = value.contiguous()
+        st = value.stride()
     if slot_mapping.dim() != 1 or slot_mapping.shape[0] != tokens:
         raise ValueError(f"slot_mapping {tuple(slot_mapping.shape)} must be [{tokens}]")
+    if tokens and not (shape[0] and shape[1]):
+        raise ValueError(f"caches {tuple(shape)} hold no slot")
     if slot_mapping.stride(0) != 1:
         slot_mapping = slot_mapping.contiguous()
-    r.out_dtype = _lib.float_code(k_cache)
     if query is not None:
-        query_out = RotaryPositions._out(query_out, query, k_cache.dtype, "query_out", dev)
-        r.q_out, r.qo_stride_tok, r.qo_stride_head = query_out.data_ptr(), query_out.stride(0), query_out.stride(1)
+        query = rope._heads(query, "query", tokens)
+        if query.dtype != key.dtype:
+            raise TypeError(f"query and key must have one dtype, got {query.dtype} and {key.dtype}")
+        query_out = rope._out(query_out, query, k_cache.dtype, "query_out")
     else:
         query_out = None
-    p.rotary = r
-    p.value, p.v_stride_tok, p.v_stride_head = value.data_ptr(), value.stride(0), value.stride(1)
-    p.slot_mapping, p.slot_dtype = slot_mapping.data_ptr(), _lib.index_code(slot_mapping)
-    p.k_cache, p.kc_stride_blk, p.kc_stride_pos, p.kc_stride_head = k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2)
-    p.v_cache, p.vc_stride_blk, p.vc_stride_pos, p.vc_stride_head = v_cache.data_ptr(), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2)
-    p.block_size, p.num_blocks = k_cache.shape[1], k_cache.shape[0]
-    if tokens and not (k_cache.shape[0] and k_cache.shape[1]):
-        raise ValueError(f"caches {tuple(k_cache.shape)} hold no slot")
-    _lib.call(dev, "akv_rotary_kv_append", ctypes.byref(p))
+    _lib.call(index, "akv_rotary_kv_append", _pack_append(
+        *rope._values(query, key, positions, query_out, None, _lib.float_code(k_cache), 0, index),
+        value.data_ptr(), st[0], st[1], slot_mapping.data_ptr(), _lib.index_code(slot_mapping),
+        k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2], shape[1], shape[0]))
     return query_out
 
 
@@ -92,19 +97,21 @@ class DensePagedAttention:
     @staticmethod
     def _rows16(x: torch.Tensor) -> bool:
         """Whether every row of a 16-bit [a, b, head_dim] tensor starts on a 16-byte boundary."""
-        return (x.stride(2) == 1 and x.stride(0) > 0 and x.stride(1) > 0
-                and not (x.data_ptr() & 15 or (x.stride(0) | x.stride(1)) & 7))
+        s = x.stride()
+        return s[2] == 1 and s[0] > 0 and s[1] > 0 and not (x.data_ptr() & 15 or (s[0] | s[1]) & 7)
 
-    def _params(self, dev, query, k_cache, v_cache, block_tables, seq_lens, num_seqs, out):
-        """Argument block of both entry points, and the output."""
-        if query.dim() != 3 or query.shape[1] != self.num_query_heads or query.shape[2] != self.head_dim:
-            raise ValueError(f"query {tuple(query.shape)} must be [tokens, {self.num_query_heads}, {self.head_dim}]")
-        _check_caches(k_cache, v_cache, self.num_kv_heads, self.head_dim)
-        if query.dtype not in (torch.float16, torch.bfloat16) or k_cache.dtype != query.dtype:
-            raise TypeError(f"query and caches must be fp16 or bf16 alike, got {query.dtype} and {k_cache.dtype}")
-        if block_tables.dim() != 2 or block_tables.shape[0] < num_seqs or seq_lens.dim() != 1 or seq_lens.shape[0] < num_seqs:
-            raise ValueError(f"block_tables {tuple(block_tables.shape)} / lengths {tuple(seq_lens.shape)} do not cover "
-                             f"{num_seqs} sequences")
+    def _values(self, query, k_cache, v_cache, block_tables, seq_lens, starts, num_seqs, out):
+        """(fields of ``akv_dense_attn_params`` up to the output, the output, tensors that must outlive the call)."""
+        qshape = query.shape
+        if len(qshape) != 3 or qshape[1] != self.num_query_heads or qshape[2] != self.head_dim:
+            raise ValueError(f"query {tuple(qshape)} must be [tokens, {self.num_query_heads}, {self.head_dim}]")
+        shape, ks, vs = _check_caches(k_cache, v_cache, self.num_kv_heads, self.head_dim)
+        dtype = query.dtype
+        if dtype not in _HALVES or k_cache.dtype != dtype:
+            raise TypeError(f"query and caches must be fp16 or bf16 alike, got {dtype} and {k_cache.dtype}")
+        tshape = block_tables.shape
+        if len(tshape) != 2 or tshape[0] < num_seqs or seq_lens.dim() != 1 or seq_lens.shape[0] < num_seqs:
+            raise ValueError(f"block_tables {tuple(tshape)} / lengths {tuple(seq_lens.shape)} do not cover {num_seqs} sequences")
         if not self._rows16(query):
             query = query.contiguous()
         if block_tables.stride(1) != 1:
@@ -112,33 +119,25 @@ class DensePagedAttention:
         if seq_lens.stride(0) != 1:
             seq_lens = seq_lens.contiguous()
         if out is None:
-            out = torch.empty_like(query, memory_format=torch.contiguous_format)
-        elif out.shape != query.shape or out.dtype != query.dtype or not self._rows16(out):
-            raise ValueError(f"out {tuple(out.shape)} {out.dtype} must be {tuple(query.shape)} {query.dtype} with rows on 16-byte "
-                             "boundaries")
-        code = _lib._FLOAT_CODES[query.dtype]
-        p = _lib.DenseAttnParams(
-            query.data_ptr(), code, query.stride(0), query.stride(1),
-            k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-            v_cache.data_ptr(), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2),
-            block_tables.data_ptr(), _lib.index_code(block_tables), block_tables.stride(0),
-            seq_lens.data_ptr(), _lib.index_code(seq_lens), None, 0,
-            num_seqs, query.shape[0], self.num_query_heads, self.num_kv_heads, self.head_dim,
-            k_cache.shape[1], block_tables.shape[1], k_cache.shape[0], self.scale, self.sliding_window,
-            out.data_ptr(), out.stride(0), out.stride(1))
-        p.stream = _lib.stream_ptr(dev)
-        return p, out, (query, block_tables, seq_lens)
+            out = torch.empty(qshape, dtype=dtype, device=query.device)
+        elif out.shape != qshape or out.dtype != dtype or not self._rows16(out):
+            raise ValueError(f"out {tuple(out.shape)} {out.dtype} must be {tuple(qshape)} {dtype} with rows on 16-byte boundaries")
+        qs, os = query.stride(), out.stride()
+        return (query.data_ptr(), _HALVES[dtype], qs[0], qs[1], k_cache.data_ptr(), ks[0], ks[1], ks[2],
+                v_cache.data_ptr(), vs[0], vs[1], vs[2], block_tables.data_ptr(), _lib.index_code(block_tables), block_tables.stride(0),
+                seq_lens.data_ptr(), _lib.index_code(seq_lens), *starts, num_seqs, qshape[0], self.num_query_heads, self.num_kv_heads,
+                self.head_dim, shape[1], tshape[1], shape[0], self.scale, self.sliding_window,
+                out.data_ptr(), os[0], os[1]), out, (query, block_tables, seq_lens)
 
     def forward(self, query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
                 context_lens: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One token per sequence: ``query`` [num_seqs, query_heads, head_dim], the last of each sequence's
         ``context_lens`` [num_seqs] tokens, over ``k_cache`` / ``v_cache`` [blocks, block_size, kv_heads, head_dim] through
         ``block_tables`` [num_seqs, max_blocks].  Returns ``out`` [num_seqs, query_heads, head_dim]."""
-        dev = _lib.require_cuda(query, k_cache, v_cache, block_tables, context_lens, out)
-        p, out, keep = self._params(dev, query, k_cache, v_cache, block_tables, context_lens, query.shape[0], out)
-        ws = torch.empty(self._decode_bytes, dtype=torch.uint8, device=dev)
-        p.workspace, p.workspace_bytes = ws.data_ptr(), self._decode_bytes
-        _lib.call(dev, "akv_dense_paged_attn", ctypes.byref(p))
+        index = _lib.cuda_index(query, k_cache, v_cache, block_tables, context_lens, out)
+        values, out, keep = self._values(query, k_cache, v_cache, block_tables, context_lens, (0, 0), query.shape[0], out)
+        ws = torch.empty(self._decode_bytes, dtype=torch.uint8, device=out.device)
+        _lib.call(index, "akv_dense_paged_attn", _pack_attn(*values, 0, ws.data_ptr(), self._decode_bytes, _lib.raw_stream(index)))
         return out
 
     def prefill(self, query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -152,25 +151,22 @@ class DensePagedAttention:
 
         Chunks run on the tensor cores for head_dim 64 and 128, at most 128 query heads per KV head and block sizes that
         are multiples of 8; other shapes attend token by token through ``forward``'s kernels."""
-        dev = _lib.require_cuda(query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, out)
+        index = _lib.cuda_index(query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, out)
         if query_start_loc.dim() != 1 or query_start_loc.shape[0] < 1:
             raise ValueError(f"query_start_loc {tuple(query_start_loc.shape)} must be [sequences + 1]")
         if query_start_loc.stride(0) != 1:
             query_start_loc = query_start_loc.contiguous()
-        qs_code = _lib.index_code(query_start_loc)
-        zero_tail = out is None
-        p, out, keep = self._params(dev, query, k_cache, v_cache, block_tables, seq_lens, query_start_loc.shape[0] - 1, out)
-        if not (self.head_dim <= 128 and self.num_query_heads <= 128 * self.num_kv_heads and k_cache.shape[1] % 8 == 0
-                and block_tables.shape[1] > 0):
+        num_seqs, zero_tail = query_start_loc.shape[0] - 1, out is None
+        values, out, keep = self._values(query, k_cache, v_cache, block_tables, seq_lens,
+                                         (query_start_loc.data_ptr(), _lib.index_code(query_start_loc)), num_seqs, out)
+        blocks, block_size, width = k_cache.shape[0], k_cache.shape[1], block_tables.shape[1]
+        if not (self.head_dim <= 128 and self.num_query_heads <= 128 * self.num_kv_heads and block_size % 8 == 0 and width > 0):
             if zero_tail:
                 out.zero_()
             return self._prefill_by_rows(query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, out)
-        nbytes = _lib.lib().akv_dense_prefill_attn_workspace_bytes(p.num_kv_heads, p.head_dim, p.num_blocks, p.block_size, p.num_seqs,
-                                                                   p.max_blocks_per_seq)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        p.workspace, p.workspace_bytes = ws.data_ptr(), nbytes
-        p.query_start_loc, p.qs_dtype, p.zero_tail = query_start_loc.data_ptr(), qs_code, int(zero_tail)
-        _lib.call(dev, "akv_dense_prefill_attn", ctypes.byref(p))
+        nbytes = _lib.lib().akv_dense_prefill_attn_workspace_bytes(self.num_kv_heads, self.head_dim, blocks, block_size, num_seqs, width)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device)
+        _lib.call(index, "akv_dense_prefill_attn", _pack_attn(*values, int(zero_tail), ws.data_ptr(), nbytes, _lib.raw_stream(index)))
         return out
 
     ROWS = 2048      # tokens of one call of the single-token kernels

@@ -17,6 +17,7 @@ import torch
 from . import _lib
 
 MAX_AXES = 4
+_pack = _lib.packer(_lib.RotaryParams)
 
 
 def axis_of_pairs(pairs: int, sections: Optional[Sequence[int]], layout: str = "blocked") -> list:
@@ -81,51 +82,50 @@ class RotaryPositions:
         self.device = self.steps.device
         self._tables = _lib.RotaryTables(self.head_dim, self.rotary_dim, self.num_axes, int(pair_layout == "adjacent"),
                                          self.steps.data_ptr(), self.axes.data_ptr(), self.scaling)
-        self._tables_ref = ctypes.pointer(self._tables)
+        self._tables_at = ctypes.addressof(self._tables)
 
-    def _positions(self, positions: torch.Tensor, tokens: int) -> Tuple[torch.Tensor, int, int]:
-        """(positions, stride over the axes, stride over the tokens) of [tokens] or [num_axes, tokens]."""
-        if positions.dim() == 1 and positions.shape[0] == tokens:
-            return positions, 0, positions.stride(0)      # text: the same position on every axis
-        if positions.dim() == 2 and positions.shape[0] == self.num_axes and positions.shape[1] == tokens:
-            return positions, positions.stride(0), positions.stride(1)
-        raise ValueError(f"positions {tuple(positions.shape)} must be [{tokens}] or [{self.num_axes}, {tokens}]")
+    def _positions(self, positions: torch.Tensor, tokens: int) -> Tuple[int, int]:
+        """(stride over the axes, stride over the tokens) of [tokens] or [num_axes, tokens]."""
+        shape = positions.shape
+        if len(shape) == 1 and shape[0] == tokens:
+            return 0, positions.stride(0)      # text: the same position on every axis
+        if len(shape) == 2 and shape[0] == self.num_axes and shape[1] == tokens:
+            return positions.stride()
+        raise ValueError(f"positions {tuple(shape)} must be [{tokens}] or [{self.num_axes}, {tokens}]")
 
     def _heads(self, x: torch.Tensor, name: str, tokens: int) -> torch.Tensor:
-        if x.dim() != 3 or x.shape[2] != self.head_dim or x.shape[0] != tokens:
-            raise ValueError(f"{name} {tuple(x.shape)} must be [{tokens}, heads, {self.head_dim}]")
+        shape = x.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or shape[0] != tokens:
+            raise ValueError(f"{name} {tuple(shape)} must be [{tokens}, heads, {self.head_dim}]")
         return x if x.stride(2) == 1 else x.contiguous()
 
-    def _params(self, query, key, positions, inverse, dev):
-        """The part of the argument block that the rotation and the append share, and tensors it must outlive."""
-        tokens = (query if query is not None else key).shape[0]
-        p = _lib.RotaryParams()
-        p.tables = self._tables_ref
-        pos, sa, st = self._positions(positions, tokens)
-        p.positions, p.pos_dtype, p.pos_stride_axis, p.pos_stride_tok = pos.data_ptr(), _lib.index_code(pos), sa, st
-        p.num_tokens = tokens
-        if query is not None:
-            query = self._heads(query, "query", tokens)
-            p.in_dtype = _lib.float_code(query)
-            p.query, p.q_stride_tok, p.q_stride_head, p.num_q_heads = query.data_ptr(), query.stride(0), query.stride(1), query.shape[1]
-        if key is not None:
-            key = self._heads(key, "key", tokens)
-            if query is not None and key.dtype != query.dtype:
-                raise TypeError(f"query and key must have one dtype, got {query.dtype} and {key.dtype}")
-            p.in_dtype = _lib.float_code(key)
-            p.key, p.k_stride_tok, p.k_stride_head, p.num_kv_heads = key.data_ptr(), key.stride(0), key.stride(1), key.shape[1]
-        p.inverse = int(inverse)
-        p.stream = _lib.stream_ptr(dev)
-        return p, query, key
-
     @staticmethod
-    def _out(out, x, dtype, name, dev):
+    def _out(out, x, dtype, name):
         if out is None:
-            return torch.empty(x.shape, dtype=dtype, device=dev)
+            return torch.empty(x.shape, dtype=dtype, device=x.device)
         if out.shape != x.shape or out.stride(2) != 1 or out.dtype != dtype:
             raise ValueError(f"{name} {tuple(out.shape)} {out.dtype} must be {tuple(x.shape)} {dtype} with a contiguous last "
                              "dimension")
         return out
+
+    def _values(self, query, key, positions, query_out, key_out, out_dtype, inverse, index):
+        """Fields of ``akv_rotary_params``: what the rotation and the append share.  Tensors are checked."""
+        tokens = (query if query is not None else key).shape[0]
+        pos_axis, pos_tok = self._positions(positions, tokens)
+        none = (0, 0, 0, 0), (0, 0, 0)
+        q, qo, k, ko = *none, *none
+        if query is not None:
+            st = query.stride()
+            q, st = (query.data_ptr(), st[0], st[1], query.shape[1]), query_out.stride()
+            qo = (query_out.data_ptr(), st[0], st[1])
+        if key is not None:
+            st = key.stride()
+            k = (key.data_ptr(), st[0], st[1], key.shape[1])
+            if key_out is not None:
+                st = key_out.stride()
+                ko = (key_out.data_ptr(), st[0], st[1])
+        return (self._tables_at, positions.data_ptr(), _lib.index_code(positions), pos_axis, pos_tok, tokens,
+                _lib.float_code(query if query is not None else key), out_dtype, *q, *qo, *k, *ko, inverse, _lib.raw_stream(index))
 
     def forward(self, query: Optional[torch.Tensor], key: Optional[torch.Tensor], positions: torch.Tensor,
                 query_out: Optional[torch.Tensor] = None, key_out: Optional[torch.Tensor] = None,
@@ -136,16 +136,22 @@ class RotaryPositions:
         gradient of the rotation."""
         if query is None and key is None:
             raise ValueError("query and key are both None")
-        dev = _lib.require_cuda(query, key, positions, query_out, key_out, self.steps)
-        p, query, key = self._params(query, key, positions, inverse, dev)
-        p.out_dtype = p.in_dtype
+        index = _lib.cuda_index(query, key, positions, query_out, key_out, self.steps)
+        tokens = (query if query is not None else key).shape[0]
         if query is not None:
-            query_out = self._out(query_out, query, query.dtype, "query_out", dev)
-            p.q_out, p.qo_stride_tok, p.qo_stride_head = query_out.data_ptr(), query_out.stride(0), query_out.stride(1)
+            query = self._heads(query, "query", tokens)
+            query_out = self._out(query_out, query, query.dtype, "query_out")
+        else:
+            query_out = None
         if key is not None:
-            key_out = self._out(key_out, key, key.dtype, "key_out", dev)
-            p.k_out, p.ko_stride_tok, p.ko_stride_head = key_out.data_ptr(), key_out.stride(0), key_out.stride(1)
-        _lib.call(dev, "akv_rotary", ctypes.byref(p))
-        return (query_out if query is not None else None), (key_out if key is not None else None)
+            key = self._heads(key, "key", tokens)
+            if query is not None and key.dtype != query.dtype:
+                raise TypeError(f"query and key must have one dtype, got {query.dtype} and {key.dtype}")
+            key_out = self._out(key_out, key, key.dtype, "key_out")
+        else:
+            key_out = None
+        code = _lib.float_code(query if query is not None else key)
+        _lib.call(index, "akv_rotary", _pack(*self._values(query, key, positions, query_out, key_out, code, int(inverse), index)))
+        return query_out, key_out
 
     __call__ = forward

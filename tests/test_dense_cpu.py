@@ -59,7 +59,7 @@ def test_rotary_refuses():
     with pytest.raises(ValueError):
         rope._heads(torch.zeros(3, 16), "query", 3)
     with pytest.raises(ValueError):
-        RotaryPositions._out(torch.zeros(3, 2, 16).half(), x, torch.float32, "query_out", None)
+        RotaryPositions._out(torch.zeros(3, 2, 16).half(), x, torch.float32, "query_out")
 
 
 def test_rotary_entry_points_refuse():
