@@ -11,10 +11,11 @@
 // negative).  Its upper 32 bits, as a signed fraction of a turn, go to float32 (2^-25 of half a turn) and sincospif.
 // No table of cosines is read: 4 bytes per pair and axis step instead of 8 per pair and position.
 //
-// Bound by HBM: every vector is read once and written once, the arithmetic (per pair ~40 instructions of sincospif,
-// shared by the heads a thread takes, and four FMAs per pair and head) stays under the copy time for two or more heads
-// per thread.  A thread owns 16 elements of a row - 8 pairs, two 16-byte loads for 16-bit types - of every HS-th head
-// of one token, so the 8 threads of a 128-element row read whole rows and a warp four neighbouring heads.
+// Bound by HBM: every vector is read once and written once.  A block takes a few tokens: first every thread works out the
+// cosine and sine of about one (token, pair) - a sincospif is some 40 instructions, so each is done once and not once per
+// head - into shared memory, while its first loads are under way; then the block streams through the heads, a thread 16
+// elements of a row at a time (8 pairs, two 16-byte loads for 16-bit types), the 8 threads of a 128-element row next to
+// each other.  That phase needs few registers, so enough loads are in flight.
 #include "common.cuh"
 
 // Mirrors of akv_rotary_tables, akv_rotary_params and akv_rotary_append_params in include/akv_b200.h.
@@ -66,7 +67,7 @@ struct RotArgs {
   void* kc; int64_t kc_sb, kc_sp, kc_sh;
   void* vc; int64_t vc_sb, vc_sp, vc_sh;
   int block_size; int64_t num_blocks;
-  int heads, head_slices;                                                        // qh + kh + vh, HS
+  int heads, tb, slice;                                                          // qh + kh + vh; tokens and heads of a block
 };
 
 // cos and sin of pos * step turns (2^64 steps to a turn), times the scaling
@@ -163,90 +164,107 @@ __device__ __forceinline__ void rot_slot(const RotArgs& a, int64_t t, int64_t& b
   if (blk >= a.num_blocks) blk = -1;
 }
 
+constexpr int ROT_MAX_PAIRS = 1024;      // (token, pair) couples of a block
+
 template <typename TI, typename TO>
-__global__ void __launch_bounds__(ROT_THREADS)
+__global__ void __launch_bounds__(ROT_THREADS, sizeof(TI) == 4 ? 3 : 4)
 rotary_rows_kernel(RotArgs a) {
-  const int units = a.D >> 4, runits = a.R >> 4;
-  const uint32_t idx = blockIdx.x * ROT_THREADS + threadIdx.x;      // the host cuts a call so that this fits
-  const uint32_t row = idx / (uint32_t)units;
-  const int u = (int)(idx - row * units);
-  const int64_t t = row / (uint32_t)a.head_slices;
-  const int h0 = (int)(row - (uint32_t)t * a.head_slices);
-  if (t >= a.tokens) return;
+  __shared__ __align__(16) float s_cos[ROT_MAX_PAIRS], s_sin[ROT_MAX_PAIRS];
+  __shared__ int64_t s_blk[16];
+  __shared__ int s_pos[16];
+  const int units = a.D >> 4, runits = a.R >> 4, half = a.R >> 1;
+  const int64_t t0 = (int64_t)blockIdx.x * a.tb;
+  const int tb = a.tokens - t0 < a.tb ? (int)(a.tokens - t0) : a.tb;
+  const int h_lo = blockIdx.y * a.slice, hs = a.heads - h_lo < a.slice ? a.heads - h_lo : a.slice;
+  const int items = tb * hs * units;
+  // item: (token, head, unit), units next to each other
+  int tt, h, u, e0, e1;
+  const TI* src;
+  TO* dst;
+  bool turned, there;
+  auto place = [&](int item) {
+    const int row = item / units;
+    u = item - row * units;
+    tt = row / hs;
+    h = h_lo + row - tt * hs;
+    const bool rot = u < runits && h < a.qh + a.kh;
+    turned = rot;
+    e0 = u < runits ? (a.adjacent ? 16 * u : 8 * u) : 16 * u;
+    e1 = u < runits && !a.adjacent ? half + 8 * u : e0 + 8;
+  };
+  Raw8<TI> r0, r1;
   int64_t blk, in_blk;
-  rot_slot(a, t, blk, in_blk);
-  const bool turned = u < runits;
-  const int half = a.R >> 1;
-  // element offsets of the thread's two groups of eight
-  const int e0 = turned ? (a.adjacent ? 16 * u : 8 * u) : 16 * u;
-  const int e1 = turned && !a.adjacent ? half + 8 * u : e0 + 8;
-  // the first batch of loads is on its way while the angles are worked out
-  constexpr int B = sizeof(TI) == 4 ? 2 : 4;
-  Raw8<TI> r0[B], r1[B];
-  auto load = [&](int h) {
-#pragma unroll
-    for (int b = 0; b < B; ++b) {
-      const TI* src;
-      TO* dst;
-      if (h + b * a.head_slices < a.heads && rot_row<TI, TO>(a, t, h + b * a.head_slices, blk, in_blk, src, dst)) {
-        r0[b] = rot_load8<TI>(src + e0);
-        r1[b] = rot_load8<TI>(src + e1);
+  int item = threadIdx.x;
+  there = false;
+  if (item < items) {
+    place(item);
+    rot_slot(a, t0 + tt, blk, in_blk);
+    there = rot_row<TI, TO>(a, t0 + tt, h, blk, in_blk, src, dst);
+    if (there) {
+      r0 = rot_load8<TI>(src + e0);
+      r1 = rot_load8<TI>(src + e1);
+    }
+  }
+  if (threadIdx.x < tb) {
+    int64_t b, p;
+    rot_slot(a, t0 + threadIdx.x, b, p);
+    s_blk[threadIdx.x] = b;
+    s_pos[threadIdx.x] = (int)p;
+  }
+  if (h_lo < a.qh + a.kh)
+    for (int x = threadIdx.x; x < tb * half; x += ROT_THREADS) {
+      const int t = x / half, p = x - t * half;
+      const int ax = a.num_axes > 1 ? a.axes[p] : 0;
+      rot_cs(load_index(a.positions, a.pos_dtype, ax * a.pos_sa + (t0 + t) * a.pos_st), a.steps[p], a, s_cos[x], s_sin[x]);
+    }
+  __syncthreads();
+#pragma unroll 1
+  while (item < items) {
+    float x0[8], x1[8];
+    TO* d = dst;
+    const int f0 = e0, f1 = e1, cs = tt * half + 8 * u;
+    const bool turn = turned, store = there;
+    if (there) {
+      rot_floats<TI>(r0, x0);
+      rot_floats<TI>(r1, x1);
+    }
+    item += ROT_THREADS;
+    if (item < items) {                     // the next item's loads before this one's arithmetic
+      place(item);
+      there = rot_row<TI, TO>(a, t0 + tt, h, s_blk[tt], s_pos[tt], src, dst);
+      if (there) {
+        r0 = rot_load8<TI>(src + e0);
+        r1 = rot_load8<TI>(src + e1);
       }
     }
-  };
-  load(h0);
-  float c[8], s[8];
-  if (turned && h0 < a.qh + a.kh) {
-    int64_t pos[ROT_MAX_AXES];
+    if (!store) continue;
+    if (turn) {
+      float c[8], s[8];
 #pragma unroll
-    for (int x = 0; x < ROT_MAX_AXES; ++x)
-      pos[x] = x < a.num_axes ? load_index(a.positions, a.pos_dtype, x * a.pos_sa + t * a.pos_st) : 0;
+      for (int i = 0; i < 2; ++i) {
+        reinterpret_cast<float4*>(c)[i] = reinterpret_cast<const float4*>(s_cos + cs)[i];
+        reinterpret_cast<float4*>(s)[i] = reinterpret_cast<const float4*>(s_sin + cs)[i];
+      }
+      if (a.adjacent) {          // x0: pairs 0..3 of the unit, x1: pairs 4..7
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int ax = a.num_axes > 1 ? a.axes[8 * u + i] : 0;
-      const int64_t p = ax == 0 ? pos[0] : ax == 1 ? pos[1] : ax == 2 ? pos[2] : pos[3];
-      rot_cs(p, a.steps[8 * u + i], a, c[i], s[i]);
-    }
-  } else {
+        for (int i = 0; i < 4; ++i) {
+          const float p = x0[2 * i], q = x0[2 * i + 1], r = x1[2 * i], w = x1[2 * i + 1];
+          x0[2 * i] = p * c[i] - q * s[i];
+          x0[2 * i + 1] = q * c[i] + p * s[i];
+          x1[2 * i] = r * c[4 + i] - w * s[4 + i];
+          x1[2 * i + 1] = w * c[4 + i] + r * s[4 + i];
+        }
+      } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { c[i] = 1.f; s[i] = 0.f; }
-  }
-#pragma unroll 1
-  for (int h1 = h0;;) {
-#pragma unroll
-    for (int b = 0; b < B; ++b) {
-      const int h = h1 + b * a.head_slices;
-      const TI* src;
-      TO* dst;
-      if (h >= a.heads || !rot_row<TI, TO>(a, t, h, blk, in_blk, src, dst)) continue;
-      float x0[8], x1[8];
-      rot_floats<TI>(r0[b], x0);
-      rot_floats<TI>(r1[b], x1);
-      if (turned && h < a.qh + a.kh) {
-        if (a.adjacent) {        // x0: pairs 0..3 of the unit, x1: pairs 4..7
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float p = x0[2 * i], q = x0[2 * i + 1], r = x1[2 * i], w = x1[2 * i + 1];
-            x0[2 * i] = p * c[i] - q * s[i];
-            x0[2 * i + 1] = q * c[i] + p * s[i];
-            x1[2 * i] = r * c[4 + i] - w * s[4 + i];
-            x1[2 * i + 1] = w * c[4 + i] + r * s[4 + i];
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float p = x0[i], q = x1[i];
-            x0[i] = p * c[i] - q * s[i];
-            x1[i] = q * c[i] + p * s[i];
-          }
+        for (int i = 0; i < 8; ++i) {
+          const float p = x0[i], q = x1[i];
+          x0[i] = p * c[i] - q * s[i];
+          x1[i] = q * c[i] + p * s[i];
         }
       }
-      rot_store8<TO>(dst + e0, x0);
-      rot_store8<TO>(dst + e1, x1);
     }
-    h1 += B * a.head_slices;
-    if (h1 >= a.heads) break;
-    load(h1);
+    rot_store8<TO>(d + f0, x0);
+    rot_store8<TO>(d + f1, x1);
   }
 }
 
@@ -285,51 +303,59 @@ rotary_elements_kernel(RotArgs a) {
 }
 
 template <typename TI, typename TO>
-int rot_launch(const RotArgs& a, bool rows16, int64_t blocks, cudaStream_t st) {
-  if (rows16) rotary_rows_kernel<TI, TO><<<(unsigned)blocks, ROT_THREADS, 0, st>>>(a);
-  else rotary_elements_kernel<TI, TO><<<(unsigned)blocks, ROT_THREADS, 0, st>>>(a);
+int rot_launch(const RotArgs& a, bool rows16, dim3 grid, cudaStream_t st) {
+  if (rows16) rotary_rows_kernel<TI, TO><<<grid, ROT_THREADS, 0, st>>>(a);
+  else rotary_elements_kernel<TI, TO><<<grid, ROT_THREADS, 0, st>>>(a);
   return check_launch(rows16 ? "rotary_rows_kernel" : "rotary_elements_kernel");
 }
 
 template <typename TI>
-int rot_launch_in(const RotArgs& a, bool rows16, int64_t blocks, cudaStream_t st) {
-  if (a.out_dtype == AKV_F16) return rot_launch<TI, __half>(a, rows16, blocks, st);
-  if (a.out_dtype == AKV_BF16) return rot_launch<TI, __nv_bfloat16>(a, rows16, blocks, st);
-  return rot_launch<TI, float>(a, rows16, blocks, st);
+int rot_launch_in(const RotArgs& a, bool rows16, dim3 grid, cudaStream_t st) {
+  if (a.out_dtype == AKV_F16) return rot_launch<TI, __half>(a, rows16, grid, st);
+  if (a.out_dtype == AKV_BF16) return rot_launch<TI, __nv_bfloat16>(a, rows16, grid, st);
+  return rot_launch<TI, float>(a, rows16, grid, st);
 }
 
 int rot_run(RotArgs a, const char* who, cudaStream_t st) {
   // 16-byte accesses: every row of every operand starts on a 16-byte boundary, and the rotated part and the row are whole
-  // units of 16 elements
+  // units of 16 elements; and a token's pairs fit into a block's shared memory
   const int64_t in_mask = a.in_dtype == AKV_F32 ? 3 : 7, out_mask = a.out_dtype == AKV_F32 ? 3 : 7;
   const uintptr_t ptrs = (uintptr_t)a.q | (uintptr_t)a.qo | (uintptr_t)a.k | (uintptr_t)a.ko | (uintptr_t)a.v | (uintptr_t)a.kc | (uintptr_t)a.vc;
   const int64_t ins = a.q_st | a.q_sh | a.k_st | a.k_sh | a.v_st | a.v_sh;
   const int64_t outs = a.qo_st | a.qo_sh | a.ko_st | a.ko_sh | a.kc_sb | a.kc_sp | a.kc_sh | a.vc_sb | a.vc_sp | a.vc_sh;
-  const bool rows16 = a.D % 16 == 0 && a.R % 16 == 0 &&
-                      ((a.R / 2) % 8 == 0) && (ptrs & 15) == 0 && (ins & in_mask) == 0 && (outs & out_mask) == 0;
   a.heads = a.qh + a.kh + a.vh;
-  const int per_row = rows16 ? a.D / 16 : a.R / 2 + (a.D - a.R);
-  // heads per thread: one while that does not fill the card (2048 threads per SM) eight times over, up to eight beyond
-  int per_thread = 1;
+  const bool rows16 = a.D % 16 == 0 && a.R % 16 == 0 && a.R / 2 <= ROT_MAX_PAIRS && (ptrs & 15) == 0 && (ins & in_mask) == 0 &&
+                      (outs & out_mask) == 0 && (int64_t)a.heads * a.D < ((int64_t)1 << 26);
+  const int per_token = a.R / 2 + (a.D - a.R);
+  int64_t most;                 // tokens of one launch: grid and thread indices stay below 2^31
   if (rows16) {
-    const int64_t threads = a.tokens * a.heads * per_row, full = (int64_t)sm_count() * 2048;
-    per_thread = (int)(threads / (2 * full));
-    if (per_thread < 1) per_thread = 1;
-    if (per_thread > 8) per_thread = 8;
+    // about one (token, pair) per thread; all heads of a token in one block where that gives every SM four blocks, else
+    // as many slices of heads as it takes, down to one item per thread (a decode step: latency)
+    a.tb = a.R > 0 ? ROT_THREADS / (a.R / 2) : 4;
+    if (a.tb < 1) a.tb = 1;
+    if (a.tb > 16) a.tb = 16;
+    const int64_t want = 4 * (int64_t)sm_count();
+    while (a.tb > 1 && (a.tokens + a.tb - 1) / a.tb < want) a.tb = (a.tb + 1) / 2;
+    const int64_t blocks = (a.tokens + a.tb - 1) / a.tb;
+    int64_t slices = blocks >= want ? 1 : (want + blocks - 1) / blocks;
+    const int64_t finest = ((int64_t)a.tb * a.heads * (a.D / 16) + ROT_THREADS - 1) / ROT_THREADS;      // one item per thread
+    if (slices > finest) slices = finest;
+    a.slice = (int)((a.heads + slices - 1) / slices);
+    most = (int64_t)a.tb << 30;
+  } else {
+    most = ((int64_t)1 << 31) / ((int64_t)a.heads * per_token);
   }
-  a.head_slices = (a.heads + per_thread - 1) / per_thread;
-  const int64_t per_token = (int64_t)(rows16 ? a.head_slices : a.heads) * per_row;
-  const int64_t most = ((int64_t)1 << 31) / per_token;      // tokens of one launch: thread indices stay below 2^31
   if (most < 1) return fail(AKV_ERR_ARG, "%s: %d heads of %d elements per token are too many", who, a.heads, a.D);
   const int isz = a.in_dtype == AKV_F32 ? 4 : 2, osz = a.out_dtype == AKV_F32 ? 4 : 2, ssz = a.slot_dtype == AKV_I64 ? 8 : 4, psz = a.pos_dtype == AKV_I64 ? 8 : 4;
   int64_t left = a.tokens;
   while (left > 0) {
     a.tokens = left < most ? left : most;
-    const int64_t blocks = (a.tokens * per_token + ROT_THREADS - 1) / ROT_THREADS;
+    const dim3 grid = rows16 ? dim3((unsigned)((a.tokens + a.tb - 1) / a.tb), (unsigned)((a.heads + a.slice - 1) / a.slice))
+                             : dim3((unsigned)((a.tokens * a.heads * per_token + ROT_THREADS - 1) / ROT_THREADS));
     int rc;
-    if (a.in_dtype == AKV_F16) rc = rot_launch_in<__half>(a, rows16, blocks, st);
-    else if (a.in_dtype == AKV_BF16) rc = rot_launch_in<__nv_bfloat16>(a, rows16, blocks, st);
-    else rc = rot_launch_in<float>(a, rows16, blocks, st);
+    if (a.in_dtype == AKV_F16) rc = rot_launch_in<__half>(a, rows16, grid, st);
+    else if (a.in_dtype == AKV_BF16) rc = rot_launch_in<__nv_bfloat16>(a, rows16, grid, st);
+    else rc = rot_launch_in<float>(a, rows16, grid, st);
     if (rc) return rc;
     left -= a.tokens;
     if (left > 0) {

@@ -119,7 +119,7 @@ class DensePagedAttention:
         if seq_lens.stride(0) != 1:
             seq_lens = seq_lens.contiguous()
         if out is None:
-            out = torch.empty(qshape, dtype=dtype, device=query.device)
+            out = torch.empty_like(query)
         elif out.shape != qshape or out.dtype != dtype or not self._rows16(out):
             raise ValueError(f"out {tuple(out.shape)} {out.dtype} must be {tuple(qshape)} {dtype} with rows on 16-byte boundaries")
         qs, os = query.stride(), out.stride()

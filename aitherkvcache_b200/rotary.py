@@ -102,7 +102,7 @@ class RotaryPositions:
     @staticmethod
     def _out(out, x, dtype, name):
         if out is None:
-            return torch.empty(x.shape, dtype=dtype, device=x.device)
+            return torch.empty_like(x) if x.dtype == dtype else torch.empty_like(x, dtype=dtype)
         if out.shape != x.shape or out.stride(2) != 1 or out.dtype != dtype:
             raise ValueError(f"{name} {tuple(out.shape)} {out.dtype} must be {tuple(x.shape)} {dtype} with a contiguous last "
                              "dimension")
