@@ -6,14 +6,14 @@
 // products are 8 D G flops for them, which mma.sync covers at a tenth of its rate.
 //
 // Work split.  The keys of a row - one sequence and one group of up to 8 NT query heads of a KV head - are cut into steps of
-// 16.  The steps of all rows are laid end to end and cut into one equal range per CTA (one per SM), so that any mixture
+// 16 (32 at D = 64).  The steps of all rows are laid end to end and cut into one equal range per CTA (one per SM), so that any mixture
 // of lengths keeps every SM busy to the end; every CTA finds its range itself from the lengths (block-wide prefix sum in shared memory).
 // A CTA walks over the pieces of rows in its range; its warps take a piece's steps in turn, each with a ring of its own
 // in shared memory filled by 16-byte cp.async copies (NS - 1 steps ahead, across the ends of pieces): no barrier in the
 // loop.  At the end of a piece the warps' results are joined in a fixed order; a piece that is a whole row is written as
 // output, others (two per CTA at most) go to the workspace and dense_decode_merge_kernel joins them, again in a fixed order.
 //
-// A step in a warp: S^T[16 keys][8 heads] = K Q^T (keys as the rows of the product, so that up to 8 heads waste nothing),
+// 16 keys in a warp: S^T[16 keys][8 heads] = K Q^T (keys as the rows of the product, so that up to 8 heads waste nothing),
 // probabilities in float32, rounded once to the cache's type, transposed in registers (movmatrix) into the second
 // operand of O^T[D][8 heads] += V^T P^T.  Scores, maxima, sums and O are float32.  The reference m moves only when a score
 // exceeds it by more than 2^8, so the shuffles and the rescaling of O run a few times per row (fp16 holds 2^8 exactly).
@@ -30,7 +30,8 @@ constexpr float DD_RESCALE = 8.0f;
 
 template <int D, int NT> struct DdL {
   static constexpr int W = D * NT >= 256 ? 4 : 8, THREADS = 32 * W;
-  static constexpr int STEP = 16 * D * 2;                     // bytes of one operand of a step
+  static constexpr int KS = D == 64 ? 32 : 16;                // keys of a step: 8 KB of keys and values at D = 64 and 128
+  static constexpr int STEP = KS * D * 2;                     // bytes of one operand of a step
   // about 192 KB of rings per SM (what 6.5 TB/s at over a microsecond of latency keep in flight, three times over), less
   // where the join buffer of 16 heads x 256 needs the room
   static constexpr int NS = D * NT == 512 ? 2 : 196608 / (2 * STEP * W);
@@ -39,7 +40,7 @@ template <int D, int NT> struct DdL {
   static constexpr int O = W * RING;                          // join buffer: [W / 2][H][OROW] float
   static constexpr int OROW = D + 4;                          // four rows apart: other banks
   static constexpr int ML = O + (W / 2) * H * OROW * 4;       // [2][W][H][2] float
-  static constexpr int PRE = ML + 2 * W * H * 2 * 4;          // prefix sums
+  static constexpr int PRE = ML + 2 * W * H * 2 * 4;          // prefix sums of the steps
   static constexpr int SMEM = PRE + (DD_MAX_SEQS + 1) * 4 + 64;
   static_assert(SMEM + 256 <= 232448, "shared memory");
 };
@@ -70,16 +71,20 @@ __device__ __forceinline__ void dd_mma(float (&c)[4], const uint32_t (&a)[4], ui
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Keys [lo, len) that a sequence's token sees, in steps of 16 from step lo / 16.
+// Keys [lo, len) that a sequence's token sees, in steps of KS from step lo / KS.
 struct DdSpan { int lo, len, first, steps; };
+template <int KS>
 __device__ __forceinline__ DdSpan dd_span(const DenseArgs& a, int s) {
   DdSpan p;
   p.len = (int)load_ctx(a.seq_lens, a.sl_dtype, s, (int64_t)a.max_blocks_per_seq * a.block_size);
   p.lo = a.window > 0 && p.len > a.window ? p.len - a.window : 0;
-  p.first = p.lo >> 4;
-  p.steps = ((p.len + 15) >> 4) - p.first;
+  p.first = p.lo / KS;
+  p.steps = (p.len + KS - 1) / KS - p.first;
   return p;
 }
+
+// What dense_decode_merge_kernel needs to know about the row whose first part CTA c wrote (parts < 2: nothing)
+struct DdDesc { int parts, slot0, s, vh; };
 
 // The CTAs that share T units: as many as are left with DD_MIN_UNITS units each (a warp gets four steps, one round of its
 // ring; a row shorter than that is not worth a second CTA and the join), at most the grid.
@@ -97,12 +102,12 @@ struct DdCursor {
   DdSpan span;
 };
 
-template <bool BF, int D, int NT, bool PAGE16>
+template <bool BF, int D, int NT, bool PAGE16>      // PAGE16: 16 aligned keys lie inside one block
 __global__ void __launch_bounds__(DdL<D, NT>::THREADS, 1)
-dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, int* plan) {
+dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, DdDesc* desc) {
   using L = DdL<D, NT>;
-  constexpr int W = L::W, NS = L::NS, H = L::H;
-  constexpr int CPR = D / 8, RPP = 32 / CPR, PASSES = 16 / RPP;     // 16-byte pieces per row, rows per pass of a warp
+  constexpr int W = L::W, NS = L::NS, H = L::H, KS = L::KS;
+  constexpr int CPR = D / 8, RPP = 32 / CPR, PASSES = KS / RPP;     // 16-byte pieces per row, rows per pass of a warp
   extern __shared__ __align__(128) uint8_t dd_smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int* pre = reinterpret_cast<int*>(dd_smem + L::PRE);
@@ -116,7 +121,7 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int s = tid * PER + i;
-      n[i] = s < seqs ? dd_span(a, seqs0 + s).steps : 0;
+      n[i] = s < seqs ? dd_span<KS>(a, seqs0 + s).steps : 0;
       sum += n[i];
     }
     int inc = sum;
@@ -138,11 +143,17 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
     }
     __syncthreads();
   }
-  if (blockIdx.x == 0)
-    for (int i = tid; i <= seqs; i += L::THREADS) plan[i] = pre[i];
+  // rows of sequences without keys: zeros
+  for (int s = blockIdx.x; s < seqs; s += gridDim.x)
+    if (pre[s + 1] == pre[s])
+      for (int e = tid; e < a.num_q_heads * D; e += L::THREADS)
+        dense_store<BF>(a.out, (int64_t)(seqs0 + s) * a.out_st + (int64_t)(e / D) * a.out_sh + e % D, 0.f);
   const int64_t units = (int64_t)pre[seqs] * vheads;
   const int n_ctas = dd_ctas(units, gridDim.x);
-  if ((int)blockIdx.x >= n_ctas || units == 0) return;
+  if ((int)blockIdx.x >= n_ctas || units == 0) {
+    if (tid == 0) desc[blockIdx.x] = DdDesc{0, 0, 0, 0};
+    return;
+  }
   const int64_t u0 = dd_begin(units, n_ctas, blockIdx.x), u1 = dd_begin(units, n_ctas, blockIdx.x + 1);
 
   // ---- the first piece ----
@@ -155,7 +166,7 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
       if ((int64_t)pre[mid] * vheads <= u0) lo = mid; else hi = mid;
     }
     cur.s = lo;
-    cur.span = dd_span(a, seqs0 + lo);
+    cur.span = dd_span<KS>(a, seqs0 + lo);
     const int64_t in_seq = u0 - (int64_t)pre[lo] * vheads;
     cur.vh = (int)(in_seq / cur.span.steps);
     cur.t = (int)(in_seq - (int64_t)cur.vh * cur.span.steps);
@@ -169,7 +180,7 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
     if (++c.vh == vheads) {
       c.vh = 0;
       do { ++c.s; } while (pre[c.s + 1] == pre[c.s]);      // left > 0: there is one with steps
-      c.span = dd_span(a, seqs0 + c.s);
+      c.span = dd_span<KS>(a, seqs0 + c.s);
     }
     c.t = 0;
     c.t_end = (int)(c.left < row_units(c) ? c.left : row_units(c));
@@ -193,32 +204,30 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
     }
   };
   settle();
-  int64_t entry = 0;            // block of the step to copy, read one step ahead
+  constexpr int KB = KS / 16;
+  int64_t entry[KB];            // blocks of the step to copy, read one step ahead
   auto fetch_entry = [&]() {
-    if (PAGE16 && more) entry = dense_block(a, seqs0 + ld.s, (ld.span.first + ld.t) * 16 / a.block_size);
+    if (PAGE16 && more)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) entry[kb] = dense_block(a, seqs0 + ld.s, ((ld.span.first + ld.t) * KS + 16 * kb) / a.block_size);
   };
   fetch_entry();
   int stage_ld = 0;
   const int my_c = lane % CPR, my_r = lane / CPR;
   auto issue = [&]() {
     if (more) {
-      const int key0 = (ld.span.first + ld.t) * 16;
+      const int key0 = (ld.span.first + ld.t) * KS;
       const int kvh = ld.vh / per_kv;
       const uint32_t dk = ring + (uint32_t)(stage_ld * 2 * L::STEP), dv = dk + L::STEP;
       const char *kp = nullptr, *vp = nullptr;
-      if (PAGE16) {
-        const int pos = key0 % a.block_size;
-        kp = kbase + 2 * (entry * a.k_sb + (int64_t)(pos + my_r) * a.k_sp + (int64_t)kvh * a.k_sh + my_c * 8);
-        vp = vbase + 2 * (entry * a.v_sb + (int64_t)(pos + my_r) * a.v_sp + (int64_t)kvh * a.v_sh + my_c * 8);
-      }
 #pragma unroll
       for (int i = 0; i < PASSES; ++i) {
         const int r = my_r + i * RPP, key = key0 + r;
         const uint32_t bytes = key >= ld.span.lo && key < ld.span.len ? 16u : 0u;
         const uint32_t off = (uint32_t)(r * (D * 2) + ((my_c ^ (r & 7)) << 4));
-        if (!PAGE16) {
-          const int64_t blk = dense_block(a, seqs0 + ld.s, key / a.block_size);
-          const int pos = key % a.block_size;
+        if (!PAGE16 || i * RPP % 16 == 0) {      // a new block may begin
+          const int64_t blk = PAGE16 ? entry[i * RPP / 16] : dense_block(a, seqs0 + ld.s, key / a.block_size);
+          const int pos = PAGE16 ? (key0 + i * RPP) % a.block_size + my_r : key % a.block_size;
           kp = kbase + 2 * (blk * a.k_sb + (int64_t)pos * a.k_sp + (int64_t)kvh * a.k_sh + my_c * 8);
           vp = vbase + 2 * (blk * a.v_sb + (int64_t)pos * a.v_sp + (int64_t)kvh * a.v_sh + my_c * 8);
         }
@@ -274,41 +283,49 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
       issue();                  // into the stage that the previous step has left
       const uint32_t sk = ring + (uint32_t)(stage * 2 * L::STEP), sv = sk + L::STEP;
       stage = stage == NS - 1 ? 0 : stage + 1;
-      float c[NT][4];
+      float c[KB][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) c[kb][nt][0] = c[kb][nt][1] = c[kb][nt][2] = c[kb][nt][3] = 0.f;
       {
         const int r = (lane & 7) + ((lane >> 3) & 1) * 8, ch = lane >> 4;
         const uint32_t row = sk + (uint32_t)(r * (D * 2));
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          uint32_t ka[4];
-          dd_ldm4(row + (uint32_t)(((2 * kk + ch) ^ (r & 7)) << 4), ka);
+        for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) dd_mma<BF>(c[nt], ka, qb[nt][kk][0], qb[nt][kk][1]);
-        }
+          for (int kb = 0; kb < KB; ++kb) {
+            uint32_t ka[4];
+            dd_ldm4(row + (uint32_t)(kb * 16 * D * 2 + (((2 * kk + ch) ^ (r & 7)) << 4)), ka);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) dd_mma<BF>(c[kb][nt], ka, qb[nt][kk][0], qb[nt][kk][1]);
+          }
       }
-      const int key0 = (cur.span.first + t) * 16;
-      const bool edge = key0 < cur.span.lo || key0 + 16 > cur.span.len;
+      const int key0 = (cur.span.first + t) * KS;
+      const bool edge = key0 < cur.span.lo || key0 + KS > cur.span.len;
+      float top[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+        top[nt][0] = top[nt][1] = -CUDART_INF_F;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          c[nt][i] *= a.scale_log2;
-          const int key = key0 + g + (i >> 1) * 8;
-          if (edge && (key < cur.span.lo || key >= cur.span.len)) c[nt][i] = -CUDART_INF_F;
-        }
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            c[kb][nt][i] *= a.scale_log2;
+            const int key = key0 + kb * 16 + g + (i >> 1) * 8;
+            if (edge && (key < cur.span.lo || key >= cur.span.len)) c[kb][nt][i] = -CUDART_INF_F;
+            top[nt][i & 1] = fmaxf(top[nt][i & 1], c[kb][nt][i]);
+          }
       }
       bool grow = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        grow = grow || fmaxf(c[nt][0], c[nt][2]) > m[nt][0] + DD_RESCALE || fmaxf(c[nt][1], c[nt][3]) > m[nt][1] + DD_RESCALE;
+      for (int nt = 0; nt < NT; ++nt) grow = grow || top[nt][0] > m[nt][0] + DD_RESCALE || top[nt][1] > m[nt][1] + DD_RESCALE;
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            float mx = fmaxf(c[nt][x], c[nt][x + 2]);
+            float mx = top[nt][x];
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
             if (mx > m[nt][x]) {
@@ -320,27 +337,32 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
             }
           }
       }
-      uint32_t pb[NT][2];
+      uint32_t pb[KB][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float m0 = m[nt][0] == -CUDART_INF_F ? 0.f : m[nt][0], m1 = m[nt][1] == -CUDART_INF_F ? 0.f : m[nt][1];
-        const float p0 = dense_ex2(c[nt][0] - m0), p1 = dense_ex2(c[nt][1] - m1);
-        const float p2 = dense_ex2(c[nt][2] - m0), p3 = dense_ex2(c[nt][3] - m1);
-        l[nt][0] += p0 + p2;
-        l[nt][1] += p1 + p3;
-        pb[nt][0] = dd_movm(dense_pack<BF>(p0, p1));
-        pb[nt][1] = dd_movm(dense_pack<BF>(p2, p3));
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          const float p0 = dense_ex2(c[kb][nt][0] - m0), p1 = dense_ex2(c[kb][nt][1] - m1);
+          const float p2 = dense_ex2(c[kb][nt][2] - m0), p3 = dense_ex2(c[kb][nt][3] - m1);
+          l[nt][0] += p0 + p2;
+          l[nt][1] += p1 + p3;
+          pb[kb][nt][0] = dd_movm(dense_pack<BF>(p0, p1));
+          pb[kb][nt][1] = dd_movm(dense_pack<BF>(p2, p3));
+        }
       }
       {
         const int r = (lane & 7) + (lane >> 4) * 8, ch = (lane >> 3) & 1;
         const uint32_t row = sv + (uint32_t)(r * (D * 2));
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          uint32_t va[4];
-          dd_ldm4t(row + (uint32_t)(((2 * i + ch) ^ (r & 7)) << 4), va);
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) dd_mma<BF>(o[nt][i], va, pb[nt][0], pb[nt][1]);
-        }
+          for (int i = 0; i < D / 16; ++i) {
+            uint32_t va[4];
+            dd_ldm4t(row + (uint32_t)(kb * 16 * D * 2 + (((2 * i + ch) ^ (r & 7)) << 4)), va);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) dd_mma<BF>(o[nt][i], va, pb[kb][nt][0], pb[kb][nt][1]);
+          }
       }
     }
 
@@ -413,6 +435,17 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
         if (d == 0) { part[h * (D + 2)] = top; part[h * (D + 2) + 1] = sum; }
       }
     }
+    if (cur.left <= 0 && tid == 0) {          // the last piece: a row that begins here and ends in another CTA's range?
+      DdDesc d{0, 0, 0, 0};
+      if (piece_t0 == 0 && cur.t_end < cur.span.steps) {
+        const int64_t end = u1 - cur.t_end + cur.span.steps;      // the row's last unit is end - 1
+        d.parts = (int)((end * n_ctas - 1) / units) - (int)blockIdx.x + 1;
+        d.slot0 = first_piece ? 0 : 1;
+        d.s = seqs0 + cur.s;
+        d.vh = cur.vh;
+      }
+      desc[blockIdx.x] = d;
+    }
     first_piece = false;
     have = next_piece(cur);
   }
@@ -420,68 +453,53 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
 }
 
 // Rows whose steps fell into several CTAs' ranges: out = sum_p 2^(m_p - M) acc_p / sum_p 2^(m_p - M) l_p, parts in the
-// order of the keys.  Rows without keys: zeros.
+// order of the keys.  Block c: the row that CTA c began.
 template <bool BF, int D, int NT>
 __global__ void __launch_bounds__(256)
-dense_decode_merge_kernel(DenseArgs a, int seqs0, int seqs, int vheads, int grid, const float* parts, const int* plan) {
+dense_decode_merge_kernel(DenseArgs a, int vheads, const float* parts, const DdDesc* desc) {
   constexpr int H = 8 * NT, P = D + 2;
   extern __shared__ float dm_f[];          // [n_parts][H] factors
   __shared__ float s_inv[H];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int tid = threadIdx.x;
-  const int s = blockIdx.x / vheads, vh = blockIdx.x - s * vheads;
+  const DdDesc d = desc[blockIdx.x];
+  if (d.parts < 2) return;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = a.num_q_heads / a.num_kv_heads, per_kv = vheads / a.num_kv_heads;
-  const int kvh = vh / per_kv, h0 = (vh - kvh * per_kv) * H;
+  const int kvh = d.vh / per_kv, h0 = (d.vh - kvh * per_kv) * H;
   const int n_heads = group - h0 < H ? group - h0 : H;
-  const int steps = plan[s + 1] - plan[s];
-  auto dst = [&](int h, int d) -> int64_t {
-    return (int64_t)(seqs0 + s) * a.out_st + (int64_t)(kvh * group + h0 + h) * a.out_sh + d;
-  };
-  if (steps == 0) {
-    for (int e = tid; e < n_heads * D; e += 256) dense_store<BF>(a.out, dst(e / D, e % D), 0.f);
-    return;
-  }
-  const int64_t units = (int64_t)plan[seqs] * vheads;
-  const int n = dd_ctas(units, grid);
-  const int64_t u0 = (int64_t)plan[s] * vheads + (int64_t)vh * steps, u1 = u0 + steps;
-  const int c0 = (int)(((u0 + 1) * n - 1) / units), c1 = (int)((u1 * n - 1) / units);
-  if (c0 == c1) return;
-  const int slot0 = dd_begin(units, n, c0) == u0 ? 0 : 1;      // later parts begin where their CTA's range begins
-  auto part = [&](int i) -> const float* { return parts + ((int64_t)(c0 + i) * 2 + (i == 0 ? slot0 : 0)) * H * P; };
-  const int n_parts = c1 - c0 + 1;
-  for (int i = tid; i < n_parts * n_heads; i += 256) {
-    const int p = i / n_heads, h = i - p * n_heads;
-    dm_f[p * H + h] = part(p)[h * P];
-  }
-  __syncthreads();
-  const int warp = tid >> 5, lane = tid & 31;
+  // later parts begin where their CTA's range begins
+  auto part = [&](int i) -> const float* { return parts + ((int64_t)(blockIdx.x + i) * 2 + (i == 0 ? d.slot0 : 0)) * H * P; };
   for (int h = warp; h < n_heads; h += 8) {
     float top = -CUDART_INF_F;
-    for (int p = lane; p < n_parts; p += 32) top = fmaxf(top, dm_f[p * H + h]);
+    for (int p = lane; p < d.parts; p += 32) {
+      const float mp = part(p)[h * P];
+      dm_f[p * H + h] = mp;
+      top = fmaxf(top, mp);
+    }
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
     float sum = 0.f;
-    for (int p = lane; p < n_parts; p += 32) {
+    for (int p = lane; p < d.parts; p += 32) {
       const float mp = dm_f[p * H + h], f = mp == -CUDART_INF_F ? 0.f : dense_ex2(mp - top);
       dm_f[p * H + h] = f;
       sum += f * part(p)[h * P + 1];
     }
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
     if (lane == 0) s_inv[h] = sum == 0.f ? 0.f : 1.f / sum;
   }
   __syncthreads();
   for (int e = tid; e < n_heads * D; e += 256) {
-    const int h = e / D, d = e - h * D;
+    const int h = e / D, x = e - h * D;
     float acc = 0.f;
 #pragma unroll 4
-    for (int p = 0; p < n_parts; ++p) acc += dm_f[p * H + h] * part(p)[h * P + 2 + d];
-    dense_store<BF>(a.out, dst(h, d), acc * s_inv[h]);
+    for (int p = 0; p < d.parts; ++p) acc += dm_f[p * H + h] * part(p)[h * P + 2 + x];
+    dense_store<BF>(a.out, (int64_t)d.s * a.out_st + (int64_t)(kvh * group + h0 + h) * a.out_sh + x, acc * s_inv[h]);
   }
 }
 
 template <bool BF, int D, int NT>
-int dd_launch(const DenseArgs& a, float* parts, int* plan, cudaStream_t st) {
+int dd_launch(const DenseArgs& a, float* parts, DdDesc* desc, cudaStream_t st) {
   using L = DdL<D, NT>;
   const int group = a.num_q_heads / a.num_kv_heads;
   const int vheads = a.num_kv_heads * ((group + L::H - 1) / L::H), grid = sm_count();
@@ -490,24 +508,24 @@ int dd_launch(const DenseArgs& a, float* parts, int* plan, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
   if (e != cudaSuccess) return fail((int)e, "dense attention: smem attribute: %s", cudaGetErrorString(e));
   // sequences of one launch: prefix sums in shared memory, and of fewer than 2^31 steps even if every sequence were full
-  const int64_t full = ((int64_t)a.max_blocks_per_seq * a.block_size + 15) / 16;
+  const int64_t full = ((int64_t)a.max_blocks_per_seq * a.block_size + L::KS - 1) / L::KS;
   int most = DD_MAX_SEQS;
   if (full * most > 0x7fffffffll) most = (int)(0x7fffffffll / full);
   for (int s0 = 0; s0 < a.num_seqs; s0 += most) {
     const int seqs = a.num_seqs - s0 < most ? a.num_seqs - s0 : most;
-    kernel<<<grid, L::THREADS, L::SMEM, st>>>(a, s0, seqs, vheads, parts, plan);
+    kernel<<<grid, L::THREADS, L::SMEM, st>>>(a, s0, seqs, vheads, parts, desc);
     if (int rc = check_launch("dense_decode_attn_kernel")) return rc;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)(seqs * vheads));
+    cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = (size_t)grid * L::H * sizeof(float);
     cfg.stream = st;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, dense_decode_merge_kernel<BF, D, NT>, a, s0, seqs, vheads, grid, (const float*)parts, (const int*)plan);
+    e = cudaLaunchKernelEx(&cfg, dense_decode_merge_kernel<BF, D, NT>, a, vheads, (const float*)parts, (const DdDesc*)desc);
     if (e != cudaSuccess) return fail((int)e, "dense attention merge: %s", cudaGetErrorString(e));
     if (int rc = check_launch("dense_decode_merge_kernel")) return rc;
   }
@@ -515,14 +533,14 @@ int dd_launch(const DenseArgs& a, float* parts, int* plan, cudaStream_t st) {
 }
 
 template <bool BF>
-int dd_dispatch(const DenseArgs& a, float* parts, int* plan, cudaStream_t st) {
+int dd_dispatch(const DenseArgs& a, float* parts, DdDesc* desc, cudaStream_t st) {
   const bool one = a.num_q_heads / a.num_kv_heads <= 8;
-  if (a.head_dim == 64) return one ? dd_launch<BF, 64, 1>(a, parts, plan, st) : dd_launch<BF, 64, 2>(a, parts, plan, st);
-  if (a.head_dim == 128) return one ? dd_launch<BF, 128, 1>(a, parts, plan, st) : dd_launch<BF, 128, 2>(a, parts, plan, st);
-  return one ? dd_launch<BF, 256, 1>(a, parts, plan, st) : dd_launch<BF, 256, 2>(a, parts, plan, st);
+  if (a.head_dim == 64) return one ? dd_launch<BF, 64, 1>(a, parts, desc, st) : dd_launch<BF, 64, 2>(a, parts, desc, st);
+  if (a.head_dim == 128) return one ? dd_launch<BF, 128, 1>(a, parts, desc, st) : dd_launch<BF, 128, 2>(a, parts, desc, st);
+  return one ? dd_launch<BF, 256, 1>(a, parts, desc, st) : dd_launch<BF, 256, 2>(a, parts, desc, st);
 }
 
-constexpr size_t DD_PLAN_BYTES = ((DD_MAX_SEQS + 1) * 4 + 255) / 256 * 256;
+size_t dd_desc_bytes() { return ((size_t)sm_count() * sizeof(DdDesc) + 255) / 256 * 256; }
 
 }  // namespace
 
@@ -569,11 +587,11 @@ int dense_common(const akv_dense_attn_params* p, const char* who, DenseArgs* a) 
 
 }  // namespace akv
 
-// Two partial rows per CTA, and the prefix sums of the steps.
+// Two partial rows per CTA, and what the merge has to know.
 AKV_EXPORT size_t akv_dense_paged_attn_workspace_bytes(int num_q_heads, int num_kv_heads, int head_dim) {
   if (num_kv_heads <= 0 || num_q_heads < num_kv_heads || head_dim <= 0) return 0;
   const int heads = num_q_heads / num_kv_heads <= 8 ? 8 : 16;
-  return akv::DD_PLAN_BYTES + (size_t)akv::sm_count() * 2 * heads * (head_dim + 2) * sizeof(float);
+  return akv::dd_desc_bytes() + (size_t)akv::sm_count() * 2 * heads * (head_dim + 2) * sizeof(float);
 }
 
 AKV_EXPORT int akv_dense_paged_attn(const akv_dense_attn_params* p) {
@@ -585,8 +603,8 @@ AKV_EXPORT int akv_dense_paged_attn(const akv_dense_attn_params* p) {
   const size_t need = akv_dense_paged_attn_workspace_bytes(a.num_q_heads, a.num_kv_heads, a.head_dim);
   if (!p->workspace || p->workspace_bytes < need || ((uintptr_t)p->workspace & 15))
     return akv::fail(AKV_ERR_WORKSPACE, "akv_dense_paged_attn: workspace of %zu bytes (16-byte aligned) needed, got %zu", need, p->workspace_bytes);
-  int* plan = reinterpret_cast<int*>(p->workspace);
-  float* parts = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + akv::DD_PLAN_BYTES);
+  akv::DdDesc* desc = reinterpret_cast<akv::DdDesc*>(p->workspace);
+  float* parts = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + akv::dd_desc_bytes());
   cudaStream_t st = reinterpret_cast<cudaStream_t>(p->stream);
-  return p->dtype == AKV_BF16 ? akv::dd_dispatch<true>(a, parts, plan, st) : akv::dd_dispatch<false>(a, parts, plan, st);
+  return p->dtype == AKV_BF16 ? akv::dd_dispatch<true>(a, parts, desc, st) : akv::dd_dispatch<false>(a, parts, desc, st);
 }
