@@ -6,7 +6,7 @@
 // products are 8 D G flops for them, which mma.sync covers at a tenth of its rate.
 //
 // Work split.  The keys of a row - one sequence and one group of up to 8 NT query heads of a KV head - are cut into steps of
-// 16 (32 at D = 64).  The steps of all rows are laid end to end and cut into one equal range per CTA (one per SM), so that any mixture
+// 16 (32 at D = 64).  The steps of all rows are laid end to end and cut into one equal range per CTA (one or two per SM), so that any mixture
 // of lengths keeps every SM busy to the end; every CTA finds its range itself from the lengths (block-wide prefix sum in shared memory).
 // A CTA walks over the pieces of rows in its range; its warps take a piece's steps in turn, each with a ring of its own
 // in shared memory filled by 16-byte cp.async copies (NS - 1 steps ahead, across the ends of pieces): no barrier in the
@@ -25,16 +25,17 @@
 namespace akv {
 namespace {
 
-constexpr int DD_MAX_SEQS = 2048;        // sequences of one launch (their prefix sums live in shared memory)
+constexpr int DD_MAX_SEQS = 1024;        // sequences of one launch (their prefix sums live in shared memory)
 constexpr float DD_RESCALE = 8.0f;
 
 template <int D, int NT> struct DdL {
-  static constexpr int W = D * NT >= 256 ? 4 : 8, THREADS = 32 * W;
+  // two CTAs per SM where their rings fit: one streams while the other joins its warps' results at the end of a piece
+  static constexpr int CTAS = D * NT <= 128 ? 2 : 1, W = 4, THREADS = 32 * W;
   static constexpr int KS = D == 64 ? 32 : 16;                // keys of a step: 8 KB of keys and values at D = 64 and 128
   static constexpr int STEP = KS * D * 2;                     // bytes of one operand of a step
   // about 192 KB of rings per SM (what 6.5 TB/s at over a microsecond of latency keep in flight, three times over), less
   // where the join buffer of 16 heads x 256 needs the room
-  static constexpr int NS = D * NT == 512 ? 2 : 196608 / (2 * STEP * W);
+  static constexpr int NS = D * NT == 512 ? 2 : 196608 / CTAS / (2 * STEP * W);
   static constexpr int RING = 2 * STEP * NS;                  // per warp
   static constexpr int H = 8 * NT;                            // heads of a row
   static constexpr int O = W * RING;                          // join buffer: [W / 2][H][OROW] float
@@ -42,7 +43,7 @@ template <int D, int NT> struct DdL {
   static constexpr int ML = O + (W / 2) * H * OROW * 4;       // [2][W][H][2] float
   static constexpr int PRE = ML + 2 * W * H * 2 * 4;          // prefix sums of the steps
   static constexpr int SMEM = PRE + (DD_MAX_SEQS + 1) * 4 + 64;
-  static_assert(SMEM + 256 <= 232448, "shared memory");
+  static_assert(CTAS * (SMEM + 256 + 1024) <= 233472, "shared memory");
 };
 
 __device__ __forceinline__ void dd_cp16(uint32_t dst, const void* src, uint32_t bytes) {
@@ -88,7 +89,7 @@ struct DdDesc { int parts, slot0, s, vh; };
 
 // The CTAs that share T units: as many as are left with DD_MIN_UNITS units each (a warp gets four steps, one round of its
 // ring; a row shorter than that is not worth a second CTA and the join), at most the grid.
-constexpr int DD_MIN_UNITS = 32;
+constexpr int DD_MIN_UNITS = 16;
 __device__ __forceinline__ int dd_ctas(int64_t units, int grid) {
   const int64_t n = units / DD_MIN_UNITS;
   return n < 1 ? 1 : (n < grid ? (int)n : grid);
@@ -103,7 +104,7 @@ struct DdCursor {
 };
 
 template <bool BF, int D, int NT, bool PAGE16>      // PAGE16: 16 aligned keys lie inside one block
-__global__ void __launch_bounds__(DdL<D, NT>::THREADS, 1)
+__global__ void __launch_bounds__(DdL<D, NT>::THREADS, DdL<D, NT>::CTAS)
 dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, DdDesc* desc) {
   using L = DdL<D, NT>;
   constexpr int W = L::W, NS = L::NS, H = L::H, KS = L::KS;
@@ -502,7 +503,7 @@ template <bool BF, int D, int NT>
 int dd_launch(const DenseArgs& a, float* parts, DdDesc* desc, cudaStream_t st) {
   using L = DdL<D, NT>;
   const int group = a.num_q_heads / a.num_kv_heads;
-  const int vheads = a.num_kv_heads * ((group + L::H - 1) / L::H), grid = sm_count();
+  const int vheads = a.num_kv_heads * ((group + L::H - 1) / L::H), grid = L::CTAS * sm_count();
   const bool page16 = a.block_size % 16 == 0;
   auto kernel = page16 ? dense_decode_kernel<BF, D, NT, true> : dense_decode_kernel<BF, D, NT, false>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
@@ -540,7 +541,7 @@ int dd_dispatch(const DenseArgs& a, float* parts, DdDesc* desc, cudaStream_t st)
   return one ? dd_launch<BF, 256, 1>(a, parts, desc, st) : dd_launch<BF, 256, 2>(a, parts, desc, st);
 }
 
-size_t dd_desc_bytes() { return ((size_t)sm_count() * sizeof(DdDesc) + 255) / 256 * 256; }
+size_t dd_desc_bytes() { return ((size_t)sm_count() * 2 * sizeof(DdDesc) + 255) / 256 * 256; }
 
 }  // namespace
 
@@ -591,7 +592,7 @@ int dense_common(const akv_dense_attn_params* p, const char* who, DenseArgs* a) 
 AKV_EXPORT size_t akv_dense_paged_attn_workspace_bytes(int num_q_heads, int num_kv_heads, int head_dim) {
   if (num_kv_heads <= 0 || num_q_heads < num_kv_heads || head_dim <= 0) return 0;
   const int heads = num_q_heads / num_kv_heads <= 8 ? 8 : 16;
-  return akv::dd_desc_bytes() + (size_t)akv::sm_count() * 2 * heads * (head_dim + 2) * sizeof(float);
+  return akv::dd_desc_bytes() + (size_t)akv::sm_count() * 4 * heads * (head_dim + 2) * sizeof(float);
 }
 
 AKV_EXPORT int akv_dense_paged_attn(const akv_dense_attn_params* p) {
