@@ -87,11 +87,10 @@ __device__ __forceinline__ DdSpan dd_span(const DenseArgs& a, int s) {
 // What dense_decode_merge_kernel needs to know about the row whose first part CTA c wrote (parts < 2: nothing)
 struct DdDesc { int parts, slot0, s, vh; };
 
-// The CTAs that share T units: as many as are left with DD_MIN_UNITS units each (a warp gets four steps, one round of its
-// ring; a row shorter than that is not worth a second CTA and the join), at most the grid.
-constexpr int DD_MIN_UNITS = 16;
-__device__ __forceinline__ int dd_ctas(int64_t units, int grid) {
-  const int64_t n = units / DD_MIN_UNITS;
+// The CTAs that share T units: as many as are left with `least` units each (four steps per warp, about a round of its ring; a
+// row shorter than that is not worth a second CTA and the join), at most the grid.
+__device__ __forceinline__ int dd_ctas(int64_t units, int grid, int least) {
+  const int64_t n = units / least;
   return n < 1 ? 1 : (n < grid ? (int)n : grid);
 }
 __device__ __forceinline__ int64_t dd_begin(int64_t units, int n, int c) { return units * c / n; }
@@ -103,12 +102,15 @@ struct DdCursor {
   DdSpan span;
 };
 
-template <bool BF, int D, int NT, bool PAGE16>      // PAGE16: 16 aligned keys lie inside one block
+// PAGE16: 16 aligned keys lie inside one block.  HEADS: the CTA's warps take a row each of four neighbouring rows.
+template <bool BF, int D, int NT, bool PAGE16, bool HEADS>
 __global__ void __launch_bounds__(DdL<D, NT>::THREADS, DdL<D, NT>::CTAS)
-dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, DdDesc* desc) {
+dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int rows, float* part_acc, float* part_ml, DdDesc* desc) {
+  // rows: of a sequence; vheads: of the sequence in the list of units (four rows at a time with HEADS)
   using L = DdL<D, NT>;
   constexpr int W = L::W, NS = L::NS, H = L::H, KS = L::KS;
   constexpr int CPR = D / 8, RPP = 32 / CPR, PASSES = KS / RPP;     // 16-byte pieces per row, rows per pass of a warp
+  const int vheads = HEADS ? rows / 4 : rows;
   extern __shared__ __align__(128) uint8_t dd_smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int* pre = reinterpret_cast<int*>(dd_smem + L::PRE);
@@ -150,7 +152,7 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
       for (int e = tid; e < a.num_q_heads * D; e += L::THREADS)
         dense_store<BF>(a.out, (int64_t)(seqs0 + s) * a.out_st + (int64_t)(e / D) * a.out_sh + e % D, 0.f);
   const int64_t units = (int64_t)pre[seqs] * vheads;
-  const int n_ctas = dd_ctas(units, gridDim.x);
+  const int n_ctas = dd_ctas(units, gridDim.x, HEADS ? 4 : 4 * W);
   if ((int)blockIdx.x >= n_ctas || units == 0) {
     if (tid == 0) desc[blockIdx.x] = DdDesc{0, 0, 0, 0};
     return;
@@ -192,16 +194,17 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
   const uint32_t ring = smem_u32(dd_smem) + (uint32_t)(warp * L::RING);
   const char* kbase = reinterpret_cast<const char*>(a.k);
   const char* vbase = reinterpret_cast<const char*>(a.v);
-  const int group = a.num_q_heads / a.num_kv_heads, per_kv = vheads / a.num_kv_heads;
+  const int group = a.num_q_heads / a.num_kv_heads, per_kv = rows / a.num_kv_heads;
+  auto row_of = [&](int vh) -> int { return HEADS ? 4 * vh + warp : vh; };
 
   // ---- producer side: this warp's next step to copy ----
   DdCursor ld = cur;
   bool more = true;
-  ld.t += warp;
+  ld.t += HEADS ? 0 : warp;
   auto settle = [&]() {         // move on to the piece that holds a step for this warp
     while (more && ld.t >= ld.t_end) {
       more = next_piece(ld);
-      ld.t += warp;
+      ld.t += HEADS ? 0 : warp;
     }
   };
   settle();
@@ -218,7 +221,7 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
   auto issue = [&]() {
     if (more) {
       const int key0 = (ld.span.first + ld.t) * KS;
-      const int kvh = ld.vh / per_kv;
+      const int kvh = row_of(ld.vh) / per_kv;
       const uint32_t dk = ring + (uint32_t)(stage_ld * 2 * L::STEP), dv = dk + L::STEP;
       const char *kp = nullptr, *vp = nullptr;
 #pragma unroll
@@ -236,7 +239,7 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
         dd_cp16(dv + off, vp, bytes);
         if (PAGE16) { kp += 2 * RPP * a.k_sp; vp += 2 * RPP * a.v_sp; }
       }
-      ld.t += W;
+      ld.t += HEADS ? 1 : W;
       settle();
       fetch_entry();
     }
@@ -254,7 +257,7 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
   bool first_piece = true;
   bool have = true;
   while (have) {
-    const int kvh = cur.vh / per_kv, h0 = (cur.vh - kvh * per_kv) * H;      // first head of the row inside its group
+    const int row = row_of(cur.vh), kvh = row / per_kv, h0 = (row - kvh * per_kv) * H;      // first head of the row inside its group
     const int n_heads = group - h0 < H ? group - h0 : H;
     uint32_t qb[NT][D / 16][2];
 #pragma unroll
@@ -278,7 +281,7 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
     }
     const int piece_t0 = cur.t;
 #pragma unroll 1
-    for (int t = cur.t + warp; t < cur.t_end; t += W) {
+    for (int t = cur.t + (HEADS ? 0 : warp); t < cur.t_end; t += HEADS ? 1 : W) {
       asm volatile("cp.async.wait_group %0;" :: "n"(NS - 2) : "memory");
       __syncwarp();
       issue();                  // into the stage that the previous step has left
@@ -367,73 +370,103 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
       }
     }
 
-    // ---- join the warps' results in a fixed order ----
-    float* ml = s_ml + parity * W * H * 2;
-    parity ^= 1;
+    const bool whole = piece_t0 == 0 && cur.t_end == cur.span.steps;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], d);
-        if (g == 0) {
-          const int h = nt * 8 + 2 * tq + x;
-          ml[(warp * H + h) * 2] = m[nt][x];
-          ml[(warp * H + h) * 2 + 1] = l[nt][x];
-        }
-      }
-    __syncthreads();            // also: everybody has read the join buffer of the previous piece
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int h = nt * 8 + 2 * tq + x;
-        float top = -CUDART_INF_F;
-#pragma unroll
-        for (int w = 0; w < W; ++w) top = fmaxf(top, ml[(w * H + h) * 2]);
-        const float f = m[nt][x] == -CUDART_INF_F ? 0.f : dense_ex2(m[nt][x] - top);
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) { o[nt][i][x] *= f; o[nt][i][x + 2] *= f; }
-      }
-    auto put = [&](int slot, bool add) {
+    if constexpr (HEADS) {
+      // the row is this warp's alone
+      const int64_t part = (((int64_t)blockIdx.x * 2 + (first_piece ? 0 : 1)) * 4 + warp) * H;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          float* dst = s_o + (slot * H + nt * 8 + 2 * tq + x) * L::OROW + g;
+          const int h = nt * 8 + 2 * tq + x;
+          if (h < n_heads) {
+            const float inv = l[nt][x] == 0.f ? 0.f : 1.f / l[nt][x];
+            const int64_t dst = (int64_t)(seqs0 + cur.s) * a.out_st + (int64_t)(kvh * group + h0 + h) * a.out_sh + g;
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            float v0 = o[nt][i][x], v1 = o[nt][i][x + 2];
-            if (add) { v0 += dst[16 * i]; v1 += dst[16 * i + 8]; }
-            dst[16 * i] = v0;
-            dst[16 * i + 8] = v1;
+            for (int i = 0; i < D / 16; ++i) {
+              if (whole) {
+                dense_store<BF>(a.out, dst + 16 * i, l[nt][x] == 0.f ? 0.f : o[nt][i][x] * inv);
+                dense_store<BF>(a.out, dst + 16 * i + 8, l[nt][x] == 0.f ? 0.f : o[nt][i][x + 2] * inv);
+              } else {
+                part_acc[(part + h) * D + g + 16 * i] = o[nt][i][x];
+                part_acc[(part + h) * D + g + 16 * i + 8] = o[nt][i][x + 2];
+              }
+            }
+            if (!whole && g == 0) reinterpret_cast<float2*>(part_ml)[part + h] = make_float2(m[nt][x], l[nt][x]);
           }
         }
-    };
-    if (warp >= W / 2) put(warp - W / 2, false);
-    __syncthreads();
-    if (warp < W / 2) put(warp, true);
-    __syncthreads();
-    const bool whole = piece_t0 == 0 && cur.t_end == cur.span.steps;
-    float* part = parts + ((int64_t)blockIdx.x * 2 + (first_piece ? 0 : 1)) * H * (D + 2);
-    for (int e = tid; e < n_heads * D; e += L::THREADS) {
-      const int h = e / D, d = e - h * D;
-      float top = -CUDART_INF_F, sum = 0.f, acc = 0.f;
+    } else {
+      // ---- join the warps' results in a fixed order ----
+      float* ml = s_ml + parity * W * H * 2;
+      parity ^= 1;
 #pragma unroll
-      for (int w = 0; w < W; ++w) top = fmaxf(top, ml[(w * H + h) * 2]);
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float mw = ml[(w * H + h) * 2];
-        sum += ml[(w * H + h) * 2 + 1] * (mw == -CUDART_INF_F ? 1.f : dense_ex2(mw - top));      // no keys: 0, or a NaN to pass on
-      }
+        for (int x = 0; x < 2; ++x) {
+          if (g == 0) {
+            const int h = nt * 8 + 2 * tq + x;
+            ml[(warp * H + h) * 2] = m[nt][x];
+            ml[(warp * H + h) * 2 + 1] = l[nt][x];
+          }
+        }
+      __syncthreads();            // also: everybody has read the join buffer of the previous piece
 #pragma unroll
-      for (int w = 0; w < W / 2; ++w) acc += s_o[(w * H + h) * L::OROW + d];
-      if (whole) {
-        dense_store<BF>(a.out, (int64_t)(seqs0 + cur.s) * a.out_st + (int64_t)(kvh * group + h0 + h) * a.out_sh + d,
-                        sum == 0.f ? 0.f : acc / sum);
-      } else {
-        part[h * (D + 2) + 2 + d] = acc;
-        if (d == 0) { part[h * (D + 2)] = top; part[h * (D + 2) + 1] = sum; }
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int h = nt * 8 + 2 * tq + x;
+          float top = -CUDART_INF_F;
+#pragma unroll
+          for (int w = 0; w < W; ++w) top = fmaxf(top, ml[(w * H + h) * 2]);
+          const float f = m[nt][x] == -CUDART_INF_F ? 0.f : dense_ex2(m[nt][x] - top);
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) { o[nt][i][x] *= f; o[nt][i][x + 2] *= f; }
+        }
+      auto put = [&](int slot, bool add) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float* dst = s_o + (slot * H + nt * 8 + 2 * tq + x) * L::OROW + g;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              float v0 = o[nt][i][x], v1 = o[nt][i][x + 2];
+              if (add) { v0 += dst[16 * i]; v1 += dst[16 * i + 8]; }
+              dst[16 * i] = v0;
+              dst[16 * i + 8] = v1;
+            }
+          }
+      };
+      if (warp >= W / 2) put(warp - W / 2, false);
+      __syncthreads();
+      if (warp < W / 2) put(warp, true);
+      __syncthreads();
+      const int64_t part = ((int64_t)blockIdx.x * 2 + (first_piece ? 0 : 1)) * H;
+      for (int e = tid; e < n_heads * D; e += L::THREADS) {
+        const int h = e / D, d = e - h * D;
+        float top = -CUDART_INF_F, sum = 0.f, acc = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) top = fmaxf(top, ml[(w * H + h) * 2]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float mw = ml[(w * H + h) * 2];
+          sum += ml[(w * H + h) * 2 + 1] * (mw == -CUDART_INF_F ? 1.f : dense_ex2(mw - top));      // no keys: 0, or a NaN to pass on
+        }
+#pragma unroll
+        for (int w = 0; w < W / 2; ++w) acc += s_o[(w * H + h) * L::OROW + d];
+        if (whole) {
+          dense_store<BF>(a.out, (int64_t)(seqs0 + cur.s) * a.out_st + (int64_t)(kvh * group + h0 + h) * a.out_sh + d,
+                          sum == 0.f ? 0.f : acc / sum);
+        } else {
+          part_acc[(part + h) * D + d] = acc;
+          if (d == 0) reinterpret_cast<float2*>(part_ml)[part + h] = make_float2(top, sum);
+        }
       }
     }
     if (cur.left <= 0 && tid == 0) {          // the last piece: a row that begins here and ends in another CTA's range?
@@ -454,58 +487,76 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int vheads, float* parts, 
 }
 
 // Rows whose steps fell into several CTAs' ranges: out = sum_p 2^(m_p - M) acc_p / sum_p 2^(m_p - M) l_p, parts in the
-// order of the keys.  Block c: the row that CTA c began.
+// order of the keys.  A warp takes one query head of one such row.  What it costs is latency: one block per SM (starting a
+// block takes some 10 ns), every warp with a CTA of its own to look after, and the reads of eight parts, their maxima and
+// sums among them, on their way together (the maximum runs along; parts in groups of eight are enough for most rows).
+constexpr int DM_THREADS = 1024;
 template <bool BF, int D, int NT>
-__global__ void __launch_bounds__(256)
-dense_decode_merge_kernel(DenseArgs a, int vheads, const float* parts, const DdDesc* desc) {
-  constexpr int H = 8 * NT, P = D + 2;
-  extern __shared__ float dm_f[];          // [n_parts][H] factors
-  __shared__ float s_inv[H];
+__global__ void __launch_bounds__(DM_THREADS)
+dense_decode_merge_kernel(DenseArgs a, int rows, int per, int ctas, const float* part_acc, const float* part_ml, const DdDesc* desc) {
+  constexpr int H = 8 * NT, V = D / 64;      // V pairs of columns per lane
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const DdDesc d = desc[blockIdx.x];
-  if (d.parts < 2) return;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int group = a.num_q_heads / a.num_kv_heads, per_kv = vheads / a.num_kv_heads;
-  const int kvh = d.vh / per_kv, h0 = (d.vh - kvh * per_kv) * H;
-  const int n_heads = group - h0 < H ? group - h0 : H;
-  // later parts begin where their CTA's range begins
-  auto part = [&](int i) -> const float* { return parts + ((int64_t)(blockIdx.x + i) * 2 + (i == 0 ? d.slot0 : 0)) * H * P; };
-  for (int h = warp; h < n_heads; h += 8) {
-    float top = -CUDART_INF_F;
-    for (int p = lane; p < d.parts; p += 32) {
-      const float mp = part(p)[h * P];
-      dm_f[p * H + h] = mp;
-      top = fmaxf(top, mp);
-    }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = a.num_q_heads / a.num_kv_heads, per_kv = rows / a.num_kv_heads;
+  const int heads = group < H ? group : H, mine = (ctas - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+  for (int job = warp; job < mine * per * heads; job += DM_THREADS / 32) {
+    const int c = blockIdx.x + job / (per * heads) * gridDim.x, y = job / heads % per, h = job % heads;
+    const DdDesc d = desc[c];
+    if (d.parts < 2) continue;
+    const int row = d.vh * per + y, kvh = row / per_kv, h0 = (row - kvh * per_kv) * H;
+    if (h >= group - h0) continue;
+    // later parts begin where their CTA's range begins
+    auto at = [&](int i) -> int64_t { return (((int64_t)(c + i) * 2 + (i == 0 ? d.slot0 : 0)) * per + y) * H + h; };
+    float top = -CUDART_INF_F, sum = 0.f;
+    float2 acc[V];
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    float sum = 0.f;
-    for (int p = lane; p < d.parts; p += 32) {
-      const float mp = dm_f[p * H + h], f = mp == -CUDART_INF_F ? 0.f : dense_ex2(mp - top);
-      dm_f[p * H + h] = f;
-      sum += f * part(p)[h * P + 1];
-    }
+    for (int i = 0; i < V; ++i) acc[i] = make_float2(0.f, 0.f);
+    constexpr int B = D == 256 ? 4 : 8;
+    for (int base = 0; base < d.parts; base += B) {
+      float2 ml[B], v[B][V];
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    if (lane == 0) s_inv[h] = sum == 0.f ? 0.f : 1.f / sum;
-  }
-  __syncthreads();
-  for (int e = tid; e < n_heads * D; e += 256) {
-    const int h = e / D, x = e - h * D;
-    float acc = 0.f;
-#pragma unroll 4
-    for (int p = 0; p < d.parts; ++p) acc += dm_f[p * H + h] * part(p)[h * P + 2 + x];
-    dense_store<BF>(a.out, (int64_t)d.s * a.out_st + (int64_t)(kvh * group + h0 + h) * a.out_sh + x, acc * s_inv[h]);
+      for (int p = 0; p < B; ++p) {
+        const bool there = base + p < d.parts;
+        ml[p] = there ? reinterpret_cast<const float2*>(part_ml)[at(base + p)] : make_float2(-CUDART_INF_F, 0.f);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          v[p][i] = there ? reinterpret_cast<const float2*>(part_acc + at(base + p) * D)[lane + 32 * i] : make_float2(0.f, 0.f);
+      }
+      float t = top;
+#pragma unroll
+      for (int p = 0; p < B; ++p) t = fmaxf(t, ml[p].x);
+      const float f0 = top == -CUDART_INF_F ? 0.f : dense_ex2(top - t);
+      sum *= f0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) { acc[i].x *= f0; acc[i].y *= f0; }
+      top = t;
+#pragma unroll
+      for (int p = 0; p < B; ++p) {
+        const float f = ml[p].x == -CUDART_INF_F ? 0.f : dense_ex2(ml[p].x - t);
+        sum += f * ml[p].y;
+#pragma unroll
+        for (int i = 0; i < V; ++i) { acc[i].x += f * v[p][i].x; acc[i].y += f * v[p][i].y; }
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (int64_t)d.s * a.out_st + (int64_t)(kvh * group + h0 + h) * a.out_sh) + lane;
+#pragma unroll
+    for (int i = 0; i < V; ++i) dst[32 * i] = dense_pack<BF>(acc[i].x * inv, acc[i].y * inv);
   }
 }
 
 template <bool BF, int D, int NT>
-int dd_launch(const DenseArgs& a, float* parts, DdDesc* desc, cudaStream_t st) {
+int dd_launch(const DenseArgs& a, float* part_acc, float* part_ml, DdDesc* desc, cudaStream_t st) {
   using L = DdL<D, NT>;
   const int group = a.num_q_heads / a.num_kv_heads;
   const int vheads = a.num_kv_heads * ((group + L::H - 1) / L::H), grid = L::CTAS * sm_count();
   const bool page16 = a.block_size % 16 == 0;
-  auto kernel = page16 ? dense_decode_kernel<BF, D, NT, true> : dense_decode_kernel<BF, D, NT, false>;
+  // head_dim 64: four rows side by side, a warp each, where a sequence's rows come in fours.  Neighbouring heads of a key are
+  // then read at the same time; its 128-byte pieces alone reach half of the HBM rate (200 windowed sequences x 8 heads: 93 us
+  // with the keys shared out among the warps, 70 us this way).  At head_dim 128 that is 162 us against 169 (16 long sequences).
+  const bool heads = D == 64 && vheads % 4 == 0;
+  auto kernel = heads ? (page16 ? dense_decode_kernel<BF, D, NT, true, true> : dense_decode_kernel<BF, D, NT, false, true>)
+                      : (page16 ? dense_decode_kernel<BF, D, NT, true, false> : dense_decode_kernel<BF, D, NT, false, false>);
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
   if (e != cudaSuccess) return fail((int)e, "dense attention: smem attribute: %s", cudaGetErrorString(e));
   // sequences of one launch: prefix sums in shared memory, and of fewer than 2^31 steps even if every sequence were full
@@ -514,19 +565,18 @@ int dd_launch(const DenseArgs& a, float* parts, DdDesc* desc, cudaStream_t st) {
   if (full * most > 0x7fffffffll) most = (int)(0x7fffffffll / full);
   for (int s0 = 0; s0 < a.num_seqs; s0 += most) {
     const int seqs = a.num_seqs - s0 < most ? a.num_seqs - s0 : most;
-    kernel<<<grid, L::THREADS, L::SMEM, st>>>(a, s0, seqs, vheads, parts, desc);
+    kernel<<<grid, L::THREADS, L::SMEM, st>>>(a, s0, seqs, vheads, part_acc, part_ml, desc);
     if (int rc = check_launch("dense_decode_attn_kernel")) return rc;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at{};
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = (size_t)grid * L::H * sizeof(float);
+    cfg.gridDim = dim3((unsigned)sm_count());
+    cfg.blockDim = dim3(DM_THREADS);
     cfg.stream = st;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, dense_decode_merge_kernel<BF, D, NT>, a, vheads, (const float*)parts, (const DdDesc*)desc);
+    e = cudaLaunchKernelEx(&cfg, dense_decode_merge_kernel<BF, D, NT>, a, vheads, heads ? 4 : 1, grid, (const float*)part_acc, (const float*)part_ml, (const DdDesc*)desc);
     if (e != cudaSuccess) return fail((int)e, "dense attention merge: %s", cudaGetErrorString(e));
     if (int rc = check_launch("dense_decode_merge_kernel")) return rc;
   }
@@ -534,11 +584,11 @@ int dd_launch(const DenseArgs& a, float* parts, DdDesc* desc, cudaStream_t st) {
 }
 
 template <bool BF>
-int dd_dispatch(const DenseArgs& a, float* parts, DdDesc* desc, cudaStream_t st) {
+int dd_dispatch(const DenseArgs& a, float* part_acc, float* part_ml, DdDesc* desc, cudaStream_t st) {
   const bool one = a.num_q_heads / a.num_kv_heads <= 8;
-  if (a.head_dim == 64) return one ? dd_launch<BF, 64, 1>(a, parts, desc, st) : dd_launch<BF, 64, 2>(a, parts, desc, st);
-  if (a.head_dim == 128) return one ? dd_launch<BF, 128, 1>(a, parts, desc, st) : dd_launch<BF, 128, 2>(a, parts, desc, st);
-  return one ? dd_launch<BF, 256, 1>(a, parts, desc, st) : dd_launch<BF, 256, 2>(a, parts, desc, st);
+  if (a.head_dim == 64) return one ? dd_launch<BF, 64, 1>(a, part_acc, part_ml, desc, st) : dd_launch<BF, 64, 2>(a, part_acc, part_ml, desc, st);
+  if (a.head_dim == 128) return one ? dd_launch<BF, 128, 1>(a, part_acc, part_ml, desc, st) : dd_launch<BF, 128, 2>(a, part_acc, part_ml, desc, st);
+  return one ? dd_launch<BF, 256, 1>(a, part_acc, part_ml, desc, st) : dd_launch<BF, 256, 2>(a, part_acc, part_ml, desc, st);
 }
 
 size_t dd_desc_bytes() { return ((size_t)sm_count() * 2 * sizeof(DdDesc) + 255) / 256 * 256; }
@@ -588,11 +638,11 @@ int dense_common(const akv_dense_attn_params* p, const char* who, DenseArgs* a) 
 
 }  // namespace akv
 
-// Two partial rows per CTA, and what the merge has to know.
+// Two times up to four partial rows for each of up to two CTAs per SM, and what the merge has to know.
 AKV_EXPORT size_t akv_dense_paged_attn_workspace_bytes(int num_q_heads, int num_kv_heads, int head_dim) {
   if (num_kv_heads <= 0 || num_q_heads < num_kv_heads || head_dim <= 0) return 0;
   const int heads = num_q_heads / num_kv_heads <= 8 ? 8 : 16;
-  return akv::dd_desc_bytes() + (size_t)akv::sm_count() * 4 * heads * (head_dim + 2) * sizeof(float);
+  return akv::dd_desc_bytes() + (size_t)akv::sm_count() * 16 * heads * (head_dim + 2) * sizeof(float);
 }
 
 AKV_EXPORT int akv_dense_paged_attn(const akv_dense_attn_params* p) {
@@ -605,7 +655,8 @@ AKV_EXPORT int akv_dense_paged_attn(const akv_dense_attn_params* p) {
   if (!p->workspace || p->workspace_bytes < need || ((uintptr_t)p->workspace & 15))
     return akv::fail(AKV_ERR_WORKSPACE, "akv_dense_paged_attn: workspace of %zu bytes (16-byte aligned) needed, got %zu", need, p->workspace_bytes);
   akv::DdDesc* desc = reinterpret_cast<akv::DdDesc*>(p->workspace);
-  float* parts = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + akv::dd_desc_bytes());
+  float* part_acc = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + akv::dd_desc_bytes());
+  float* part_ml = part_acc + (size_t)akv::sm_count() * 16 * (a.num_q_heads / a.num_kv_heads <= 8 ? 8 : 16) * a.head_dim;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(p->stream);
-  return p->dtype == AKV_BF16 ? akv::dd_dispatch<true>(a, parts, desc, st) : akv::dd_dispatch<false>(a, parts, desc, st);
+  return p->dtype == AKV_BF16 ? akv::dd_dispatch<true>(a, part_acc, part_ml, desc, st) : akv::dd_dispatch<false>(a, part_acc, part_ml, desc, st);
 }

@@ -902,44 +902,74 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
   }
 }
 
-// Row tiles that were cut: out = sum_p 2^(m_p - M) acc_p / sum_p 2^(m_p - M) l_p in the order of the keys.  Block (c, y, r):
-// rows 32 y .. + 31 of the row tile that CTA c began in round r; a thread takes 4 columns of one row, neighbouring threads
-// neighbouring rows (the partials' layout).
+// Row tiles that were cut: out = sum_p 2^(m_p - M) acc_p / sum_p 2^(m_p - M) l_p in the order of the keys.  Block (c, y):
+// rows 128 y .. + 127 of the row tiles that CTA c began, round by round; a thread takes 16 columns of one row (a 32-byte sector), neighbouring
+// threads neighbouring rows (the partials' layout).  Two blocks per SM: starting a
+// block costs some 10 ns.  The first parts' maxima, sums and columns are read together (most row tiles have two).
+constexpr int PM_THREADS = 1024;
 template <bool BF, int D>
-__global__ void __launch_bounds__(256)
-dense_prefill_merge_kernel(DenseArgs a, int G, int TT, int tail, const DpDesc* desc, const float* part_ml, const float* part_acc) {
+__global__ void __launch_bounds__(PM_THREADS)
+dense_prefill_merge_kernel(DenseArgs a, int G, int TT, int rounds, int tail, const DpDesc* desc, const float* part_ml, const float* part_acc) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (tail >= 0 && blockIdx.z == 0) {      // rows behind the last sequence (`tail` of them in this launch) come out as zeros
+  if (tail >= 0) {              // rows behind the last sequence (`tail` of them in this launch) come out as zeros
     int64_t row = load_index(a.starts, a.qs_dtype, tail);
     if (row < 0) row = 0;
     for (row += blockIdx.y * gridDim.x + blockIdx.x; row < a.n_tokens; row += gridDim.x * gridDim.y)
-      for (int e = threadIdx.x; e < a.num_q_heads * (D / 8); e += 256)
+      for (int e = threadIdx.x; e < a.num_q_heads * (D / 8); e += PM_THREADS)
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.out_st + (int64_t)(e / (D / 8)) * a.out_sh + e % (D / 8) * 8) =
             make_uint4(0u, 0u, 0u, 0u);
   }
-  const DpDesc d = desc[blockIdx.z * gridDim.x + blockIdx.x];
-  if (d.parts < 2) return;
-  constexpr int ROWS = 256 / (D / 4);      // rows of the block at a time
-  const int c4 = threadIdx.x / ROWS;
-  for (int r = blockIdx.y * 32 + threadIdx.x % ROWS; r < blockIdx.y * 32 + 32; r += ROWS) {
-    const int in_half = r & 127, t = in_half / G, tok = (r >> 7) * TT + t;
-    if (t >= TT || tok >= d.ntok) continue;
-    auto slot = [&](int p) -> int64_t { return ((int64_t)blockIdx.z * gridDim.x + blockIdx.x + p) * 2 + (p == 0 ? d.slot0 : 0); };
-    float top = -CUDART_INF_F;
-    for (int p = 0; p < d.parts; ++p) top = fmaxf(top, part_ml[(slot(p) * 256 + r) * 2]);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-    for (int p = 0; p < d.parts; ++p) {
-      const float2 ml = *reinterpret_cast<const float2*>(part_ml + (slot(p) * 256 + r) * 2);
-      if (ml.x == -CUDART_INF_F) continue;      // the part saw no key of this row
-      const float f = dense_ex2(ml.x - top);
-      const float4 v = reinterpret_cast<const float4*>(part_acc)[slot(p) * 64 * D + c4 * 256 + r];
-      sum += f * ml.y;
-      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+  for (int z = 0; z < rounds; ++z) {
+    const DpDesc d = desc[z * gridDim.x + blockIdx.x];
+    if (d.parts < 2) continue;
+    for (int item = threadIdx.x; item < 128 * (D / 16); item += PM_THREADS) {
+      const int in_half = item & 127, r = blockIdx.y * 128 + in_half, c16 = item >> 7, t = in_half / G, tok = (int)blockIdx.y * TT + t;
+      if (t >= TT || tok >= d.ntok) continue;
+      auto slot = [&](int p) -> int64_t { return ((int64_t)z * gridDim.x + blockIdx.x + p) * 2 + (p == 0 ? d.slot0 : 0); };
+      float top = -CUDART_INF_F, sum = 0.f;
+      float4 acc[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      constexpr int B = 2;
+      for (int base = 0; base < d.parts; base += B) {
+        float2 ml[B];
+        float4 v[B][4];
+#pragma unroll
+        for (int p = 0; p < B; ++p) {
+          const bool there = base + p < d.parts;
+          ml[p] = there ? *reinterpret_cast<const float2*>(part_ml + (slot(base + p) * 256 + r) * 2) : make_float2(-CUDART_INF_F, 0.f);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            v[p][k] = there ? reinterpret_cast<const float4*>(part_acc)[slot(base + p) * 64 * D + (4 * c16 + k) * 256 + r] : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float t2 = top;
+#pragma unroll
+        for (int p = 0; p < B; ++p) t2 = fmaxf(t2, ml[p].x);
+        const float f0 = top == -CUDART_INF_F ? 0.f : dense_ex2(top - t2);
+        sum *= f0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { acc[k].x *= f0; acc[k].y *= f0; acc[k].z *= f0; acc[k].w *= f0; }
+        top = t2;
+#pragma unroll
+        for (int p = 0; p < B; ++p) {
+          if (ml[p].x == -CUDART_INF_F) continue;      // the part saw no key of this row
+          const float f = dense_ex2(ml[p].x - t2);
+          sum += f * ml[p].y;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) { acc[k].x += f * v[p][k].x; acc[k].y += f * v[p][k].y; acc[k].z += f * v[p][k].z; acc[k].w += f * v[p][k].w; }
+        }
+      }
+      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+      uint32_t o[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        o[2 * k] = dense_pack<BF>(acc[k].x * inv, acc[k].y * inv);
+        o[2 * k + 1] = dense_pack<BF>(acc[k].z * inv, acc[k].w * inv);
+      }
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (int64_t)(d.row0 + tok) * a.out_st + (int64_t)(d.kvh * G + in_half - t * G) * a.out_sh + 16 * c16);
+      dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+      dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
     }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (int64_t)(d.row0 + tok) * a.out_st + (int64_t)(d.kvh * G + in_half - t * G) * a.out_sh + 4 * c4) =
-        make_uint2(dense_pack<BF>(acc.x * inv, acc.y * inv), dense_pack<BF>(acc.z * inv, acc.w * inv));
   }
 }
 
@@ -1030,9 +1060,9 @@ int dp_launch(const DenseArgs& all, const DpMaps& maps, int G, int TT, int box, 
     if (e != cudaSuccess) return fail((int)e, "dense prefill attention: %s", cudaGetErrorString(e));
     if (int rc = check_launch("dense_prefill_attn_kernel")) return rc;
     cfg.dynamicSmemBytes = 0;
-    cfg.gridDim = dim3((unsigned)grid, 8, (unsigned)rounds);
-    cfg.blockDim = dim3(256);
-    e = cudaLaunchKernelEx(&cfg, dense_prefill_merge_kernel<BF, D>, a, G, TT, zero_tail && s0 + seqs == all.num_seqs ? seqs : -1, (const DpDesc*)w.desc, (const float*)w.ml, (const float*)w.acc);
+    cfg.gridDim = dim3((unsigned)grid, 2);
+    cfg.blockDim = dim3(PM_THREADS);
+    e = cudaLaunchKernelEx(&cfg, dense_prefill_merge_kernel<BF, D>, a, G, TT, rounds, zero_tail && s0 + seqs == all.num_seqs ? seqs : -1, (const DpDesc*)w.desc, (const float*)w.ml, (const float*)w.acc);
     if (e != cudaSuccess) return fail((int)e, "dense prefill merge: %s", cudaGetErrorString(e));
     if (int rc = check_launch("dense_prefill_merge_kernel")) return rc;
   }
