@@ -11,10 +11,10 @@ from aitherkvcache_b200 import *  # noqa: F401,F403
 from aitherkvcache_b200 import __all__, __version__  # noqa: F401
 
 _SUBMODULES = ("quantizer", "codebook", "rotation", "packing", "fused_attention", "fused_kv_update",
-               "hybrid_quantizer", "parallel", "triattention", "triattention.config", "triattention.encoder",
+               "rotary", "dense_kv", "hybrid_quantizer", "parallel", "triattention", "triattention.config", "triattention.encoder",
                "triattention.attention", "triattention.spectral", "vllm", "vllm.ops", "vllm.backend", "vllm.plugin")
 for _name in _SUBMODULES:
     sys.modules[f"{__name__}.{_name}"] = importlib.import_module(f"aitherkvcache_b200.{_name}")
 for _name in ("quantizer", "codebook", "rotation", "packing", "fused_attention", "fused_kv_update",
-              "hybrid_quantizer", "parallel", "triattention", "vllm"):
+              "rotary", "dense_kv", "hybrid_quantizer", "parallel", "triattention", "vllm"):
     setattr(sys.modules[__name__], _name, sys.modules[f"{__name__}.{_name}"])

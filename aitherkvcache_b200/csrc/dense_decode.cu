@@ -608,7 +608,7 @@ int dense_common(const akv_dense_attn_params* p, const char* who, DenseArgs* a) 
   if ((int64_t)p->max_blocks_per_seq * p->block_size > 0x7fffff00ll)
     return fail(AKV_ERR_UNSUPPORTED, "%s: %d blocks of %d per sequence pass 2^31 keys", who, p->max_blocks_per_seq, p->block_size);
   if ((p->bt_dtype | p->sl_dtype | p->qs_dtype) & ~1) return fail(AKV_ERR_ARG, "%s: unknown index type", who);
-  if (!(p->scale == p->scale)) return fail(AKV_ERR_ARG, "%s: scale is not a number", who);
+  if (!(p->scale > 0.f && p->scale <= 1.0e38f)) return fail(AKV_ERR_ARG, "%s: scale %g (positive and finite)", who, (double)p->scale);
   if (p->num_tokens > 0 && p->num_seqs > 0) {
     if (!p->query || !p->out || !p->seq_lens) return fail(AKV_ERR_ARG, "%s: null query, out or lengths", who);
     if (p->max_blocks_per_seq > 0 && (!p->block_tables || !p->k_cache || !p->v_cache || p->num_blocks == 0))

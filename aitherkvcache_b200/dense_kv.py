@@ -6,6 +6,7 @@ vLLM's kernels; here they run in ``akv_rotary_kv_append``, ``akv_dense_paged_att
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Optional
 
@@ -70,6 +71,31 @@ def rotary_kv_append(query: Optional[torch.Tensor], key: torch.Tensor, value: to
     return query_out
 
 
+def kv_append(key: torch.Tensor, value: torch.Tensor, slot_mapping: torch.Tensor, k_cache: torch.Tensor,
+              v_cache: torch.Tensor) -> None:
+    """``rotary_kv_append`` of keys that carry their rotation already (or need none): ``key`` and ``value`` [tokens, heads,
+    head_dim] go to their slots as they are, converted to the caches' dtype."""
+    index = _lib.cuda_index(key, value, slot_mapping, k_cache, v_cache)
+    if key.dim() != 3 or value.shape != key.shape or value.dtype != key.dtype:
+        raise ValueError(f"key {tuple(key.shape)} {key.dtype} and value {tuple(value.shape)} {value.dtype} must be one [tokens, heads, "
+                         "head_dim]")
+    tokens, heads, head_dim = key.shape
+    shape, ks, vs = _check_caches(k_cache, v_cache, heads, head_dim)
+    key, value = (x if x.stride(2) == 1 else x.contiguous() for x in (key, value))
+    if slot_mapping.dim() != 1 or slot_mapping.shape[0] != tokens:
+        raise ValueError(f"slot_mapping {tuple(slot_mapping.shape)} must be [{tokens}]")
+    if tokens and not (shape[0] and shape[1]):
+        raise ValueError(f"caches {tuple(shape)} hold no slot")
+    slot_mapping = slot_mapping.contiguous()
+    tables = _lib.RotaryTables(head_dim, 0, 1, 0, None, None, 1.0)      # nothing is rotated
+    k, v = key.stride(), value.stride()
+    _lib.call(index, "akv_rotary_kv_append", _pack_append(
+        ctypes.addressof(tables), 0, 0, 0, 0, tokens, _lib.float_code(key), _lib.float_code(k_cache), 0, 0, 0, 0, 0, 0, 0,
+        key.data_ptr(), k[0], k[1], heads, 0, 0, 0, 0, _lib.raw_stream(index),
+        value.data_ptr(), v[0], v[1], slot_mapping.data_ptr(), _lib.index_code(slot_mapping),
+        k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2], shape[1], shape[0]))
+
+
 class DensePagedAttention:
     """``DensePagedAttention(head_dim, query_heads, kv_heads).forward(query, k_cache, v_cache, block_tables, context_lens)``.
 
@@ -87,6 +113,8 @@ class DensePagedAttention:
             raise ValueError(f"head_dim must be 64, 128 or 256, got {head_dim}")
         if num_kv_heads <= 0 or num_query_heads <= 0 or num_query_heads % num_kv_heads:
             raise ValueError(f"{num_query_heads} query heads are not a multiple of {num_kv_heads} KV heads")
+        if scale is not None and not (0.0 < scale < math.inf):
+            raise ValueError(f"scale must be positive and finite, got {scale}")
         if sliding_window < 0:
             raise ValueError(f"sliding_window must not be negative, got {sliding_window}")
         self.head_dim, self.num_query_heads, self.num_kv_heads = head_dim, num_query_heads, num_kv_heads
@@ -136,7 +164,7 @@ class DensePagedAttention:
         ``block_tables`` [num_seqs, max_blocks].  Returns ``out`` [num_seqs, query_heads, head_dim]."""
         index = _lib.cuda_index(query, k_cache, v_cache, block_tables, context_lens, out)
         values, out, keep = self._values(query, k_cache, v_cache, block_tables, context_lens, (0, 0), query.shape[0], out)
-        ws = torch.empty(self._decode_bytes, dtype=torch.uint8, device=out.device)
+        ws = out.new_empty((self._decode_bytes + 1) // 2)      # half the host time of torch.empty
         _lib.call(index, "akv_dense_paged_attn", _pack_attn(*values, 0, ws.data_ptr(), self._decode_bytes, _lib.raw_stream(index)))
         return out
 
@@ -165,7 +193,7 @@ class DensePagedAttention:
                 out.zero_()
             return self._prefill_by_rows(query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, out)
         nbytes = _lib.lib().akv_dense_prefill_attn_workspace_bytes(self.num_kv_heads, self.head_dim, blocks, block_size, num_seqs, width)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=out.device)
+        ws = out.new_empty((nbytes + 1) // 2)
         _lib.call(index, "akv_dense_prefill_attn", _pack_attn(*values, int(zero_tail), ws.data_ptr(), nbytes, _lib.raw_stream(index)))
         return out
 

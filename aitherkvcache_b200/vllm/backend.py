@@ -12,6 +12,10 @@ with its own causal context length and its sequence's block-table row, built on 
 without a host synchronisation.  Nothing is decompressed to fp16.  The reference's shadow mode,
 cold tier and block selection are not part of this build.
 
+A layer whose cache tensor is fp16 or bf16 stays uncompressed (a cache dtype of ``auto`` or ``bfloat16`` outside primary
+mode, or the layers that vLLM exempts from the compressed dtype): it is written by ``kv_append`` / ``rotary_kv_append`` and
+attended by ``DensePagedAttention`` (``dense_kv.py``) behind the same methods, block tables and slots.
+
 The codec is picked like the reference does (``vllm/backend.py:618-626``): ``AITHER_TQ_MODE=tq35``
 selects the hybrid codec, otherwise ``AITHER_TQ_BITS`` (default 4) the uniform one; a
 ``tq-t4nc`` / ``tq-t3nc`` / ``tq-t2nc`` / ``tq-t35nc`` cache-dtype string overrides both.  The
@@ -28,6 +32,7 @@ import torch
 
 KV_DTYPE_BITS = {"tq-t4nc": 4, "tq-t3nc": 3, "tq-t2nc": 2}
 KV_DTYPE_HYBRID = {"tq-t35nc": "tq35", "tq-t25nc": "tq25"}
+DENSE_DTYPES = (torch.float16, torch.bfloat16)      # cache tensors of layers that stay uncompressed
 
 
 def bits_from_env_or_dtype(cache_dtype_str: Optional[str] = None) -> int:
@@ -165,7 +170,12 @@ class TurboQuantImplBase:
         return kn, _LayerState.v_norms[layer_name]
 
     def do_kv_cache_update(self, layer, key, value, kv_cache, slot_mapping) -> None:
-        """Encode ``key`` / ``value`` [tokens, kv_heads, head_size] into the packed cache in place."""
+        """Encode ``key`` / ``value`` [tokens, kv_heads, head_size] into the packed cache in place (a 16-bit cache takes them
+        as they are)."""
+        if kv_cache.dtype in DENSE_DTYPES:
+            from ..dense_kv import kv_append
+            kv_append(key[:slot_mapping.shape[0]], value[:slot_mapping.shape[0]], slot_mapping, kv_cache[:, 0], kv_cache[:, 1])
+            return
         pd, bs = self.packed_dim, kv_cache.shape[2]
         if self.tq_codec == "hybrid":
             from ..hybrid_quantizer import hybrid_kv_update
@@ -180,7 +190,36 @@ class TurboQuantImplBase:
             fused_tq4_kv_update(x, slot_mapping, rows, norms, tq.rotation,
                                 tq.boundaries_inner, bs, kv_cache.shape[0], rotation_t=tq.rotation_T)
 
+    def rope_and_kv_cache_update(self, layer, query, key, value, positions, rope, kv_cache, slot_mapping, query_out=None):
+        """``do_kv_cache_update`` of keys that are not rotated yet: ``query`` [tokens, heads, head_size] and ``key`` are turned
+        to ``positions`` by ``rope`` (a ``RotaryPositions``) on the way.  Returns the rotated query.  One launch for a 16-bit
+        cache; in front of the codecs the rotation is a launch of its own."""
+        if kv_cache.dtype in DENSE_DTYPES:
+            from ..dense_kv import rotary_kv_append
+            return rotary_kv_append(query, key, value, positions, slot_mapping, kv_cache[:, 0], kv_cache[:, 1], rope, query_out)
+        query_out, key = rope.forward(query, key, positions, query_out=query_out)
+        self.do_kv_cache_update(layer, key, value, kv_cache, slot_mapping)
+        return query_out
+
+    def _dense_attention(self, kv_cache: torch.Tensor):
+        """The attention object of this impl's uncompressed layers; ``sliding_window`` as vLLM's impls keep it: None, a number
+        of tokens, or (tokens to the left, tokens to the right) with -1 for no limit."""
+        window = getattr(self, "sliding_window", None)
+        if isinstance(window, (tuple, list)):
+            window = window[0] + 1 if window and window[0] >= 0 else 0
+        window = int(window or 0)
+        key_ = ("dense", self.head_size, self.num_heads, self.num_kv_heads, self.scale, window, str(kv_cache.device))
+        attn = _LayerState.attention.get(key_)
+        if attn is None:
+            from ..dense_kv import DensePagedAttention
+            attn = DensePagedAttention(self.head_size, self.num_heads, self.num_kv_heads, scale=self.scale, sliding_window=window)
+            _LayerState.attention[key_] = attn
+        return attn
+
     def _attend(self, layer, q, out, kv_cache, block_table, context_lens) -> None:
+        if kv_cache.dtype in DENSE_DTYPES:
+            self._dense_attention(kv_cache).forward(q, kv_cache[:, 0], kv_cache[:, 1], block_table, context_lens, out=out)
+            return
         pd, bs = self.packed_dim, kv_cache.shape[2]
         kc, vc = self._codes(kv_cache)
         key_ = (self.head_size, self.tq_codec, self.tq_mode or self.tq_bits, self.num_heads, str(kv_cache.device))
@@ -207,6 +246,10 @@ class TurboQuantImplBase:
         one pass over its packed blocks); False when they are not built for the case (3- / 2-bit codes in a batch too
         ragged for the staged tensor-core kernel, rows that are not readable in 16-byte pieces), in which case every
         token becomes a row of the decode kernels."""
+        if kv_cache.dtype in DENSE_DTYPES:
+            self._dense_attention(kv_cache).prefill(q, kv_cache[:, 0], kv_cache[:, 1], md.block_table, md.seq_lens,
+                                                    md.query_start_loc, out=out)
+            return True
         pd, bs = self.packed_dim, kv_cache.shape[2]
         if self.tq_codec == "hybrid":      # tq35 records: staged tensor-core kernel over decoded operand images
             key_ = (self.head_size, self.tq_codec, self.tq_mode or self.tq_bits, self.num_heads, str(kv_cache.device))

@@ -471,7 +471,7 @@ int akv_rotary_kv_append(const akv_rotary_append_params* params);
  * num_kv_heads, head_dim] and out [num_tokens, num_q_heads, head_dim] all of `dtype` (AKV_F16 / AKV_BF16), any strides whose
  * rows start on 16-byte boundaries, last dimension contiguous; num_q_heads a multiple of num_kv_heads; head_dim 64, 128 or
  * 256; any block_size.  block_tables [num_seqs, max_blocks_per_seq] and seq_lens [num_seqs] int32 / int64; entries outside
- * the pool are clamped to it, lengths to [0, max_blocks_per_seq * block_size].  window 0, or the number of keys a token
+ * the pool are clamped to it, lengths to [0, max_blocks_per_seq * block_size].  scale positive and finite.  window 0, or the number of keys a token
  * sees, itself included.  A row that sees no key is zero.  Pages behind a sequence's end may hold anything, NaN included.
  *
  * akv_dense_paged_attn: one token per sequence, row s of query and out, the last of its seq_lens[s] tokens (rows behind

@@ -135,3 +135,76 @@ def test_dense_structures_match_the_header_layout(tmp_path):
         body = re.sub(r"/\*.*?\*/", "", re.search(r"typedef struct %s \{(.*?)\} %s;" % (cname, cname), header, re.S).group(1), flags=re.S)
         names = [re.findall(r"[A-Za-z_]\w*", part)[-1] for decl in body.split(";") if decl.strip() for part in decl.split(",")]
         assert names == [f for f, _ in st._fields_], cname
+
+
+def test_attention_refuses():
+    from aitherkvcache_b200 import DensePagedAttention
+    for args, kw in (((96, 8, 2), {}), ((128, 7, 2), {}), ((128, 0, 1), {}), ((128, 4, 0), {}), ((128, 4, 2), dict(sliding_window=-1)),
+                     ((128, 4, 2), dict(scale=0.0)), ((128, 4, 2), dict(scale=-1.0)), ((128, 4, 2), dict(scale=math.inf)),
+                     ((128, 4, 2), dict(scale=math.nan))):
+        with pytest.raises(ValueError):
+            DensePagedAttention(*args, **kw)
+    a = DensePagedAttention(64, 4, 2)
+    q, c = torch.zeros(3, 4, 64).half(), torch.zeros(5, 16, 2, 64).half()
+    bt, n, st = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    for call in (lambda: a.forward(q, c, c, bt, n), lambda: a.prefill(q, c, c, bt, n, st)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+    good = (q, c, c, bt, n, (0, 0), 3, None)
+    a._values(*good)
+    for at, bad in ((0, q[:, :3]), (0, q[0]), (1, c[:, :, :1]), (2, c[:4]), (3, bt[:2]), (3, bt[0]), (4, n[:2]), (4, bt), (7, q[:2]), (7, q.transpose(1, 2))):
+        with pytest.raises(ValueError):
+            a._values(*good[:at], bad, *good[at + 1:])
+    for at, bad in ((0, q.float()), (0, q.bfloat16()), (3, bt.short()), (4, n.float())):
+        with pytest.raises(TypeError):
+            a._values(*good[:at], bad, *good[at + 1:])
+
+
+def test_attention_entry_points_refuse():
+    """Argument blocks that the C entry points turn into errors before any launch."""
+    from aitherkvcache_b200 import _lib
+    L = _lib.lib()
+
+    def call(name, **kw):
+        p = _lib.DenseAttnParams()
+        for f in ("query", "k_cache", "v_cache", "block_tables", "seq_lens", "query_start_loc", "out", "workspace"):
+            setattr(p, f, 256)
+        p.q_stride_tok = p.out_stride_tok = p.k_stride_pos = p.v_stride_pos = 256
+        p.q_stride_head = p.out_stride_head = p.k_stride_head = p.v_stride_head = 128
+        p.k_stride_blk = p.v_stride_blk = 4096
+        p.num_seqs, p.num_tokens, p.num_q_heads, p.num_kv_heads, p.head_dim, p.block_size = 2, 4, 2, 2, 128, 16
+        p.max_blocks_per_seq, p.num_blocks, p.scale = 3, 9, 1.0
+        for k, v in kw.items():
+            setattr(p, k, v)
+        return getattr(L, name)(ctypes.byref(p))
+
+    for name in ("akv_dense_paged_attn", "akv_dense_prefill_attn"):
+        assert getattr(L, name)(None) == _lib.AKV_ERR_ARG
+        assert call(name) == _lib.AKV_ERR_WORKSPACE      # everything but the workspace is right
+        for kw in (dict(num_seqs=-1), dict(num_q_heads=3), dict(num_kv_heads=0), dict(block_size=0), dict(num_blocks=-1), dict(window=-1),
+                   dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(bt_dtype=2),
+                   dict(sl_dtype=3), dict(qs_dtype=-1), dict(query=None), dict(out=None), dict(seq_lens=None), dict(block_tables=None),
+                   dict(k_cache=None), dict(v_cache=None), dict(num_blocks=0), dict(query=264), dict(out=264), dict(k_cache=264),
+                   dict(k_stride_pos=260), dict(v_stride_head=4), dict(q_stride_tok=258), dict(out_stride_head=1)):
+            assert call(name, **kw) == _lib.AKV_ERR_ARG, (name, kw)
+        for kw in (dict(head_dim=96), dict(dtype=_lib.AKV_F32), dict(max_blocks_per_seq=1 << 28)):
+            assert call(name, **kw) == _lib.AKV_ERR_UNSUPPORTED, (name, kw)
+        assert call(name, num_seqs=0) == 0
+    assert call("akv_dense_paged_attn", num_tokens=1) == _lib.AKV_ERR_ARG
+    assert call("akv_dense_prefill_attn", query_start_loc=None) == _lib.AKV_ERR_ARG
+    for kw in (dict(head_dim=256), dict(block_size=12), dict(num_q_heads=258), dict(max_blocks_per_seq=0)):
+        assert call("akv_dense_prefill_attn", **kw) == _lib.AKV_ERR_UNSUPPORTED, kw
+    assert L.akv_dense_prefill_attn_workspace_bytes(8, 128, 10, 16, 1, 10) > 0
+    small, large = (L.akv_dense_prefill_attn_workspace_bytes(8, 128, n, 16, 4, 1 << 20) for n in (100, 1 << 20))
+    assert large == 4 * small or large > 3.9 * small      # up to four rounds
+
+
+def test_backend_window_of_uncompressed_layers():
+    from aitherkvcache_b200.vllm.backend import TurboQuantImplBase
+    impl = TurboQuantImplBase()
+    impl._tq_setup(8, 128, 0.1, 2, "auto")
+    cache = torch.zeros(1, dtype=torch.bfloat16)
+    for value, window in ((None, 0), ((-1, -1), 0), ((127, 0), 128), (64, 64), ((0, 0), 1)):
+        impl.sliding_window = value
+        attn = impl._dense_attention(cache)
+        assert (attn.sliding_window, attn.scale, attn.head_dim, attn.num_kv_heads) == (window, 0.1, 128, 2)
