@@ -76,7 +76,7 @@ template <int D> struct DpL {
 };
 // barriers (bytes behind BAR)
 constexpr uint32_t P_PAIR = 0 /* V of tile g and K of tile g + 1 are there */, P_KFIRST = 32, P_KFREE = 64, P_VFREE = 96, P_QFULL = 128, P_QFREE = 144, P_SFULL = 160, P_PFULL = 192, P_PVDONE = 224,
-                   P_TAIL = 240, P_DRAIN = 248, P_TMEM = 264, P_FAILED = 268;
+                   P_TAIL = 240, P_DRAIN = 248, P_TMEM = 264, P_FAILED = 268, P_JOIN = 272, P_OFULL = 288;
 
 // What dense_prefill_merge_kernel needs to know about the row tile whose first part CTA c wrote (parts < 2: nothing)
 struct DpDesc { int parts, slot0, row0, ntok, kvh, pad[3]; };
@@ -266,7 +266,8 @@ struct DpCursor {
   DpSeq q;
   int off, cnt;                 // key tiles at.t.t0 + off .. + cnt - 1
   int64_t left;                 // units behind this piece
-  int nq;                       // halves with tokens
+  int nq;                       // halves that work
+  bool twin;                    // tokens for one half only, and key tiles for two: half h takes tiles off + h, off + h + 2 ... for the same rows
   int round;
   bool first;                   // the first piece of this CTA's part of the round
 
@@ -276,8 +277,13 @@ struct DpCursor {
     off = at.off > DP_PIECE ? at.off - DP_PIECE : 0;
     cnt = end - DP_PIECE - off;
     left = avail - (end - at.off);
-    nq = 2 * at.t.ntok > w.tt2 ? 2 : 1;
+    const bool one = 2 * at.t.ntok <= w.tt2;
+    twin = one && cnt > 1;
+    nq = one && !twin ? 1 : 2;
   }
+  // key tiles of half h (h < nq), and whether its first one is the piece's first
+  __device__ __forceinline__ int tiles(int h) const { return twin ? (cnt + 1 - h) >> 1 : cnt; }
+  __device__ __forceinline__ bool leads(int h) const { return h < nq && !(twin && h == 1); }
   // the part of the next round that has one; false: there is none
   __device__ __forceinline__ bool next_round(const DpWork& w, const DpRound* rounds) {
     do {
@@ -326,11 +332,13 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_QFULL + 8 * i));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_QFREE + 8 * i));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_PVDONE + 8 * i));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_OFULL + 8 * i));
     }
     for (int i = 0; i < 4; ++i) {           // half, sub-tile
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_SFULL + 8 * i));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 4;" :: "r"(bar_s + P_PFULL + 8 * i));
     }
+    for (int i = 0; i < 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 4;" :: "r"(bar_s + P_JOIN + 8 * i));
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_TAIL));
     asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_KFIRST));
     for (int i = 0; i < 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" :: "r"(bar_s + P_DRAIN + 8 * i));
@@ -484,13 +492,14 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
       if (u == 1 && last) umma_commit(bar_s + P_QFREE + 8 * h);
       if (u == 1) umma_commit(bar_s + P_KFREE + 8 * (uint32_t)(g % NP));
     };
-    // O += P V of sub-tile u; first: the piece's first tile
-    auto issue_pv = [&](int g, int u, bool first) {
+    // O += P V of sub-tile u; first, last: the half's first and last tile of the piece
+    auto issue_pv = [&](int g, int u, bool first, bool last) {
       const uint32_t vd = v_d + (uint32_t)(2 * (g % NP)) * (L::TILE >> 4) + (uint32_t)(u * (8192 >> 4));
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
         dp_mma_ts(t_o, t_s + (uint32_t)(u * 64 + kk * 8), vd + (uint32_t)(kk * (2048 >> 4)), v_hi, IDESC_O, (u | kk) != 0 || !first ? 1u : 0u);
       umma_commit(bar_s + P_PVDONE + 8 * h);
+      if (u == 1 && last) umma_commit(bar_s + P_OFULL + 8 * h);
       if (u == 1) umma_commit(bar_s + P_VFREE + 8 * (uint32_t)(g % NP));
     };
     auto q_there = [&]() -> bool {
@@ -508,16 +517,16 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
       return __all_sync(0xffffffffu, done != 0u);
     };
     bool go = wait_warp(bar_s + P_KFIRST, 0u), there = false;
-    if (go && h < cur.nq) {
+    if (go && cur.leads(h)) {
       go = q_there();
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       if (go && withhold != 0 && dp_elect()) {
-        issue_s(0, 0, cur.cnt == 1);
-        issue_s(0, 1, cur.cnt == 1);
+        issue_s(0, 0, cur.tiles(h) == 1);
+        issue_s(0, 1, cur.tiles(h) == 1);
       }
       __syncwarp();
     } else if (go && lane == 0) {
-      dp_arrive(bar_s + P_KFREE);           // no rows in this half: the tile is free as far as it goes
+      dp_arrive(bar_s + P_KFREE);           // not this half's: the tile is free as far as it goes
     }
     __syncwarp();
     // One tile: P V of its sub-tiles, each followed by the scores of the next tile's.  V of this tile and K of the next are
@@ -534,19 +543,72 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
     };
     int g = 0;
     while (go) {
+      if (cur.twin) {
+        // ---- every other tile is this half's; those between are free as far as it goes ----
+        there = false;
+        const int end = g + cur.cnt;
+        if (h == 1) {                       // its first scores
+          if (!pair_there(g) || !q_there()) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (g + 1 != withhold && dp_elect()) {
+            issue_s(g + 1, 0, cur.cnt <= 3);
+            issue_s(g + 1, 1, cur.cnt <= 3);
+          }
+          __syncwarp();
+          if (lane == 0) dp_arrive(bar_s + P_VFREE + 8 * (uint32_t)(g % NP));
+          __syncwarp();
+          ++g;
+        }
+        for (bool first = true; g < end; g += 2, first = false) {
+          const bool other = g + 1 < end, next = g + 2 < end;
+          if (!pair_there(g)) { go = false; break; }
+          if (other && lane == 0) dp_arrive(bar_s + P_KFREE + 8 * (uint32_t)((g + 1) % NP));
+          __syncwarp();
+          if (!p_there(0)) { go = false; break; }
+          if (dp_elect()) issue_pv(g, 0, first, false);
+          __syncwarp();
+          if (other && !pair_there(g + 1)) { go = false; break; }
+          if (next && g + 2 != withhold && dp_elect()) issue_s(g + 2, 0, false);
+          __syncwarp();
+          if (!p_there(1)) { go = false; break; }
+          if (dp_elect()) {
+            issue_pv(g, 1, false, !next);
+            if (next && g + 2 != withhold) issue_s(g + 2, 1, g + 4 >= end);
+          }
+          __syncwarp();
+          if (other && lane == 0) dp_arrive(bar_s + P_VFREE + 8 * (uint32_t)((g + 1) % NP));
+          __syncwarp();
+          p_phase ^= 1u;
+        }
+        if (!go) break;
+        g = end;                            // the first tile of the next piece, whose keys are there
+        if (!cur.next(a, w, s_round)) break;
+        if (cur.leads(h)) {
+          if (!q_there()) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (g != withhold && dp_elect()) {
+            issue_s(g, 0, cur.tiles(h) == 1);
+            issue_s(g, 1, cur.tiles(h) == 1);
+          }
+        } else if (lane == 0) {
+          dp_arrive(bar_s + P_KFREE + 8 * (uint32_t)(g % NP));
+        }
+        __syncwarp();
+        continue;
+      }
       // ---- tiles of the piece that are followed by another of the same piece: the loop that counts ----
       if (h < cur.nq) {
         for (int j = 0; j + 1 < cur.cnt; ++j, ++g) {
           if (!pair_there(g) || !p_there(0)) { go = false; break; }
           if (dp_elect()) {
-            issue_pv(g, 0, j == 0);
+            issue_pv(g, 0, j == 0, false);
             if (g + 1 != withhold) issue_s(g + 1, 0, false);
           }
           __syncwarp();
           if (!p_there(1)) { go = false; break; }
           test_pair(g + 1);
           if (dp_elect()) {
-            issue_pv(g, 1, false);
+            issue_pv(g, 1, false, false);
             if (g + 1 != withhold) issue_s(g + 1, 1, j + 2 == cur.cnt);
           }
           __syncwarp();
@@ -566,13 +628,13 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
       if (!go) break;
       // ---- the piece's last tile, with the scores of the next piece's first ----
       DpCursor ahead = cur;
-      const bool more = ahead.next(a, w, s_round), pv = h < cur.nq, sc = more && h < ahead.nq;
+      const bool more = ahead.next(a, w, s_round), pv = h < cur.nq, sc = more && ahead.leads(h);
       if (!pair_there(g)) break;
 #pragma unroll 1
       for (int u = 0; u < 2 && go; ++u) {
         if (pv) {
           go = p_there(u);
-          if (go && dp_elect()) issue_pv(g, u, cur.cnt == 1);
+          if (go && dp_elect()) issue_pv(g, u, cur.cnt == 1, true);
           __syncwarp();
         }
         if (go && sc) {
@@ -580,7 +642,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
             go = q_there();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           }
-          if (go && g + 1 != withhold && dp_elect()) issue_s(g + 1, u, ahead.cnt == 1);
+          if (go && g + 1 != withhold && dp_elect()) issue_s(g + 1, u, ahead.tiles(h) == 1);
           __syncwarp();
         }
       }
@@ -632,7 +694,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
 #pragma unroll
           for (int x = 0; x < L::HALVES; ++x)
             dp_tma3(base_s + L::Q + (uint32_t)(h * L::TILE + x * 16384), &maps.q, bar_s + P_QFULL + 8 * h, 64 * x, c.at.kvh * G,
-                    c.q.q0 + c.at.t.tok0 + h * TT);
+                    c.q.q0 + c.at.t.tok0 + (c.twin ? 0 : h * TT));
         }
         __syncwarp();
       }
@@ -713,16 +775,18 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
       heads4 |= (uint32_t)(rr - t * G) << (8 * e);
     }
     int step = 0;               // sub-tiles of this half
+    uint32_t joined = 0, pieces = 0;      // parities of the next join and of this half's next piece
     bool ok = true;
     do {
       if (half < cur.nq) {
-        const int tok = cur.at.t.tok0 + half * TT + r_tok;
+        const int of = cur.twin ? 0 : half;         // the half of the row tile that its rows are
+        const int tok = cur.at.t.tok0 + of * TT + r_tok;
         const bool live = r_tok < TT && tok < cur.q.qlen;
         const int lim = live ? cur.q.total - cur.q.qlen + tok + 1 : 0x7fffffff;      // keys below it; a row without a token masks nothing
         const int low = live && a.window > 0 && lim > a.window ? lim - a.window : 0;
         const int lim_w = __reduce_min_sync(0xffffffffu, lim), low_w = __reduce_max_sync(0xffffffffu, low);
         float m = -CUDART_INF_F, l = 0.f;      // reference in log2 units, sum of the weights
-        for (int x = 0; x < 2 * cur.cnt; ++x) {
+        for (int x = 0; x < 2 * cur.tiles(half); ++x) {
           const int u = x & 1;
           if (!wait_warp(bar_s + P_SFULL + 8 * (uint32_t)(2 * half + u), (uint32_t)((step >> 1) & 1))) { ok = false; break; }
           ++step;
@@ -731,7 +795,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
           tmem_ld32(t_s + 64 * u, *reinterpret_cast<uint32_t (*)[32]>(&v[0]));
           tmem_ld32(t_s + 64 * u + 32, *reinterpret_cast<uint32_t (*)[32]>(&v[32]));
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          const int key0 = (cur.at.t.t0 + cur.off) * DP_KT + 64 * x;
+          const int key0 = (cur.at.t.t0 + cur.off) * DP_KT + 64 * x + (cur.twin ? (x >> 1) * DP_KT + half * DP_KT : 0);
           if (key0 + 64 > lim_w || key0 < low_w) {
             // a bit per key: those below the limit and not below the window's edge (bits by constant position become predicates
             // several at a time)
@@ -799,10 +863,50 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
           __syncwarp();
           if (lane == 0) dp_arrive(bar_s + P_PFULL + 8 * (uint32_t)(2 * half + u));
         }
-        // the last two products (the scores of the last sub-tile say that the ones before are done)
-        if (!ok || !wait_warp(bar_s + P_PVDONE + 8 * half, (uint32_t)((step - 2) & 1)) ||
-            !wait_warp(bar_s + P_PVDONE + 8 * half, (uint32_t)((step - 1) & 1))) { ok = false; break; }
+        // all products of the piece have a barrier of their own: the one that counts sub-tiles may be two ahead of a warp that
+        // waits here, which a parity does not tell
+        if (!ok || !wait_warp(bar_s + P_OFULL + 8 * half, pieces)) { ok = false; break; }
+        pieces ^= 1u;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (cur.twin) {
+          // The same rows' other tiles: half 1 hands over its maximum and sum; its O lies in the same lanes of tensor memory, and
+          // half 0 adds it to its own:  O = 2^(m0 - M) O0 + 2^(m1 - M) O1.
+          float2* ml = reinterpret_cast<float2*>(base + L::STAGE + (4 + quad) * 32 * L::SROW) + lane;
+          if (half == 1) {
+            *ml = make_float2(m, l);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) dp_arrive(bar_s + P_JOIN);
+            if (!wait_warp(bar_s + P_JOIN + 8, joined)) { ok = false; break; }      // O and the staging are free again
+            joined ^= 1u;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            continue;
+          }
+          if (!wait_warp(bar_s + P_JOIN, joined)) { ok = false; break; }
+          joined ^= 1u;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const float2 o1 = *ml;
+          const float top = fmaxf(m, o1.x);
+          const bool has0 = m != -CUDART_INF_F, has1 = o1.x != -CUDART_INF_F;      // a side that saw no key adds nothing
+          const float f0 = has0 ? dense_ex2(m - top) : 0.f, f1 = has1 ? dense_ex2(o1.x - top) : 0.f;
+          m = top;
+          l = f0 * l + f1 * o1.y;
+#pragma unroll 1
+          for (int y = 0; y < D / 32; ++y) {
+            uint32_t o[32], p[32];
+            tmem_ld32(t_o + 32 * y, o);
+            tmem_ld32(t_o + 128 + 32 * y, p);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              o[i] = __float_as_uint((has0 ? __uint_as_float(o[i]) * f0 : 0.f) + (has1 ? __uint_as_float(p[i]) * f1 : 0.f));
+            tmem_st32(t_o + 32 * y, o);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) dp_arrive(bar_s + P_JOIN + 8);
+        }
         const bool whole = cur.cnt == cur.at.t.n;
         const int64_t slot = ((int64_t)cur.round * gridDim.x + blockIdx.x) * 2 + (cur.first ? 0 : 1);
         const float inv = l == 0.f ? 0.f : 1.0f / l;
@@ -814,7 +918,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
         char* dst4[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int t = (rows4 >> (8 * e)) & 255, hd = (heads4 >> (8 * e)) & 255, tok_e = cur.at.t.tok0 + half * TT + t;
+          const int t = (rows4 >> (8 * e)) & 255, hd = (heads4 >> (8 * e)) & 255, tok_e = cur.at.t.tok0 + of * TT + t;
           if (t < TT && tok_e < cur.q.qlen) alive |= 1u << e;
           dst4[e] = static_cast<char*>(a.out) + 2 * ((int64_t)(cur.q.q0 + tok_e) * a.out_st + (int64_t)(cur.at.kvh * G + hd) * a.out_sh + 8 * c4);
         }
@@ -844,7 +948,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
           }
         } else {
           // float4 of 4 columns, rows fastest: a store instruction writes 512 bytes in a row
-          float4* part = reinterpret_cast<float4*>(part_acc) + slot * 64 * D + half * 128 + r;
+          float4* part = reinterpret_cast<float4*>(part_acc) + slot * 64 * D + of * 128 + r;
 #pragma unroll 1
           for (int x = 0; x < D / 32; ++x) {
             uint32_t o[32];
@@ -856,8 +960,8 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
           }
         }
         if (live && !whole) {
-          part_ml[(slot * 256 + half * 128 + r) * 2] = m;
-          part_ml[(slot * 256 + half * 128 + r) * 2 + 1] = l;
+          part_ml[(slot * 256 + of * 128 + r) * 2] = m;
+          part_ml[(slot * 256 + of * 128 + r) * 2 + 1] = l;
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       }

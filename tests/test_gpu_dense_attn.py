@@ -288,6 +288,34 @@ def test_chunks_many_sequences_and_repeatability():
         assert torch.equal(a.prefill(q, kc, vc, bt, cl, starts), out)
 
 
+def test_chunks_many_short_pieces_repeatedly():
+    """Row tiles of one to four key tiles, one or two halves of rows each: every end of a piece has its own wait, which no
+    delay of a warp may carry past its barrier."""
+    from aitherkvcache_b200 import _lib
+    g = torch.Generator().manual_seed(3)
+    new = torch.randint(0, 9, (380,), generator=g).tolist()
+    new[::7] = [100] * len(new[::7])
+    lens = [n + int(x) for n, x in zip(new, torch.randint(0, 500, (380,), generator=g))]
+    for D, bs in ((64, 16), (128, 32)):
+        q, kc, vc, bt, cl, starts = make(lens, new, 4, 2, D, bs, torch.float16, seed=3, stale=math.nan)
+        a = attn(4, 2, D)
+        out = a.prefill(q, kc, vc, bt, cl, starts)
+        check(out, q, kc, vc, bt, cl, starts)
+        for _ in range(200):
+            assert torch.equal(a.prefill(q, kc, vc, bt, cl, starts), out)
+    assert _lib.device_status()["attn_window"] == 0
+
+
+@pytest.mark.parametrize("D,bs", [(64, 32), (128, 16), (128, 8), (64, 256)])
+@pytest.mark.parametrize("window", [0, 3, 130, 1000])
+def test_chunks_of_few_rows(D, bs, window):
+    """Few rows per sequence: the two halves take alternate key tiles of the same rows.  Ends just behind a key tile's edge
+    leave rows that see nothing of the last tile, windows leave rows that see nothing of the others."""
+    lens = [1, 128, 129, 130, 131, 133, 256, 257, 259, 384, 385, 390, 1030, 3333, 12000, 5]
+    new = [1, 1, 1, 4, 7, 9, 2, 3, 9, 1, 8, 8, 9, 5, 3, 5]
+    run_chunks(lens, new, 14, 2, D, bs, torch.bfloat16, window=window, seed=bs + window, scale_q=2.0)
+
+
 def test_chunks_in_rounds():
     """Keys and values of 245 MB: the call goes over its (sequence, KV head) pairs in rounds, every one of them cut into
     ranges for all SMs (four rounds of three sequences: rounds begin between the KV heads of a sequence)."""
