@@ -33,7 +33,9 @@
 // Rounds.  The CTAs' ranges begin anywhere in the keys, so a KV head's keys and values are wanted at all times of its round,
 // and what does not fit into L2 comes from HBM again for every row tile: at a power limit that costs clock (131 MB of
 // keys and values ran at 1.34 GHz, 24 MB at 1.47).  So the (sequence, KV head) pairs are taken in rounds of about
-// DP_ROUND_BYTES of keys and values, each cut into ranges for all SMs.
+// DP_ROUND_BYTES of keys and values, each cut into ranges for all SMs.  Sequences of one row tile read their keys once and do
+// not count: a round more costs some 10 us (its cuts, and the SMs' wait for the first keys), and 32 sequences of 4096 keys with
+// 4 new tokens (4 KV heads of 64) took 54 us in two rounds, 43 in one.
 //
 // Every wait is bounded (umma.cuh): a wait that gives up sets g_dense_prefill_status and a flag that ends all loops.
 #include "dense_attn.cuh"
@@ -65,7 +67,7 @@ template <int D> struct DpL {
   static constexpr int NP = D == 128 ? 2 : 4;              // ring slots of K tiles, and of V tiles
   static constexpr int Q = 0, KV = 2 * TILE, BAR = KV + 2 * NP * TILE;      // K slot, V slot, K slot ...
   static constexpr int PRE = BAR + 512;                    // int64 [DP_MAX_SEQS + 1]: units before a sequence ...
-  static constexpr int PREK = PRE + (DP_MAX_SEQS + 1) * 8; // ... and keys before it
+  static constexpr int PREK = PRE + (DP_MAX_SEQS + 1) * 8; // ... and keys before it that several row tiles read
   static constexpr int SROW = 80;                          // staging of results: 64 bytes of a row, padded to other banks
   static constexpr int SEQ = PRE + (DP_MAX_SEQS + 1) * 16;       // int [DP_MAX_SEQS][3]: DpSeq of every sequence
   static constexpr int STAGE = (SEQ + DP_MAX_SEQS * 12 + 15) / 16 * 16;     // [8 warps][32 rows][SROW]
@@ -365,7 +367,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
     for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
     if (lane == 0) {
       pre[s + 1] = n * a.num_kv_heads;
-      prek[s + 1] = tiles == 0 ? 0 : (a.window > 0 && a.window + q.qlen < q.total ? a.window + q.qlen : q.total);
+      prek[s + 1] = tiles < 2 ? 0 : (a.window > 0 && a.window + q.qlen < q.total ? a.window + q.qlen : q.total);
     }
     my_tiles += tiles;
   }
@@ -391,7 +393,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
   }
   __syncthreads();
   const int64_t units = pre[seqs];
-  // rounds: as many as it takes for a round's keys and values to stay in L2 while the CTAs walk over them
+  // rounds: as many as it takes for a round's keys and values to stay in L2 while the CTAs walk over them again and again
   const int64_t kv_bytes = prek[seqs] * a.num_kv_heads * (4 * D);
   int n_rounds = (int)((kv_bytes + DP_ROUND_BYTES - 1) / DP_ROUND_BYTES < max_rounds ? (kv_bytes + DP_ROUND_BYTES - 1) / DP_ROUND_BYTES : max_rounds);
   if (n_rounds < 1) n_rounds = 1;
