@@ -11,19 +11,24 @@
 //   O[128][D]  += P V        A = P in tensor memory (over the columns of S), B = the values as they lie in the pages:
 //                            [key][dim] rows are the MN-major form of the operand, nothing is transposed.
 // K, V and Q come by TMA with the 128-byte swizzle straight out of the paged tensors (a box per run of keys inside a
-// block); rows of values behind the sequence's end are zeroed in shared memory, since 0 * NaN is NaN.
+// block); rows of values that no row may see (behind the sequence's end, before all windows) are zeroed
+// in shared memory, since 0 * NaN is NaN.
 //
-// Ten warps: 0-3 softmax of half 0 and 4-7 of half 1 (thread = row), 8 issues the MMAs, 9 the copies.  A half's tile goes
-// through in two sub-tiles of 64 keys with a score buffer each, and the MMAs are issued in the order
-//   P V of (half 0, sub-tile u), S of (half 0, u + 2), then the same of half 1,
-// so while a softmax warp works on sub-tile u the scores of u + 1 are there already: it never waits for the tensor pipe's
-// round trip (P written -> P V and the next S: 1300 cycles and more), and the two halves' warps, two per scheduler, fill
-// each other's gaps in the exponential unit.  64-key scores cost the tensor pipe 385 cycles instead of 256 (the operands'
-// shared-memory traffic), 2485 per tile pair in all where 2048 would be the least; with whole 128-key tiles in one buffer a
-// tile pair took 4850 cycles, 2900 of each half's period waiting for that round trip.
+// Twelve warps: 0-3 softmax of half 0 and 4-7 of half 1 (thread = row), 8 and 10 issue the MMAs of one half each, 9 copies the
+// keys and Q, 11 the values.  A half's tile goes through in two sub-tiles of 64 keys with a score buffer each, and its MMAs
+// are issued in the order  P V of sub-tile u, S of u + 2,  so while a softmax warp works on sub-tile u the scores of u + 1
+// are there already: it never waits for the tensor pipe's round trip (P written -> P V and the next S: 1300 cycles and more),
+// and the two halves' warps, two per scheduler, fill each other's gaps in the exponential unit.  64-key scores cost the tensor
+// pipe 385 cycles instead of 256 (the operands' shared-memory traffic), 2485 per tile pair in all where 2048 would be the least;
+// with whole 128-key tiles in one buffer a tile pair took 4850 cycles, 2900 of each half's period waiting for that round trip.
 // MMAs complete in order, so "S of u is there" also says that P V of u - 2 is done and the buffer of P u - 2 was free.
 // The row's reference maximum moves only when a score exceeds it by more than 2^8 (fp16 and bf16 hold 2^8 exactly), so O
 // is rescaled a few times per row; that waits for P V of u - 1.
+//
+// Few rows.  Where a row tile has rows for one half only (at most TT new tokens left), the halves take alternate key tiles of
+// the same rows, half 0 the piece's first, third ..., half 1 the others, and at the piece's end half 0 adds half 1's O, which
+// lies in the same lanes of tensor memory, to its own.  1 to 8 new tokens behind 32 sequences of 4000 (28 / 4 heads of
+// 64): 56.7 us, against 65.7 with one half idle.
 //
 // Work split.  The (row tile, key tile) pairs of the whole call are laid end to end and cut into equal ranges, one per SM:
 // every SM finishes at the same time whatever the lengths.  Row tiles that are cut (at most two per CTA) leave float32
@@ -36,6 +41,11 @@
 // DP_ROUND_BYTES of keys and values, each cut into ranges for all SMs.  Sequences of one row tile read their keys once and do
 // not count: a round more costs some 10 us (its cuts, and the SMs' wait for the first keys), and 32 sequences of 4096 keys with
 // 4 new tokens (4 KV heads of 64) took 54 us in two rounds, 43 in one.
+//
+// Measured: 2048 tokens behind 30000 (32 / 8 heads of 128) 0.99 ms in a sustained run at the power limit, 1.05 PFLOP/s, 77 % of
+// the measured sustained matrix rate (0.87 ms, 1.2 PFLOP/s in short bursts; 3000 cycles per tile pair); twelve prompts of 1 to
+// 2000 tokens 157 us, 0.75 PFLOP/s (10 pieces per CTA, each with some 3.6 us of its own: the last P V, the epilogue and the first
+// scores); the 1 to 8 new tokens above 47 us, 3 TB/s.
 //
 // Every wait is bounded (umma.cuh): a wait that gives up sets g_dense_prefill_status and a flag that ends all loops.
 #include "dense_attn.cuh"
@@ -54,7 +64,7 @@ constexpr int DP_KT = 128;                       // keys per tile
 constexpr int DP_MAX_SEQS = 384;                 // sequences of one launch
 constexpr int DP_MAX_ROUNDS = 4;
 constexpr int64_t DP_ROUND_BYTES = 68 << 20;     // keys and values of a round
-constexpr int DP_SNAP = 4;
+constexpr int DP_SNAP = 4;                       // a cut this near to a row tile's edge is moved there, in key tiles
 constexpr int DP_PIECE = 2;                      // what a row tile costs besides its key tiles, in key tiles
 constexpr float DP_RESCALE = 8.0f;
 
@@ -726,9 +736,12 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
           if (g >= NP) go = wait_warp(bar_s + P_VFREE + 8 * slot, (uint32_t)((g / NP - 1) & 1));
           if (!go) break;
           const uint32_t full = bar_s + P_PAIR + 8 * slot, dst = base_s + L::KV + (2 * slot + 1) * L::TILE;
-          const int z = cur.q.total - (cur.at.t.t0 + cur.off + j) * DP_KT;      // rows inside the sequence
-          copy(&maps.v, dst, z < DP_KT ? bar_s + P_TAIL : full, blk_j, pos_j, cur.at.kvh);
-          if (z < DP_KT) {                  // values behind the sequence's end are zeroed before the tile is handed over
+          // keys of the tile that a row of the row tile may see: inside the sequence, and not before all rows' windows
+          const int key0 = (cur.at.t.t0 + cur.off + j) * DP_KT, z = cur.q.total - key0;
+          const int before = a.window > 0 ? cur.q.total - cur.q.qlen + cur.at.t.tok0 + 1 - a.window - key0 : 0;
+          const bool part = z < DP_KT || before > 0;
+          copy(&maps.v, dst, part ? bar_s + P_TAIL : full, blk_j, pos_j, cur.at.kvh);
+          if (part) {                       // the other values are zeroed before the tile is handed over
             const bool there = __all_sync(0xffffffffu, mbar_wait(bar_s + P_TAIL, (uint32_t)(tails++ & 1)));      // also when others gave up: the copy is in flight
             if (!there) {
               g_dense_prefill_status = 1;
@@ -736,10 +749,14 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
               go = false;
               break;
             }
-            for (int e = (z < 0 ? 0 : z) * 8 + lane; e < DP_KT * 8; e += 32)
+            auto zero = [&](int from, int to) {      // keys of the tile
+              for (int e = from * 8 + lane; e < to * 8; e += 32)
 #pragma unroll
-              for (int x = 0; x < L::HALVES; ++x)
-                asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" :: "r"(dst + (uint32_t)(x * 16384 + e * 16)), "r"(0u) : "memory");
+                for (int x = 0; x < L::HALVES; ++x)
+                  asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" :: "r"(dst + (uint32_t)(x * 16384 + e * 16)), "r"(0u) : "memory");
+            };
+            zero(0, before < DP_KT ? before : DP_KT);
+            zero(z < 0 ? 0 : z, DP_KT);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) dp_arrive(full);

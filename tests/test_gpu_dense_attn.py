@@ -316,6 +316,46 @@ def test_chunks_of_few_rows(D, bs, window):
     run_chunks(lens, new, 14, 2, D, bs, torch.bfloat16, window=window, seed=bs + window, scale_q=2.0)
 
 
+@pytest.mark.parametrize("D,bs", [(64, 16), (128, 32), (256, 16)])
+@pytest.mark.parametrize("new", [1, 3, 150])
+def test_chunks_pages_that_have_left_the_window(D, bs, new):
+    """A cache of sliding windows gives its pages back: what lies before the first window of a chunk may be anything."""
+    lens, window = [999, 130, 400, 700], 100
+    q, kc, vc, bt, cl, starts = make(lens, [new if n >= new else n for n in lens], 8, 2, D, bs, torch.bfloat16, seed=new, stale=math.nan)
+    want, bound = od.attention(q, kc, vc, bt, cl.tolist(), starts.tolist(), 1 / math.sqrt(D), window)
+    for s, n in enumerate(lens):
+        first = n - (new if n >= new else n) + 1 - window           # the first key that a row sees
+        for j in range(max(first, 0)):
+            kc[bt[s, j // bs], j % bs] = vc[bt[s, j // bs], j % bs] = math.nan if j % 2 else math.inf
+    out = attn(8, 2, D, sliding_window=window).prefill(q, kc, vc, bt, cl, starts)
+    assert bool(((out.double() - want).abs() <= bound).all())
+    if new == 1:
+        out = attn(8, 2, D, sliding_window=window).forward(q, kc, vc, bt, cl)
+        assert bool(((out.double() - want).abs() <= bound).all())
+
+
+def test_no_blocks_and_no_tokens():
+    """Block tables without columns, sequences without tokens, calls without rows."""
+    for D in (64, 128, 256):
+        kc, vc = (torch.full((3, 16, 2, D), math.nan, dtype=torch.float16, device="cuda") for _ in range(2))
+        q = torch.randn(4, 4, D, device="cuda").half()
+        a = attn(4, 2, D)
+        none, zeros = torch.zeros(4, 0, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+        lens = torch.tensor([5, 0, 1, 9], dtype=torch.int32, device="cuda")      # clamped to what the table addresses
+        starts = torch.tensor([0, 1, 1, 3, 4], dtype=torch.int32, device="cuda")
+        assert bool((a.forward(q, kc, vc, none, lens) == 0).all())
+        assert bool((a.prefill(q, kc, vc, none, lens, starts) == 0).all())
+        table = torch.zeros(4, 1, dtype=torch.int32, device="cuda")
+        assert bool((a.forward(q, kc, vc, table, zeros) == 0).all())
+        assert bool((a.prefill(q, kc, vc, table, zeros, starts) == 0).all())
+        assert a.forward(q[:0], kc, vc, table, zeros).shape == (0, 4, D)
+        assert a.prefill(q[:0], kc, vc, table, zeros, zeros[:1]).shape == (0, 4, D)
+        assert bool((a.prefill(q, kc, vc, table, zeros, zeros[:1]) == 0).all())
+        out = torch.ones_like(q)
+        a.prefill(q, kc, vc, table, zeros, starts[:3], out=out)
+        assert bool((out[:1] == 0).all()) and bool((out[1:] == 1).all())
+
+
 def test_chunks_in_rounds():
     """Keys and values of 245 MB: the call goes over its (sequence, KV head) pairs in rounds, every one of them cut into
     ranges for all SMs (four rounds of three sequences: rounds begin between the KV heads of a sequence)."""

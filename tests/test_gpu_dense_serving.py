@@ -180,3 +180,30 @@ def test_calls_on_two_streams_at_once():
     for i in range(2):
         for res in got[i]:
             assert all(torch.equal(x, y) for x, y in zip(res, want[i]))
+
+
+@pytest.mark.parametrize("src,dst", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16)])
+@pytest.mark.parametrize("heads,D,bs", [(2, 128, 16), (3, 64, 5), (1, 40, 1)])
+def test_kv_append(src, dst, heads, D, bs):
+    """Keys as they are: slices of a fused projection, a transposed one, padding, and what lies around the slots."""
+    from aitherkvcache_b200 import kv_append
+    g = torch.Generator().manual_seed(D + bs)
+    for n in (0, 1, 77):
+        blocks = 2 * n // bs + 2
+        slots = torch.randperm(blocks * bs, generator=g)[:n]
+        if n > 3:
+            slots[1], slots[2] = -1, blocks * bs
+        qkv = torch.randn(n, heads * 4, D, generator=g).to(src).cuda()
+        caches = torch.randn(blocks, 2, bs, heads, D, generator=g).to(dst).cuda()
+        want = caches.clone()
+        key, value = qkv[:, heads:2 * heads], qkv[:, 2 * heads:3 * heads]
+        for t, s in enumerate(slots.tolist()):
+            if 0 <= s < blocks * bs:
+                want[s // bs, 0, s % bs], want[s // bs, 1, s % bs] = key[t].to(dst), value[t].to(dst)
+        for form in (lambda x: x, lambda x: x.transpose(1, 2).contiguous().transpose(1, 2)):
+            got = caches.clone()
+            kv_append(form(key), form(value), slots.cuda(), got[:, 0], got[:, 1])
+            assert torch.equal(got, want)
+            got = caches.clone()
+            kv_append(key, form(value), slots.int().cuda(), got[:, 0], got[:, 1])
+            assert torch.equal(got, want)
