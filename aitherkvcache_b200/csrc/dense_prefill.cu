@@ -44,7 +44,7 @@
 //
 // Measured: 2048 tokens behind 30000 (32 / 8 heads of 128) 0.99 ms in a sustained run at the power limit, 1.05 PFLOP/s, 77 % of
 // the measured sustained matrix rate (0.87 ms, 1.2 PFLOP/s in short bursts; 3000 cycles per tile pair); twelve prompts of 1 to
-// 2000 tokens 157 us, 0.75 PFLOP/s (10 pieces per CTA, each with some 3.6 us of its own: the last P V, the epilogue and the first
+// 2000 tokens 153 us, 0.76 PFLOP/s (10 pieces per CTA, each with some 3.6 us of its own: the last P V, the epilogue and the first
 // scores); the 1 to 8 new tokens above 47 us, 3 TB/s.
 //
 // Every wait is bounded (umma.cuh): a wait that gives up sets g_dense_prefill_status and a flag that ends all loops.
@@ -64,7 +64,7 @@ constexpr int DP_KT = 128;                       // keys per tile
 constexpr int DP_MAX_SEQS = 384;                 // sequences of one launch
 constexpr int DP_MAX_ROUNDS = 4;
 constexpr int64_t DP_ROUND_BYTES = 68 << 20;     // keys and values of a round
-constexpr int DP_SNAP = 4;                       // a cut this near to a row tile's edge is moved there, in key tiles
+constexpr int DP_SNAP = 2;                       // a cut this near to a row tile's edge is moved there, in key tiles (0 and 6: 158 us for the prompts above, 4: 156, 2: 153)
 constexpr int DP_PIECE = 2;                      // what a row tile costs besides its key tiles, in key tiles
 constexpr float DP_RESCALE = 8.0f;
 

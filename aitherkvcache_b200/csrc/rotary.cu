@@ -18,8 +18,7 @@
 // each other.  That phase needs few registers, so enough loads are in flight.
 // Measured (inside a graph): 32768 tokens of 32 + 8 + 8 heads of 128, fp16, into the cache, 806 MB in 151 us, 5.3 TB/s, 81 % of
 // the measured copy bandwidth; 8192 tokens of 32 + 8 heads with three axes, 168 MB in 35 us, 4.8 TB/s; 16 tokens 2.2 us, with the
-// append 2.7.  With the
-// angles worked out again for every head the first two took 225 and 67 us.
+// append 2.7.  With the angles worked out again for every head the first two took 225 and 67 us.
 #include "common.cuh"
 
 // Mirrors of akv_rotary_tables, akv_rotary_params and akv_rotary_append_params in include/akv_b200.h.
