@@ -180,18 +180,14 @@ rotary_rows_kernel(RotArgs a) {
   const int tb = a.tokens - t0 < a.tb ? (int)(a.tokens - t0) : a.tb;
   const int h_lo = blockIdx.y * a.slice, hs = a.heads - h_lo < a.slice ? a.heads - h_lo : a.slice;
   const int items = tb * hs * units;
-  // item: (token, head, unit), units next to each other
+  // item: (token, head, unit), units next to each other; a thread's next item is ROT_THREADS further on
+  const int row_step = ROT_THREADS / units, u_step = ROT_THREADS - row_step * units, t_step = row_step / hs, h_step = row_step - t_step * hs;
   int tt, h, u, e0, e1;
   const TI* src;
   TO* dst;
   bool turned, there;
-  auto place = [&](int item) {
-    const int row = item / units;
-    u = item - row * units;
-    tt = row / hs;
-    h = h_lo + row - tt * hs;
-    const bool rot = u < runits && h < a.qh + a.kh;
-    turned = rot;
+  auto spans = [&]() {
+    turned = u < runits && h < a.qh + a.kh;
     e0 = u < runits ? (a.adjacent ? 16 * u : 8 * u) : 16 * u;
     e1 = u < runits && !a.adjacent ? half + 8 * u : e0 + 8;
   };
@@ -200,7 +196,11 @@ rotary_rows_kernel(RotArgs a) {
   int item = threadIdx.x;
   there = false;
   if (item < items) {
-    place(item);
+    const int row = item / units;
+    u = item - row * units;
+    tt = row / hs;
+    h = h_lo + row - tt * hs;
+    spans();
     rot_slot(a, t0 + tt, blk, in_blk);
     there = rot_row<TI, TO>(a, t0 + tt, h, blk, in_blk, src, dst);
     if (there) {
@@ -233,7 +233,12 @@ rotary_rows_kernel(RotArgs a) {
     }
     item += ROT_THREADS;
     if (item < items) {                     // the next item's loads before this one's arithmetic
-      place(item);
+      u += u_step;
+      tt += t_step;
+      h += h_step;
+      if (u >= units) { u -= units; ++h; }
+      if (h >= h_lo + hs) { h -= hs; ++tt; }
+      spans();
       there = rot_row<TI, TO>(a, t0 + tt, h, s_blk[tt], s_pos[tt], src, dst);
       if (there) {
         r0 = rot_load8<TI>(src + e0);
