@@ -16,9 +16,11 @@
 // head - into shared memory, while its first loads are under way; then the block streams through the heads, a thread 16
 // elements of a row at a time (8 pairs, two 16-byte loads for 16-bit types), the 8 threads of a 128-element row next to
 // each other.  That phase needs few registers, so enough loads are in flight.
-// Measured (inside a graph): 32768 tokens of 32 + 8 + 8 heads of 128, fp16, into the cache, 806 MB in 151 us, 5.3 TB/s, 81 % of
-// the measured copy bandwidth; 8192 tokens of 32 + 8 heads with three axes, 168 MB in 35 us, 4.8 TB/s; 16 tokens 2.2 us, with the
-// append 2.7.  With the angles worked out again for every head the first two took 225 and 67 us.
+// Measured (inside a graph): 32768 tokens of 32 + 8 + 8 heads of 128, fp16, into the cache, 806 MB in 136 us, 5.9 TB/s, 90 % of
+// the measured copy bandwidth; 8192 tokens of 32 + 8 heads with three axes, 168 MB in 32.5 us, 5.2 TB/s; 16 tokens 2.3 us, with the
+// append 3.1.  With the angles worked out again for every head the first two took 225 and 67 us; with blocks of 256 threads
+// 144 and 33.6 (eight blocks of 128 per SM have their first loads and their last stores at more different times), of 64
+// threads 138 and 32.4, with one couple per thread 141 and 32.6.
 #include "common.cuh"
 
 // Mirrors of akv_rotary_tables, akv_rotary_params and akv_rotary_append_params in include/akv_b200.h.
@@ -51,7 +53,7 @@ struct akv_rotary_append_params {
 namespace akv {
 namespace {
 
-constexpr int ROT_THREADS = 256;
+constexpr int ROT_THREADS = 128;
 constexpr int ROT_MAX_AXES = 4;
 
 struct RotArgs {
@@ -170,7 +172,7 @@ __device__ __forceinline__ void rot_slot(const RotArgs& a, int64_t t, int64_t& b
 constexpr int ROT_MAX_PAIRS = 1024;      // (token, pair) couples of a block
 
 template <typename TI, typename TO>
-__global__ void __launch_bounds__(ROT_THREADS, sizeof(TI) == 4 ? 3 : 4)
+__global__ void __launch_bounds__(ROT_THREADS, sizeof(TI) == 4 ? 6 : 8)
 rotary_rows_kernel(RotArgs a) {
   __shared__ __align__(16) float s_cos[ROT_MAX_PAIRS], s_sin[ROT_MAX_PAIRS];
   __shared__ int64_t s_blk[16];
@@ -337,15 +339,15 @@ int rot_run(RotArgs a, const char* who, cudaStream_t st) {
   const int per_token = a.R / 2 + (a.D - a.R);
   int64_t most;                 // tokens of one launch: grid and thread indices stay below 2^31
   if (rows16) {
-    // about one (token, pair) per thread; all heads of a token in one block where that gives every SM four blocks, else
+    // two (token, pair) couples per thread; all heads of a token in one block where that gives every SM eight blocks, else
     // as many slices of heads as it takes, down to one item per thread (a decode step: latency)
-    a.tb = a.R > 0 ? ROT_THREADS / (a.R / 2) : 4;
+    a.tb = a.R > 0 ? 2 * ROT_THREADS / (a.R / 2) : 4;
     if (a.tb < 1) a.tb = 1;
     if (a.tb > 16) a.tb = 16;
-    const int64_t want = 4 * (int64_t)sm_count();
+    const int64_t want = 8 * (int64_t)sm_count();
     if (a.tokens / want < a.tb) a.tb = a.tokens / want > 1 ? (int)(a.tokens / want) : 1;
-    // between half and all of that, the number whose items fill the threads best: 4099 tokens of 12 x 96 float32 take 11.8 us
-    // six at a time (432 items for 256 threads, twice) and 14.0 four at a time (288); 5003 of 18 x 64 bf16 9.4 us against 10.4
+    // between half and all of that, the number whose items fill the threads best: with blocks of 256 threads, 4099 tokens of
+    // 12 x 96 float32 took 11.8 us six at a time (432 items, two rounds) and 14.0 four at a time (288, also two)
     double best = 0.0;
     for (int tb = a.tb, lo = (a.tb + 1) / 2; tb >= lo; --tb) {
       const int64_t items = (int64_t)tb * a.heads * (a.D / 16);
