@@ -16,11 +16,11 @@
 // head - into shared memory, while its first loads are under way; then the block streams through the heads, a thread 16
 // elements of a row at a time (8 pairs, two 16-byte loads for 16-bit types), the 8 threads of a 128-element row next to
 // each other.  That phase needs few registers, so enough loads are in flight.
-// Measured (inside a graph): 32768 tokens of 32 + 8 + 8 heads of 128, fp16, into the cache, 806 MB in 136 us, 5.9 TB/s, 90 % of
-// the measured copy bandwidth; 8192 tokens of 32 + 8 heads with three axes, 168 MB in 32.5 us, 5.2 TB/s; 16 tokens 2.3 us, with the
-// append 3.1.  With the angles worked out again for every head the first two took 225 and 67 us; with blocks of 256 threads
-// 144 and 33.6 (eight blocks of 128 per SM have their first loads and their last stores at more different times), of 64
-// threads 138 and 32.4, with one couple per thread 141 and 32.6.
+// Measured (inside a graph): 32768 tokens of 32 + 8 + 8 heads of 128, fp16, into the cache, 806 MB in 134 us, 6.0 TB/s, 92 % of
+// the measured copy bandwidth; 8192 tokens of 32 + 8 heads with three axes, 168 MB in 32.4 us, 5.2 TB/s; 4099 tokens of 9 + 3
+// heads of 96 float32, adjacent pairs, 38 MB in 10.5 us; 16 tokens 2.3 us, with the append 3.1.  With the angles worked out
+// again for every head the first two took 225 and 67 us; with blocks of 256 threads 144 and 33.6, of 64 threads 138 and 32.4,
+// with one couple per thread 141 and 32.6; with loads that pass L1 by 136 and 32.5, the third 11.3 (its sectors are read in halves).
 #include "common.cuh"
 
 // Mirrors of akv_rotary_tables, akv_rotary_params and akv_rotary_append_params in include/akv_b200.h.
@@ -90,7 +90,7 @@ template <typename T> __device__ __forceinline__ Raw8<T> rot_load8(const T* p) {
   Raw8<T> r;
 #pragma unroll
   for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+    asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r.w[i].x), "=r"(r.w[i].y), "=r"(r.w[i].z), "=r"(r.w[i].w) : "l"(reinterpret_cast<const uint4*>(p) + i));
   return r;
 }
