@@ -1025,63 +1025,108 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
   }
 }
 
-// Row tiles that were cut: out = sum_p 2^(m_p - M) acc_p / sum_p 2^(m_p - M) l_p in the order of the keys.  Block (c, y):
-// rows 128 y .. + 127 of the row tiles that CTA c began, round by round; a thread takes 16 columns of one row (a 32-byte sector), neighbouring
-// threads neighbouring rows (the partials' layout).  Two blocks per SM: starting a
-// block costs some 10 ns.  The first parts' maxima, sums and columns are read together (most row tiles have two).
-constexpr int PM_THREADS = 1024;
-template <bool BF, int D>
+// Row tiles that were cut: out = sum_p 2^(m_p - M) acc_p / sum_p 2^(m_p - M) l_p.  A slice is 16 columns (a 32-byte sector) of
+// 128 rows, half of a row tile; a thread takes a row of it, neighbouring threads neighbouring rows (the partials' layout).  Two
+// blocks per SM: starting a block costs some 10 ns.
+// !SPREAD: a block per half of the row tile that a CTA began, round by round.  Most have two or three parts.
+// SPREAD, for calls of few row tiles, which have many parts each: every block lists the halves that have parts, the slices are
+// spread over all blocks, and where that leaves threads idle, `groups` of 128 threads share a slice: group g takes parts g,
+// g + groups, ..., and the groups are joined in order through shared memory (their number depends on the call's lengths alone,
+// so results repeat).  100 tokens behind 20000 (32 / 8 heads of 128, 18 parts per row tile) take 86 us with it and 118 without, 5
+// tokens (8 / 1 heads, 20 parts) 33 and 37; 5 tokens behind 5000 (5 parts) 23.7 and 22.6, 30 tokens behind 8 sequences of 3000
+// 50.7 and 49.3.
+constexpr int PM_THREADS = 1024, PM_LIST = DP_MAX_ROUNDS * 256 * 2;      // at most 256 SMs
+constexpr int PM_SMEM = PM_THREADS * 18 * (int)sizeof(float);
+template <bool BF, int D, bool SPREAD>
 __global__ void __launch_bounds__(PM_THREADS)
-dense_prefill_merge_kernel(DenseArgs a, int G, int TT, int rounds, int tail, const DpDesc* desc, const float* part_ml, const float* part_acc) {
+dense_prefill_merge_kernel(DenseArgs a, int G, int TT, int rounds, int ctas, int tail, const DpDesc* desc, const float* part_ml, const float* part_acc) {
+  extern __shared__ float s_part[];                    // [18][PM_THREADS]: maximum, sum, 16 columns
+  __shared__ uint16_t s_list[SPREAD ? PM_LIST : 1];    // 2 * place in desc + half
+  __shared__ int s_count[32], s_most[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (tail >= 0) {              // rows behind the last sequence (`tail` of them in this launch) come out as zeros
     int64_t row = load_index(a.starts, a.qs_dtype, tail);
     if (row < 0) row = 0;
-    for (row += blockIdx.y * gridDim.x + blockIdx.x; row < a.n_tokens; row += gridDim.x * gridDim.y)
-      for (int e = threadIdx.x; e < a.num_q_heads * (D / 8); e += PM_THREADS)
+    for (row += blockIdx.x; row < a.n_tokens; row += gridDim.x)
+      for (int e = tid; e < a.num_q_heads * (D / 8); e += PM_THREADS)
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.out_st + (int64_t)(e / (D / 8)) * a.out_sh + e % (D / 8) * 8) =
             make_uint4(0u, 0u, 0u, 0u);
   }
-  for (int z = 0; z < rounds; ++z) {
-    const DpDesc d = desc[z * gridDim.x + blockIdx.x];
-    if (d.parts < 2) continue;
-    for (int item = threadIdx.x; item < 128 * (D / 16); item += PM_THREADS) {
-      const int in_half = item & 127, r = blockIdx.y * 128 + in_half, c16 = item >> 7, t = in_half / G, tok = (int)blockIdx.y * TT + t;
-      if (t >= TT || tok >= d.ntok) continue;
-      auto slot = [&](int p) -> int64_t { return ((int64_t)z * gridDim.x + blockIdx.x + p) * 2 + (p == 0 ? d.slot0 : 0); };
-      float top = -CUDART_INF_F, sum = 0.f;
-      float4 acc[4];
+  const int in_half = tid & 127, tok_in = in_half / G;
+  // columns 16 c16 .. + 15 of half `half` of the row tile whose first part is described at `first`
+  auto slice = [&](bool there, int first, int half, int c16, int group, int groups) {
+    DpDesc d{0, 0, 0, 0, 0, {0, 0, 0}};
+    if (there) d = desc[first];
+    const int r = half * 128 + in_half, tok = half * TT + tok_in;
+    const bool live = d.parts > 1 && tok_in < TT && tok < d.ntok;
+    float top = -CUDART_INF_F, sum = 0.f;
+    float4 acc[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < 4; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    // one more set of values: maximum, sum and columns
+    auto add = [&](const float2& ml, const float4 (&v)[4], float t) {
+      if (ml.x == -CUDART_INF_F) return;      // no key of this row was seen
+      const float f = dense_ex2(ml.x - t);
+      sum += f * ml.y;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) { acc[k].x += f * v[k].x; acc[k].y += f * v[k].y; acc[k].z += f * v[k].z; acc[k].w += f * v[k].w; }
+    };
+    auto rise = [&](float t) {
+      const float f = top == -CUDART_INF_F ? 0.f : dense_ex2(top - t);
+      top = t;
+      sum *= f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) { acc[k].x *= f; acc[k].y *= f; acc[k].z *= f; acc[k].w *= f; }
+    };
+    if (live) {
+      auto slot = [&](int p) -> int64_t { return ((int64_t)first + p) * 2 + (p == 0 ? d.slot0 : 0); };
       constexpr int B = 2;
-      for (int base = 0; base < d.parts; base += B) {
+      for (int base = group; base < d.parts; base += B * groups) {
         float2 ml[B];
         float4 v[B][4];
 #pragma unroll
-        for (int p = 0; p < B; ++p) {
-          const bool there = base + p < d.parts;
-          ml[p] = there ? *reinterpret_cast<const float2*>(part_ml + (slot(base + p) * 256 + r) * 2) : make_float2(-CUDART_INF_F, 0.f);
+        for (int b = 0; b < B; ++b) {
+          const int p = base + b * groups;
+          const bool in = p < d.parts;
+          ml[b] = in ? *reinterpret_cast<const float2*>(part_ml + (slot(p) * 256 + r) * 2) : make_float2(-CUDART_INF_F, 0.f);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            v[p][k] = there ? reinterpret_cast<const float4*>(part_acc)[slot(base + p) * 64 * D + (4 * c16 + k) * 256 + r] : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[b][k] = in ? reinterpret_cast<const float4*>(part_acc)[slot(p) * 64 * D + (4 * c16 + k) * 256 + r] : make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        float t2 = top;
+        rise(fmaxf(fmaxf(top, ml[0].x), ml[1].x));
 #pragma unroll
-        for (int p = 0; p < B; ++p) t2 = fmaxf(t2, ml[p].x);
-        const float f0 = top == -CUDART_INF_F ? 0.f : dense_ex2(top - t2);
-        sum *= f0;
+        for (int b = 0; b < B; ++b) add(ml[b], v[b], top);
+      }
+    }
+    if (SPREAD && groups > 1) {
+      s_part[tid] = top;
+      s_part[PM_THREADS + tid] = sum;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) { acc[k].x *= f0; acc[k].y *= f0; acc[k].z *= f0; acc[k].w *= f0; }
-        top = t2;
+      for (int k = 0; k < 4; ++k) {
+        s_part[(2 + 4 * k) * PM_THREADS + tid] = acc[k].x;
+        s_part[(3 + 4 * k) * PM_THREADS + tid] = acc[k].y;
+        s_part[(4 + 4 * k) * PM_THREADS + tid] = acc[k].z;
+        s_part[(5 + 4 * k) * PM_THREADS + tid] = acc[k].w;
+      }
+      __syncthreads();
+      if (group == 0 && live) {
+        float t = top;
+        for (int g = 1; g < groups; ++g) t = fmaxf(t, s_part[tid + 128 * g]);
+        rise(t);
+#pragma unroll 1
+        for (int g = 1; g < groups; ++g) {
+          const float* from = s_part + tid + 128 * g;
+          float4 v[4];
 #pragma unroll
-        for (int p = 0; p < B; ++p) {
-          if (ml[p].x == -CUDART_INF_F) continue;      // the part saw no key of this row
-          const float f = dense_ex2(ml[p].x - t2);
-          sum += f * ml[p].y;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) { acc[k].x += f * v[p][k].x; acc[k].y += f * v[p][k].y; acc[k].z += f * v[p][k].z; acc[k].w += f * v[p][k].w; }
+          for (int k = 0; k < 4; ++k)
+            v[k] = make_float4(from[(2 + 4 * k) * PM_THREADS], from[(3 + 4 * k) * PM_THREADS], from[(4 + 4 * k) * PM_THREADS], from[(5 + 4 * k) * PM_THREADS]);
+          add(make_float2(from[0], from[PM_THREADS]), v, top);
         }
       }
+      __syncthreads();
+    }
+    if (group == 0 && live) {
       const float inv = sum == 0.f ? 0.f : 1.0f / sum;
       uint32_t o[8];
 #pragma unroll
@@ -1089,9 +1134,47 @@ dense_prefill_merge_kernel(DenseArgs a, int G, int TT, int rounds, int tail, con
         o[2 * k] = dense_pack<BF>(acc[k].x * inv, acc[k].y * inv);
         o[2 * k + 1] = dense_pack<BF>(acc[k].z * inv, acc[k].w * inv);
       }
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (int64_t)(d.row0 + tok) * a.out_st + (int64_t)(d.kvh * G + in_half - t * G) * a.out_sh + 16 * c16);
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (int64_t)(d.row0 + tok) * a.out_st + (int64_t)(d.kvh * G + in_half - tok_in * G) * a.out_sh + 16 * c16);
       dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
       dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    }
+  };
+  if constexpr (!SPREAD) {
+    const int half = (int)blockIdx.x >= ctas ? 1 : 0, c = (int)blockIdx.x - half * ctas;
+    for (int z = 0; z < rounds; ++z) slice(tid < 128 * (D / 16), z * ctas + c, half, tid >> 7, 0, 1);
+  } else {
+    // ---- the halves with parts, in the order of desc (the same list in every block) ----
+    int entries = 0, most = 0;
+    for (int base = 0; base < rounds * ctas; base += PM_THREADS) {
+      const int at = base + tid;
+      int parts = 0, n = 0;
+      if (at < rounds * ctas) {
+        parts = desc[at].parts;
+        n = parts < 2 ? 0 : (desc[at].ntok > TT ? 2 : 1);
+      }
+      int inc = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += x;
+      }
+      const int top = __reduce_max_sync(0xffffffffu, n > 0 ? parts : 0);
+      if (lane == 31) s_count[warp] = inc;
+      if (lane == 0) s_most[warp] = top;
+      __syncthreads();
+      const int c = s_count[lane], before = __reduce_add_sync(0xffffffffu, lane < warp ? c : 0);
+      most = max(most, __reduce_max_sync(0xffffffffu, s_most[lane]));
+      for (int h = 0; h < n; ++h) s_list[entries + before + inc - n + h] = (uint16_t)(2 * at + h);
+      entries += __reduce_add_sync(0xffffffffu, c);
+      __syncthreads();
+    }
+    const int slices = entries * (D / 16);
+    int groups = 1;      // four parts each at least
+    while (groups < 8 && groups * 4 < most && slices * groups * 2 <= (int)gridDim.x * (PM_THREADS / 128)) groups *= 2;
+    const int at_once = PM_THREADS / 128 / groups, sub = (tid >> 7) / groups, group = (tid >> 7) - sub * groups;
+    for (int s0 = blockIdx.x * at_once; s0 < slices; s0 += gridDim.x * at_once) {      // the same rounds for all threads of the block
+      const int s = s0 + sub, entry = s < slices ? s_list[s / (D / 16)] : 0;
+      slice(s < slices, entry >> 1, entry & 1, s % (D / 16), group, groups);
     }
   }
 }
@@ -1160,7 +1243,16 @@ int dp_launch(const DenseArgs& all, const DpMaps& maps, int G, int TT, int box, 
   using L = DpL<D>;
   cudaError_t e = cudaFuncSetAttribute(dense_prefill_kernel<BF, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
   if (e != cudaSuccess) return fail((int)e, "dense prefill attention: smem attribute: %s", cudaGetErrorString(e));
-  const int grid = sm_count();
+  const int grid = sm_count(), tt2 = 2 * TT;
+  // few row tiles (at most a quarter of the SMs' number, so four parts or more each) that may be long (64 key tiles, eight parts)
+  const bool spread = (int64_t)all.max_blocks_per_seq * all.block_size >= 64 * DP_KT &&
+                      ((int64_t)all.n_tokens / tt2 + (all.num_seqs < all.n_tokens ? all.num_seqs : all.n_tokens)) * all.num_kv_heads <= grid / 4 &&
+                      grid <= PM_LIST / 2 / DP_MAX_ROUNDS;
+  auto merge = spread ? dense_prefill_merge_kernel<BF, D, true> : dense_prefill_merge_kernel<BF, D, false>;
+  if (spread) {
+    e = cudaFuncSetAttribute(merge, cudaFuncAttributeMaxDynamicSharedMemorySize, PM_SMEM);
+    if (e != cudaSuccess) return fail((int)e, "dense prefill merge: smem attribute: %s", cudaGetErrorString(e));
+  }
   for (int s0 = 0; s0 < all.num_seqs; s0 += DP_MAX_SEQS) {
     const int seqs = all.num_seqs - s0 < DP_MAX_SEQS ? all.num_seqs - s0 : DP_MAX_SEQS;
     DenseArgs a = all;
@@ -1182,10 +1274,10 @@ int dp_launch(const DenseArgs& all, const DpMaps& maps, int G, int TT, int box, 
     e = cudaLaunchKernelEx(&cfg, dense_prefill_kernel<BF, D>, a, maps, seqs, G, TT, box, rounds, w.desc, w.ml, w.acc);
     if (e != cudaSuccess) return fail((int)e, "dense prefill attention: %s", cudaGetErrorString(e));
     if (int rc = check_launch("dense_prefill_attn_kernel")) return rc;
-    cfg.dynamicSmemBytes = 0;
-    cfg.gridDim = dim3((unsigned)grid, 2);
+    cfg.dynamicSmemBytes = spread ? PM_SMEM : 0;
+    cfg.gridDim = dim3((unsigned)(2 * grid));
     cfg.blockDim = dim3(PM_THREADS);
-    e = cudaLaunchKernelEx(&cfg, dense_prefill_merge_kernel<BF, D>, a, G, TT, rounds, zero_tail && s0 + seqs == all.num_seqs ? seqs : -1, (const DpDesc*)w.desc, (const float*)w.ml, (const float*)w.acc);
+    e = cudaLaunchKernelEx(&cfg, merge, a, G, TT, rounds, grid, zero_tail && s0 + seqs == all.num_seqs ? seqs : -1, (const DpDesc*)w.desc, (const float*)w.ml, (const float*)w.acc);
     if (e != cudaSuccess) return fail((int)e, "dense prefill merge: %s", cudaGetErrorString(e));
     if (int rc = check_launch("dense_prefill_merge_kernel")) return rc;
   }

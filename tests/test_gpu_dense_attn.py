@@ -418,3 +418,11 @@ def test_chunks_a_wait_that_runs_out_is_reported():
         _lib.check(_lib.lib().akv_debug_tc_withhold(3, -1), "hook")
     assert torch.equal(a.prefill(q, kc, vc, bt, cl, starts), want)
     assert _lib.device_status()["attn_window"] == 0
+
+
+@pytest.mark.parametrize("lens,new,qh,kvh,D", [([20000], [5], 8, 1, 128), ([17000, 3, 9001], [70, 3, 40], 16, 2, 64), ([12345], [100], 32, 8, 128),
+                                               ([8300], [1], 1, 1, 64), ([9000, 8200], [64, 130], 4, 1, 128)])
+def test_chunks_cut_into_many_parts(lens, new, qh, kvh, D):
+    """Few row tiles of long sequences: every one is cut into many parts, which several groups of threads join."""
+    out = run_chunks(lens, new, qh, kvh, D, 16, torch.bfloat16, seed=sum(lens), scale_q=2.0)
+    assert torch.equal(run_chunks(lens, new, qh, kvh, D, 16, torch.bfloat16, seed=sum(lens), scale_q=2.0), out)
