@@ -38,9 +38,10 @@
 // Rounds.  The CTAs' ranges begin anywhere in the keys, so a KV head's keys and values are wanted at all times of its round,
 // and what does not fit into L2 comes from HBM again for every row tile: at a power limit that costs clock (131 MB of
 // keys and values ran at 1.34 GHz, 24 MB at 1.47).  So the (sequence, KV head) pairs are taken in rounds of about
-// DP_ROUND_BYTES of keys and values, each cut into ranges for all SMs.  Sequences of one row tile read their keys once and do
-// not count: a round more costs some 10 us (its cuts, and the SMs' wait for the first keys), and 32 sequences of 4096 keys with
-// 4 new tokens (4 KV heads of 64) took 54 us in two rounds, 43 in one.
+// DP_ROUND_BYTES of keys and values, each cut into ranges for all SMs.  A round more costs some 10 us (its cuts, and the SMs' wait
+// for the first keys), so only the keys of sequences with DP_ROUND_TILES row tiles or more count (32 / 8 heads of 128): 2048
+// tokens behind 60000 take 1.81 ms in rounds and 2.07 without, 1000 behind 60000 0.95 and 1.09, 800 behind 40000 514 us and 550;
+// 440 behind 20000 152 us and 134, 100 behind 20000 85 and 62; 32 sequences of 4096 with 4 new tokens (4 KV heads of 64) 54 and 43.
 //
 // Measured: 2048 tokens behind 30000 (32 / 8 heads of 128) 0.99 ms in a sustained run at the power limit, 1.05 PFLOP/s, 77 % of
 // the measured sustained matrix rate (0.87 ms, 1.2 PFLOP/s in short bursts; 3000 cycles per tile pair); twelve prompts of 1 to
@@ -64,6 +65,7 @@ constexpr int DP_KT = 128;                       // keys per tile
 constexpr int DP_MAX_SEQS = 384;                 // sequences of one launch
 constexpr int DP_MAX_ROUNDS = 4;
 constexpr int64_t DP_ROUND_BYTES = 68 << 20;     // keys and values of a round
+constexpr int DP_ROUND_TILES = 8;                // row tiles that make keys worth keeping in L2
 constexpr int DP_SNAP = 2;                       // a cut this near to a row tile's edge is moved there, in key tiles (0 and 6: 158 us for the prompts above, 4: 156, 2: 153)
 constexpr int DP_PIECE = 2;                      // what a row tile costs besides its key tiles, in key tiles
 constexpr float DP_RESCALE = 8.0f;
@@ -77,7 +79,7 @@ template <int D> struct DpL {
   static constexpr int NP = D == 128 ? 2 : 4;              // ring slots of K tiles, and of V tiles
   static constexpr int Q = 0, KV = 2 * TILE, BAR = KV + 2 * NP * TILE;      // K slot, V slot, K slot ...
   static constexpr int PRE = BAR + 512;                    // int64 [DP_MAX_SEQS + 1]: units before a sequence ...
-  static constexpr int PREK = PRE + (DP_MAX_SEQS + 1) * 8; // ... and keys before it that several row tiles read
+  static constexpr int PREK = PRE + (DP_MAX_SEQS + 1) * 8; // ... and keys before it that count towards the rounds
   static constexpr int SROW = 80;                          // staging of results: 64 bytes of a row, padded to other banks
   static constexpr int SEQ = PRE + (DP_MAX_SEQS + 1) * 16;       // int [DP_MAX_SEQS][3]: DpSeq of every sequence
   static constexpr int STAGE = (SEQ + DP_MAX_SEQS * 12 + 15) / 16 * 16;     // [8 warps][32 rows][SROW]
@@ -377,7 +379,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
     for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
     if (lane == 0) {
       pre[s + 1] = n * a.num_kv_heads;
-      prek[s + 1] = tiles < 2 ? 0 : (a.window > 0 && a.window + q.qlen < q.total ? a.window + q.qlen : q.total);
+      prek[s + 1] = tiles < DP_ROUND_TILES ? 0 : (a.window > 0 && a.window + q.qlen < q.total ? a.window + q.qlen : q.total);
     }
     my_tiles += tiles;
   }
@@ -1032,7 +1034,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
 // SPREAD, for calls of few row tiles, which have many parts each: every block lists the halves that have parts, the slices are
 // spread over all blocks, and where that leaves threads idle, `groups` of 128 threads share a slice: group g takes parts g,
 // g + groups, ..., and the groups are joined in order through shared memory (their number depends on the call's lengths alone,
-// so results repeat).  100 tokens behind 20000 (32 / 8 heads of 128, 18 parts per row tile) take 86 us with it and 118 without, 5
+// so results repeat).  100 tokens behind 20000 (32 / 8 heads of 128, in two rounds, 18 parts per row tile) took 86 us with it and 118 without, 5
 // tokens (8 / 1 heads, 20 parts) 33 and 37; 5 tokens behind 5000 (5 parts) 23.7 and 22.6, 30 tokens behind 8 sequences of 3000
 // 50.7 and 49.3.
 constexpr int PM_THREADS = 1024, PM_LIST = DP_MAX_ROUNDS * 256 * 2;      // at most 256 SMs
