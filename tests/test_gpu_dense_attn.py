@@ -356,10 +356,15 @@ def test_no_blocks_and_no_tokens():
         assert bool((out[:1] == 0).all()) and bool((out[1:] == 1).all())
 
 
-def test_chunks_in_rounds():
-    """Keys and values of 245 MB: the call goes over its (sequence, KV head) pairs in rounds, every one of them cut into
-    ranges for all SMs (four rounds of three sequences: rounds begin between the KV heads of a sequence)."""
+def test_chunks_of_many_keys():
+    """Keys and values of 245 MB under few row tiles each."""
     run_chunks([20000, 300, 25000, 14700], [70, 300, 130, 1], 16, 8, 128, 16, torch.float16, seed=12)
+
+
+def test_chunks_of_many_row_tiles_in_rounds():
+    """Keys and values of 146 MB that eight row tiles and more read: three rounds, which begin between the KV heads of a
+    sequence, among sequences that do not count towards them."""
+    run_chunks([30000, 300, 40000, 900], [130, 20, 150, 3], 64, 4, 128, 16, torch.float16, seed=13)
 
 
 def test_chunks_past_32_bit_offsets():
