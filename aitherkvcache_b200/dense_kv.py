@@ -104,7 +104,7 @@ class DensePagedAttention:
     ``sliding_window``: keys a token sees, itself included (0: all).  ``scale`` defaults to 1/sqrt(head_dim).
 
     A row that sees no key is zero.  Block-table entries outside the pool are clamped to it, and what pages hold behind
-    a sequence's end does not matter.  Scratch is allocated per call (stream-ordered, so calls on several streams and
+    a sequence's end or before all windows does not matter.  ``out`` overlaps no input.  Scratch is allocated per call (stream-ordered, so calls on several streams and
     captured graphs share nothing)."""
 
     def __init__(self, head_dim: int, num_query_heads: int, num_kv_heads: int, scale: Optional[float] = None,

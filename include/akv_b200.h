@@ -471,8 +471,9 @@ int akv_rotary_kv_append(const akv_rotary_append_params* params);
  * num_kv_heads, head_dim] and out [num_tokens, num_q_heads, head_dim] all of `dtype` (AKV_F16 / AKV_BF16), any strides whose
  * rows start on 16-byte boundaries, last dimension contiguous; num_q_heads a multiple of num_kv_heads; head_dim 64, 128 or
  * 256; any block_size.  block_tables [num_seqs, max_blocks_per_seq] and seq_lens [num_seqs] int32 / int64; entries outside
- * the pool are clamped to it, lengths to [0, max_blocks_per_seq * block_size].  scale positive and finite.  window 0, or the number of keys a token
- * sees, itself included.  A row that sees no key is zero.  Pages behind a sequence's end may hold anything, NaN included.
+ * the pool are clamped to it, lengths to [0, max_blocks_per_seq * block_size].  scale positive and at most 1e38.  window 0,
+ * or the number of keys a token sees, itself included.  A row that sees no key is zero.  What pages hold behind a sequence's
+ * end, or before the first window of a call's rows, may be anything, NaN included.  out overlaps no input.
  *
  * akv_dense_paged_attn: one token per sequence, row s of query and out, the last of its seq_lens[s] tokens (rows behind
  * num_seqs are left alone; query_start_loc is ignored).  Two launches, capturable; the workspace is used by the call alone
@@ -481,8 +482,8 @@ int akv_rotary_kv_append(const akv_rotary_append_params* params);
  * akv_dense_prefill_attn: chunks of new tokens.  Sequence s brings rows query_start_loc[s] .. query_start_loc[s + 1] - 1
  * (int32 / int64, [num_seqs + 1], ascending, from 0), the last of its seq_lens[s] tokens, whose keys and values are in the
  * cache already; token i of n sees the first seq_lens[s] - (n - 1 - i) keys, the last `window` of them with a window.
- * Rows behind the last sequence are left alone, or zeroed with zero_tail.  Two launches, capturable, no host bound on any length needed; workspace as
- * above, 256-byte aligned.  head_dim 64 or 128, at most 128 query heads per KV head, block_size a multiple of 8:
+ * Rows behind the last sequence are left alone, or zeroed with zero_tail.  Two launches, capturable, no host bound on any
+ * length needed; workspace as above, 256-byte aligned.  head_dim 64 or 128, at most 128 query heads per KV head, block_size a multiple of 8:
  * AKV_ERR_UNSUPPORTED otherwise (attend row by row with akv_dense_paged_attn then).  A value that is not finite reaches the
  * rows of its sequence that see its key, and may reach rows of the same 128 keys' tile that do not. */
 typedef struct akv_dense_attn_params {
