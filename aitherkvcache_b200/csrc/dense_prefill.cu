@@ -43,10 +43,11 @@
 // tokens behind 60000 take 1.81 ms in rounds and 2.07 without, 1000 behind 60000 0.95 and 1.09, 800 behind 40000 514 us and 550;
 // 440 behind 20000 152 us and 134, 100 behind 20000 85 and 62; 32 sequences of 4096 with 4 new tokens (4 KV heads of 64) 54 and 43.
 //
-// Measured: 2048 tokens behind 30000 (32 / 8 heads of 128) 0.99 ms in a sustained run at the power limit, 1.05 PFLOP/s, 77 % of
-// the measured sustained matrix rate (0.87 ms, 1.2 PFLOP/s in short bursts; 3000 cycles per tile pair); twelve prompts of 1 to
-// 2000 tokens 153 us, 0.76 PFLOP/s (10 pieces per CTA, each with some 3.6 us of its own: the last P V, the epilogue and the first
-// scores); the 1 to 8 new tokens above 47 us, 3 TB/s.
+// Measured: 2048 tokens behind 30000 (32 / 8 heads of 128) 0.99 ms in a sustained run at the power limit (1.45 GHz), 1.05 PFLOP/s,
+// 77 % of the measured sustained matrix rate; 0.87 ms, 1.2 PFLOP/s in short bursts, 0.77 ms with zero data; 2900 cycles per tile
+// pair.  Some SMs take 14 % longer than the others for the same share and set the end.  Twelve prompts of 1 to 2000 tokens 153
+// us, 0.76 PFLOP/s (10 pieces per CTA, each with 1700 cycles of its own for the last P V and the first scores, and 2600 for the
+// epilogue); the 1 to 8 new tokens above 47 us, 3 TB/s.
 //
 // Every wait is bounded (umma.cuh): a wait that gives up sets g_dense_prefill_status and a flag that ends all loops.
 #include "dense_attn.cuh"
@@ -66,7 +67,8 @@ constexpr int DP_MAX_SEQS = 384;                 // sequences of one launch
 constexpr int DP_MAX_ROUNDS = 4;
 constexpr int64_t DP_ROUND_BYTES = 68 << 20;     // keys and values of a round
 constexpr int DP_ROUND_TILES = 8;                // row tiles that make keys worth keeping in L2
-constexpr int DP_SNAP = 2;                       // a cut this near to a row tile's edge is moved there, in key tiles (0 and 6: 158 us for the prompts above, 4: 156, 2: 153)
+// a cut this near to a row tile's edge is moved there, in key tiles (0 and 6: 158 us for the prompts above, 4: 156, 2: 153)
+constexpr int DP_SNAP = 2;
 constexpr int DP_PIECE = 2;                      // what a row tile costs besides its key tiles, in key tiles
 constexpr float DP_RESCALE = 8.0f;
 
