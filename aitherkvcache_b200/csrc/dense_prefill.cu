@@ -31,8 +31,8 @@
 // 64): 56.7 us, against 65.7 with one half idle.
 //
 // Work split.  The (row tile, key tile) pairs of the whole call are laid end to end and cut into equal ranges, one per SM:
-// every SM finishes at the same time whatever the lengths.  Row tiles that are cut (at most two per CTA) leave float32
-// partials in the workspace, joined by dense_prefill_merge_kernel in the order of the keys; a cut within DP_SNAP tiles of a
+// every SM has the same share whatever the lengths.  Row tiles that are cut (at most two per CTA) leave float32 partials in
+// the workspace, joined by dense_prefill_merge_kernel in a fixed order; a cut within DP_SNAP tiles of a
 // row tile's edge is moved to the edge (a partial costs about as much as two key tiles).
 //
 // Rounds.  The CTAs' ranges begin anywhere in the keys, so a KV head's keys and values are wanted at all times of its round,

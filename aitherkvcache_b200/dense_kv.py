@@ -209,7 +209,8 @@ class DensePagedAttention:
         seq = torch.bucketize(tok, ends, right=True)
         there = (seq < ends.shape[0])[:, None, None]
         seq = seq.clamp_(max=ends.shape[0] - 1)
-        ctx = (seq_lens.to(torch.int64)[seq] - (ends[seq] - 1 - tok)).clamp_(min=0)
+        lens = seq_lens.to(torch.int64).clamp(0, block_tables.shape[1] * k_cache.shape[1])
+        ctx = (lens[seq] - (ends[seq] - 1 - tok)).clamp_(min=0)
         for lo in range(0, n, self.ROWS):
             hi = min(n, lo + self.ROWS)
             rows = self.forward(query[lo:hi], k_cache, v_cache, block_tables[seq[lo:hi]], ctx[lo:hi])

@@ -431,3 +431,13 @@ def test_chunks_cut_into_many_parts(lens, new, qh, kvh, D):
     """Few row tiles of long sequences: every one is cut into many parts, which several groups of threads join."""
     out = run_chunks(lens, new, qh, kvh, D, 16, torch.bfloat16, seed=sum(lens), scale_q=2.0)
     assert torch.equal(run_chunks(lens, new, qh, kvh, D, 16, torch.bfloat16, seed=sum(lens), scale_q=2.0), out)
+
+
+@pytest.mark.parametrize("D,bs", [(128, 16), (256, 16), (64, 5)])
+def test_chunks_longer_than_their_table(D, bs):
+    """Lengths are clamped to what a row of the table addresses, in every path."""
+    q, kc, vc, bt, cl, starts = make([3 * bs, 4 * bs], [9, 12], 4, 2, D, bs, torch.float16, seed=5, stale=math.nan)
+    a = attn(4, 2, D)
+    want = a.prefill(q, kc, vc, bt, torch.full_like(cl, 4 * bs), starts)
+    assert torch.equal(a.prefill(q, kc, vc, bt, torch.tensor([4 * bs + 1, 1 << 40], device="cuda"), starts), want)
+    assert bool((a.prefill(q, kc, vc, bt, torch.full_like(cl, -3), starts) == 0).all())
