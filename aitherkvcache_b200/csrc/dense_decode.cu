@@ -631,7 +631,8 @@ int dense_common(const akv_dense_attn_params* p, const char* who, DenseArgs* a) 
   a->num_q_heads = p->num_q_heads; a->num_kv_heads = p->num_kv_heads; a->head_dim = p->head_dim;
   a->block_size = p->block_size; a->max_blocks_per_seq = p->max_blocks_per_seq; a->num_blocks = p->num_blocks;
   a->scale_log2 = p->scale * 1.4426950408889634f;
-  a->window = p->window;
+  // one that no sequence fills is none (and positions minus the window stay above -2^31)
+  a->window = p->window >= (int64_t)p->max_blocks_per_seq * p->block_size ? 0 : p->window;
   a->out = p->out; a->out_st = p->out_stride_tok; a->out_sh = p->out_stride_head;
   return AKV_OK;
 }

@@ -381,7 +381,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
     for (int d = 16; d > 0; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
     if (lane == 0) {
       pre[s + 1] = n * a.num_kv_heads;
-      prek[s + 1] = tiles < DP_ROUND_TILES ? 0 : (a.window > 0 && a.window + q.qlen < q.total ? a.window + q.qlen : q.total);
+      prek[s + 1] = tiles < DP_ROUND_TILES ? 0 : (a.window > 0 && a.window < q.total - q.qlen ? a.window + q.qlen : q.total);
     }
     my_tiles += tiles;
   }

@@ -119,7 +119,7 @@ class DensePagedAttention:
             raise ValueError(f"sliding_window must not be negative, got {sliding_window}")
         self.head_dim, self.num_query_heads, self.num_kv_heads = head_dim, num_query_heads, num_kv_heads
         self.scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
-        self.sliding_window = int(sliding_window)
+        self.sliding_window = min(int(sliding_window), 0x7fffffff)
         self._decode_bytes = _lib.lib().akv_dense_paged_attn_workspace_bytes(num_query_heads, num_kv_heads, head_dim)
 
     @staticmethod

@@ -441,3 +441,12 @@ def test_chunks_longer_than_their_table(D, bs):
     want = a.prefill(q, kc, vc, bt, torch.full_like(cl, 4 * bs), starts)
     assert torch.equal(a.prefill(q, kc, vc, bt, torch.tensor([4 * bs + 1, 1 << 40], device="cuda"), starts), want)
     assert bool((a.prefill(q, kc, vc, bt, torch.full_like(cl, -3), starts) == 0).all())
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 40, 2 ** 31 - 200, 1500])
+def test_windows_that_no_sequence_fills(window):
+    lens, new = [1400, 300, 1290, 1500], [300, 300, 200, 1]
+    q, kc, vc, bt, cl, starts = make(lens, new, 8, 2, 128, 16, torch.float16, seed=6, stale=math.nan)
+    wide, none = attn(8, 2, 128, sliding_window=window), attn(8, 2, 128)
+    assert torch.equal(wide.prefill(q, kc, vc, bt, cl, starts), none.prefill(q, kc, vc, bt, cl, starts))
+    assert torch.equal(wide.forward(q[:4], kc, vc, bt, cl), none.forward(q[:4], kc, vc, bt, cl))
