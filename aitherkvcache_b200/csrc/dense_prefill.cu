@@ -435,8 +435,9 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
     };
     const int round = warp >> 1;
     const int64_t lo = edge(round), hi = edge(round + 1);
-    // CTAs that share it: all, but not more than there are row tiles or groups of eight units (less is not worth a cut)
-    int64_t want = (hi - lo) >> 3;
+    // CTAs that share it: all, but not more than there are row tiles or groups of six units: a part costs about two (5 tokens
+    // behind 20000, 8 / 1 heads of 128: 22.0 us; with eight units 23.8), and four or fewer could be moved away whole
+    int64_t want = (hi - lo) / 6;
     if (n_rounds == 1) {
       int64_t rts = 0;
       for (int x = 0; x < L::WARPS; ++x) rts += s_tiles[x];
@@ -1047,9 +1048,8 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
 // SPREAD, for calls of few row tiles, which have many parts each: every block lists the halves that have parts, the slices are
 // spread over all blocks, and where that leaves threads idle, `groups` of 128 threads share a slice: group g takes parts g,
 // g + groups, ..., and the groups are joined in order through shared memory (their number depends on the call's lengths alone,
-// so results repeat).  100 tokens behind 20000 (32 / 8 heads of 128, in two rounds, 18 parts per row tile) took 86 us with it and 118 without, 5
-// tokens (8 / 1 heads, 20 parts) 33 and 37; 5 tokens behind 5000 (5 parts) 23.7 and 22.6, 30 tokens behind 8 sequences of 3000
-// 50.7 and 49.3.
+// so results repeat).  100 tokens behind 20000 (32 / 8 heads of 128, 18 parts per row tile) take 58 us with it and 65 without, 60
+// tokens (8 / 1 heads, two row tiles of 20 parts) 36 and 48, 5 tokens 24 and 29; 5 tokens behind 5000 (5 parts) 23.8 and 22.8.
 constexpr int PM_THREADS = 1024, PM_LIST = DP_MAX_ROUNDS * 256 * 2;      // at most 256 SMs
 constexpr int PM_SMEM = PM_THREADS * 18 * (int)sizeof(float);
 template <bool BF, int D, bool SPREAD>
