@@ -376,15 +376,18 @@ def packer(cls):
 
 
 def cuda_index(*tensors) -> int:
-    """Index of the one CUDA device that the tensors (None: left out) are on."""
-    index = -1
+    """Index of the one CUDA device that the tensors (None: left out) are on; raises when one is in host memory (whose
+    index reads -1), when they are on several devices and when there is none."""
+    index = None
     for t in tensors:
         if t is not None:
             i = t.get_device()
             if i != index:
-                if index >= 0 or i < 0:
+                if index is not None or i < 0:
                     require_cuda(*tensors)      # raises what is wrong
                 index = i
+    if index is None:
+        raise RuntimeError("no tensor to take the device from")
     return index
 
 
