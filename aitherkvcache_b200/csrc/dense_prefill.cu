@@ -1253,6 +1253,13 @@ int dp_rounds(int num_kv_heads, int head_dim, int64_t num_blocks, int block_size
   return n <= 1.0 ? 1 : (n >= DP_MAX_ROUNDS ? DP_MAX_ROUNDS : (int)ceil(n));
 }
 
+// A call without sequences: every row is behind the last one.  The merge without parts writes their zeros.
+template <int D>
+int dp_launch_zeros(const DenseArgs& a, int G, int TT, cudaStream_t st) {
+  dense_prefill_merge_kernel<false, D, false><<<2 * sm_count(), PM_THREADS, 0, st>>>(a, G, TT, 0, sm_count(), 0, nullptr, nullptr, nullptr);
+  return check_launch("dense_prefill_merge_kernel");
+}
+
 template <bool BF, int D>
 int dp_launch(const DenseArgs& all, const DpMaps& maps, int G, int TT, int box, int rounds, bool zero_tail, const DpWorkspace& w, cudaStream_t st) {
   using L = DpL<D>;
@@ -1323,24 +1330,26 @@ AKV_EXPORT size_t akv_dense_prefill_attn_workspace_bytes(int num_kv_heads, int h
 AKV_EXPORT int akv_dense_prefill_attn(const akv_dense_attn_params* p) {
   akv::DenseArgs a;
   if (int rc = akv::dense_common(p, "akv_dense_prefill_attn", &a)) return rc;
-  if (a.num_seqs == 0 || a.n_tokens == 0) return AKV_OK;
+  if (a.n_tokens == 0 || (a.num_seqs == 0 && !p->zero_tail)) return AKV_OK;
+  if (!a.out) return akv::fail(AKV_ERR_ARG, "akv_dense_prefill_attn: null out");
   if (!a.starts) return akv::fail(AKV_ERR_ARG, "akv_dense_prefill_attn: null query_start_loc");
   const int G = a.num_q_heads / a.num_kv_heads;
   const int box = a.block_size % 128 == 0 ? 128 : akv::gcd(a.block_size, 128);
   if (a.head_dim == 256 || G > 128 || box < 8 || a.max_blocks_per_seq == 0 || a.num_blocks > 0x7fffffffll)
     return akv::fail(AKV_ERR_UNSUPPORTED, "akv_dense_prefill_attn: head_dim %d, %d query heads per KV head, block_size %d, %d blocks per "
                      "sequence (64 or 128, at most 128, a multiple of 8, at least 1)", a.head_dim, G, a.block_size, a.max_blocks_per_seq);
+  const int TT = 128 / G;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(p->stream);
+  if (a.num_seqs == 0) return a.head_dim == 128 ? akv::dp_launch_zeros<128>(a, G, TT, st) : akv::dp_launch_zeros<64>(a, G, TT, st);
   akv::DpWorkspace w;
   const int rounds = akv::dp_rounds(a.num_kv_heads, a.head_dim, a.num_blocks, a.block_size, a.num_seqs, a.max_blocks_per_seq);
   const size_t need = akv::dp_workspace(a.head_dim, rounds, static_cast<char*>(p->workspace), &w);
   if (!p->workspace || p->workspace_bytes < need || ((uintptr_t)p->workspace & 255))
     return akv::fail(AKV_ERR_WORKSPACE, "akv_dense_prefill_attn: workspace of %zu bytes (256-byte aligned) needed, got %zu", need, p->workspace_bytes);
-  const int TT = 128 / G;
   akv::DpMaps maps;
   const bool bf = p->dtype == AKV_BF16;
   if (!akv::dp_make_maps(a, bf, G, TT, box, &maps))
     return akv::fail(AKV_ERR_UNSUPPORTED, "akv_dense_prefill_attn: these strides cannot be described to the copy unit");
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(p->stream);
   if (a.head_dim == 128) return bf ? akv::dp_launch<true, 128>(a, maps, G, TT, box, rounds, p->zero_tail != 0, w, st) : akv::dp_launch<false, 128>(a, maps, G, TT, box, rounds, p->zero_tail != 0, w, st);
   return bf ? akv::dp_launch<true, 64>(a, maps, G, TT, box, rounds, p->zero_tail != 0, w, st) : akv::dp_launch<false, 64>(a, maps, G, TT, box, rounds, p->zero_tail != 0, w, st);
 }

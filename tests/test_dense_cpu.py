@@ -199,6 +199,21 @@ def test_attention_entry_points_refuse():
     assert large == 4 * small or large > 3.9 * small      # up to four rounds
 
 
+def test_chunk_entry_point_without_sequences():
+    """Rows of a call without sequences are zeroed (zero_tail): their output and the start must be there."""
+    from aitherkvcache_b200 import _lib
+    L = _lib.lib()
+    p = _lib.DenseAttnParams()
+    p.num_tokens, p.num_q_heads, p.num_kv_heads, p.head_dim, p.block_size, p.max_blocks_per_seq, p.num_blocks, p.scale = 4, 2, 2, 128, 16, 3, 9, 1.0
+    assert L.akv_dense_prefill_attn(ctypes.byref(p)) == 0      # nothing asked for
+    p.zero_tail = 1
+    assert L.akv_dense_prefill_attn(ctypes.byref(p)) == _lib.AKV_ERR_ARG
+    p.out = 256
+    assert L.akv_dense_prefill_attn(ctypes.byref(p)) == _lib.AKV_ERR_ARG
+    p.num_tokens = 0
+    assert L.akv_dense_prefill_attn(ctypes.byref(p)) == 0
+
+
 def test_backend_window_of_uncompressed_layers():
     from aitherkvcache_b200.vllm.backend import TurboQuantImplBase
     impl = TurboQuantImplBase()

@@ -450,3 +450,20 @@ def test_windows_that_no_sequence_fills(window):
     wide, none = attn(8, 2, 128, sliding_window=window), attn(8, 2, 128)
     assert torch.equal(wide.prefill(q, kc, vc, bt, cl, starts), none.prefill(q, kc, vc, bt, cl, starts))
     assert torch.equal(wide.forward(q[:4], kc, vc, bt, cl), none.forward(q[:4], kc, vc, bt, cl))
+
+
+@pytest.mark.parametrize("D,bs", [(64, 16), (128, 16), (256, 16), (128, 5)])
+@pytest.mark.parametrize("n", [1, 4, 3000])
+def test_no_sequences_in_memory_that_held_something_else(D, bs, n):
+    """Rows of a call without sequences are behind the last one: zeros, whatever the block that the allocator hands out held."""
+    q = torch.randn(n, 4, D, device="cuda").half()
+    kc, vc = (torch.randn(3, bs, 2, D, device="cuda").half() for _ in range(2))
+    table, none = torch.zeros(0, 2, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda")
+    a = attn(4, 2, D)
+    for starts in (torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda")):
+        used = torch.full_like(q, math.nan)
+        del used
+        assert bool((a.prefill(q, kc, vc, table, none, starts) == 0).all())
+        out = torch.full((n, 6, D), 5.0, dtype=torch.float16, device="cuda")
+        a.prefill(q, kc, vc, table, none, starts, out=out[:, 1:5])
+        assert bool((out == 5.0).all())
