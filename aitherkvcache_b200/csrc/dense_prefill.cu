@@ -1054,20 +1054,21 @@ constexpr int PM_THREADS = 1024, PM_LIST = DP_MAX_ROUNDS * 256 * 2;      // at m
 constexpr int PM_SMEM = PM_THREADS * 18 * (int)sizeof(float);
 template <bool BF, int D, bool SPREAD>
 __global__ void __launch_bounds__(PM_THREADS)
-dense_prefill_merge_kernel(DenseArgs a, int G, int TT, int rounds, int ctas, int tail, const DpDesc* desc, const float* part_ml, const float* part_acc) {
+dense_prefill_merge_kernel(DenseArgs a, int G, int TT, int rounds, int ctas, int head, int tail, const DpDesc* desc, const float* part_ml, const float* part_acc) {
   extern __shared__ float s_part[];                    // [18][PM_THREADS]: maximum, sum, 16 columns
   __shared__ uint16_t s_list[SPREAD ? PM_LIST : 1];    // 2 * place in desc + half
   __shared__ int s_count[32], s_most[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (tail >= 0) {              // rows behind the last sequence (`tail` of them in this launch) come out as zeros
-    int64_t row = load_index(a.starts, a.qs_dtype, tail);
-    if (row < 0) row = 0;
-    for (row += blockIdx.x; row < a.n_tokens; row += gridDim.x)
+  auto zeros = [&](int64_t from, int64_t to) {
+    for (int64_t row = (from > 0 ? from : 0) + blockIdx.x; row < to && row < a.n_tokens; row += gridDim.x)
       for (int e = tid; e < a.num_q_heads * (D / 8); e += PM_THREADS)
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.out_st + (int64_t)(e / (D / 8)) * a.out_sh + e % (D / 8) * 8) =
             make_uint4(0u, 0u, 0u, 0u);
-  }
+  };
+  // rows before the first sequence and behind the last (`tail` of them in this launch) come out as zeros
+  if (head) zeros(0, load_index(a.starts, a.qs_dtype, 0));
+  if (tail >= 0) zeros(load_index(a.starts, a.qs_dtype, tail), a.n_tokens);
   const int in_half = tid & 127, tok_in = in_half / G;
   // columns 16 c16 .. + 15 of half `half` of the row tile whose first part is described at `first`
   auto slice = [&](bool there, int first, int half, int c16, int group, int groups) {
@@ -1253,10 +1254,10 @@ int dp_rounds(int num_kv_heads, int head_dim, int64_t num_blocks, int block_size
   return n <= 1.0 ? 1 : (n >= DP_MAX_ROUNDS ? DP_MAX_ROUNDS : (int)ceil(n));
 }
 
-// A call without sequences: every row is behind the last one.  The merge without parts writes their zeros.
+// A call without sequences: no row belongs to one.  The merge without parts writes their zeros.
 template <int D>
 int dp_launch_zeros(const DenseArgs& a, int G, int TT, cudaStream_t st) {
-  dense_prefill_merge_kernel<false, D, false><<<2 * sm_count(), PM_THREADS, 0, st>>>(a, G, TT, 0, sm_count(), 0, nullptr, nullptr, nullptr);
+  dense_prefill_merge_kernel<false, D, false><<<2 * sm_count(), PM_THREADS, 0, st>>>(a, G, TT, 0, sm_count(), 1, 0, nullptr, nullptr, nullptr);
   return check_launch("dense_prefill_merge_kernel");
 }
 
@@ -1299,7 +1300,7 @@ int dp_launch(const DenseArgs& all, const DpMaps& maps, int G, int TT, int box, 
     cfg.dynamicSmemBytes = spread ? PM_SMEM : 0;
     cfg.gridDim = dim3((unsigned)(2 * grid));
     cfg.blockDim = dim3(PM_THREADS);
-    e = cudaLaunchKernelEx(&cfg, merge, a, G, TT, rounds, grid, zero_tail && s0 + seqs == all.num_seqs ? seqs : -1, (const DpDesc*)w.desc, (const float*)w.ml, (const float*)w.acc);
+    e = cudaLaunchKernelEx(&cfg, merge, a, G, TT, rounds, grid, zero_tail && s0 == 0 ? 1 : 0, zero_tail && s0 + seqs == all.num_seqs ? seqs : -1, (const DpDesc*)w.desc, (const float*)w.ml, (const float*)w.acc);
     if (e != cudaSuccess) return fail((int)e, "dense prefill merge: %s", cudaGetErrorString(e));
     if (int rc = check_launch("dense_prefill_merge_kernel")) return rc;
   }

@@ -173,8 +173,8 @@ class DensePagedAttention:
                 max_seq_len: Optional[int] = None) -> torch.Tensor:
         """Chunks of new tokens: rows ``query_start_loc[s] .. query_start_loc[s + 1]`` of ``query`` [tokens, query_heads,
         head_dim] are the last tokens of sequence s, whose keys and values (counted in ``seq_lens``) are in the cache
-        already; each attends causally up to its own position.  Rows behind the last sequence are left as they are in
-        ``out`` (zero when ``out`` is allocated here).  Lengths stay on the device: ``max_seq_len``, which
+        already; each attends causally up to its own position.  Rows before the first sequence and behind the last are left as
+        they are in ``out`` (zero when ``out`` is allocated here).  Lengths stay on the device: ``max_seq_len``, which
         ``TQPagedAttention.prefill`` sizes its scratch by, is accepted and not needed.
 
         Chunks run on the tensor cores for head_dim 64 and 128, at most 128 query heads per KV head and block sizes that
@@ -207,7 +207,7 @@ class DensePagedAttention:
         tok = torch.arange(n, device=query.device, dtype=torch.int64)
         ends = query_start_loc[1:].to(torch.int64).contiguous()
         seq = torch.bucketize(tok, ends, right=True)
-        there = (seq < ends.shape[0])[:, None, None]
+        there = ((seq < ends.shape[0]) & (tok >= query_start_loc[0]))[:, None, None]
         seq = seq.clamp_(max=ends.shape[0] - 1)
         lens = seq_lens.to(torch.int64).clamp(0, block_tables.shape[1] * k_cache.shape[1])
         ctx = (lens[seq] - (ends[seq] - 1 - tok)).clamp_(min=0)

@@ -480,9 +480,9 @@ int akv_rotary_kv_append(const akv_rotary_append_params* params);
  * until it has finished.
  *
  * akv_dense_prefill_attn: chunks of new tokens.  Sequence s brings rows query_start_loc[s] .. query_start_loc[s + 1] - 1
- * (int32 / int64, [num_seqs + 1], ascending, from 0), the last of its seq_lens[s] tokens, whose keys and values are in the
+ * (int32 / int64, [num_seqs + 1], ascending), the last of its seq_lens[s] tokens, whose keys and values are in the
  * cache already; token i of n sees the first seq_lens[s] - (n - 1 - i) keys, the last `window` of them with a window.
- * Rows behind the last sequence are left alone, or zeroed with zero_tail.  Two launches, capturable, no host bound on any
+ * Rows before the first sequence and behind the last are left alone, or zeroed with zero_tail (also with num_seqs 0).  Two launches, capturable, no host bound on any
  * length needed; workspace as above, 256-byte aligned.  head_dim 64 or 128, at most 128 query heads per KV head, block_size a multiple of 8:
  * AKV_ERR_UNSUPPORTED otherwise (attend row by row with akv_dense_paged_attn then).  A value that is not finite reaches the
  * rows of its sequence that see its key, and may reach rows of the same 128 keys' tile that do not. */
@@ -497,7 +497,7 @@ typedef struct akv_dense_attn_params {
   int64_t num_blocks;
   float scale; int window;
   void* out; int64_t out_stride_tok, out_stride_head;
-  int zero_tail;   /* akv_dense_prefill_attn: write zeros to the rows behind the last sequence */
+  int zero_tail;   /* akv_dense_prefill_attn: write zeros to the rows that belong to no sequence */
   void* workspace; size_t workspace_bytes;
   void* stream;
 } akv_dense_attn_params;

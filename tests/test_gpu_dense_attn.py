@@ -467,3 +467,24 @@ def test_no_sequences_in_memory_that_held_something_else(D, bs, n):
         out = torch.full((n, 6, D), 5.0, dtype=torch.float16, device="cuda")
         a.prefill(q, kc, vc, table, none, starts, out=out[:, 1:5])
         assert bool((out == 5.0).all())
+
+
+@pytest.mark.parametrize("D,bs,first,seqs", [(64, 16, 3, 2), (128, 16, 700, 2), (256, 16, 5, 2), (128, 5, 5, 2), (64, 16, 40, 400), (128, 16, 9, 1)])
+def test_chunks_rows_before_the_first_sequence(D, bs, first, seqs):
+    """query_start_loc of a batch's later sequences: the rows of those before belong to no sequence of the call."""
+    lens, new = [first + 50] + [70 + i % 5 for i in range(seqs)], [first] + [33 - i % 30 for i in range(seqs)]
+    q, kc, vc, bt, cl, starts = make(lens, new, 4, 2, D, bs, torch.float16, seed=D + first, tail=6)
+    a = attn(4, 2, D)
+    want = a.prefill(q, kc, vc, bt, cl, starts)
+    used = torch.full_like(q, math.nan)
+    del used
+    out = a.prefill(q, kc, vc, bt[1:], cl[1:], starts[1:])
+    assert bool((out[:first] == 0).all()) and bool((out[-6:] == 0).all())
+    want[:first] = 0
+    _, bound = od.attention(q, kc, vc, bt, cl.tolist(), starts.tolist(), 1 / math.sqrt(D), 0)
+    # both are within the bound of the same values (their cuts may differ)
+    assert bool(((out.double() - want.double()).abs() <= 2 * bound)[first:-6].all())
+    out = torch.full((q.shape[0], 6, D), 5.0, dtype=torch.float16, device="cuda")
+    a.prefill(q, kc, vc, bt[1:], cl[1:], starts[1:], out=out[:, 1:5])
+    assert bool((out[:first] == 5.0).all()) and bool((out[-6:] == 5.0).all()) and bool((out[:, 0] == 5.0).all())
+    assert bool(((out[:, 1:5].double() - want.double()).abs() <= 2 * bound)[first:-6].all())
