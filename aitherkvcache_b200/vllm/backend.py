@@ -169,10 +169,24 @@ class TurboQuantImplBase:
             _LayerState.v_norms[layer_name] = torch.zeros_like(kn)
         return kn, _LayerState.v_norms[layer_name]
 
+    def _dense(self, kv_cache: torch.Tensor) -> bool:
+        """Whether this layer's cache stays in 16 bits.  Its operators apply scale and sliding window and nothing else of
+        what vLLM's impls are given: the rest is refused by name."""
+        if kv_cache.dtype not in DENSE_DTYPES:
+            return False
+        asked = [name for name, none in (("logits_soft_cap", (None, 0)), ("chunk_lookback", (None, -1))) if getattr(self, name, None) not in none]
+        asked += [name for name in ("alibi_slopes", "sinks") if getattr(self, name, None) is not None]
+        kind = getattr(self, "attn_type", None)
+        if getattr(kind, "value", kind) not in (None, "decoder"):
+            asked.append("attn_type")
+        if asked:
+            raise NotImplementedError(f"a layer with a {kv_cache.dtype} cache applies no {' and no '.join(asked)}")
+        return True
+
     def do_kv_cache_update(self, layer, key, value, kv_cache, slot_mapping) -> None:
         """Encode ``key`` / ``value`` [tokens, kv_heads, head_size] into the packed cache in place (a 16-bit cache takes them
         as they are)."""
-        if kv_cache.dtype in DENSE_DTYPES:
+        if self._dense(kv_cache):
             from ..dense_kv import kv_append
             kv_append(key[:slot_mapping.shape[0]], value[:slot_mapping.shape[0]], slot_mapping, kv_cache[:, 0], kv_cache[:, 1])
             return
@@ -194,7 +208,7 @@ class TurboQuantImplBase:
         """``do_kv_cache_update`` of keys that are not rotated yet: ``query`` [tokens, heads, head_size] and ``key`` are turned
         to ``positions`` by ``rope`` (a ``RotaryPositions``) on the way.  Returns the rotated query.  One launch for a 16-bit
         cache; in front of the codecs the rotation is a launch of its own."""
-        if kv_cache.dtype in DENSE_DTYPES:
+        if self._dense(kv_cache):
             from ..dense_kv import rotary_kv_append
             return rotary_kv_append(query, key, value, positions, slot_mapping, kv_cache[:, 0], kv_cache[:, 1], rope, query_out)
         query_out, key = rope.forward(query, key, positions, query_out=query_out)
@@ -217,7 +231,7 @@ class TurboQuantImplBase:
         return attn
 
     def _attend(self, layer, q, out, kv_cache, block_table, context_lens) -> None:
-        if kv_cache.dtype in DENSE_DTYPES:
+        if self._dense(kv_cache):
             self._dense_attention(kv_cache).forward(q, kv_cache[:, 0], kv_cache[:, 1], block_table, context_lens, out=out)
             return
         pd, bs = self.packed_dim, kv_cache.shape[2]
@@ -246,7 +260,7 @@ class TurboQuantImplBase:
         one pass over its packed blocks); False when they are not built for the case (3- / 2-bit codes in a batch too
         ragged for the staged tensor-core kernel, rows that are not readable in 16-byte pieces), in which case every
         token becomes a row of the decode kernels."""
-        if kv_cache.dtype in DENSE_DTYPES:
+        if self._dense(kv_cache):
             self._dense_attention(kv_cache).prefill(q, kv_cache[:, 0], kv_cache[:, 1], md.block_table, md.seq_lens,
                                                     md.query_start_loc, out=out)
             return True

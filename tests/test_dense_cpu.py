@@ -223,3 +223,52 @@ def test_backend_window_of_uncompressed_layers():
         impl.sliding_window = value
         attn = impl._dense_attention(cache)
         assert (attn.sliding_window, attn.scale, attn.head_dim, attn.num_kv_heads) == (window, 0.1, 128, 2)
+
+
+class _Enum:
+    value = "encoder_only"
+
+
+@pytest.mark.parametrize("name,value", [("logits_soft_cap", 30.0), ("alibi_slopes", [0.5] * 8), ("sinks", torch.zeros(8)),
+                                        ("attn_type", "encoder"), ("attn_type", _Enum()), ("chunk_lookback", 1)])
+def test_backend_refuses_what_uncompressed_layers_do_not_compute(name, value):
+    """Scale and sliding window are all that the 16-bit path applies: an impl that asks for more is refused by name, in
+    every method that meets the cache, before anything is written or launched."""
+    from aitherkvcache_b200.vllm.backend import TurboQuantImplBase
+    cache = torch.zeros(3, 2, 16, 2, 128, dtype=torch.bfloat16)
+    q, k, n = torch.zeros(4, 8, 128, dtype=torch.bfloat16), torch.zeros(4, 2, 128, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int64)
+    impl = TurboQuantImplBase()
+    impl._tq_setup(8, 128, 0.1, 2, "auto")
+    setattr(impl, name, value)
+    for run in (lambda: impl.do_kv_cache_update(None, k, k, cache, n), lambda: impl.rope_and_kv_cache_update(None, q, k, k, n, None, cache, n),
+                lambda: impl._attend(None, q, q, cache, n[:, None], n), lambda: impl._prefill(None, q, q, cache, None)):
+        with pytest.raises(NotImplementedError, match=name):
+            run()
+
+
+def test_backend_takes_uncompressed_layers_without_them():
+    """What vLLM's impls hold where none of these is asked for."""
+    from aitherkvcache_b200.vllm.backend import TurboQuantImplBase
+    cache, k, n = torch.zeros(3, 2, 16, 2, 128, dtype=torch.bfloat16), torch.zeros(4, 2, 128, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int64)
+    for cap, kind in ((None, "decoder"), (0, "decoder"), (0.0, None)):
+        impl = TurboQuantImplBase()
+        impl._tq_setup(8, 128, 0.1, 2, "auto")
+        impl.logits_soft_cap, impl.alibi_slopes, impl.sinks, impl.attn_type, impl.chunk_lookback = cap, None, None, kind, -1
+        with pytest.raises(RuntimeError, match="CUDA tensors only"):      # as far as a host without a GPU gets
+            impl.do_kv_cache_update(None, k, k, cache, n)
+
+
+def test_backend_under_vllm_reads_its_impl(monkeypatch):
+    """The attributes are those that vLLM's own constructor sets."""
+    pytest.importorskip("vllm")
+    from aitherkvcache_b200.vllm.backend import TurboQuantBackend
+    for name in ("AITHER_TQ_MODE", "AITHER_TQ_BITS"):
+        monkeypatch.delenv(name, raising=False)
+    make = lambda **kw: TurboQuantBackend.get_impl_cls()(num_heads=8, head_size=128, scale=0.1, num_kv_heads=2, sliding_window=None,  # noqa: E731
+                                                         kv_cache_dtype="auto", **{"alibi_slopes": None, **kw})
+    cache = torch.zeros(3, 2, 16, 2, 128, dtype=torch.bfloat16)
+    assert make()._dense(cache) and not make()._dense(cache.view(torch.uint8))
+    for kw in (dict(logits_soft_cap=50.0), dict(alibi_slopes=[0.5] * 8), dict(sinks=torch.zeros(8))):
+        with pytest.raises(NotImplementedError, match=next(iter(kw))):
+            make(**kw)._dense(cache)
+        assert not make(**kw)._dense(cache.view(torch.uint8))
