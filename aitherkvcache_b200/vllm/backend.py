@@ -24,11 +24,14 @@ classes are created on first attribute access so that importing this module does
 from __future__ import annotations
 
 import inspect
+import logging
 import types
 import os
 from typing import Dict, Optional, Tuple
 
 import torch
+
+logger = logging.getLogger("aitherkvcache_b200.backend")
 
 KV_DTYPE_BITS = {"tq-t4nc": 4, "tq-t3nc": 3, "tq-t2nc": 2}
 KV_DTYPE_HYBRID = {"tq-t35nc": "tq35", "tq-t25nc": "tq25"}
@@ -61,6 +64,7 @@ class _LayerState:
     attention: Dict[tuple, object] = {}
     k_norms: Dict[str, torch.Tensor] = {}
     v_norms: Dict[str, torch.Tensor] = {}
+    told: set = set()      # what has been logged once
 
 
 def _quantizer(head_size: int, bits: int, device):
@@ -107,6 +111,7 @@ class TurboQuantImplBase:
                   kv_cache_dtype: str = "auto") -> None:
         self.num_heads, self.head_size, self.scale = num_heads, head_size, float(scale)
         self.num_kv_heads = num_kv_heads
+        self.tq_named_dtype = kv_cache_dtype if kv_cache_dtype in KV_DTYPE_BITS or kv_cache_dtype in KV_DTYPE_HYBRID else ""
         self.tq_codec, what = codec_from_env_or_dtype(kv_cache_dtype)
         if self.tq_codec == "hybrid":
             from ..hybrid_quantizer import HybridTurboQuant
@@ -171,9 +176,16 @@ class TurboQuantImplBase:
 
     def _dense(self, kv_cache: torch.Tensor) -> bool:
         """Whether this layer's cache stays in 16 bits.  Its operators apply scale and sliding window and nothing else of
-        what vLLM's impls are given: the rest is refused by name."""
+        what vLLM's impls are given: the rest is refused by name.  So is a layer whose own cache dtype is a compressed one;
+        where only the environment names a codec, the layer may be an exempt one, and that is said once."""
         if kv_cache.dtype not in DENSE_DTYPES:
             return False
+        if self.tq_named_dtype:
+            raise TypeError(f"the cache of a layer with cache dtype {self.tq_named_dtype} must be uint8, got {kv_cache.dtype}")
+        codec = os.environ.get("AITHER_TQ_MODE") or os.environ.get("AITHER_TQ_BITS")
+        if codec not in (None, "", "0") and kv_cache.dtype not in _LayerState.told:
+            _LayerState.told.add(kv_cache.dtype)
+            logger.warning("the environment names codec %s, but layers were given a %s cache: they stay uncompressed", codec, kv_cache.dtype)
         asked = [name for name, none in (("logits_soft_cap", (None, 0)), ("chunk_lookback", (None, -1))) if getattr(self, name, None) not in none]
         asked += [name for name in ("alibi_slopes", "sinks") if getattr(self, name, None) is not None]
         kind = getattr(self, "attn_type", None)

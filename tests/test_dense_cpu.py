@@ -272,3 +272,36 @@ def test_backend_under_vllm_reads_its_impl(monkeypatch):
         with pytest.raises(NotImplementedError, match=next(iter(kw))):
             make(**kw)._dense(cache)
         assert not make(**kw)._dense(cache.view(torch.uint8))
+
+
+@pytest.mark.parametrize("name", ["tq-t4nc", "tq-t3nc", "tq-t2nc", "tq-t35nc", "tq-t25nc"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_backend_refuses_16_bit_caches_of_layers_with_a_compressed_dtype(name, dtype):
+    """A layer that was set up with a compressed cache dtype is not stored uncompressed without a word."""
+    from aitherkvcache_b200.vllm.backend import TurboQuantImplBase
+    cache, n = torch.zeros(3, 2, 16, 2, 128, dtype=dtype), torch.zeros(4, dtype=torch.int64)
+    q, k = torch.zeros(4, 8, 128, dtype=dtype), torch.zeros(4, 2, 128, dtype=dtype)
+    impl = TurboQuantImplBase()
+    impl._tq_setup(8, 128, 0.1, 2, name)
+    for run in (lambda: impl.do_kv_cache_update(None, k, k, cache, n), lambda: impl.rope_and_kv_cache_update(None, q, k, k, n, None, cache, n),
+                lambda: impl._attend(None, q, q, cache, n[:, None], n), lambda: impl._prefill(None, q, q, cache, None)):
+        with pytest.raises(TypeError, match=name):
+            run()
+
+
+@pytest.mark.parametrize("env,value,words", [("AITHER_TQ_MODE", "tq35", 1), ("AITHER_TQ_BITS", "3", 1), (None, "", 0)])
+def test_backend_says_once_that_a_layer_stays_uncompressed(monkeypatch, caplog, env, value, words):
+    """Where the environment names a codec and the layer's dtype does not, a 16-bit cache is taken and said so, once."""
+    from aitherkvcache_b200.vllm import backend
+    for name in ("AITHER_TQ_MODE", "AITHER_TQ_BITS"):
+        monkeypatch.delenv(name, raising=False)
+    if env:
+        monkeypatch.setenv(env, value)
+    monkeypatch.setattr(backend._LayerState, "told", set())
+    impl = backend.TurboQuantImplBase()
+    impl._tq_setup(8, 128, 0.1, 2, "auto")
+    with caplog.at_level("WARNING"):
+        for _ in range(3):
+            assert impl._dense(torch.zeros(3, 2, 16, 2, 128, dtype=torch.bfloat16))
+            assert not impl._dense(torch.zeros(3, 2, 16, 2, 128, dtype=torch.uint8))
+    assert sum("uncompressed" in r.getMessage() for r in caplog.records) == words
