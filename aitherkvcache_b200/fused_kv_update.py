@@ -53,6 +53,8 @@ def fused_tq4_kv_update(
     bits = _BITS_FROM_BOUNDARIES.get(boundaries.numel())
     if bits is None:
         raise ValueError(f"expected 15, 7 or 3 boundaries, got {boundaries.numel()}")
+    if slot_mapping.numel() < num_tokens:
+        raise ValueError(f"slot_mapping has {slot_mapping.numel()} slots for {num_tokens} tokens")
     dev = _lib.require_cuda(x, slot_mapping, out_packed, out_norms, rotation, boundaries)
     if x.dtype not in _lib._FLOAT_CODES:
         x = x.float()

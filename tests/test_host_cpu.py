@@ -299,3 +299,35 @@ def test_ctypes_structures_match_the_header_layout(tmp_path):
         assert ctypes.sizeof(st) == int(size), cname
         got = [getattr(st, f).offset for f, _ in st._fields_]
         assert got == [int(o) for o in offs], (cname, names[cname], [f for f, _ in st._fields_])
+
+
+@pytest.mark.parametrize("dtype", ["tq-t4nc", "tq-t3nc", "tq-t35nc"])
+def test_backend_update_of_a_padded_batch(monkeypatch, dtype):
+    """Keys and values padded behind the slots' length (vLLM pads the token dimension): the codecs are given the tokens
+    that have a slot, no more."""
+    import types
+    from aitherkvcache_b200 import fused_kv_update, hybrid_quantizer
+    from aitherkvcache_b200.vllm import backend
+    seen = []
+    monkeypatch.setattr(fused_kv_update, "fused_tq4_kv_update", lambda x, slots, *a, **k: seen.append((x, slots)))
+    monkeypatch.setattr(hybrid_quantizer, "hybrid_kv_update", lambda htq, x, slots, *a, **k: seen.append((x, slots)))
+    tq = types.SimpleNamespace(rotation=None, rotation_T=None, boundaries_inner=None)
+    monkeypatch.setattr(backend, "_quantizer", lambda *a: tq)
+    monkeypatch.setattr(backend, "_hybrid_quantizer", lambda *a: tq)
+    impl = backend.TurboQuantImplBase()
+    impl._tq_setup(8, 128, 0.1, 2, dtype)
+    key, value = torch.randn(9, 2, 128), torch.randn(9, 2, 128)
+    slots = torch.arange(6)
+    impl.do_kv_cache_update(types.SimpleNamespace(layer_name="x"), key, value, torch.zeros(4, 2, 16, 2, 128, dtype=torch.uint8), slots)
+    assert len(seen) == 2
+    for (x, s), whole in zip(seen, (key, value)):
+        assert torch.equal(x, whole[:6]) and s is slots
+
+
+def test_packed_update_refuses_fewer_slots_than_tokens():
+    """A slot per token: with fewer the kernel would read behind them.  Refused before anything looks for a device."""
+    from aitherkvcache_b200 import fused_tq4_kv_update
+    x, bounds = torch.zeros(5, 2, 128), torch.zeros(15)
+    for slots in (torch.arange(4), torch.zeros(0, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="slot_mapping"):
+            fused_tq4_kv_update(x, slots, torch.zeros(2, 16, 2, 64, dtype=torch.uint8), torch.zeros(2, 16, 2), torch.zeros(128, 128), bounds)
