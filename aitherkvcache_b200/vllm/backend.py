@@ -219,10 +219,14 @@ class TurboQuantImplBase:
 
     def rope_and_kv_cache_update(self, layer, query, key, value, positions, rope, kv_cache, slot_mapping, query_out=None):
         """``do_kv_cache_update`` of keys that are not rotated yet: ``query`` [tokens, heads, head_size] and ``key`` are turned
-        to ``positions`` by ``rope`` (a ``RotaryPositions``) on the way.  Returns the rotated query.  One launch for a 16-bit
-        cache; in front of the codecs the rotation is a launch of its own."""
+        to ``positions`` by ``rope`` (a ``RotaryPositions``) on the way.  Returns the rotated query, padding (tokens behind the
+        length of ``slot_mapping``) included.  One launch for a 16-bit cache; in front of the codecs the rotation is a launch of
+        its own.  For callers that own their rotation: vLLM's layers rotate by themselves and call ``do_kv_cache_update``."""
         if self._dense(kv_cache):
             from ..dense_kv import rotary_kv_append
+            padding = key.shape[0] - slot_mapping.shape[0]
+            if padding > 0:
+                slot_mapping = torch.nn.functional.pad(slot_mapping, (0, padding), value=-1)
             return rotary_kv_append(query, key, value, positions, slot_mapping, kv_cache[:, 0], kv_cache[:, 1], rope, query_out)
         query_out, key = rope.forward(query, key, positions, query_out=query_out)
         self.do_kv_cache_update(layer, key, value, kv_cache, slot_mapping)

@@ -305,3 +305,23 @@ def test_backend_says_once_that_a_layer_stays_uncompressed(monkeypatch, caplog, 
             assert impl._dense(torch.zeros(3, 2, 16, 2, 128, dtype=torch.bfloat16))
             assert not impl._dense(torch.zeros(3, 2, 16, 2, 128, dtype=torch.uint8))
     assert sum("uncompressed" in r.getMessage() for r in caplog.records) == words
+
+
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+def test_backend_rotating_update_of_a_padded_batch(monkeypatch, index):
+    """Tokens behind the slots' length are padding: turned, and without a slot.  Other batches go through as they are."""
+    from aitherkvcache_b200 import dense_kv
+    from aitherkvcache_b200.vllm.backend import TurboQuantImplBase
+    seen = []
+    monkeypatch.setattr(dense_kv, "rotary_kv_append", lambda *a: seen.append(a) or "query")
+    impl = TurboQuantImplBase()
+    impl._tq_setup(8, 128, 0.1, 2, "auto")
+    cache = torch.zeros(3, 2, 16, 2, 128, dtype=torch.bfloat16)
+    q, k, v, pos = torch.zeros(9, 8, 128), torch.zeros(9, 2, 128), torch.zeros(9, 2, 128), torch.zeros(3, 9, dtype=torch.int64)
+    for n in (6, 9, 0):
+        slots = torch.arange(n, dtype=index)
+        assert impl.rope_and_kv_cache_update(None, q, k, v, pos, "rope", cache, slots, "out") == "query"
+        got = seen.pop()
+        assert got[0] is q and got[1] is k and got[2] is v and got[3] is pos and got[7:] == ("rope", "out")
+        assert got[4].dtype == index and got[4].tolist() == list(range(n)) + [-1] * (9 - n)
+        assert n < 9 or got[4] is slots

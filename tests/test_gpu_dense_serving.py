@@ -207,3 +207,30 @@ def test_kv_append(src, dst, heads, D, bs):
             got = caches.clone()
             kv_append(key, form(value), slots.int().cuda(), got[:, 0], got[:, 1])
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("kind", ["dense", "packed"])
+@pytest.mark.parametrize("pad", [1, 30])
+def test_backend_rotating_update_of_a_padded_batch(kind, pad):
+    """Query, key, value and positions padded behind the slots' length: what has a slot is stored as without the padding,
+    nothing else is touched, and every query row is turned."""
+    QH, H, D, bs, n = 8, 2, 128, 16, 37
+    from aitherkvcache_b200 import RotaryPositions
+    impl, rope = _impl(QH, H, D), RotaryPositions(D, base=1e4)
+    layer = types.SimpleNamespace(layer_name="padded")
+    g = torch.Generator().manual_seed(pad)
+    q, k, v = (torch.randn(n + pad, h, D, generator=g).half().cuda() for h in (QH, H, H))
+    slots, pos = torch.randperm(64, generator=g)[:n].cuda(), torch.arange(n + pad).cuda()
+    dtype = torch.float16 if kind == "dense" else torch.uint8
+    a, b = (torch.zeros(4, 2, bs, H, D, dtype=dtype, device="cuda") for _ in range(2))
+    qa = impl.rope_and_kv_cache_update(layer, q, k, v, pos, rope, a, slots)
+    qb = impl.rope_and_kv_cache_update(layer, q[:n], k[:n], v[:n], pos[:n], rope, b, slots)
+    assert torch.equal(a, b) and int((a != 0).sum()) > 0
+    assert torch.equal(qa[:n], qb) and torch.equal(qa, rope.forward(q, None, pos)[0])
+    graph = torch.cuda.CUDAGraph()
+    out = torch.empty_like(q)
+    a.zero_()
+    with torch.cuda.graph(graph):
+        impl.rope_and_kv_cache_update(layer, q, k, v, pos, rope, a, slots, out)
+    graph.replay()
+    assert torch.equal(a, b) and torch.equal(out, qa)
