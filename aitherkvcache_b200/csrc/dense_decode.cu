@@ -614,11 +614,14 @@ int dense_common(const akv_dense_attn_params* p, const char* who, DenseArgs* a) 
     if (p->max_blocks_per_seq > 0 && (!p->block_tables || !p->k_cache || !p->v_cache || p->num_blocks == 0))
       return fail(AKV_ERR_ARG, "%s: null block tables or caches, or a cache without blocks", who);
   }
-  const int64_t strides = p->k_stride_blk | p->k_stride_pos | p->k_stride_head | p->v_stride_blk | p->v_stride_pos | p->v_stride_head;
-  if ((((uintptr_t)p->k_cache | (uintptr_t)p->v_cache) & 15) || (strides & 7))
+  // the stride of a dimension of one element is never used
+  auto used = [](int64_t stride, int64_t n) -> int64_t { return n > 1 ? stride : 0; };
+  const int64_t caches = used(p->k_stride_blk | p->v_stride_blk, p->num_blocks) | used(p->k_stride_pos | p->v_stride_pos, p->block_size) |
+                         used(p->k_stride_head | p->v_stride_head, p->num_kv_heads);
+  if ((((uintptr_t)p->k_cache | (uintptr_t)p->v_cache) & 15) || (caches & 7))
     return fail(AKV_ERR_ARG, "%s: cache rows must start on 16-byte boundaries", who);
-  if (((uintptr_t)p->query & 15) || ((p->q_stride_tok | p->q_stride_head) & 7) || ((uintptr_t)p->out & 15) ||
-      ((p->out_stride_tok | p->out_stride_head) & 7))
+  const int64_t rows = used(p->q_stride_tok | p->out_stride_tok, p->num_tokens) | used(p->q_stride_head | p->out_stride_head, p->num_q_heads);
+  if ((((uintptr_t)p->query | (uintptr_t)p->out) & 15) || (rows & 7))
     return fail(AKV_ERR_ARG, "%s: query and output rows must start on 16-byte boundaries", who);
   *a = DenseArgs{};
   a->q = p->query; a->q_st = p->q_stride_tok; a->q_sh = p->q_stride_head;

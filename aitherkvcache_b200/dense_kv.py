@@ -124,9 +124,11 @@ class DensePagedAttention:
 
     @staticmethod
     def _rows16(x: torch.Tensor) -> bool:
-        """Whether every row of a 16-bit [a, b, head_dim] tensor starts on a 16-byte boundary."""
-        s = x.stride()
-        return s[2] == 1 and s[0] > 0 and s[1] > 0 and not (x.data_ptr() & 15 or (s[0] | s[1]) & 7)
+        """Whether every row of a 16-bit [a, b, head_dim] tensor starts on a 16-byte boundary (the stride of a dimension of
+        one element is never used)."""
+        n, s = x.shape, x.stride()
+        a, b = s[0] if n[0] > 1 else 8, s[1] if n[1] > 1 else 8
+        return s[2] == 1 and a > 0 and b > 0 and not (x.data_ptr() & 15 or (a | b) & 7)
 
     def _values(self, query, k_cache, v_cache, block_tables, seq_lens, starts, num_seqs, out):
         """(fields of ``akv_dense_attn_params`` up to the output, the output, tensors that must outlive the call)."""
@@ -140,8 +142,8 @@ class DensePagedAttention:
         tshape = block_tables.shape
         if len(tshape) != 2 or tshape[0] < num_seqs or seq_lens.dim() != 1 or seq_lens.shape[0] < num_seqs:
             raise ValueError(f"block_tables {tuple(tshape)} / lengths {tuple(seq_lens.shape)} do not cover {num_seqs} sequences")
-        if not self._rows16(query):
-            query = query.contiguous()
+        if not self._rows16(query):      # clone: contiguous() leaves a tensor at an odd offset where it is
+            query = query.clone(memory_format=torch.contiguous_format)
         if block_tables.stride(1) != 1:
             block_tables = block_tables.contiguous()
         if seq_lens.stride(0) != 1:

@@ -325,3 +325,43 @@ def test_backend_rotating_update_of_a_padded_batch(monkeypatch, index):
         assert got[0] is q and got[1] is k and got[2] is v and got[3] is pos and got[7:] == ("rope", "out")
         assert got[4].dtype == index and got[4].tolist() == list(range(n)) + [-1] * (9 - n)
         assert n < 9 or got[4] is slots
+
+
+def test_rows_on_16_byte_boundaries():
+    """Which query rows are readable as they are: strides of dimensions with one element say nothing."""
+    from aitherkvcache_b200 import DensePagedAttention
+    flat = torch.zeros(4096, dtype=torch.float16)
+    assert flat.data_ptr() % 16 == 0
+    rows16 = DensePagedAttention._rows16
+    for shape, strides, offset, good in (((3, 4, 64), (256, 64, 1), 0, True), ((3, 4, 64), (264, 64, 1), 8, True), ((3, 4, 64), (260, 64, 1), 0, False),
+                                         ((3, 4, 64), (256, 64, 1), 1, False), ((3, 4, 64), (256, 64, 1), 4, False), ((1, 4, 64), (257, 64, 1), 0, True),
+                                         ((1, 4, 64), (257, 64, 1), 1, False), ((1, 4, 64), (0, 64, 1), 0, True), ((3, 1, 64), (64, 1, 1), 0, True),
+                                         ((3, 1, 64), (65, 1, 1), 0, False), ((1, 1, 64), (3, 5, 1), 0, True), ((3, 4, 64), (0, 64, 1), 0, False),
+                                         ((3, 4, 64), (64, 0, 1), 0, False), ((1, 4, 64), (0, 65, 1), 0, False), ((3, 4, 32), (256, 64, 2), 0, False)):
+        assert rows16(flat.as_strided(shape, strides, offset)) is good, (shape, strides, offset)
+
+
+def test_attention_entry_points_ignore_strides_of_single_elements():
+    """A dimension of one element may have any stride: only the workspace is missing."""
+    from aitherkvcache_b200 import _lib
+    L = _lib.lib()
+    for name in ("akv_dense_paged_attn", "akv_dense_prefill_attn"):
+        p = _lib.DenseAttnParams()
+        for f in ("query", "k_cache", "v_cache", "block_tables", "seq_lens", "query_start_loc", "out", "workspace"):
+            setattr(p, f, 256)
+        p.num_seqs = p.num_tokens = p.num_q_heads = p.num_kv_heads = p.num_blocks = p.max_blocks_per_seq = 1
+        p.head_dim, p.block_size, p.scale, p.k_stride_pos, p.v_stride_pos = 128, 16, 1.0, 128, 128
+        p.q_stride_tok, p.q_stride_head, p.out_stride_tok, p.out_stride_head = 257, 1, 3, 129
+        p.k_stride_blk, p.k_stride_head, p.v_stride_blk, p.v_stride_head = 33, 1, 77, 5
+        assert getattr(L, name)(ctypes.byref(p)) == _lib.AKV_ERR_WORKSPACE
+        for kw in (dict(num_tokens=2), dict(num_blocks=2)):
+            for f, v in kw.items():
+                setattr(p, f, v)
+            assert getattr(L, name)(ctypes.byref(p)) == _lib.AKV_ERR_ARG, kw
+            for f in kw:
+                setattr(p, f, 1)
+        for heads in (dict(num_q_heads=2, q_stride_head=128), dict(num_q_heads=2, out_stride_head=128, q_stride_head=1)):
+            for f, v in heads.items():
+                setattr(p, f, v)
+            assert getattr(L, name)(ctypes.byref(p)) == _lib.AKV_ERR_ARG, heads
+            p.num_q_heads = 1

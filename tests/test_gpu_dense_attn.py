@@ -488,3 +488,32 @@ def test_chunks_rows_before_the_first_sequence(D, bs, first, seqs):
     a.prefill(q, kc, vc, bt[1:], cl[1:], starts[1:], out=out[:, 1:5])
     assert bool((out[:first] == 5.0).all()) and bool((out[-6:] == 5.0).all()) and bool((out[:, 0] == 5.0).all())
     assert bool(((out[:, 1:5].double() - want.double()).abs() <= 2 * bound)[first:-6].all())
+
+
+@pytest.mark.parametrize("D,bs", [(64, 16), (128, 16), (256, 16), (128, 5)])
+@pytest.mark.parametrize("n", [1, 3])
+def test_queries_that_start_anywhere(D, bs, n):
+    """A contiguous query off the 16-byte boundaries, one token of an odd pitch and heads of one element's stride: the same
+    bits as from a query of its own, in both forms."""
+    H = 2
+    lens, new = [70] + [33] * (n - 1), [1] * n
+    for QH in (8, 2):
+        q, kc, vc, bt, cl, starts = make(lens, new, QH, H, D, bs, torch.float16, seed=D + n)
+        a = attn(QH, H, D)
+        want, chunk = a.forward(q, kc, vc, bt, cl), a.prefill(q, kc, vc, bt, cl, starts)
+        wide = torch.randn(n * (QH * D + 3) + 16, device="cuda").half()
+        for pitch, offset in ((QH * D, 1), (QH * D, 4), (QH * D + 3, 0), (QH * D + 3, 5)):
+            at = wide.as_strided((n, QH, D), (pitch, D, 1), offset)
+            at.copy_(q)
+            assert torch.equal(a.forward(at, kc, vc, bt, cl), want)
+            assert torch.equal(a.prefill(at, kc, vc, bt, cl, starts), chunk)
+    # one query head and one KV head, whose strides say nothing; in the output too
+    q, kc, vc, bt, cl, starts = make(lens, new, 1, 1, D, bs, torch.float16, seed=D)
+    a = attn(1, 1, D)
+    want, chunk = a.forward(q, kc, vc, bt, cl), a.prefill(q, kc, vc, bt, cl, starts)
+    q1, k1, v1 = q.as_strided(q.shape, (D, 1, 1)), *(x.as_strided(x.shape, (x.stride(0), x.stride(1), 7, 1)) for x in (kc, vc))
+    out = torch.full((n, D), 5.0, dtype=torch.float16, device="cuda")
+    assert torch.equal(a.forward(q1, k1, v1, bt, cl, out=out.as_strided((n, 1, D), (D, 3, 1))), want) and torch.equal(out, want[:, 0])
+    out.fill_(5.0)
+    assert torch.equal(a.prefill(q1, k1, v1, bt, cl, starts, out=out.as_strided((n, 1, D), (D, 3, 1))), chunk) and torch.equal(out, chunk[:, 0])
+    assert torch.equal(a.forward(q1, k1, v1, bt, cl), want) and torch.equal(a.prefill(q1, k1, v1, bt, cl, starts), chunk)
