@@ -79,10 +79,21 @@ class RotaryPositions:
         self.inv_freq = torch.tensor(freq, dtype=torch.float64)
         self.steps = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64, device=device)
         self.axes = torch.tensor(axes, dtype=torch.int32, device=device)
+        self._bind()
+
+    def _bind(self) -> None:
+        """The argument block that points at the tables."""
         self.device = self.steps.device
-        self._tables = _lib.RotaryTables(self.head_dim, self.rotary_dim, self.num_axes, int(pair_layout == "adjacent"),
+        self._tables = _lib.RotaryTables(self.head_dim, self.rotary_dim, self.num_axes, int(self.pair_layout == "adjacent"),
                                          self.steps.data_ptr(), self.axes.data_ptr(), self.scaling)
         self._tables_at = ctypes.addressof(self._tables)
+
+    def __getstate__(self) -> dict:      # copies and pickles: addresses stay behind
+        return {k: v for k, v in vars(self).items() if k not in ("_tables", "_tables_at")}
+
+    def __setstate__(self, state: dict) -> None:
+        vars(self).update(state)
+        self._bind()
 
     def _positions(self, positions: torch.Tensor, tokens: int) -> Tuple[int, int]:
         """(stride over the axes, stride over the tokens) of [tokens] or [num_axes, tokens]."""

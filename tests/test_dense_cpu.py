@@ -365,3 +365,31 @@ def test_attention_entry_points_ignore_strides_of_single_elements():
                 setattr(p, f, v)
             assert getattr(L, name)(ctypes.byref(p)) == _lib.AKV_ERR_ARG, heads
             p.num_q_heads = 1
+
+
+@pytest.mark.parametrize("how", ["copy", "deepcopy", "pickle", "module"])
+def test_rotary_positions_are_copied(how):
+    """A copy has an argument block of its own that points at its own tables, and outlives the original."""
+    import copy
+    import gc
+    import pickle
+    from aitherkvcache_b200 import RotaryPositions
+    rope = RotaryPositions(32, rotary_dim=16, base=5e5, sections=(4, 3, 1), section_layout="cycled", pair_layout="adjacent", scaling=1.5, device="cpu")
+    if how == "module":
+        layer = torch.nn.Module()
+        layer.rope = rope
+        twin = copy.deepcopy(layer).rope
+    else:
+        twin = {"copy": copy.copy, "deepcopy": copy.deepcopy, "pickle": lambda x: pickle.loads(pickle.dumps(x))}[how](rope)
+    plain = {k: v for k, v in vars(rope).items() if not k.startswith("_")}
+    assert set(plain) == {k for k in vars(twin) if not k.startswith("_")}
+    for k, v in plain.items():
+        assert torch.equal(v, getattr(twin, k)) if isinstance(v, torch.Tensor) else v == getattr(twin, k)
+    if how != "copy":
+        assert twin.steps.data_ptr() != rope.steps.data_ptr() and twin.axes.data_ptr() != rope.axes.data_ptr()
+    assert twin._tables_at != rope._tables_at
+    del rope
+    gc.collect()
+    t = ctypes.cast(twin._tables_at, ctypes.POINTER(type(twin._tables))).contents
+    assert (t.head_dim, t.rotary_dim, t.num_axes, t.adjacent, t.scaling) == (32, 16, 3, 1, 1.5)
+    assert (t.steps, t.axes) == (twin.steps.data_ptr(), twin.axes.data_ptr())

@@ -215,3 +215,18 @@ def test_append_replays_from_a_graph_with_new_inputs():
         out = rotary_kv_append(q, k, v, pos, slots, k2, v2, rope)
         assert torch.equal(out, qo) and torch.equal(k2, kc) and torch.equal(v2, vc)
         _check(qo, q, pos, rope)
+
+
+def test_copies_of_rotary_positions():
+    """A deep copy on the device rotates alike after the original and its tables are gone."""
+    import copy
+    from aitherkvcache_b200 import RotaryPositions
+    rope = RotaryPositions(64, base=1e5, sections=(16, 8, 8))
+    q = torch.randn(50, 3, 64, device="cuda")
+    pos = torch.randint(0, 10 ** 6, (3, 50), device="cuda")
+    want = rope.forward(q, None, pos)[0]
+    twin = copy.deepcopy(rope)
+    rope.steps.fill_(0)      # what the copy must not look at
+    rope.axes.fill_(0)
+    del rope
+    assert torch.equal(twin.forward(q, None, pos)[0], want)
