@@ -51,6 +51,15 @@ __device__ __forceinline__ float dense_ex2(float x) {
   return y;
 }
 
+// A row's reference m in log2 units: it moves when a score exceeds what the largest weight may be, to the score minus
+// DENSE_SHIFT.  fp16 ends at 2^-24 below, so weights relative to the largest score itself would vanish from the product below
+// 2^-25 of the largest weight while the sum still counts them: 40000 keys of 2^-26 each, 6e-4 of the result, came out as
+// zeros.  With the factor 2^7 the largest weight stays at or below 2^15 (65504 is the end above) and what vanishes is 2^-32
+// of it and less.  bf16 has the range of float32.
+constexpr float DENSE_RESCALE = 8.0f;
+template <bool BF> constexpr float DENSE_SHIFT = BF ? 0.0f : 7.0f;
+template <bool BF> constexpr float DENSE_TOP = DENSE_RESCALE + DENSE_SHIFT<BF>;      // log2 of the largest weight
+
 template <bool BF> __device__ __forceinline__ uint32_t dense_pack(float lo, float hi) {
   if (BF) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);

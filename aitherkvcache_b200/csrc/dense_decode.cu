@@ -15,8 +15,8 @@
 //
 // 16 keys in a warp: S^T[16 keys][8 heads] = K Q^T (keys as the rows of the product, so that up to 8 heads waste nothing),
 // probabilities in float32, rounded once to the cache's type, transposed in registers (movmatrix) into the second
-// operand of O^T[D][8 heads] += V^T P^T.  Scores, maxima, sums and O are float32.  The reference m moves only when a score
-// exceeds it by more than 2^8, so the shuffles and the rescaling of O run a few times per row (fp16 holds 2^8 exactly).
+// operand of O^T[D][8 heads] += V^T P^T.  Scores, maxima, sums and O are float32.  The reference m moves only when a weight
+// would pass 2^8 times the last reference's (DENSE_TOP in dense_attn.cuh), so the shuffles and the rescaling of O run a few times per row.
 // Keys outside the range are filled with zeros by the copy and masked: whatever stale pages hold does not matter.
 #include "dense_attn.cuh"
 #include "umma.cuh"
@@ -26,7 +26,6 @@ namespace akv {
 namespace {
 
 constexpr int DD_MAX_SEQS = 1024;        // sequences of one launch (their prefix sums live in shared memory)
-constexpr float DD_RESCALE = 8.0f;
 
 template <int D, int NT> struct DdL {
   // two CTAs per SM where their rings fit: one streams while the other joins its warps' results at the end of a piece
@@ -323,7 +322,7 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int rows, float* part_acc,
       }
       bool grow = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) grow = grow || top[nt][0] > m[nt][0] + DD_RESCALE || top[nt][1] > m[nt][1] + DD_RESCALE;
+      for (int nt = 0; nt < NT; ++nt) grow = grow || top[nt][0] > m[nt][0] + DENSE_TOP<BF> || top[nt][1] > m[nt][1] + DENSE_TOP<BF>;
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -332,6 +331,7 @@ dense_decode_kernel(DenseArgs a, int seqs0, int seqs, int rows, float* part_acc,
             float mx = top[nt][x];
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            mx -= DENSE_SHIFT<BF>;
             if (mx > m[nt][x]) {
               const float f = dense_ex2(m[nt][x] - mx);      // -inf before the first key: 0
               m[nt][x] = mx;

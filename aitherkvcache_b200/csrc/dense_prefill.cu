@@ -22,7 +22,7 @@
 // pipe 385 cycles instead of 256 (the operands' shared-memory traffic), 2485 per tile pair in all where 2048 would be the least;
 // with whole 128-key tiles in one buffer a tile pair took 4850 cycles, 2900 of each half's period waiting for that round trip.
 // MMAs complete in order, so "S of u is there" also says that P V of u - 2 is done and the buffer of P u - 2 was free.
-// The row's reference maximum moves only when a score exceeds it by more than 2^8 (fp16 and bf16 hold 2^8 exactly), so O
+// The row's reference moves only when a weight would pass 2^8 times the last reference's (DENSE_TOP in dense_attn.cuh), so O
 // is rescaled a few times per row; that waits for P V of u - 1.
 //
 // Few rows.  Where a row tile has rows for one half only (at most TT new tokens left), the halves take alternate key tiles of
@@ -70,7 +70,6 @@ constexpr int DP_ROUND_TILES = 8;                // row tiles that make keys wor
 // a cut this near to a row tile's edge is moved there, in key tiles (0 and 6: 158 us for the prompts above, 4: 156, 2: 153)
 constexpr int DP_SNAP = 2;
 constexpr int DP_PIECE = 2;                      // what a row tile costs besides its key tiles, in key tiles
-constexpr float DP_RESCALE = 8.0f;
 
 struct DpMaps { CUtensorMap q, k, v; };
 
@@ -846,10 +845,10 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
           mx[0] = dp_max3(mx[0], __uint_as_float(v[60]), __uint_as_float(v[61]));
           mx[1] = dp_max3(mx[1], __uint_as_float(v[62]), __uint_as_float(v[63]));
           const float top = dp_max3(mx[0], mx[1], dp_max3(mx[2], mx[3], mx[3])) * c;
-          const bool grow = live && !(top <= m + DP_RESCALE);      // also for a NaN, which then stays
+          const bool grow = live && !(top <= m + DENSE_TOP<BF>);      // also for a NaN, which then stays
           if (__any_sync(0xffffffffu, grow)) {
-            const float f = grow ? dense_ex2(m - top) : 1.0f;      // m = -inf: 0
-            if (grow) { m = top; l *= f; }
+            const float to = top - DENSE_SHIFT<BF>, f = grow ? dense_ex2(m - to) : 1.0f;      // m = -inf: 0
+            if (grow) { m = to; l *= f; }
             if (x > 0) {                    // O holds the products of the sub-tiles before: P V of the last one may still run
               if (!wait_warp(bar_s + P_PVDONE + 8 * half, (uint32_t)((step - 2) & 1))) { ok = false; break; }
               asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");

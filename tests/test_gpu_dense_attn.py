@@ -517,3 +517,39 @@ def test_queries_that_start_anywhere(D, bs, n):
     out.fill_(5.0)
     assert torch.equal(a.prefill(q1, k1, v1, bt, cl, starts, out=out.as_strided((n, 1, D), (D, 3, 1))), chunk) and torch.equal(out, chunk[:, 0])
     assert torch.equal(a.forward(q1, k1, v1, bt, cl), want) and torch.equal(a.prefill(q1, k1, v1, bt, cl, starts), chunk)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,QH", [(64, 4), (64, 16), (128, 8), (256, 2)])
+@pytest.mark.parametrize("at", [0, 20000, 39990])
+def test_many_small_weights_beside_a_large_one(dtype, D, QH, at):
+    """One key takes nearly all of the weight, 40000 others e^-18 = 2^-26 of it each, and only theirs have values: what they
+    add up to must not be lost, although each is below the smallest step of fp16 (2^-24).
+
+    Bound, relative to the result: a weight is rounded to the type: u, and for fp16 half a step 2^-25 of 2^-26 times the
+    factor 2^7 that weights carry there, 2^-6; the exponential 2^-21 and the score (its error is 64 to 256 additions of zeros, one product and the
+    reference's subtraction, 2^-22 of 26: 2^-17); float32 sums of n terms above and below, 2 n 2^-23; u of the result."""
+    n, new, bs = 40000, 150, 16
+    blocks = n // bs
+    kc, vc = torch.zeros(blocks, bs, 1, D, dtype=dtype, device="cuda"), torch.ones(blocks, bs, 1, D, dtype=dtype, device="cuda")
+    kc[:, :, 0, 3] = -18.0
+    kc[at // bs, at % bs, 0, 3] = 0.0
+    vc[at // bs, at % bs] = 0.0
+    bt = torch.arange(blocks, dtype=torch.int32, device="cuda").view(1, -1)
+    q = torch.zeros(new, QH, D, dtype=dtype, device="cuda")
+    q[:, :, 3] = 1.0
+    a, u = attn(QH, 1, D, scale=1.0), torch.finfo(dtype).eps / 2
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+
+    def near(out, keys):
+        seen = (keys > at).double()      # rows that do not see the large key: all ones
+        rest = (keys - seen) * math.exp(-18.0)
+        want = torch.where(seen > 0, rest / (1 + rest), torch.ones_like(rest))[:, None, None]
+        bound = want * (2 * u + 2.0 ** -6 + 2.0 ** -21 + 2.0 ** -16 + 2 * n * 2.0 ** -23) + 2.0 ** -25
+        assert bool(((out.double() - want).abs() <= bound).all()), (out.flatten()[:3].tolist(), want.flatten()[:3].tolist())
+
+    full = torch.full((1,), n, dtype=torch.float64, device="cuda")
+    near(a.forward(q[:1], kc, vc, bt, lens), full)
+    for m in (1, 3, new):
+        starts = torch.tensor([0, m], dtype=torch.int32, device="cuda")
+        near(a.prefill(q[:m], kc, vc, bt, lens, starts), full - m + 1 + torch.arange(m, device="cuda"))
