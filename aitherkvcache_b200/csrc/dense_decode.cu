@@ -555,8 +555,9 @@ int dd_launch(const DenseArgs& a, float* part_acc, float* part_ml, DdDesc* desc,
   // then read at the same time; its 128-byte pieces alone reach half of the HBM rate (200 windowed sequences x 8 heads: 93 us
   // with the keys shared out among the warps, 70 us this way).  At head_dim 128 that is 162 us against 169 (16 long sequences).
   const bool heads = D == 64 && vheads % 4 == 0;
-  auto kernel = heads ? (page16 ? dense_decode_kernel<BF, D, NT, true, true> : dense_decode_kernel<BF, D, NT, false, true>)
-                      : (page16 ? dense_decode_kernel<BF, D, NT, true, false> : dense_decode_kernel<BF, D, NT, false, false>);
+  auto kernel = page16 ? dense_decode_kernel<BF, D, NT, true, false> : dense_decode_kernel<BF, D, NT, false, false>;
+  if constexpr (D == 64)
+    if (heads) kernel = page16 ? dense_decode_kernel<BF, D, NT, true, true> : dense_decode_kernel<BF, D, NT, false, true>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
   if (e != cudaSuccess) return fail((int)e, "dense attention: smem attribute: %s", cudaGetErrorString(e));
   // sequences of one launch: prefix sums in shared memory, and of fewer than 2^31 steps even if every sequence were full
