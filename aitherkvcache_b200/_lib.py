@@ -266,6 +266,7 @@ _SIGNATURES = {
     "akv_rotary": (c_int, [C.POINTER(RotaryParams)]),
     "akv_rotary_kv_append": (c_int, [C.POINTER(RotaryAppendParams)]),
     "akv_dense_paged_attn_workspace_bytes": (C.c_size_t, [c_int] * 3),
+    "akv_dense_prefill_attn_call_bytes": (C.c_size_t, [c_int, c_int, c_int, c_int, c_i64, c_int, c_int, c_int]),
     "akv_dense_prefill_attn_workspace_bytes": (C.c_size_t, [c_int, c_int, c_i64, c_int, c_int, c_int]),
     "akv_dense_prefill_attn": (c_int, [C.POINTER(DenseAttnParams)]),
     "akv_dense_paged_attn": (c_int, [C.POINTER(DenseAttnParams)]),

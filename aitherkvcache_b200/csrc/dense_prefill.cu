@@ -1246,8 +1246,11 @@ size_t dp_workspace(int head_dim, int rounds, char* base, DpWorkspace* w) {
   return d + ml + acc;
 }
 
-// Rounds that a call may need: its keys and values are at most those of the pool, or of full block-table rows.
-int dp_rounds(int num_kv_heads, int head_dim, int64_t num_blocks, int block_size, int num_seqs, int max_blocks_per_seq) {
+// Rounds that a call may need: its keys and values are at most those of the pool, or of full block-table rows, and only
+// sequences of DP_ROUND_TILES row tiles count, which fewer new tokens than that cannot have (for one drafted token over a large pool
+// at head_dim 128 the workspace is 40 MB instead of the 158 of four rounds).
+int dp_rounds(int num_tokens, int group, int num_kv_heads, int head_dim, int64_t num_blocks, int block_size, int num_seqs, int max_blocks_per_seq) {
+  if (group > 0 && num_tokens <= (DP_ROUND_TILES - 1) * 2 * (128 / group)) return 1;
   const double rows = (double)num_seqs * max_blocks_per_seq, blocks = rows < (double)num_blocks ? rows : (double)num_blocks;
   const double n = blocks * block_size * num_kv_heads * 4.0 * head_dim / (double)DP_ROUND_BYTES;
   return n <= 1.0 ? 1 : (n >= DP_MAX_ROUNDS ? DP_MAX_ROUNDS : (int)ceil(n));
@@ -1324,7 +1327,15 @@ int dense_prefill_withhold(int tile) {
 AKV_EXPORT size_t akv_dense_prefill_attn_workspace_bytes(int num_kv_heads, int head_dim, int64_t num_blocks, int block_size, int num_seqs,
                                                           int max_blocks_per_seq) {
   if (num_kv_heads <= 0 || head_dim <= 0 || num_blocks < 0 || block_size <= 0 || num_seqs < 0 || max_blocks_per_seq < 0) return 0;
-  return akv::dp_workspace(head_dim, akv::dp_rounds(num_kv_heads, head_dim, num_blocks, block_size, num_seqs, max_blocks_per_seq), nullptr, nullptr);
+  return akv::dp_workspace(head_dim, akv::dp_rounds(0x7fffffff, 1, num_kv_heads, head_dim, num_blocks, block_size, num_seqs, max_blocks_per_seq), nullptr, nullptr);
+}
+
+AKV_EXPORT size_t akv_dense_prefill_attn_call_bytes(int num_tokens, int num_q_heads, int num_kv_heads, int head_dim, int64_t num_blocks,
+                                                    int block_size, int num_seqs, int max_blocks_per_seq) {
+  if (num_tokens < 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || head_dim <= 0 || num_blocks < 0 || block_size <= 0 || num_seqs < 0 ||
+      max_blocks_per_seq < 0) return 0;
+  return akv::dp_workspace(head_dim, akv::dp_rounds(num_tokens, num_q_heads / num_kv_heads, num_kv_heads, head_dim, num_blocks, block_size, num_seqs, max_blocks_per_seq),
+                           nullptr, nullptr);
 }
 
 AKV_EXPORT int akv_dense_prefill_attn(const akv_dense_attn_params* p) {
@@ -1342,7 +1353,7 @@ AKV_EXPORT int akv_dense_prefill_attn(const akv_dense_attn_params* p) {
   cudaStream_t st = reinterpret_cast<cudaStream_t>(p->stream);
   if (a.num_seqs == 0) return a.head_dim == 128 ? akv::dp_launch_zeros<128>(a, G, TT, st) : akv::dp_launch_zeros<64>(a, G, TT, st);
   akv::DpWorkspace w;
-  const int rounds = akv::dp_rounds(a.num_kv_heads, a.head_dim, a.num_blocks, a.block_size, a.num_seqs, a.max_blocks_per_seq);
+  const int rounds = akv::dp_rounds(a.n_tokens, G, a.num_kv_heads, a.head_dim, a.num_blocks, a.block_size, a.num_seqs, a.max_blocks_per_seq);
   const size_t need = akv::dp_workspace(a.head_dim, rounds, static_cast<char*>(p->workspace), &w);
   if (!p->workspace || p->workspace_bytes < need || ((uintptr_t)p->workspace & 255))
     return akv::fail(AKV_ERR_WORKSPACE, "akv_dense_prefill_attn: workspace of %zu bytes (256-byte aligned) needed, got %zu", need, p->workspace_bytes);

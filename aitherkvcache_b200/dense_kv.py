@@ -194,7 +194,8 @@ class DensePagedAttention:
             if zero_tail:
                 out.zero_()
             return self._prefill_by_rows(query, k_cache, v_cache, block_tables, seq_lens, query_start_loc, out)
-        nbytes = _lib.lib().akv_dense_prefill_attn_workspace_bytes(self.num_kv_heads, self.head_dim, blocks, block_size, num_seqs, width)
+        nbytes = _lib.lib().akv_dense_prefill_attn_call_bytes(query.shape[0], self.num_query_heads, self.num_kv_heads, self.head_dim,
+                                                              blocks, block_size, num_seqs, width)
         ws = out.new_empty((nbytes + 1) // 2)
         _lib.call(index, "akv_dense_prefill_attn", _pack_attn(*values, int(zero_tail), ws.data_ptr(), nbytes, _lib.raw_stream(index)))
         return out

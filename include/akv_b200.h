@@ -503,6 +503,9 @@ typedef struct akv_dense_attn_params {
 } akv_dense_attn_params;
 size_t akv_dense_paged_attn_workspace_bytes(int num_q_heads, int num_kv_heads, int head_dim);
 int akv_dense_paged_attn(const akv_dense_attn_params* params);
+/* Workspace of akv_dense_prefill_attn: what a call needs, and a bound for any number of tokens and query heads. */
+size_t akv_dense_prefill_attn_call_bytes(int num_tokens, int num_q_heads, int num_kv_heads, int head_dim, int64_t num_blocks, int block_size,
+                                         int num_seqs, int max_blocks_per_seq);
 size_t akv_dense_prefill_attn_workspace_bytes(int num_kv_heads, int head_dim, int64_t num_blocks, int block_size, int num_seqs,
                                               int max_blocks_per_seq);
 int akv_dense_prefill_attn(const akv_dense_attn_params* params);

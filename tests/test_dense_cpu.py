@@ -393,3 +393,18 @@ def test_rotary_positions_are_copied(how):
     t = ctypes.cast(twin._tables_at, ctypes.POINTER(type(twin._tables))).contents
     assert (t.head_dim, t.rotary_dim, t.num_axes, t.adjacent, t.scaling) == (32, 16, 3, 1, 1.5)
     assert (t.steps, t.axes) == (twin.steps.data_ptr(), twin.axes.data_ptr())
+
+
+def test_chunk_workspace_goes_by_the_call():
+    """Rounds are for sequences of eight row tiles of 256 rows: calls with fewer tokens need one round's workspace, whatever the
+    pool; the bound without tokens covers every call."""
+    from aitherkvcache_b200 import _lib
+    L = _lib.lib()
+    for heads, kv, D in ((32, 8, 128), (8, 8, 64), (28, 4, 64), (128, 1, 128)):
+        need = lambda n: L.akv_dense_prefill_attn_call_bytes(n, heads, kv, D, 1 << 20, 16, 4, 1 << 20)  # noqa: E731
+        few = 7 * 2 * (128 // (heads // kv))
+        bound = L.akv_dense_prefill_attn_workspace_bytes(kv, D, 1 << 20, 16, 4, 1 << 20)
+        assert need(0) == need(1) == need(few) and need(few + 1) == need(1 << 30) == bound
+        assert 3.9 * need(1) < bound <= 4 * need(1)
+    for bad in ((-1, 8, 8, 64, 9, 16, 4, 9), (1, 4, 8, 64, 9, 16, 4, 9), (1, 8, 0, 64, 9, 16, 4, 9), (1, 8, 8, 64, 9, 0, 4, 9), (1, 8, 8, 64, -1, 16, 4, 9)):
+        assert L.akv_dense_prefill_attn_call_bytes(*bad) == 0

@@ -553,3 +553,21 @@ def test_many_small_weights_beside_a_large_one(dtype, D, QH, at):
     for m in (1, 3, new):
         starts = torch.tensor([0, m], dtype=torch.int32, device="cuda")
         near(a.prefill(q[:m], kc, vc, bt, lens, starts), full - m + 1 + torch.arange(m, device="cuda"))
+
+
+def test_scratch_of_few_tokens_over_a_large_pool():
+    """One drafted token over a pool of 300 MB takes the scratch of one round; more tokens may take four."""
+    nb = 4600
+    kc, vc = (torch.randn(nb, 16, 8, 128, device="cuda").half() for _ in range(2))
+    bt = torch.randperm(nb, generator=torch.Generator().manual_seed(0))[:4500].view(1, -1).int().cuda()
+    a, cl = attn(32, 8, 128), torch.tensor([72000], dtype=torch.int32, device="cuda")
+    for n, most in ((1, 45 << 20), (448, 45 << 20), (449, 170 << 20)):
+        q = torch.randn(n, 32, 128, device="cuda").half()
+        starts = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        out = a.prefill(q, kc, vc, bt, cl, starts)
+        assert torch.cuda.max_memory_allocated() - before - out.numel() * 2 <= most
+        if n == 1:
+            check(out, q, kc, vc, bt, cl, starts)
