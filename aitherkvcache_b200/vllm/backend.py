@@ -198,7 +198,9 @@ class TurboQuantImplBase:
     def do_kv_cache_update(self, layer, key, value, kv_cache, slot_mapping) -> None:
         """Encode ``key`` / ``value`` [tokens, kv_heads, head_size] into the packed cache in place (a 16-bit cache takes them
         as they are).  Tokens behind the length of ``slot_mapping`` are padding."""
-        key, value = key[:slot_mapping.shape[0]], value[:slot_mapping.shape[0]]
+        n = slot_mapping.shape[0]
+        if key.shape[0] > n:
+            key, value = key[:n], value[:n]
         if self._dense(kv_cache):
             from ..dense_kv import kv_append
             kv_append(key, value, slot_mapping, kv_cache[:, 0], kv_cache[:, 1])
