@@ -234,3 +234,43 @@ def test_backend_rotating_update_of_a_padded_batch(kind, pad):
         impl.rope_and_kv_cache_update(layer, q, k, v, pos, rope, a, slots, out)
     graph.replay()
     assert torch.equal(a, b) and torch.equal(out, qa)
+
+
+def test_compressed_and_exempt_layers_side_by_side():
+    """A layer with a compressed cache dtype and one that is exempt from it, in one process, with the same block tables and
+    slots and pages of one shape: each gives what it gives alone."""
+    from aitherkvcache_b200.vllm.backend import TurboQuantImplBase
+    QH, H, D, bs, dtype = 8, 2, 128, 16, torch.bfloat16
+    g = torch.Generator().manual_seed(7)
+    packed, exempt = TurboQuantImplBase(), TurboQuantImplBase()
+    packed._tq_setup(QH, D, 1 / math.sqrt(D), H, "tq-t4nc")
+    exempt._tq_setup(QH, D, 1 / math.sqrt(D), H, "auto")
+    layers = [types.SimpleNamespace(layer_name=n) for n in ("side.0", "side.1")]
+    new = [[48, 32], [1, 1], [5, 1]]
+    _, bt = _pages(2, 4, bs, H, D, dtype, 3)
+    x = [[torch.randn(2, 64, h, D, generator=g).to(dtype).cuda() for h in (QH, H, H)] for _ in layers]      # per layer: q, k, v by sequence
+
+    def serve(which):
+        caches = [torch.zeros(11, 2, bs, H, D, dtype=torch.uint8, device="cuda"), torch.zeros(11, 2, bs, H, D, dtype=dtype, device="cuda")]
+        done, outs = [0, 0], {i: [] for i in which}
+        for step in new:
+            cut = [slice(d, d + n) for d, n in zip(done, step)]
+            slots = torch.cat([_slots(bt, bs, s, d, n) for s, (d, n) in enumerate(zip(done, step))])
+            done = [d + n for d, n in zip(done, step)]
+            md = types.SimpleNamespace(num_actual_tokens=sum(step), max_query_len=max(step), block_table=bt, max_seq_len=max(done),
+                                       seq_lens=torch.tensor(done, dtype=torch.int32, device="cuda"),
+                                       query_start_loc=torch.tensor([0, step[0], sum(step)], dtype=torch.int32, device="cuda"))
+            for i in which:
+                q, k, v = (torch.cat([t[s, c] for s, c in enumerate(cut)]) for t in x[i])
+                impl = (packed, exempt)[i]
+                impl.do_kv_cache_update(layers[i], k, v, caches[i], slots)
+                outs[i].append(impl.forward(layers[i], q.flatten(1), None, None, caches[i], md, output=torch.zeros(sum(step), QH * D, dtype=dtype, device="cuda")))
+        return caches, outs
+
+    both, both_outs = serve((0, 1))
+    for i in (0, 1):
+        alone, outs = serve((i,))
+        assert torch.equal(alone[i], both[i]) and all(torch.equal(a, b) for a, b in zip(outs[i], both_outs[i]))
+    q, k, v = ([t[s].double() for s in range(2)] for t in x[1])
+    want, bound = _expect(q, k, v, [48, 32], [48, 32], 0, 1 / math.sqrt(D))
+    assert bool(((both_outs[1][0].view(-1, QH, D).double() - want).abs() <= bound).all())
