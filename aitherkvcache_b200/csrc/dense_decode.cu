@@ -553,7 +553,8 @@ int dd_launch(const DenseArgs& a, float* part_acc, float* part_ml, DdDesc* desc,
   const bool page16 = a.block_size % 16 == 0;
   // head_dim 64: four rows side by side, a warp each, where a sequence's rows come in fours.  Neighbouring heads of a key are
   // then read at the same time; its 128-byte pieces alone reach half of the HBM rate (200 windowed sequences x 8 heads: 93 us
-  // with the keys shared out among the warps, 70 us this way).  At head_dim 128 that is 162 us against 169 (16 long sequences).
+  // with the keys shared out among the warps, 70 us this way).  At head_dim 128 it gains nothing: 16 sequences of 6 K to 32 K tokens
+  // (32 / 8 heads) take 203 to 206 us both ways.
   const bool heads = D == 64 && vheads % 4 == 0;
   auto kernel = page16 ? dense_decode_kernel<BF, D, NT, true, false> : dense_decode_kernel<BF, D, NT, false, false>;
   if constexpr (D == 64)

@@ -28,7 +28,7 @@
 // Few rows.  Where a row tile has rows for one half only (at most TT new tokens left), the halves take alternate key tiles of
 // the same rows, half 0 the piece's first, third ..., half 1 the others, and at the piece's end half 0 adds half 1's O, which
 // lies in the same lanes of tensor memory, to its own.  1 to 8 new tokens behind 32 sequences of 4000 (28 / 4 heads of
-// 64): 56.7 us, against 65.7 with one half idle.
+// 64): 56.7 us against 65.7 with one half idle when this came, 48 now.
 //
 // Work split.  The (row tile, key tile) pairs of the whole call are laid end to end and cut into equal ranges, one per SM:
 // every SM has the same share whatever the lengths.  Row tiles that are cut (at most two per CTA) leave float32 partials in
@@ -39,15 +39,16 @@
 // and what does not fit into L2 comes from HBM again for every row tile: at a power limit that costs clock (131 MB of
 // keys and values ran at 1.34 GHz, 24 MB at 1.47).  So the (sequence, KV head) pairs are taken in rounds of about
 // DP_ROUND_BYTES of keys and values, each cut into ranges for all SMs.  A round more costs some 10 us (its cuts, and the SMs' wait
-// for the first keys), so only the keys of sequences with DP_ROUND_TILES row tiles or more count (32 / 8 heads of 128): 2048
-// tokens behind 60000 take 1.81 ms in rounds and 2.07 without, 1000 behind 60000 0.95 and 1.09, 800 behind 40000 514 us and 550;
-// 440 behind 20000 152 us and 134, 100 behind 20000 85 and 62; 32 sequences of 4096 with 4 new tokens (4 KV heads of 64) 54 and 43.
+// for the first keys), so only the keys of sequences with DP_ROUND_TILES row tiles or more count.  Inside a graph, keys from HBM
+// (32 / 8 heads of 128): 2048 tokens behind 60000 take 1.89 ms in rounds and 2.13 without, 1000 behind 60000 0.99 and 1.13, 800
+// behind 40000 536 us and 578.  With the keys of all sequences counted, 440 behind 20000 would take 166 us instead of 148, 100
+// behind 20000 76 instead of 61, and 32 sequences of 4096 with 4 new tokens (4 KV heads of 64) 52 instead of 45.
 //
-// Measured: 2048 tokens behind 30000 (32 / 8 heads of 128) 0.99 ms in a sustained run at the power limit (1.45 GHz), 1.05 PFLOP/s,
+// Measured: 2048 tokens behind 30000 (32 / 8 heads of 128) 0.98 ms in a sustained run at the power limit (1.45 GHz), 1.06 PFLOP/s,
 // 77 % of the measured sustained matrix rate; 0.87 ms, 1.2 PFLOP/s in short bursts, 0.77 ms with zero data; 2900 cycles per tile
-// pair.  Some SMs take 14 % longer than the others for the same share and set the end.  Twelve prompts of 1 to 2000 tokens 153
-// us, 0.76 PFLOP/s (10 pieces per CTA, each with 1700 cycles of its own for the last P V and the first scores, and 2600 for the
-// epilogue); the 1 to 8 new tokens above 47 us, 3 TB/s.
+// pair.  Some SMs take 14 % longer than the others for the same share and set the end.  Twelve prompts of 1 to 2000 tokens 174 us
+// with keys from HBM, 0.67 PFLOP/s, and 153 us with keys in L2 (10 pieces per CTA, each with 1700 cycles of its own for the last
+// P V and the first scores, and 2600 for the epilogue); the 1 to 8 new tokens above 48 us, 3 TB/s.
 //
 // Every wait is bounded (umma.cuh): a wait that gives up sets g_dense_prefill_status and a flag that ends all loops.
 #include "dense_attn.cuh"
@@ -67,7 +68,7 @@ constexpr int DP_MAX_SEQS = 384;                 // sequences of one launch
 constexpr int DP_MAX_ROUNDS = 4;
 constexpr int64_t DP_ROUND_BYTES = 68 << 20;     // keys and values of a round
 constexpr int DP_ROUND_TILES = 8;                // row tiles that make keys worth keeping in L2
-// a cut this near to a row tile's edge is moved there, in key tiles (0 and 6: 158 us for the prompts above, 4: 156, 2: 153)
+// a cut this near to a row tile's edge is moved there, in key tiles (0 and 6: 158 us for the prompts above with keys in L2, 4: 156, 2: 153)
 constexpr int DP_SNAP = 2;
 constexpr int DP_PIECE = 2;                      // what a row tile costs besides its key tiles, in key tiles
 
@@ -435,7 +436,7 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
     const int round = warp >> 1;
     const int64_t lo = edge(round), hi = edge(round + 1);
     // CTAs that share it: all, but not more than there are row tiles or groups of six units: a part costs about two (5 tokens
-    // behind 20000, 8 / 1 heads of 128: 22.0 us; with eight units 23.8), and four or fewer could be moved away whole
+    // behind 20000, 8 / 1 heads of 128: 25 us; with eight units 28), and four or fewer could be moved away whole
     int64_t want = (hi - lo) / 6;
     if (n_rounds == 1) {
       int64_t rts = 0;
@@ -1047,8 +1048,9 @@ dense_prefill_kernel(const __grid_constant__ DenseArgs a, const __grid_constant_
 // SPREAD, for calls of few row tiles, which have many parts each: every block lists the halves that have parts, the slices are
 // spread over all blocks, and where that leaves threads idle, `groups` of 128 threads share a slice: group g takes parts g,
 // g + groups, ..., and the groups are joined in order through shared memory (their number depends on the call's lengths alone,
-// so results repeat).  100 tokens behind 20000 (32 / 8 heads of 128, 18 parts per row tile) take 58 us with it and 65 without, 60
-// tokens (8 / 1 heads, two row tiles of 20 parts) 36 and 48, 5 tokens 24 and 29; 5 tokens behind 5000 (5 parts) 23.8 and 22.8.
+// so results repeat).  Inside a graph, keys from HBM: 100 tokens behind 20000 (32 / 8 heads of 128, 18 parts per row tile) take 61 us
+// with it and 68 without, 60 tokens (8 / 1 heads, two row tiles of 20 parts) 34 and 56, 5 tokens 25 and 34; 5 tokens behind 5000 (5
+// parts) 20.7 either way.
 constexpr int PM_THREADS = 1024, PM_LIST = DP_MAX_ROUNDS * 256 * 2;      // at most 256 SMs
 constexpr int PM_SMEM = PM_THREADS * 18 * (int)sizeof(float);
 template <bool BF, int D, bool SPREAD>

@@ -143,8 +143,8 @@ class RotaryPositions:
                 inverse: bool = False) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
         """``query`` [tokens, query_heads, head_dim] and ``key`` [tokens, kv_heads, head_dim] (either may be None, any
         strides with a contiguous last dimension) turned to ``positions``: [tokens] or [num_axes, tokens], int32 or int64.
-        Returns (query, key) in their dtype.  ``query_out=query`` works in place.  ``inverse`` turns back; it is also the
-        gradient of the rotation."""
+        Returns (query, key) in their dtype.  ``query_out=query`` works in place.  ``inverse`` turns by the negative angles:
+        the rotation taken back at scaling 1, and its gradient at any scaling."""
         if query is None and key is None:
             raise ValueError("query and key are both None")
         index = _lib.cuda_index(query, key, positions, query_out, key_out, self.steps)

@@ -12,9 +12,12 @@ with its own causal context length and its sequence's block-table row, built on 
 without a host synchronisation.  Nothing is decompressed to fp16.  The reference's shadow mode,
 cold tier and block selection are not part of this build.
 
-A layer whose cache tensor is fp16 or bf16 stays uncompressed (a cache dtype of ``auto`` or ``bfloat16`` outside primary
-mode, or the layers that vLLM exempts from the compressed dtype): it is written by ``kv_append`` / ``rotary_kv_append`` and
-attended by ``DensePagedAttention`` (``dense_kv.py``) behind the same methods, block tables and slots.
+A layer whose cache tensor is fp16 or bf16 stays uncompressed: it is written by ``kv_append`` and attended by
+``DensePagedAttention`` (``dense_kv.py``) behind the same methods, block tables and slots.  These are layers with a cache
+dtype of ``auto`` or ``bfloat16`` outside primary mode, those that vLLM exempts from the compressed dtype among them (pages
+have one shape for both kinds there).  In primary mode every page has the size and shape of packed records
+(``engine.py``), so no layer can be exempt.  vLLM's layers rotate queries and keys themselves; ``rope_and_kv_cache_update``
+is for callers that leave it to ``rotary_kv_append``.
 
 The codec is picked like the reference does (``vllm/backend.py:618-626``): ``AITHER_TQ_MODE=tq35``
 selects the hybrid codec, otherwise ``AITHER_TQ_BITS`` (default 4) the uniform one; a
