@@ -176,7 +176,8 @@ class DensePagedAttention:
         """Chunks of new tokens: rows ``query_start_loc[s] .. query_start_loc[s + 1]`` of ``query`` [tokens, query_heads,
         head_dim] are the last tokens of sequence s, whose keys and values (counted in ``seq_lens``) are in the cache
         already; each attends causally up to its own position.  Rows before the first sequence and behind the last are left as
-        they are in ``out`` (zero when ``out`` is allocated here).  Lengths stay on the device: ``max_seq_len``, which
+        they are in ``out`` (zero when ``out`` is allocated here).  A value that is not finite, of a key that some of a
+        chunk's tokens see, may reach the chunk's earlier tokens too.  Lengths stay on the device: ``max_seq_len``, which
         ``TQPagedAttention.prefill`` sizes its scratch by, is accepted and not needed.
 
         Chunks run on the tensor cores for head_dim 64 and 128, at most 128 query heads per KV head and block sizes that
